@@ -261,11 +261,145 @@ int moe_lm_head_upload(moe_ctx *ctx, const moe_tensor *output_weight, const moe_
  * asynchronous on the context's stream (status via moe_device_status). */
 int moe_lm_head(moe_ctx *ctx, int32_t T, const float *normed, float *logits, int32_t n_logits, int32_t ptr_kind);
 
+/* ---- the attention sublayer: norms and rotation, paged 8-bit KV cache, attention ----
+ * The step between two FFN sublayers of the reference's token loop
+ * (src/qwen_deepseek.rs:984-1097: per-head norms, rotation, KV store, grouped
+ * query attention), from the rows of the q/k/v projection to the rows of the
+ * output projection's input. Device pointers on the context's device
+ * throughout; asynchronous on the context's stream; the caller owns all memory
+ * named here, the context a fixed workspace. The first of these calls on a
+ * context allocates it (about 20 MiB), so make that call before capturing the
+ * stream into a graph. Calls on one context, replays of graphs captured from
+ * it among them, are serialised by the caller as every other call.
+ *
+ * What the device finds wrong in batch arrays or page tables (a slot or page id
+ * out of range, row_start not ascending or past n_tokens, more than max_new
+ * rows, a negative past, a sequence longer than its page table, a slot twice in
+ * one append) skips that sequence, or that page, and is reported by
+ * moe_device_status as MOE_ERR_TENSOR_BOUNDS. */
+
+/* Types of activation rows: ggml_type ids. */
+typedef enum moe_act {
+    MOE_ACT_F32 = 0,
+    MOE_ACT_F16 = 1,
+    MOE_ACT_BF16 = 30
+} moe_act;
+
+#define MOE_KV_BLOCK_TOKENS 16   /* tokens that share a scale, as the blocks of the reference's arena (src/kv.rs:1-4) */
+
+/* One layer's KV cache. A block of 16 tokens and one head is held as signed
+ * bytes q with one f32 scale s, each value s * q: s = f32(max|x| / 127) over
+ * the block's tokens, q = x / s rounded to nearest even. Values that are NaN
+ * count as 0, infinite ones as +-127 (the maximum is over the finite ones), and
+ * blocks whose largest magnitude is below 1e-20 are zeros with s = 0. Token t of
+ * slot r lives in page page_table[r * table_stride + t / page_tokens]. The
+ * tokens of a sequence's last, not yet full, block are also kept in f32
+ * (open_k, open_v), and their block is quantised anew when tokens join it: its
+ * bits depend on its tokens only, not on the calls that brought them. */
+typedef struct moe_kv_cache {
+    int32_t head_dim;      /* D: 64 or 128 */
+    int32_t kv_heads;
+    int32_t page_tokens;   /* 16, 32, 64, 128 or 256 */
+    int32_t n_pages;
+    int32_t n_slots;       /* rows of page_table, open_k and open_v */
+    int32_t table_stride;  /* page ids of a row */
+    const int32_t *page_table;   /* [n_slots][table_stride]; entries past a sequence's end are not read */
+    int8_t *k;             /* [n_pages][kv_heads][page_tokens / 16][D / 64][16][64] */
+    int8_t *v;             /* [n_pages][kv_heads][page_tokens / 16][D][16] */
+    float *k_scale, *v_scale;    /* [n_pages][kv_heads][page_tokens / 16] */
+    float *open_k, *open_v;      /* [n_slots][kv_heads][16][D]; moe_kv_append and moe_attention only */
+} moe_kv_cache;
+
+/* A batch of sequences: sequence b has past[b] tokens before this call and the
+ * rows row_start[b] .. row_start[b + 1] - 1, at positions past[b], past[b] + 1, ... */
+typedef struct moe_kv_batch {
+    int32_t n_seqs;
+    int32_t n_tokens;           /* rows of q / k / v; rows from row_start[n_seqs] on are left as they were */
+    const int32_t *past;        /* [n_seqs] */
+    const int32_t *row_start;   /* [n_seqs + 1], or NULL: sequence b has the one row b */
+    const int32_t *slot;        /* [n_seqs] rows of the page table, or NULL: sequence b has slot b */
+    int32_t max_new;            /* upper bound on a sequence's rows (chooses kernels); 0: n_tokens */
+    int32_t _pad;
+} moe_kv_batch;
+
+/* Norm and rotation of query and key heads: x * rsqrt(mean(x^2) + eps) * norm
+ * (per head, where the weight is given), then the first rope_dim values rotated
+ * by position * inv_freq[i] and scaled by mscale. Angles are formed in f64; the
+ * keys of the cache in f64 throughout, then rounded to f32. */
+typedef struct moe_rope {
+    int32_t rope_dim;           /* even, 0 .. head_dim; 0: no rotation */
+    int32_t interleaved;        /* 0: value i turns with i + rope_dim / 2; 1: 2i with 2i + 1 */
+    double theta;               /* inv_freq[i] = theta^(-2i / rope_dim) where inv_freq is NULL */
+    const double *inv_freq;     /* host memory, [rope_dim / 2], or NULL */
+    double mscale;              /* 0 counts as 1 */
+    double eps;
+    const float *q_norm, *k_norm;   /* device, [head_dim] each, or NULL: no norm */
+} moe_rope;
+
+/* Rows of queries, keys and values: head h of row t at x + t * x_stride +
+ * h * head_dim (strides in elements, multiples of 16 bytes, as the pointers). */
+typedef struct moe_qkv_rows {
+    int32_t act;                /* moe_act of q, k and v */
+    int32_t q_heads, kv_heads, head_dim;
+    void *q, *k, *v;
+    int64_t q_stride, k_stride, v_stride;
+} moe_qkv_rows;
+
+typedef struct moe_attn_opts {
+    float scale;                /* of q . k; 0: 1 / sqrt(head_dim) */
+    int32_t window;             /* a row sees the last `window` tokens, itself included; 0: all */
+} moe_attn_opts;
+
+/* Norms and rotates the query and key heads of a batch's rows in one pass
+ * (rmsnorm per head and the rotation, src/qwen_deepseek.rs:984-1097) into
+ * out->q and out->k, which may be in's. out has in's act, heads and head_dim;
+ * a NULL in->q or in->k is passed over. batch->slot is not read. */
+int moe_qk_norm_rope(moe_ctx *ctx, const moe_kv_batch *batch, const moe_rope *rope, const moe_qkv_rows *in,
+                     const moe_qkv_rows *out);
+
+/* Appends rows->k (normed and rotated on the way; rope == NULL: as they are)
+ * and rows->v to the cache, the KV store of src/qwen_deepseek.rs:984-1097 on
+ * blocks of src/kv.rs. A slot may occur once in a batch, and the pages that
+ * take new tokens belong to one sequence (full ones before them may be shared).
+ * The caller advances its past counts. Tokens can be taken back (a smaller past
+ * in the next call) down to the start of the block left open; further back,
+ * append from that block's first token on. */
+int moe_kv_append(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rope *rope,
+                  const moe_qkv_rows *rows);
+
+/* The cached tokens past[b] .. past[b] + rows - 1 of each sequence as rows into
+ * out->k and out->v (either may be NULL), each value s * q rounded to out->act
+ * (for a host path that takes over a sequence, and for tests). */
+int moe_kv_read(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_qkv_rows *out);
+
+/* Grouped-query attention of rows->q over the cached tokens: row i of sequence
+ * b sees the tokens at positions <= past[b] + i (its own key must be cached),
+ * the last opts->window of them; query head h reads key head
+ * h / (q_heads / kv_heads). out rows hold q_heads * head_dim values of
+ * rows->act, out_stride elements apart. A row whose every page is bad gets
+ * zeros. Softmax and sums in f32; with F32 rows the products carry 22 bits of
+ * the queries and weights, with 16-bit rows 11. opts may be NULL. */
+int moe_kv_attention(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_attn_opts *opts,
+                     const moe_qkv_rows *rows, void *out, int64_t out_stride);
+
+/* The whole step: moe_kv_append of rows->k and rows->v, then moe_kv_attention
+ * of rows->q, normed and rotated (in f32) as it is read. */
+int moe_attention(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rope *rope,
+                  const moe_attn_opts *opts, const moe_qkv_rows *rows, void *out, int64_t out_stride);
+
+/* Whether a context of max_tokens takes a moe_attention call with these
+ * arguments, by the same checks, without a device (nothing is read but the
+ * structures and a host inv_freq); the message is moe_last_error_message(NULL)'s. */
+int moe_attention_check(int32_t max_tokens, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rope *rope,
+                        const moe_attn_opts *opts, const moe_qkv_rows *rows, const void *out, int64_t out_stride);
+
 int moe_residency_summary(const moe_ctx *ctx, moe_residency *out);
 
 /* Reads and clears the device status word of ctx (synchronises the context
  * stream). *status != 0 (and MOE_ERR_TIMEOUT) when a bounded wait inside a
- * kernel gave up since the last check; host-pointer forwards check it themselves. */
+ * kernel gave up since the last check; host-pointer forwards check it themselves.
+ * *status != 0 and MOE_ERR_TENSOR_BOUNDS when an attention call since the last
+ * check met a bad batch entry or page (above). */
 int moe_device_status(moe_ctx *ctx, int32_t *status);
 
 /* ---- per-kernel timing (the device counterpart of PassTiming, src/engine.rs:136) ---- */

@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "../../include/jeromoe.h"
+#include "attn.h"
 #include "ep_p2p.h"
 #include "ep_plan.h"
 #include "kernels.h"
@@ -189,6 +190,7 @@ struct moe_ctx {
         MatMaps maps_tc{};       // tensor-core boxes (128 rows), when tc
         bool tc = false;         // the head suits the int8 tensor-core down launch
     } head;
+    void *attn_ws = nullptr;   // attention calls: the status word, then the workspace of split sequences
     Profiler prof;
     EpState ep;
 };
@@ -217,6 +219,13 @@ int cuda_fail(moe_ctx *ctx, cudaError_t e, const char *what)
         cudaError_t e_ = (call);                             \
         if (e_ != cudaSuccess) return cuda_fail(ctx, e_, what); \
     } while (0)
+
+// Puts the calling thread's current device back at the end of a call.
+struct DeviceGuard {
+    int dev = -1;
+    DeviceGuard() { if (cudaGetDevice(&dev) != cudaSuccess) dev = -1; }
+    ~DeviceGuard() { if (dev >= 0) cudaSetDevice(dev); }
+};
 
 // ------------------------------------------------------------ validation
 
@@ -852,6 +861,7 @@ int moe_ctx_destroy(moe_ctx *ctx)
     if (ctx->stack_buf) cudaFree(ctx->stack_buf);
     if (ctx->head.block) cudaFree(ctx->head.block);
     if (ctx->head.buf) cudaFree(ctx->head.buf);
+    if (ctx->attn_ws) cudaFree(ctx->attn_ws);
     EpState &ep = ctx->ep;
     if (ep.comm) {
         if (const NcclApi *nc = nccl_api()) nc->CommDestroy(ep.comm);
@@ -1438,6 +1448,22 @@ int moe_device_status(moe_ctx *ctx, int32_t *status)
 {
     if (!ctx || !status) return fail(nullptr, MOE_ERR_INVALID_ARGS, "null argument");
     *status = 0;
+    if (ctx->attn_ws) {   // the attention calls' own word
+        DeviceGuard guard;
+        CUDA_TRY(ctx, cudaSetDevice(ctx->spec.device), "cudaSetDevice");
+        CUDA_TRY(ctx, cudaMemcpyAsync(ctx->status_host, ctx->attn_ws, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream),
+                 "copy status");
+        CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream), "status sync");
+        *status = *ctx->status_host;
+        if (*status) {
+            CUDA_TRY(ctx, cudaMemsetAsync(ctx->attn_ws, 0, sizeof(int), ctx->stream), "clear status");
+            if (*status != kErrKvBounds)
+                return fail(ctx, MOE_ERR_TIMEOUT, "a bounded device wait ran out in an attention call (status %d)",
+                            *status);
+            return fail(ctx, MOE_ERR_TENSOR_BOUNDS,
+                        "an attention call met a batch entry, slot or page id out of range (or a slot twice)");
+        }
+    }
     // the context's word, or (LM head calls before any layer upload) the head's own
     int *word = ctx->scratch.err ? ctx->scratch.err : ctx->head.errw;
     CUDA_TRY(ctx, cudaSetDevice(ctx->spec.device), "cudaSetDevice");
@@ -2064,6 +2090,271 @@ int moe_forward_ep(moe_ctx *ctx, int32_t layer, int32_t T, const float *x, float
         }
     }
     return MOE_OK;
+}
+
+// ------------------------------------------------- the attention sublayer
+
+static bool misaligned(const void *p) { return ((uintptr_t)p & 15) != 0; }
+
+static size_t act_size(int act) { return act == MOE_ACT_F32 ? 4 : 2; }
+
+static int check_batch(moe_ctx *ctx, int max_tokens, const moe_kv_batch *b, KvBatchDev *out)
+{
+    if (!b) return fail(ctx, MOE_ERR_INVALID_ARGS, "null batch");
+    if (b->n_seqs < 0 || b->n_tokens < 0 || b->max_new < 0)
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "negative sequence, token or max_new count");
+    if (b->n_tokens > max_tokens)
+        return fail(ctx, MOE_ERR_CONTEXT_LENGTH, "%d rows exceed max_tokens %d", b->n_tokens, max_tokens);
+    if (b->n_seqs > 65536) return fail(ctx, MOE_ERR_CAPABILITY_MISMATCH, "%d sequences (at most 65536)", b->n_seqs);
+    if (b->n_seqs && b->n_tokens && !b->past) return fail(ctx, MOE_ERR_INVALID_ARGS, "null past");
+    if (!b->row_start && b->n_tokens != b->n_seqs)
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "without row_start a batch has one row per sequence (%d rows, %d sequences)",
+                    b->n_tokens, b->n_seqs);
+    out->B = b->n_seqs;
+    out->T = b->n_tokens;
+    out->max_new = !b->row_start ? 1 : b->max_new ? std::min(b->max_new, b->n_tokens) : b->n_tokens;
+    out->past = b->past;
+    out->row_start = b->row_start;
+    out->slot = b->slot;
+    return MOE_OK;
+}
+
+static int check_rope(moe_ctx *ctx, const moe_rope *r, int head_dim, RopeDev *out)
+{
+    if (r->rope_dim < 0 || r->rope_dim > head_dim || r->rope_dim % 2)
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "rope_dim %d must be even, 0..%d", r->rope_dim, head_dim);
+    if (!std::isfinite(r->eps) || r->eps < 0.0) return fail(ctx, MOE_ERR_INVALID_ARGS, "eps must be finite and >= 0");
+    if (!std::isfinite(r->mscale)) return fail(ctx, MOE_ERR_INVALID_ARGS, "mscale must be finite");
+    if (r->rope_dim && !r->inv_freq && !(std::isfinite(r->theta) && r->theta > 0.0))
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "theta must be positive where inv_freq is not given");
+    out->R = r->rope_dim;
+    out->interleaved = r->interleaved != 0;
+    out->eps = r->eps;
+    out->mscale = r->mscale == 0.0 ? 1.0 : r->mscale;
+    out->q_norm = r->q_norm;
+    out->k_norm = r->k_norm;
+    for (int i = 0; i < r->rope_dim / 2; i++) {
+        out->inv[i] = r->inv_freq ? r->inv_freq[i] : std::pow(r->theta, -2.0 * i / r->rope_dim);
+        if (!std::isfinite(out->inv[i])) return fail(ctx, MOE_ERR_INVALID_ARGS, "inv_freq[%d] is not finite", i);
+    }
+    return MOE_OK;
+}
+
+// The rows' type, heads and strides; `need`: the tensors (q 1, k 2, v 4) that must be there.
+static int check_rows(moe_ctx *ctx, const moe_qkv_rows *r, int need, AttnRows *out)
+{
+    if (!r) return fail(ctx, MOE_ERR_INVALID_ARGS, "null rows");
+    if (r->act != MOE_ACT_F32 && r->act != MOE_ACT_F16 && r->act != MOE_ACT_BF16)
+        return fail(ctx, MOE_ERR_CAPABILITY_MISMATCH, "unsupported activation type %d", r->act);
+    if (r->head_dim != 64 && r->head_dim != 128)
+        return fail(ctx, MOE_ERR_CAPABILITY_MISMATCH, "head_dim %d (64 or 128)", r->head_dim);
+    const struct { const char *name; const void *p; int heads; int64_t stride; int bit; } t[] = {
+        {"q", r->q, r->q_heads, r->q_stride, 1}, {"k", r->k, r->kv_heads, r->k_stride, 2}, {"v", r->v, r->kv_heads, r->v_stride, 4}};
+    for (const auto &x : t) {
+        if (!x.p) {
+            if (need & x.bit) return fail(ctx, MOE_ERR_INVALID_ARGS, "null %s rows", x.name);
+            continue;
+        }
+        if (x.heads <= 0 || x.heads > 1024) return fail(ctx, MOE_ERR_CAPABILITY_MISMATCH, "%d heads of %s (1..1024)", x.heads, x.name);
+        if (x.stride < (int64_t)x.heads * r->head_dim)
+            return fail(ctx, MOE_ERR_TENSOR_BOUNDS, "%s row stride %lld is below %d heads of %d", x.name, (long long)x.stride,
+                        x.heads, r->head_dim);
+        if (x.stride > ((int64_t)1 << 40)) return fail(ctx, MOE_ERR_TENSOR_BOUNDS, "%s row stride out of range", x.name);
+        if (misaligned(x.p) || x.stride * act_size(r->act) % 16)
+            return fail(ctx, MOE_ERR_INVALID_ARGS, "%s rows must start on 16-byte boundaries", x.name);
+    }
+    *out = AttnRows{r->act, r->q_heads, r->kv_heads, r->q, r->k, r->v, r->q_stride, r->k_stride, r->v_stride};
+    return MOE_OK;
+}
+
+static int check_cache(moe_ctx *ctx, const moe_kv_cache *c, const moe_kv_batch *b, bool open, KvCacheDev *out)
+{
+    if (!c) return fail(ctx, MOE_ERR_INVALID_ARGS, "null cache");
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return fail(ctx, MOE_ERR_CAPABILITY_MISMATCH, "cache head_dim %d (64 or 128)", c->head_dim);
+    if (c->kv_heads <= 0 || c->kv_heads > 1024) return fail(ctx, MOE_ERR_CAPABILITY_MISMATCH, "%d key heads (1..1024)", c->kv_heads);
+    int shift = 0;
+    while (shift < 5 && (kKvBlock << shift) != c->page_tokens) shift++;
+    if (shift == 5) return fail(ctx, MOE_ERR_CAPABILITY_MISMATCH, "page_tokens %d (16, 32, 64, 128 or 256)", c->page_tokens);
+    if (c->n_pages < 0 || c->n_slots < 0 || c->table_stride < 0)
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "negative page, slot or table size");
+    if (!c->page_table || !c->k || !c->v || !c->k_scale || !c->v_scale || (open && (!c->open_k || !c->open_v)))
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "null cache array");
+    if (misaligned(c->k) || misaligned(c->v) || misaligned(c->open_k) || misaligned(c->open_v))
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "cache arrays must be 16-byte aligned");
+    if (!b->slot && b->n_seqs > c->n_slots)
+        return fail(ctx, MOE_ERR_TENSOR_BOUNDS, "%d sequences without slots, %d slots", b->n_seqs, c->n_slots);
+    *out = KvCacheDev{c->head_dim, c->kv_heads, c->n_pages, c->n_slots, c->table_stride, shift, c->page_table,
+                      c->k, c->v, c->k_scale, c->v_scale, c->open_k, c->open_v};
+    return MOE_OK;
+}
+
+// The workspace, allocated by the first attention call of a context. The
+// caller has set the device.
+static int attn_workspace(moe_ctx *ctx)
+{
+    if (ctx->attn_ws) return MOE_OK;
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    CUDA_TRY(ctx, cudaStreamIsCapturing(ctx->stream, &cap), "cudaStreamIsCapturing");
+    if (cap != cudaStreamCaptureStatusNone)
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "the first attention call of a context allocates: make it before capturing");
+    void *ws = nullptr;
+    const size_t bytes = attn_workspace_bytes(ctx->num_sms);
+    if (cudaMalloc(&ws, bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(ctx, MOE_ERR_INSUFFICIENT_MEMORY, "attention workspace of %zu bytes", bytes);
+    }
+    cudaError_t e = cudaMemset(ws, 0, bytes);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();   // the context stream does not wait for the legacy stream
+    if (e != cudaSuccess) {
+        cudaFree(ws);
+        return cuda_fail(ctx, e, "cudaMemset(attention workspace)");
+    }
+    ctx->attn_ws = ws;
+    return MOE_OK;
+}
+
+int moe_qk_norm_rope(moe_ctx *ctx, const moe_kv_batch *batch, const moe_rope *rope, const moe_qkv_rows *in,
+                     const moe_qkv_rows *out)
+{
+    if (!ctx) return fail(nullptr, MOE_ERR_INVALID_ARGS, "null context");
+    if (!rope) return fail(ctx, MOE_ERR_INVALID_ARGS, "null rope");
+    KvBatchDev b;
+    RopeDev r;
+    AttnRows ri, ro;
+    int rc;
+    if ((rc = check_batch(ctx, ctx->spec.max_tokens, batch, &b)) || (rc = check_rows(ctx, in, 0, &ri))) return rc;
+    if (!in->q && !in->k) return fail(ctx, MOE_ERR_INVALID_ARGS, "null q and k rows");
+    if ((rc = check_rows(ctx, out, (in->q ? 1 : 0) | (in->k ? 2 : 0), &ro)) || (rc = check_rope(ctx, rope, in->head_dim, &r)))
+        return rc;
+    if (in->act != out->act || in->head_dim != out->head_dim || (in->q && in->q_heads != out->q_heads) ||
+        (in->k && in->kv_heads != out->kv_heads))
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "input and output rows differ in type or heads");
+    if (b.B == 0 || b.T == 0) return MOE_OK;
+    DeviceGuard guard;
+    CUDA_TRY(ctx, cudaSetDevice(ctx->spec.device), "cudaSetDevice");
+    if ((rc = attn_workspace(ctx))) return rc;
+    const cudaError_t e = launch_qk_norm_rope(b, r, ri, ro, in->head_dim, static_cast<int *>(ctx->attn_ws), ctx->stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "norm and rotation");
+    return MOE_OK;
+}
+
+int moe_kv_append(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rope *rope,
+                  const moe_qkv_rows *rows)
+{
+    if (!ctx) return fail(nullptr, MOE_ERR_INVALID_ARGS, "null context");
+    KvBatchDev b;
+    KvCacheDev c;
+    RopeDev r{};
+    AttnRows rr;
+    int rc;
+    if ((rc = check_batch(ctx, ctx->spec.max_tokens, batch, &b)) || (rc = check_cache(ctx, cache, batch, true, &c)) ||
+        (rc = check_rows(ctx, rows, 2 | 4, &rr)))
+        return rc;
+    if (rope && (rc = check_rope(ctx, rope, cache->head_dim, &r))) return rc;
+    if (rows->head_dim != cache->head_dim || rows->kv_heads != cache->kv_heads)
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "rows of %d heads of %d, cache of %d heads of %d", rows->kv_heads,
+                    rows->head_dim, cache->kv_heads, cache->head_dim);
+    if (b.B == 0 || b.T == 0) return MOE_OK;
+    DeviceGuard guard;
+    CUDA_TRY(ctx, cudaSetDevice(ctx->spec.device), "cudaSetDevice");
+    if ((rc = attn_workspace(ctx))) return rc;
+    const cudaError_t e = launch_kv_append(c, b, rope ? &r : nullptr, rr, static_cast<int *>(ctx->attn_ws), ctx->stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cache append");
+    return MOE_OK;
+}
+
+int moe_kv_read(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_qkv_rows *out)
+{
+    if (!ctx) return fail(nullptr, MOE_ERR_INVALID_ARGS, "null context");
+    KvBatchDev b;
+    KvCacheDev c;
+    AttnRows ro;
+    int rc;
+    if ((rc = check_batch(ctx, ctx->spec.max_tokens, batch, &b)) || (rc = check_cache(ctx, cache, batch, false, &c)) ||
+        (rc = check_rows(ctx, out, 0, &ro)))
+        return rc;
+    if (!out->k && !out->v) return fail(ctx, MOE_ERR_INVALID_ARGS, "null k and v rows");
+    if (out->head_dim != cache->head_dim || out->kv_heads != cache->kv_heads)
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "rows of %d heads of %d, cache of %d heads of %d", out->kv_heads,
+                    out->head_dim, cache->kv_heads, cache->head_dim);
+    if (b.B == 0 || b.T == 0) return MOE_OK;
+    DeviceGuard guard;
+    CUDA_TRY(ctx, cudaSetDevice(ctx->spec.device), "cudaSetDevice");
+    if ((rc = attn_workspace(ctx))) return rc;
+    const cudaError_t e = launch_kv_read(c, b, ro, static_cast<int *>(ctx->attn_ws), ctx->stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cache read");
+    return MOE_OK;
+}
+
+// The argument checks of moe_kv_attention, and with append of moe_attention;
+// fills the kernels' parameters.
+static int check_attention(moe_ctx *ctx, int max_tokens, const moe_kv_cache *cache, const moe_kv_batch *batch,
+                           const moe_rope *rope, const moe_attn_opts *opts, const moe_qkv_rows *rows, void *out,
+                           int64_t out_stride, bool append, AttnParams *p)
+{
+    int rc;
+    if ((rc = check_batch(ctx, max_tokens, batch, &p->b)) || (rc = check_cache(ctx, cache, batch, append, &p->c)) ||
+        (rc = check_rows(ctx, rows, append ? 1 | 2 | 4 : 1, &p->rows)))
+        return rc;
+    if (rope && (rc = check_rope(ctx, rope, cache->head_dim, &p->rope))) return rc;
+    if (rows->head_dim != cache->head_dim || rows->kv_heads != cache->kv_heads || rows->q_heads % cache->kv_heads)
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "rows of %d query and %d key heads of %d, cache of %d heads of %d",
+                    rows->q_heads, rows->kv_heads, rows->head_dim, cache->kv_heads, cache->head_dim);
+    p->use_rope = rope != nullptr;
+    p->scale = opts && opts->scale != 0.0f ? opts->scale : (float)(1.0 / std::sqrt((double)cache->head_dim));
+    if (!std::isfinite(p->scale)) return fail(ctx, MOE_ERR_INVALID_ARGS, "scale must be finite");
+    p->window = opts ? opts->window : 0;
+    if (p->window < 0) return fail(ctx, MOE_ERR_INVALID_ARGS, "negative window");
+    if (!out || misaligned(out) || out_stride * (int64_t)act_size(rows->act) % 16)
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "out rows must start on 16-byte boundaries");
+    if (out_stride < (int64_t)rows->q_heads * rows->head_dim || out_stride > ((int64_t)1 << 40))
+        return fail(ctx, MOE_ERR_TENSOR_BOUNDS, "out row stride %lld for %d heads of %d", (long long)out_stride,
+                    rows->q_heads, rows->head_dim);
+    p->out = out;
+    p->out_stride = out_stride;
+    return MOE_OK;
+}
+
+static int attention_impl(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rope *rope,
+                          const moe_attn_opts *opts, const moe_qkv_rows *rows, void *out, int64_t out_stride, bool append)
+{
+    if (!ctx) return fail(nullptr, MOE_ERR_INVALID_ARGS, "null context");
+    AttnParams p{};
+    int rc;
+    if ((rc = check_attention(ctx, ctx->spec.max_tokens, cache, batch, rope, opts, rows, out, out_stride, append, &p)))
+        return rc;
+    if (p.b.B == 0 || p.b.T == 0) return MOE_OK;
+    DeviceGuard guard;
+    CUDA_TRY(ctx, cudaSetDevice(ctx->spec.device), "cudaSetDevice");
+    if ((rc = attn_workspace(ctx))) return rc;
+    p.err = static_cast<int *>(ctx->attn_ws);
+    p.num_sms = ctx->num_sms;
+    p.ws = ctx->attn_ws;
+    cudaError_t e;
+    if (append && (e = launch_kv_append(p.c, p.b, rope ? &p.rope : nullptr, p.rows, p.err, ctx->stream)) != cudaSuccess)
+        return cuda_fail(ctx, e, "cache append");
+    if ((e = launch_attention(p, ctx->stream)) != cudaSuccess) return cuda_fail(ctx, e, "attention");
+    return MOE_OK;
+}
+
+int moe_attention_check(int32_t max_tokens, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rope *rope,
+                        const moe_attn_opts *opts, const moe_qkv_rows *rows, const void *out, int64_t out_stride)
+{
+    AttnParams p{};
+    return check_attention(nullptr, max_tokens, cache, batch, rope, opts, rows, const_cast<void *>(out), out_stride, true, &p);
+}
+
+int moe_kv_attention(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_attn_opts *opts,
+                     const moe_qkv_rows *rows, void *out, int64_t out_stride)
+{
+    return attention_impl(ctx, cache, batch, nullptr, opts, rows, out, out_stride, false);
+}
+
+int moe_attention(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rope *rope,
+                  const moe_attn_opts *opts, const moe_qkv_rows *rows, void *out, int64_t out_stride)
+{
+    return attention_impl(ctx, cache, batch, rope, opts, rows, out, out_stride, true);
 }
 
 uint64_t moe_row_bytes(int32_t quant, int32_t cols) { return gguf_row_bytes(quant, cols); }

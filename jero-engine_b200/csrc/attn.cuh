@@ -1,0 +1,148 @@
+// attn.cuh -- device helpers of the attention sublayer: activation types, batch
+// and page lookups with their checks, and the norm and rotation of a query head.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <limits.h>
+
+#include "../../include/jeromoe.h"
+#include "attn.h"
+#include "ptx.cuh"
+
+namespace jmoe {
+
+template <int ACT> struct ActType;
+template <> struct ActType<MOE_ACT_F32> { using T = float; };
+template <> struct ActType<MOE_ACT_F16> { using T = __half; };
+template <> struct ActType<MOE_ACT_BF16> { using T = __nv_bfloat16; };
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+// one rounding to the row's type, to nearest even
+__device__ __forceinline__ void from_f32(float &d, float v) { d = v; }
+__device__ __forceinline__ void from_f32(__half &d, float v) { d = __float2half_rn(v); }
+__device__ __forceinline__ void from_f32(__nv_bfloat16 &d, float v) { d = __float2bfloat16_rn(v); }
+
+// N consecutive values (N * size a multiple of 8 bytes, so aligned) to and from f32.
+template <int N, typename T>
+__device__ __forceinline__ void load_vals(const T *p, float (&v)[N])
+{
+    constexpr int kBytes = N * (int)sizeof(T), kWord = kBytes % 16 == 0 ? 16 : kBytes % 8 == 0 ? 8 : 4;
+    static_assert(kBytes % kWord == 0, "vector");
+    alignas(16) T t[N];
+#pragma unroll
+    for (int i = 0; i < kBytes / kWord; i++) {
+        if (kWord == 16) reinterpret_cast<uint4 *>(t)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+        else if (kWord == 8) reinterpret_cast<uint2 *>(t)[i] = __ldg(reinterpret_cast<const uint2 *>(p) + i);
+        else reinterpret_cast<uint32_t *>(t)[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = to_f32(t[i]);
+}
+
+template <int N, typename T>
+__device__ __forceinline__ void store_vals(T *p, const float (&v)[N])
+{
+    constexpr int kBytes = N * (int)sizeof(T), kWord = kBytes % 16 == 0 ? 16 : kBytes % 8 == 0 ? 8 : 4;
+    static_assert(kBytes % kWord == 0, "vector");
+    alignas(16) T t[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) from_f32(t[i], v[i]);
+#pragma unroll
+    for (int i = 0; i < kBytes / kWord; i++) {
+        if (kWord == 16) reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(t)[i];
+        else if (kWord == 8) reinterpret_cast<uint2 *>(p)[i] = reinterpret_cast<const uint2 *>(t)[i];
+        else reinterpret_cast<uint32_t *>(p)[i] = reinterpret_cast<const uint32_t *>(t)[i];
+    }
+}
+
+__device__ __forceinline__ void kv_error(int *err) { atomicExch(err, kErrKvBounds); }
+
+__device__ __forceinline__ int row_of(const KvBatchDev &b, int s) { return b.row_start ? __ldg(b.row_start + s) : s; }
+
+struct SeqInfo {
+    int past, row0, n;
+};
+
+// Sequence s of the batch; false where its entries are out of range.
+__device__ __forceinline__ bool seq_info(const KvBatchDev &b, int s, SeqInfo &q)
+{
+    q.past = __ldg(b.past + s);
+    q.row0 = row_of(b, s);
+    const int end = row_of(b, s + 1);
+    q.n = end - q.row0;
+    return q.row0 >= 0 && end >= q.row0 && end <= b.T && q.n <= b.max_new && q.past >= 0 &&
+           q.past <= INT_MAX - 4096 - q.n;
+}
+
+// The same against a cache: the slot exists and its table holds the sequence's tokens.
+__device__ __forceinline__ bool seq_in_cache(const KvCacheDev &c, const KvBatchDev &b, int s, const SeqInfo &q, int &slot)
+{
+    slot = b.slot ? __ldg(b.slot + s) : s;
+    return slot >= 0 && slot < c.n_slots &&
+           ((int64_t)q.past + q.n + kKvBlock - 1) / kKvBlock <= ((int64_t)c.table_stride << c.page_shift);
+}
+
+// Block `blk` of a slot's sequence: index of (page, block in page) for head 0
+// in units of blocks, with the head stride page_blocks; -1 for a bad page id.
+__device__ __forceinline__ int64_t block_index(const KvCacheDev &c, int slot, int blk, int head)
+{
+    const int page = __ldg(c.table + (int64_t)slot * c.table_stride + (blk >> c.page_shift));
+    if (page < 0 || page >= c.n_pages) return -1;
+    return (((int64_t)page * c.heads + head) << c.page_shift) + (blk & ((1 << c.page_shift) - 1));
+}
+
+// cos and sin of an angle in f64, reduced there to [-pi, pi] so that far
+// positions lose nothing, then in f32.
+__device__ __forceinline__ void turn_f32(double angle, float &c, float &s)
+{
+    const double n = rint(angle * 0.15915494309189535);
+    double r = fma(-n, 6.283185307179586, angle);
+    r = fma(-n, 2.4492935982947064e-16, r);   // the rest of 2 pi
+    sincosf((float)r, &s, &c);
+}
+
+// Indices of pair i of a head's first R values.
+__device__ __forceinline__ int2 rope_pair(const RopeDev &r, int i)
+{
+    return r.interleaved ? make_int2(2 * i, 2 * i + 1) : make_int2(i, i + r.R / 2);
+}
+
+// One warp: head row x[D] normed (w != nullptr) and rotated at position pos
+// into y[D] (shared memory), all in f32 but the angles.
+template <int D, typename T>
+__device__ __forceinline__ void norm_rope_head(const T *x, const float *w, const RopeDev &r, int pos, float *y, int lane)
+{
+    constexpr int N = D / 32;
+    float v[N];
+    load_vals<N>(x + lane * N, v);
+    if (w) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; i++) ss = fmaf(v[i], v[i], ss);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = 1.0f / sqrtf(ss * (1.0f / D) + (float)r.eps);
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = v[i] * inv * __ldg(w + lane * N + i);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < N; i++) y[lane * N + i] = v[i];
+    __syncwarp();
+    for (int i = lane; i < r.R / 2; i += 32) {
+        float c, s;
+        turn_f32((double)pos * r.inv[i], c, s);
+        c *= (float)r.mscale;
+        s *= (float)r.mscale;
+        const int2 ab = rope_pair(r, i);
+        const float a = y[ab.x], b = y[ab.y];
+        y[ab.x] = a * c - b * s;
+        y[ab.y] = b * c + a * s;
+    }
+    __syncwarp();
+}
+
+}  // namespace jmoe

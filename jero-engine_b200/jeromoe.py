@@ -27,7 +27,7 @@ LIB_PATH = os.path.join(HERE, "libjeromoe.so")
 from moe_types import (  # noqa: F401,E402
     MOE_OK, MOE_ERR_INVALID_ARGS, MOE_ERR_CAPABILITY_MISMATCH, MOE_ERR_INSUFFICIENT_MEMORY,
     MOE_ERR_RESOURCE_EXHAUSTED, MOE_ERR_TENSOR_BOUNDS, MOE_ERR_CONTEXT_LENGTH, MOE_ERR_NOT_UPLOADED, MOE_ERR_CUDA,
-    MOE_ERR_NCCL, MOE_ERR_TIMEOUT, F32, Q8_0, Q4_K, QUANT_NAMES, ROUTE_SOFTMAX_TOPK, ROUTE_GROUP_LIMITED, MoeError,
+    MOE_ERR_NCCL, MOE_ERR_TIMEOUT, F32, F16, BF16, Q8_0, Q4_K, QUANT_NAMES, ROUTE_SOFTMAX_TOPK, ROUTE_GROUP_LIMITED, MoeError,
     InvalidArguments, CapabilityMismatch, InsufficientLockableMemory, ResourceExhausted, TensorBoundsError,
     ContextLengthExceeded, NotUploaded, CudaError, NcclError, DeviceTimeout, Tensor, f32_tensor, ModelWeights,
     RouteSpec, ERRORS as _ERRORS)
@@ -40,6 +40,8 @@ FLAG_INT8_TENSOR_CORES_NEVER, FLAG_INT8_TENSOR_CORES_ALWAYS = 8, 16
 FLAG_FUSED_TC_NEVER = 32   # small batches: no fused tensor-core expert launch
 FLAG_FUSED_I8_NEVER, FLAG_FUSED_I8_ALWAYS = 64, 128   # the fused launch's f16 / int8 form
 TENSOR_CORE_MIN_TOKENS = 256
+STREAM_LEGACY = 1       # Context.set_stream: the legacy default stream (0 is the context's own)
+KV_BLOCK_TOKENS = 16
 
 # ------------------------------------------------------------------- structs
 
@@ -85,6 +87,49 @@ class moe_kernel_time(C.Structure):
     _fields_ = [("name", C.c_char * 32), ("total_ms", C.c_double), ("launches", C.c_int64)]
 
 
+class KvCache(C.Structure):
+    """moe_kv_cache: one layer's paged 8-bit cache, device pointers as integers."""
+    _fields_ = [("head_dim", C.c_int32), ("kv_heads", C.c_int32), ("page_tokens", C.c_int32), ("n_pages", C.c_int32),
+                ("n_slots", C.c_int32), ("table_stride", C.c_int32), ("page_table", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("open_k", C.c_void_p),
+                ("open_v", C.c_void_p)]
+
+
+class KvBatch(C.Structure):
+    """moe_kv_batch: past, row_start and slot are device pointers."""
+    _fields_ = [("n_seqs", C.c_int32), ("n_tokens", C.c_int32), ("past", C.c_void_p), ("row_start", C.c_void_p),
+                ("slot", C.c_void_p), ("max_new", C.c_int32), ("_pad", C.c_int32)]
+
+
+class _moe_rope(C.Structure):
+    _fields_ = [("rope_dim", C.c_int32), ("interleaved", C.c_int32), ("theta", C.c_double), ("inv_freq", C.c_void_p),
+                ("mscale", C.c_double), ("eps", C.c_double), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p)]
+
+
+class Rope(_moe_rope):
+    """moe_rope: q_norm and k_norm are device pointers, inv_freq a host array [rope_dim / 2] or None."""
+
+    def __init__(self, rope_dim=0, interleaved=False, theta=0.0, eps=0.0, mscale=1.0, q_norm=0, k_norm=0, inv_freq=None):
+        f = None if inv_freq is None else np.ascontiguousarray(inv_freq, dtype=np.float64)
+        if f is not None and f.size < rope_dim // 2:
+            raise InvalidArguments(MOE_ERR_INVALID_ARGS, f"{f.size} inverse frequencies for rope_dim {rope_dim}")
+        super().__init__(rope_dim, int(bool(interleaved)), theta, f.ctypes.data if f is not None else None, mscale, eps,
+                         q_norm or None, k_norm or None)
+        self._keep = f
+
+
+class QkvRows(C.Structure):
+    """moe_qkv_rows: rows of queries, keys and values; strides in elements."""
+    _fields_ = [("act", C.c_int32), ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64)]
+
+
+class AttnOpts(C.Structure):
+    """moe_attn_opts."""
+    _fields_ = [("scale", C.c_float), ("window", C.c_int32)]
+
+
 # ------------------------------------------------------------------- library
 
 EXPORTS = {
@@ -102,6 +147,17 @@ EXPORTS = {
     "moe_prefill_ffn_layers": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int32]),
     "moe_lm_head_upload": (C.c_int, [C.c_void_p, C.POINTER(moe_tensor), C.POINTER(moe_tensor), C.c_int32]),
     "moe_lm_head": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32]),
+    "moe_qk_norm_rope": (C.c_int, [C.c_void_p, C.POINTER(KvBatch), C.POINTER(_moe_rope), C.POINTER(QkvRows),
+                                   C.POINTER(QkvRows)]),
+    "moe_kv_append": (C.c_int, [C.c_void_p, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(_moe_rope),
+                                C.POINTER(QkvRows)]),
+    "moe_kv_read": (C.c_int, [C.c_void_p, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(QkvRows)]),
+    "moe_kv_attention": (C.c_int, [C.c_void_p, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(AttnOpts),
+                                   C.POINTER(QkvRows), C.c_void_p, C.c_int64]),
+    "moe_attention": (C.c_int, [C.c_void_p, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(_moe_rope),
+                                C.POINTER(AttnOpts), C.POINTER(QkvRows), C.c_void_p, C.c_int64]),
+    "moe_attention_check": (C.c_int, [C.c_int32, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(_moe_rope),
+                                      C.POINTER(AttnOpts), C.POINTER(QkvRows), C.c_void_p, C.c_int64]),
     "moe_residency_summary": (C.c_int, [C.c_void_p, C.POINTER(moe_residency)]),
     "moe_device_status": (C.c_int, [C.c_void_p, C.POINTER(C.c_int32)]),
     "moe_ctx_set_profiling": (C.c_int, [C.c_void_p, C.c_int32]),
@@ -350,6 +406,30 @@ class Context:
         _check(lib.moe_prefill_ffn_layers(self.h, first_layer, n_layers, T, _ptr(rows), PTR_HOST), self.h)
         return rows
 
+    # ---- the attention sublayer (device pointers; asynchronous on the context's stream)
+
+    def qk_norm_rope(self, batch: KvBatch, rope: Rope, rows: QkvRows, out: QkvRows):
+        """Per-head norms and rotation of rows.q and rows.k into out.q and out.k (moe_qk_norm_rope)."""
+        _check(lib.moe_qk_norm_rope(self.h, batch, rope, rows, out), self.h)
+
+    def kv_append(self, cache: KvCache, batch: KvBatch, rope: Optional[Rope], rows: QkvRows):
+        """Appends rows.k (normed and rotated; rope None: as they are) and rows.v to the cache (moe_kv_append)."""
+        _check(lib.moe_kv_append(self.h, cache, batch, rope, rows), self.h)
+
+    def kv_read(self, cache: KvCache, batch: KvBatch, out: QkvRows):
+        """Cached tokens past[b] .. of each sequence as rows into out.k and out.v (moe_kv_read)."""
+        _check(lib.moe_kv_read(self.h, cache, batch, out), self.h)
+
+    def kv_attention(self, cache: KvCache, batch: KvBatch, opts: Optional[AttnOpts], rows: QkvRows, out_ptr: int,
+                     out_stride: int):
+        """Attention of rows.q over the cached tokens (moe_kv_attention)."""
+        _check(lib.moe_kv_attention(self.h, cache, batch, opts, rows, out_ptr, out_stride), self.h)
+
+    def attention(self, cache: KvCache, batch: KvBatch, rope: Optional[Rope], opts: Optional[AttnOpts], rows: QkvRows,
+                  out_ptr: int, out_stride: int):
+        """Append, then attention of the normed and rotated queries (moe_attention)."""
+        _check(lib.moe_attention(self.h, cache, batch, rope, opts, rows, out_ptr, out_stride), self.h)
+
     # ---- expert parallelism (moe_ep_init / moe_forward_ep)
 
     def ep_init(self, rank: int, world: int, uid: bytes):
@@ -461,6 +541,12 @@ def admission_check(device: int, max_tokens: int, descs: Sequence[moe_layer_desc
         insp = C.byref(moe_mem_inspector(free_bytes, total_bytes or free_bytes))
     _check(lib.moe_admission_check(C.byref(spec), arr, len(descs), insp, C.byref(fp)))
     return fp
+
+
+def attention_check(max_tokens: int, cache: KvCache, batch: KvBatch, rope: Optional[Rope], opts: Optional[AttnOpts],
+                    rows: QkvRows, out_ptr: int, out_stride: int):
+    """Raises what Context.attention would for these arguments; needs no device (moe_attention_check)."""
+    _check(lib.moe_attention_check(max_tokens, cache, batch, rope, opts, rows, out_ptr, out_stride))
 
 
 def probe_tensor(device: int, kind: int, m: int, n: int, a_tmem: bool = False, n_acc: int = 1, ctas_per_sm: int = 1,

@@ -26,6 +26,7 @@ MOE_ERR_NCCL = 21
 MOE_ERR_TIMEOUT = 22
 
 F32, Q8_0, Q4_K = 0, 8, 12
+F16, BF16 = 1, 30   # activation rows of the attention calls (F32 too)
 QUANT_NAMES = {F32: "F32", Q8_0: "Q8_0", Q4_K: "Q4_K"}
 ROUTE_SOFTMAX_TOPK, ROUTE_GROUP_LIMITED = 0, 1
 

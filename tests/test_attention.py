@@ -1,0 +1,788 @@
+"""The attention sublayer (moe_qk_norm_rope, moe_kv_append, moe_kv_read,
+moe_kv_attention, moe_attention) against the plain 64-bit oracle.
+
+Tolerances. u = 2^-24 is a rounding to f32; a rounding to a row's type is at
+most half a step, eps / 2 relative.
+
+Norm and rotation in f32 of a head of D values: sum of squares (D/32 + 5 chained
+roundings, halved by the root), root, quotient, two products: under 12 u; the
+angle, reduced in f64, is rounded once (pi u) and its sine and cosine are good to
+2 ulp, two products and a sum follow: under 12 u of |a| + |b|. In all 24 u (|a| + |b|).
+
+Attention: a logit is a sum of D products of exact 8-bit values with queries of
+22 bits (F32 rows) or exact ones (16-bit rows, scaled by a power of two), scaled
+in f32: its error is at most A (2^-22 + (D + 8) u) with A = scale * max sum
+|q_d k_d|. A weight is then off by twice that (the maximum is off too) and the
+exponential's 2^-21, relative; weights enter the product with 22 bits, or 11
+with 16-bit rows; sums over L tokens add (L + 64) u in numerator and in
+denominator. Each part moves the output by at most that share of max|v|, twice
+(numerator and denominator)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import attn_oracle as ao
+import jeromoe as jm
+
+U = 2.0 ** -24
+ACTS = {"f32": jm.F32, "f16": jm.F16, "bf16": jm.BF16}
+HALF_STEP = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+# ------------------------------------------------------------------ refusals
+
+
+def _args(**over):
+    """A moe_attention call that is taken; pointers are only checked, never read."""
+    P = 1 << 20
+    a = {"max_tokens": 64, "out": P, "out_stride": 32 * 128,
+         "cache": dict(head_dim=128, kv_heads=4, page_tokens=64, n_pages=10, n_slots=4, table_stride=4, page_table=P, k=P,
+                       v=P, k_scale=P, v_scale=P, open_k=P, open_v=P),
+         "batch": dict(n_seqs=4, n_tokens=4, past=P),
+         "rope": dict(rope_dim=128, theta=1e6, eps=1e-6, q_norm=P, k_norm=P),
+         "opts": dict(),
+         "rows": dict(act=jm.F32, q_heads=32, kv_heads=4, head_dim=128, q=P, k=P, v=P, q_stride=4096, k_stride=512,
+                      v_stride=512)}
+    for key, v in over.items():
+        part, _, name = key.partition("__")
+        if name:
+            a[part] = {**a[part], name: v}
+        else:
+            a[part] = v
+    return a
+
+
+def _check(a):
+    jm.attention_check(a["max_tokens"], jm.KvCache(**a["cache"]), jm.KvBatch(**a["batch"]), jm.Rope(**a["rope"]),
+                       jm.AttnOpts(**a["opts"]), jm.QkvRows(**a["rows"]), a["out"], a["out_stride"])
+
+
+def test_check_takes_good_arguments():
+    _check(_args())
+    _check(_args(rows__act=jm.BF16, cache__page_tokens=16, opts__window=100, rope__rope_dim=0))
+    _check(_args(batch=dict(n_seqs=2, n_tokens=7, past=1 << 20, row_start=1 << 20, slot=1 << 20)))
+    _check(_args(batch=dict(n_seqs=0, n_tokens=0)))
+
+
+@pytest.mark.parametrize("over,error", [
+    (dict(cache__head_dim=96), jm.CapabilityMismatch),
+    (dict(cache__head_dim=256, rows__head_dim=256), jm.CapabilityMismatch),
+    (dict(cache__page_tokens=24), jm.CapabilityMismatch),
+    (dict(cache__page_tokens=512), jm.CapabilityMismatch),
+    (dict(cache__page_tokens=0), jm.CapabilityMismatch),
+    (dict(cache__kv_heads=0), jm.CapabilityMismatch),
+    (dict(cache__n_pages=-1), jm.InvalidArguments),
+    (dict(cache__n_slots=3), jm.TensorBoundsError),
+    (dict(cache__k=0), jm.InvalidArguments),
+    (dict(cache__v=(1 << 20) + 8), jm.InvalidArguments),
+    (dict(cache__open_k=0), jm.InvalidArguments),
+    (dict(cache__page_table=0), jm.InvalidArguments),
+    (dict(batch__n_tokens=5), jm.InvalidArguments),
+    (dict(batch__n_seqs=-1), jm.InvalidArguments),
+    (dict(batch__max_new=-1), jm.InvalidArguments),
+    (dict(batch__past=0), jm.InvalidArguments),
+    (dict(max_tokens=3), jm.ContextLengthExceeded),
+    (dict(rope__rope_dim=3), jm.InvalidArguments),
+    (dict(rope__rope_dim=130), jm.InvalidArguments),
+    (dict(rope__rope_dim=-2), jm.InvalidArguments),
+    (dict(rope__theta=0.0), jm.InvalidArguments),
+    (dict(rope__theta=float("nan")), jm.InvalidArguments),
+    (dict(rope__eps=-1.0), jm.InvalidArguments),
+    (dict(rope__eps=float("inf")), jm.InvalidArguments),
+    (dict(rope__mscale=float("nan")), jm.InvalidArguments),
+    (dict(rope__inv_freq=[float("inf")] * 64), jm.InvalidArguments),
+    (dict(rope__inv_freq=[1.0] * 63), jm.InvalidArguments),
+    (dict(opts__window=-1), jm.InvalidArguments),
+    (dict(opts__scale=float("inf")), jm.InvalidArguments),
+    (dict(rows__act=8), jm.CapabilityMismatch),
+    (dict(rows__q_heads=30), jm.InvalidArguments),
+    (dict(rows__q_heads=0), jm.CapabilityMismatch),
+    (dict(rows__kv_heads=2), jm.InvalidArguments),
+    (dict(rows__head_dim=64), jm.InvalidArguments),
+    (dict(rows__q=0), jm.InvalidArguments),
+    (dict(rows__v=0), jm.InvalidArguments),
+    (dict(rows__q=(1 << 20) + 4), jm.InvalidArguments),
+    (dict(rows__q_stride=4095), jm.TensorBoundsError),
+    (dict(rows__k_stride=514), jm.InvalidArguments),
+    (dict(out=0), jm.InvalidArguments),
+    (dict(out=(1 << 20) + 4), jm.InvalidArguments),
+    (dict(out_stride=4095), jm.InvalidArguments),
+    (dict(out_stride=2048), jm.TensorBoundsError),
+])
+def test_check_refuses(over, error):
+    with pytest.raises(error):
+        _check(_args(**over))
+
+
+def test_struct_sizes_match_the_header():
+    assert [C.sizeof(t) for t in (jm.KvCache, jm.KvBatch, jm.Rope, jm.QkvRows, jm.AttnOpts)] == [80, 40, 56, 64, 8]
+
+
+def test_quantiser_of_the_oracle():
+    x = np.zeros((16, 64), np.float32)
+    x[0, :4] = [127.0, 0.5, 1.5, -2.5]     # scale 1: ties go to even
+    q, s = ao.quantise(x)
+    assert s == 1.0 and q[0, :4].tolist() == [127, 0, 2, -2]
+    x[1, :3] = [np.nan, np.inf, -np.inf]
+    q, s = ao.quantise(x)
+    assert s == 1.0 and q[1, :3].tolist() == [0, 127, -127]
+    assert ao.quantise(np.full((16, 64), 1e-21, np.float32))[1] == 0.0
+
+
+# ----------------------------------------------------------------- GPU set-up
+
+
+class Setup:
+    """A context, a cache and a batch on the GPU with the oracle's view of the same."""
+
+    def __init__(self, act="f32", D=128, q_heads=8, kv_heads=2, page=32, n_slots=4, pages_per_slot=6, seed=0, poison=True):
+        import torch
+        self.t = torch
+        self.act, self.D, self.hq, self.hk, self.page = act, D, q_heads, kv_heads, page
+        self.dtype = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[act]
+        self.rng = np.random.default_rng(seed)
+        self.n_slots, self.stride = n_slots, pages_per_slot
+        self.n_pages = n_slots * pages_per_slot + 3
+        pb = page // 16
+        dev = "cuda"
+        # pages hold what earlier users left: any bytes, and scales that must not leak
+        self.k = torch.full((self.n_pages, kv_heads, pb, D // 64, 16, 64), 99, dtype=torch.int8, device=dev)
+        self.v = torch.full((self.n_pages, kv_heads, pb, D, 16), -77, dtype=torch.int8, device=dev)
+        bad = float("nan") if poison else 0.0
+        self.k_scale = torch.full((self.n_pages, kv_heads, pb), bad, device=dev)
+        self.v_scale = torch.full((self.n_pages, kv_heads, pb), bad, device=dev)
+        self.open_k = torch.full((n_slots, kv_heads, 16, D), float("nan"), device=dev)
+        self.open_v = torch.full((n_slots, kv_heads, 16, D), float("nan"), device=dev)
+        self.table_np = self.rng.permutation(self.n_pages)[: n_slots * pages_per_slot].reshape(n_slots, pages_per_slot)
+        self.table = torch.tensor(self.table_np, dtype=torch.int32, device=dev)
+        self.ctx = jm.Context(0, max_tokens=4096)
+        self.ctx.set_stream(jm.STREAM_LEGACY)
+        self.cache = jm.KvCache(head_dim=D, kv_heads=kv_heads, page_tokens=page, n_pages=self.n_pages, n_slots=n_slots,
+                                table_stride=pages_per_slot, page_table=self.table.data_ptr(), k=self.k.data_ptr(),
+                                v=self.v.data_ptr(), k_scale=self.k_scale.data_ptr(), v_scale=self.v_scale.data_ptr(),
+                                open_k=self.open_k.data_ptr(), open_v=self.open_v.data_ptr())
+        self.ref = ao.Cache()
+        self.lens = [0] * n_slots
+        self.keep = []
+
+    def close(self):
+        self.t.cuda.synchronize()
+        self.ctx.close()
+
+    def ints(self, v):
+        x = self.t.tensor(v, dtype=self.t.int32, device="cuda")
+        self.keep.append(x)
+        return x.data_ptr()
+
+    def batch(self, past, new, slots, behind=0, max_new=0):
+        rs = np.concatenate(([0], np.cumsum(new)))
+        return jm.KvBatch(n_seqs=len(past), n_tokens=int(rs[-1]) + behind, past=self.ints(list(past)),
+                          row_start=self.ints(rs.tolist()), slot=self.ints(list(slots)), max_new=max_new)
+
+    def rows(self, T, scale=1.0, pad=0):
+        """Random rows of a fused projection (with `pad` 16-byte units between rows) and their f64 values."""
+        t = self.t
+        width = (self.hq + 2 * self.hk) * self.D + pad * (4 if self.act == "f32" else 8)
+        x = t.tensor(self.rng.standard_normal((max(T, 1), width)) * scale, dtype=self.dtype, device="cuda")
+        self.keep.append(x)
+        a, b = self.hq * self.D, (self.hq + self.hk) * self.D
+        size = x.element_size()
+        r = jm.QkvRows(act=ACTS[self.act], q_heads=self.hq, kv_heads=self.hk, head_dim=self.D, q=x.data_ptr(),
+                       k=x.data_ptr() + a * size, v=x.data_ptr() + b * size, q_stride=width, k_stride=width, v_stride=width)
+        f = x.double().cpu().numpy()
+        return r, x, f[:, :a].reshape(-1, self.hq, self.D), f[:, a:b].reshape(-1, self.hk, self.D), \
+            f[:, b:b + self.hk * self.D].reshape(-1, self.hk, self.D)
+
+    def out(self, T, heads, fill=123.0):
+        x = self.t.full((max(T, 1), heads, self.D), fill, dtype=self.dtype, device="cuda")
+        self.keep.append(x)
+        return x
+
+    def into(self, q=None, k=None, v=None):
+        return jm.QkvRows(act=ACTS[self.act], q_heads=self.hq, kv_heads=self.hk, head_dim=self.D,
+                          q=q.data_ptr() if q is not None else 0, k=k.data_ptr() if k is not None else 0,
+                          v=v.data_ptr() if v is not None else 0, q_stride=self.hq * self.D, k_stride=self.hk * self.D,
+                          v_stride=self.hk * self.D)
+
+    def rope(self, rope_dim=None, interleaved=False, norm=True, **kw):
+        R = self.D if rope_dim is None else rope_dim
+        w = {n: (1.0 + 0.3 * self.rng.standard_normal(self.D)).astype(np.float32) for n in ("q", "k")} if norm else {}
+        dev = {n: self.t.tensor(x, device="cuda") for n, x in w.items()}
+        self.keep.append(dev)
+        kw = {"theta": 1e6, "eps": 1e-6, **kw}
+        r = jm.Rope(rope_dim=R, interleaved=interleaved, q_norm=dev["q"].data_ptr() if norm else 0,
+                    k_norm=dev["k"].data_ptr() if norm else 0, **kw)
+
+        def plain(x, which, pos):
+            return ao.norm_rope(x, w.get(which), pos, R, interleaved, theta=kw["theta"], eps=kw["eps"],
+                                mscale=kw.get("mscale", 1.0), inv_freq=kw.get("inv_freq"))
+        return r, plain
+
+    def append(self, past, new, slots, rope=None, plain=None, rows=None, behind=0):
+        """Appends random rows on both sides; the oracle takes keys rounded to f32 as the library does."""
+        T = int(np.sum(new))
+        r, x, q, k, v = rows or self.rows(T + behind)
+        b = self.batch(past, new, slots, behind)
+        self.ctx.kv_append(self.cache, b, rope, r)
+        at = 0
+        for p, n, s in zip(past, new, slots):
+            if n:
+                kk = k[at:at + n] if plain is None else plain(k[at:at + n], "k", p + np.arange(n))
+                self.ref.append(s, p, kk, v[at:at + n])
+                self.lens[s] = p + n
+            at += n
+        return b, r, q
+
+    def device_blocks(self, slot):
+        """(kq, ks, vq, vs) of a slot as the oracle's blocks() lays them out."""
+        n = self.lens[slot]
+        nb = -(-n // 16)
+        pb = self.page // 16
+        blocks = np.arange(nb)
+        pages = self.t.tensor(self.table_np[slot][blocks // pb], device="cuda")
+        at = self.t.tensor(blocks % pb, device="cuda")
+        kq = self.k[pages, :, at].permute(1, 0, 3, 2, 4).reshape(self.hk, nb, 16, self.D).cpu().numpy()
+        vq = self.v[pages, :, at].permute(1, 0, 3, 2).cpu().numpy()
+        ks, vs = (s[pages, :, at].t().cpu().numpy() for s in (self.k_scale, self.v_scale))
+        return kq, ks, vq, vs
+
+    def check_blocks(self, slot, exact_keys=False):
+        kq, ks, vq, vs = self.device_blocks(slot)
+        rq, rs = self.ref.blocks(slot, "v")
+        np.testing.assert_array_equal(vq, rq)
+        np.testing.assert_array_equal(vs, rs)
+        rq, rs = self.ref.blocks(slot, "k")
+        if exact_keys:
+            np.testing.assert_array_equal(kq, rq)
+            np.testing.assert_array_equal(ks, rs)
+            return
+        # numpy's and the device's f64 functions may differ in the last place, which
+        # the rounding to f32 shows once in some 10^8 values: scales within one ulp of
+        # f32 (and its rounding), values within one step and all but never off
+        assert np.all(np.abs(ks.astype(np.float64) - rs) <= 4 * U * rs)
+        d = np.abs(kq.astype(int) - rq.astype(int))
+        assert d.max(initial=0) <= 1 and np.count_nonzero(d) <= 1 + kq.size // 100000
+
+    def check_attention(self, got, q, past, new, slots, scale=None, window=0, q_err=0.0, bad=()):
+        """got [T, hq, D] f64 against the oracle over the device's own cache bits."""
+        scale = scale or 1.0 / np.sqrt(self.D)
+        at = 0
+        for p, n, s in zip(past, new, slots):
+            if not n:
+                continue
+            kq, ks, vq, vs = self.device_blocks(s)
+            o, A, vmax = ao.attend(q[at:at + n], kq, ks, vq, vs, p, scale, window, bad)
+            L = p + n
+            logit = A * (2.0 ** -22 + (self.D + 8) * U + q_err)
+            part = 2 * logit + 2.0 ** -21 + (2.0 ** -22 if self.act == "f32" else 2.0 ** -11) + (L + 64) * U
+            tol = 2 * part * vmax + HALF_STEP[self.act] * np.abs(o)
+            err = np.abs(got[at:at + n] - o)
+            assert np.all(err <= tol), (s, float((err - tol).max()), float(err.max()), float(np.min(tol)))
+            at += n
+
+    def attend(self, past, new, slots, q=None, rows=None, opts=None, behind=0, max_new=0, scale=None, window=0, bad=()):
+        T = int(np.sum(new))
+        if rows is None:
+            rows, _, q, _, _ = self.rows(T + behind)
+        out = self.out(T + behind, self.hq)
+        opts = opts or jm.AttnOpts(window=window, scale=scale or 0.0)
+        self.ctx.kv_attention(self.cache, self.batch(past, new, slots, behind, max_new), opts, rows, out.data_ptr(),
+                              self.hq * self.D)
+        got = out.double().cpu().numpy()
+        self.check_attention(got[:T], q, past, new, slots, scale, window, bad=bad)
+        assert np.all(got[T:T + behind] == 123.0), "rows behind the last sequence were written"
+        return got
+
+
+@pytest.fixture
+def make():
+    made = []
+
+    def f(*a, **kw):
+        made.append(Setup(*a, **kw))
+        return made[-1]
+    yield f
+    for s in made:
+        s.close()
+
+
+# ----------------------------------------------------------- norm and rotation
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,R,interleaved,norm", [(128, 128, False, True), (64, 64, True, True), (128, 64, True, False),
+                                                  (128, 2, False, True), (64, 0, False, True), (128, 0, False, False),
+                                                  (64, 34, False, True)])
+def test_norm_rope(make, act, D, R, interleaved, norm):
+    s = make(act, D=D, q_heads=6, kv_heads=3)
+    rope, plain = s.rope(R, interleaved, norm, mscale=1.25)
+    past, new = [0, 5, 1 << 20, 130], [1, 0, 7, 3]
+    r, x, q, k, _ = s.rows(13, pad=1)
+    oq, ok = s.out(13, s.hq), s.out(13, s.hk)
+    s.ctx.qk_norm_rope(s.batch(past, new, range(4), behind=2), rope, r, s.into(oq, ok))
+    pos = np.concatenate([p + np.arange(n) for p, n in zip(past, new)])
+    for got, x, which in ((oq, q, "q"), (ok, k, "k")):
+        ref = plain(x[:11], which, pos)
+        got = got.double().cpu().numpy()
+        size = 2 * np.max(np.abs(ref), axis=-1, keepdims=True) * np.sqrt(2.0)   # at least |a| + |b| of any pair
+        assert np.all(np.abs(got[:11] - ref) <= 24 * U * size + HALF_STEP[act] * np.abs(ref) * (1 + 2 ** -7))
+        assert np.all(got[11:] == 123.0)
+
+
+@pytest.mark.gpu
+def test_norm_rope_in_place_and_one_tensor(make):
+    s = make("f32")
+    rope, plain = s.rope()
+    r, x, q, k, _ = s.rows(5)
+    b = jm.KvBatch(n_seqs=5, n_tokens=5, past=s.ints([3, 1, 4, 1, 5]))
+    before = x.clone()
+    only_k = jm.QkvRows(**{f: getattr(r, f) for f, _ in r._fields_})
+    only_k.q = None
+    s.ctx.qk_norm_rope(b, rope, only_k, only_k)
+    ref = plain(k, "k", [3, 1, 4, 1, 5])
+    a, e = s.hq * s.D, (s.hq + s.hk) * s.D
+    got = x[:, a:e].double().cpu().numpy().reshape(ref.shape)
+    assert np.all(np.abs(got - ref) <= 24 * U * 4 * np.max(np.abs(ref), axis=-1, keepdims=True))
+    assert s.t.equal(x[:, :a], before[:, :a]) and s.t.equal(x[:, e:], before[:, e:])
+
+
+@pytest.mark.gpu
+def test_norm_rope_given_frequencies_far_positions(make):
+    """Angles of far positions: a frequency of 1 at position 2^30 turns by 2^30 radians."""
+    s = make("f32", D=64)
+    f = 1.0 / (1.0 + np.arange(32))
+    rope, plain = s.rope(64, False, False, inv_freq=f)
+    pos = [1 << 30, (1 << 30) + 1, 7]
+    r, x, q, k, _ = s.rows(3)
+    oq, ok = s.out(3, s.hq), s.out(3, s.hk)
+    s.ctx.qk_norm_rope(jm.KvBatch(n_seqs=3, n_tokens=3, past=s.ints(pos)), rope, r, s.into(oq, ok))
+    ref = plain(q, "q", pos)
+    # numpy reduces 2^30 radians exactly; the angle itself is a product in f64: 2^30 * 2^-53 = 2^-23
+    size = np.max(np.abs(q), axis=-1, keepdims=True) * 2
+    assert np.all(np.abs(oq.double().cpu().numpy() - ref) <= (24 * U + 2.0 ** -22) * size)
+
+
+# ------------------------------------------------------------------ the cache
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,page", [(128, 32), (64, 16), (128, 256)])
+def test_append_blocks_are_the_tokens_own(make, act, D, page):
+    """Histories built by different splits hold the same bits, the oracle's, open blocks among them."""
+    n = 83
+    splits = [[n], [1] * n, [16, 16, 51], [5, 11, 1, 15, 33, 18]]
+    s = make(act, D=D, page=page, pages_per_slot=-(-96 // page) + 1)
+    rope, plain = s.rope(D // 2, True)
+    r, x, q, k, v = s.rows(n)
+    size = x.element_size()
+    for slot, parts in enumerate(splits):
+        past = 0
+        for m in parts:
+            rr = jm.QkvRows(**{f: getattr(r, f) for f, _ in r._fields_})
+            for name in ("q", "k", "v"):
+                setattr(rr, name, getattr(r, name) + past * r.q_stride * size)
+            s.append([past], [m], [slot], rope, plain, rows=(rr, x, q[past:], k[past:], v[past:]))
+            past += m
+    first = s.device_blocks(0)
+    s.check_blocks(0)
+    for slot in range(1, 4):
+        for a, b in zip(first, s.device_blocks(slot)):
+            np.testing.assert_array_equal(a, b)
+    want_k, want_v = (np.asarray(x[0][80:83]) for x in ([s.ref.k[0]], [s.ref.v[0]]))
+    for slot in range(4):
+        got_k, got_v = (o[slot, :, :3].transpose(0, 1).cpu().numpy() for o in (s.open_k, s.open_v))
+        np.testing.assert_allclose(got_k, want_k, rtol=4 * U, atol=0)
+        np.testing.assert_array_equal(got_v, want_v)
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_append_ragged_batch_strided_rows(make):
+    s = make("bf16", q_heads=3, kv_heads=3, D=64, page=16, n_slots=6, pages_per_slot=20)
+    rope, plain = s.rope()
+    lens = {4: 0, 1: 0, 5: 0, 0: 0, 2: 0}
+    for step in range(4):
+        slots = [4, 1, 5, 0, 2]
+        new = s.rng.integers(0, 60, 5).tolist() if step else [0, 16, 1, 17, 100]
+        r = s.rows(sum(new) + 3, pad=step)
+        s.append([lens[i] for i in slots], new, slots, rope, plain, rows=r, behind=3)
+        for i, n in zip(slots, new):
+            lens[i] += n
+    untouched = s.k_scale.clone()
+    for i, n in lens.items():
+        if n:
+            s.check_blocks(i)
+    assert np.isnan(untouched[s.table[3].long()].cpu().numpy()).all(), "an unused slot's pages were written"
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_append_odd_values(make):
+    """NaN, infinities, zeros, tiny blocks and ties of the rounding, without norm or rotation."""
+    s = make("f32", D=64, q_heads=2, kv_heads=2)
+    r, x, q, k, v = s.rows(40)
+    a, b = s.hq * s.D, (s.hq + s.hk) * s.D
+    x[16:32] = 0.0
+    x[32:, a:b] *= 1e-22
+    x[0, a] = float("nan")
+    x[1, a + 1] = float("inf")
+    x[2, b] = -float("inf")
+    x[3, b + 1] = float("nan")
+    x[:16, b + 64:] = s.t.tensor(np.resize(np.arange(-127, 128) / 2.0, (16, 64)), device="cuda", dtype=s.dtype)
+    x[0, b + 64] = 127.0
+    f = x.double().cpu().numpy()
+    k, v = f[:, a:b].reshape(-1, 2, 64), f[:, b:].reshape(-1, 2, 64)
+    s.append([0], [40], [2], rows=(r, x, q, k, v))
+    s.check_blocks(2, exact_keys=True)
+    kq, ks, vq, vs = s.device_blocks(2)
+    assert ks[:, 1].tolist() == [0, 0] and ks[:, 2].tolist() == [0, 0] and vs[1, 0] == 1.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+def test_read_rounds_once(make, act):
+    s = make(act, D=128, page=64)
+    s.append([0, 0], [70, 33], [3, 1], rows=s.rows(103))
+    ok, ov = s.out(50, s.hk), s.out(50, s.hk)
+    s.ctx.kv_read(s.cache, s.batch([21, 3], [30, 18], [3, 1], behind=2), s.into(k=ok, v=ov))
+    at = 0
+    for slot, lo, n in ((3, 21, 30), (1, 3, 18)):
+        kq, ks, vq, vs = s.device_blocks(slot)
+        for got, qv, sc in ((ok, kq, ks), (ov, vq, vs)):
+            val = (qv.astype(np.float32) * sc[..., None, None]).reshape(s.hk, -1, s.D)[:, lo:lo + n].transpose(1, 0, 2)
+            want = s.t.tensor(val).to(s.dtype)
+            assert s.t.equal(got[at:at + n].cpu(), want)
+        at += n
+    assert np.all(ok[48:].double().cpu().numpy() == 123.0)
+    alone = s.out(1, s.hk)
+    s.ctx.kv_read(s.cache, s.batch([21], [1], [3]), s.into(v=alone))
+    assert s.t.equal(alone[0], ov[0])
+
+
+# ------------------------------------------------------------------ attention
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,hq,hk,page", [(128, 8, 1, 64), (64, 14, 2, 16), (128, 2, 2, 32), (64, 16, 1, 128),
+                                          (128, 15, 3, 16), (128, 33, 1, 64)])
+def test_attention_lengths(make, act, D, hq, hk, page):
+    """Single tokens, drafts and prompts over histories around block, page and tile ends."""
+    s = make(act, D=D, q_heads=hq, kv_heads=hk, page=page, n_slots=8, pages_per_slot=-(-448 // page))
+    total = [1, 2, 15, 16, 17, 64, 129, 300]
+    s.append([0] * 8, total, range(8), rows=s.rows(sum(total)))
+    for new in ([1] * 8, [1, 2, 3, 5, 8, 9, 17, 33], [1, 0, 15, 16, 1, 64, 129, 300]):
+        slots = s.rng.permutation(8)
+        n = [new[i] for i in slots]
+        s.attend([total[i] - new[i] for i in slots], n, slots, behind=2, max_new=max(n))
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [1, 2, 16, 63, 100, 10000])
+def test_attention_window(make, act, window):
+    s = make(act, D=64, q_heads=4, kv_heads=2, page=16, n_slots=3, pages_per_slot=20)
+    total = [300, 77, 16]
+    s.append([0] * 3, total, range(3), rows=s.rows(sum(total)))
+    # blocks that no row sees hold poison
+    for i, t in enumerate(total):
+        for b in range(max(0, t - 30 - window + 1) // 16):
+            s.k_scale[int(s.table_np[i][b]), :, 0] = float("nan")
+            s.v_scale[int(s.table_np[i][b]), :, 0] = float("inf")
+    blocks = s.device_blocks
+
+    def clean(slot):
+        return tuple(np.nan_to_num(x, nan=0.0, posinf=0.0) for x in blocks(slot))
+    s.device_blocks = clean
+    for new in ([1, 1, 1], [30, 9, 16]):
+        s.attend([t - n for t, n in zip(total, new)], new, range(3), window=window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16"])
+def test_attention_long_history_and_extreme_scales(make, act):
+    """Work split over a long history; heads whose value blocks differ by orders of magnitude."""
+    s = make(act, D=128, q_heads=8, kv_heads=2, page=64, n_slots=2, pages_per_slot=70)
+    n = 4000
+    r, x, q, k, v = s.rows(n)
+    b = (s.hq + s.hk) * s.D
+    gain = np.ones((n, 1), np.float32)
+    gain[::3] = 1e-3
+    gain[512:1024] = 1e-4 if act == "f16" else 1e-7
+    gain[2000:2500] = 30.0 if act == "f16" else 1e6
+    gain[3000:3100] = 0.0
+    x[:, b:b + s.D] *= s.t.tensor(gain, device="cuda", dtype=s.dtype)
+    f = x.double().cpu().numpy()
+    v = f[:, b:].reshape(-1, 2, 128)
+    s.append([0], [n], [1], rows=(r, x, q, k, v))
+    s.check_blocks(1, exact_keys=True)
+    s.attend([n - 1], [1], [1])
+    s.attend([n - 6], [6], [1])
+    s.attend([700], [1], [1])
+    s.attend([n - 1], [1], [1], scale=3.0)
+
+
+@pytest.mark.gpu
+def test_attention_extreme_queries(make):
+    """Queries beyond half precision's range and a head of zeros."""
+    s = make("f32", D=64, q_heads=4, kv_heads=2, n_slots=1, pages_per_slot=8)
+    s.append([0], [200], [0], rows=s.rows(200))
+    r, x, q, _, _ = s.rows(3)
+    x[0, :64] *= 1e7
+    x[1, 64:128] = 0.0
+    x[2, 128:192] *= 1e-9
+    q = x[:, : 4 * 64].double().cpu().numpy().reshape(3, 4, 64)
+    s.attend([197], [3], [0], q=q, rows=r, scale=1e-6)
+    s.attend([197], [3], [0], q=q, rows=r, scale=1e-2)
+
+
+@pytest.mark.gpu
+def test_attention_bad_entries_are_skipped_and_reported(make):
+    s = make("f32", D=64, q_heads=4, kv_heads=2, page=16, n_slots=4, pages_per_slot=8)
+    total = [100, 60, 30, 20]
+    s.append([0] * 4, total, range(4), rows=s.rows(sum(total)))
+    assert s.ctx.device_status() == 0
+
+    def status():
+        with pytest.raises(jm.TensorBoundsError):
+            s.ctx.device_status()
+        assert s.ctx.device_status() == 0
+
+    # page ids out of range: those blocks count as absent; a row that sees no other gets zeros
+    good = s.table.clone()
+    s.table[0, 2] = -1
+    s.table[0, 4] = s.n_pages
+    s.attend([99], [1], [0], bad=(2, 4))
+    status()
+    s.attend([40], [60], [0], bad=(2, 4), max_new=60)
+    status()
+    s.table[3, :2] = 1 << 30
+    r, _, q, _, _ = s.rows(2)
+    out = s.out(2, s.hq)
+    s.ctx.kv_attention(s.cache, s.batch([19, 59], [1, 1], [3, 1]), None, r, out.data_ptr(), s.hq * s.D)
+    got = out.double().cpu().numpy()
+    assert np.all(got[0] == 0.0)
+    s.check_attention(got[1:], q[1:], [59], [1], [1])
+    status()
+    s.table.copy_(good)
+    # sequences out of range are passed over, the others computed
+    for past, new, slots in (([99, 59, 29], [1, 1, 1], [0, 4, 2]), ([99, 59, 29], [1, 1, 1], [0, -1, 2]),
+                             ([99, -1, 29], [1, 1, 1], [0, 1, 2]), ([99, 8 * 16, 29], [1, 1, 1], [0, 1, 2]),
+                             ([99, 2147483647, 29], [1, 1, 1], [0, 1, 2])):
+        r, _, q, _, _ = s.rows(3)
+        out = s.out(3, s.hq)
+        s.ctx.kv_attention(s.cache, s.batch(past, new, slots), None, r, out.data_ptr(), s.hq * s.D)
+        got = out.double().cpu().numpy()
+        assert np.all(got[1] == 123.0)
+        s.check_attention(got[:1], q[:1], [99], [1], [0])
+        s.check_attention(got[2:], q[2:], [29], [1], [2])
+        status()
+    # more rows than max_new, rows past the end, rows that go back
+    r, _, q, _, _ = s.rows(4)
+    out = s.out(4, s.hq)
+    for rs, n in (([0, 3, 4], 2), ([0, 5, 4], 4), ([-1, 3, 4], 4)):
+        b = jm.KvBatch(n_seqs=2, n_tokens=4, past=s.ints([0, 59]), row_start=s.ints(rs), slot=s.ints([2, 1]), max_new=n)
+        out.fill_(123.0)
+        s.ctx.kv_attention(s.cache, b, None, r, out.data_ptr(), s.hq * s.D)
+        got = out.double().cpu().numpy()
+        assert np.all(got[:3] == 123.0)
+        status()
+
+
+@pytest.mark.gpu
+def test_append_and_read_bad_entries(make):
+    s = make("f32", D=64, q_heads=2, kv_heads=2, page=16, n_slots=4, pages_per_slot=4)
+    s.append([0], [20], [0], rows=s.rows(20))
+
+    def status():
+        with pytest.raises(jm.TensorBoundsError):
+            s.ctx.device_status()
+        assert s.ctx.device_status() == 0
+
+    state = [t.clone() for t in (s.k, s.v, s.k_scale, s.open_k)]
+    for past, new, slots in (([20], [1], [4]), ([20], [1], [-1]), ([60], [5], [0]), ([-3], [1], [0])):
+        r = s.rows(sum(new))[0]
+        s.ctx.kv_append(s.cache, s.batch(past, new, slots), None, r)
+        status()
+        for a, b in zip(state, (s.k, s.v, s.k_scale, s.open_k)):
+            assert s.t.equal(a.nan_to_num(-5.0), b.nan_to_num(-5.0))
+        ok = s.out(sum(new), 2)
+        s.ctx.kv_read(s.cache, s.batch(past, new, slots), s.into(k=ok))
+        status()
+        assert np.all(ok.double().cpu().numpy() == 123.0)
+    # a slot twice: the first is appended, the second passed over
+    r, x, q, k, v = s.rows(4)
+    s.ctx.kv_append(s.cache, s.batch([20, 0, 22], [2, 1, 1], [0, 1, 0]), None, r)
+    status()
+    s.ref.append(0, 20, k[:2], v[:2])
+    s.ref.append(1, 0, k[2:3], v[2:3])
+    s.lens[0], s.lens[1] = 22, 1
+    s.check_blocks(0, exact_keys=True)
+    s.check_blocks(1, exact_keys=True)
+    # a page out of range: its tokens are not held, the others are
+    s.table[2, 1] = 99
+    r, x, q, k, v = s.rows(40)
+    s.ctx.kv_append(s.cache, s.batch([0], [40], [2]), None, r)
+    status()
+    ok = s.out(40, 2)
+    s.ctx.kv_read(s.cache, s.batch([0], [40], [2]), s.into(k=ok))
+    status()
+    got = ok.double().cpu().numpy()
+    assert np.all(got[16:32] == 0.0) and np.all(np.abs(got[:16] - k[:16]) < 0.05) and np.all(np.abs(got[32:] - k[32:]) < 0.05)
+
+
+# ------------------------------------------------------------ the whole step
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,D,hq,hk,page", [("f32", 128, 8, 2, 64), ("bf16", 64, 14, 2, 16), ("f16", 128, 4, 4, 32)])
+def test_attention_step_prompts_then_decode(make, act, D, hq, hk, page):
+    """Ragged prompts, then single tokens and drafts, through moe_attention."""
+    s = make(act, D=D, q_heads=hq, kv_heads=hk, page=page, n_slots=4, pages_per_slot=-(-256 // page))
+    rope, plain = s.rope(D, D == 64)
+    lens = [0, 0, 0, 0]
+    for step, new in enumerate(([37, 150, 1, 0], [1, 1, 1, 20], [4, 1, 0, 1]) + tuple([1, 1, 1, 1] for _ in range(6))):
+        T = sum(new)
+        r, x, q, k, v = s.rows(T, pad=step % 2)
+        out = s.out(T, hq)
+        s.ctx.attention(s.cache, s.batch(lens, new, range(4)), rope, None, r, out.data_ptr(), hq * D)
+        got = out.double().cpu().numpy()
+        at, qr = 0, []
+        for i, n in enumerate(new):
+            if n:
+                pos = lens[i] + np.arange(n)
+                s.ref.append(i, lens[i], plain(k[at:at + n], "k", pos), v[at:at + n])
+                qr.append(plain(q[at:at + n], "q", pos))
+                s.lens[i] = lens[i] + n
+                s.check_blocks(i)
+            at += n
+        qr = np.concatenate(qr)
+        s.check_attention(got, qr, lens, new, range(4), q_err=48 * U)
+        lens = [a + b for a, b in zip(lens, new)]
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_decoder_layers_attention_then_ffn():
+    """Attention and the FFN sublayer in turn on one context, as a decoder layer runs them:
+    the FFN's results are those of a context of its own."""
+    import torch
+    import synth
+    cfg = synth.CONFIGS[2].scaled(E=16, I=256, H=512)
+    w = synth.build_weights(cfg)
+    s = Setup("f32", D=64, q_heads=8, kv_heads=2, n_slots=3)
+    d, keep = synth.desc_for(cfg, w)
+    alone = jm.Context(0, 8, 1)
+    for c in (s.ctx, alone):
+        c.upload(0, d)
+        c.set_ffn_norm(0, None, 1e-6)
+    rope, plain = s.rope()
+    past = [0, 0, 0]
+    hidden = torch.from_numpy(synth.gen_x(cfg, 3)).cuda()
+    for step in range(5):
+        r, x, q, k, v = s.rows(3)
+        out = s.out(3, 8)
+        b = s.batch(past, [1, 1, 1], range(3))
+        s.ctx.attention(s.cache, b, rope, None, r, out.data_ptr(), 512)
+        after = hidden + 0.1 * out.view(3, 512)
+        torch.cuda.synchronize()
+        got = torch.empty_like(after)
+        s.ctx.forward_block_ptrs(0, 3, after.data_ptr(), got.data_ptr())
+        torch.cuda.synchronize()
+        ref, _, _ = alone.forward_block(0, after.cpu().numpy())
+        np.testing.assert_array_equal(got.cpu().numpy(), ref)
+        pos = np.array(past)
+        for i in range(3):
+            s.ref.append(i, past[i], plain(k[i:i + 1], "k", pos[i:i + 1]), v[i:i + 1])
+            s.lens[i] = past[i] + 1
+        s.check_attention(out.double().cpu().numpy(), plain(q, "q", pos), past, [1] * 3, range(3), q_err=48 * U)
+        past = [p + 1 for p in past]
+        hidden = got
+    assert s.ctx.device_status() == 0
+    alone.close()
+    s.close()
+
+
+@pytest.mark.gpu
+def test_captured_step_replays_over_growing_histories(make):
+    """One graph of the step, replayed while the batch's past counts, rows and page table move on."""
+    import torch
+    s = make("f32", D=128, q_heads=8, kv_heads=2, page=16, n_slots=3, pages_per_slot=10)
+    rope, plain = s.rope()
+    stream = torch.cuda.Stream()
+    past = torch.tensor([0, 40, 70], dtype=torch.int32, device="cuda")
+    s.append([0, 0], [40, 70], [1, 2], rope, plain)
+    r, x, _, _, _ = s.rows(3)
+    out = s.out(3, 8)
+    batch = jm.KvBatch(n_seqs=3, n_tokens=3, past=past.data_ptr())
+    torch.cuda.synchronize()
+    s.ctx.set_stream(stream.cuda_stream)
+    fresh = jm.Context(0, max_tokens=8)
+    fresh.set_stream(stream.cuda_stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        with pytest.raises(jm.InvalidArguments):      # a context's first call allocates: refused while capturing
+            fresh.attention(s.cache, batch, rope, None, r, out.data_ptr(), 1024)
+        s.ctx.attention(s.cache, batch, rope, None, r, out.data_ptr(), 1024)
+    fresh.close()
+    for step in range(20):
+        x.copy_(torch.tensor(s.rng.standard_normal(tuple(x.shape)), dtype=s.dtype))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        f = x.double().cpu().numpy()
+        q, k, v = (f[:, a * 128:b * 128].reshape(3, -1, 128) for a, b in ((0, 8), (8, 10), (10, 12)))
+        pos = past.cpu().numpy()
+        for i in range(3):
+            s.ref.append(i, int(pos[i]), plain(k[i:i + 1], "k", pos[i:i + 1]), v[i:i + 1])
+            s.lens[i] = int(pos[i]) + 1
+            s.check_blocks(i)
+        s.check_attention(out.double().cpu().numpy(), plain(q, "q", pos), pos.tolist(), [1] * 3, range(3), q_err=48 * U)
+        past += 1
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_results_do_not_change_between_runs(make):
+    s = make("bf16", D=128, q_heads=32, kv_heads=4, page=64, n_slots=5, pages_per_slot=40)
+    total = [2500, 3, 700, 64, 1999]
+    s.append([0] * 3, total[:3], range(3), rows=s.rows(sum(total[:3])))
+    s.append([0] * 2, total[3:], [3, 4], rows=s.rows(sum(total[3:])))
+    for new in ([1] * 5, [70, 3, 5, 1, 200]):
+        r = s.rows(sum(new))[0]
+        b = s.batch([t - n for t, n in zip(total, new)], new, range(5))
+        first = None
+        for _ in range(4):
+            out = s.out(sum(new), 32)
+            s.ctx.kv_attention(s.cache, b, None, r, out.data_ptr(), 32 * 128)
+            first = out if first is None else first
+            assert s.t.equal(first, out)
+
+
+@pytest.mark.gpu
+def test_two_contexts_on_two_streams(make):
+    """Contexts have workspaces of their own: calls at once on two streams give what they give alone."""
+    import torch
+    s = make("f32", D=128, q_heads=8, kv_heads=2, page=64, n_slots=2, pages_per_slot=60)
+    s.append([0], [3500], [0], rows=s.rows(3500))
+    s.append([0], [3000], [1], rows=s.rows(3000))
+    other = jm.Context(0, max_tokens=64)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    work = []
+    for i, ctx in enumerate((s.ctx, other)):
+        r, _, q, _, _ = s.rows(1)
+        work.append((ctx, s.batch([s.lens[i] - 1], [1], [i]), r, s.out(1, 8), q))
+    torch.cuda.synchronize()
+    for (ctx, b, r, out, q), st in zip(work, streams):
+        ctx.set_stream(st.cuda_stream)
+    for _ in range(20):
+        for ctx, b, r, out, q in work:
+            ctx.kv_attention(s.cache, b, None, r, out.data_ptr(), 1024)
+    torch.cuda.synchronize()
+    for i, (ctx, b, r, out, q) in enumerate(work):
+        s.check_attention(out.double().cpu().numpy(), q, [s.lens[i] - 1], [1], [i])
+    other.close()
