@@ -2,97 +2,615 @@
 //   o = sum_j p_j (sv_j V_j) / sum_j p_j,  p_j = exp(scale q . (sk_j K_j) - m),
 // over the tokens j <= position of the row (and inside its window), with the
 // running maximum m and the sums in f32, in one pass over the cache.
+//
+// attend_stream_kernel: the whole batch's (sequence, row chunk, key head, tile
+// of 64 tokens) list is cut into equal runs, one per CTA, found on the device
+// from the batch arrays. A run's tiles go to the CTA's warps in turn; each warp
+// keeps the softmax of its row tile in registers, and the warps' (and, where a
+// run ends inside a sequence, the CTAs') parts are joined by their maxima.
+//
+// The products run on mma.m16n8k16 with f16 operands: a decode row tile has 8
+// rows, which the 128-row tcgen05 form would leave 15/16 empty, and the kernel
+// is bound by the cache's bytes. Cache bytes are exact in f16. Queries are
+// scaled per row by a power of two; with F32 rows they and the weights are
+// split in two f16 halves that take the upper and lower 8 rows of the same
+// instruction, so 22 bits cost no more than 11.
+//
+// The value scale sv of a block enters as a term of the exponent: the weights
+// w = exp2(s + log2 sv - m) stay in (0, 1] whatever the scales, and p = w / sv
+// is summed for the denominator.
 #include "attn.cuh"
 #include "kernels.h"
+#include "tc_common.cuh"
 
 namespace jmoe {
 namespace {
 
-constexpr int kSimpleWarps = 4;
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kTile = 64;                    // tokens of a tile: 4 blocks
+constexpr int kMaxRows = 128;                // rows of a chunk (8 warps x 16)
+// A run has at least this many tiles: fewer CTAs share a short sequence.
+constexpr int kMinTiles = 2;
 
-// One warp per (row, query head): lanes split the head's values, tokens go by
-// one after another.
-template <int D, typename T>
-__global__ void __launch_bounds__(kSimpleWarps * 32) attention_simple_kernel(const __grid_constant__ AttnParams p)
+// Workspace: status word | arrival counters [ctas] | partials [ctas][2].
+constexpr size_t kCounterOff = 256;
+size_t partial_off(int ctas) { return kCounterOff + ((size_t)ctas * 4 + 255) / 256 * 256; }
+constexpr size_t kPartialBytes = (size_t)kMaxRows * (kMaxHeadDim + 2) * 4;
+
+// Values of a sequence without a scale (an all-zero block): far below any real
+// scale (>= 2^-74), so its weights stay small and its sums in range.
+constexpr float kNoScaleLog2 = -80.0f;
+
+__device__ __forceinline__ float ex2(float x)
 {
-    __shared__ float s_q[kSimpleWarps][D];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const KvCacheDev &c = p.c;
-    if (blockIdx.x == 0)
-        for (int s = threadIdx.x; s < p.b.B; s += blockDim.x) {
-            SeqInfo q;
-            int slot;
-            if (!seq_info(p.b, s, q) || !seq_in_cache(c, p.b, s, q, slot)) kv_error(p.err);
-        }
-    const int64_t item = (int64_t)blockIdx.x * kSimpleWarps + warp;
-    const int row = (int)(item / p.rows.q_heads), head = (int)(item - (int64_t)row * p.rows.q_heads);
-    if (row >= p.b.T) return;
-    int lo = 0, hi = p.b.B - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (row_of(p.b, mid) <= row) lo = mid;
-        else hi = mid - 1;
-    }
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(smem_addr(bar))
+                 : "memory");
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Four signed bytes to f16 pairs: byte + 128 under the exponent of 1024, minus 1152.
+__device__ __forceinline__ void bytes_f16(uint32_t w, uint32_t &lo, uint32_t &hi)
+{
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), bias), y = __hsub2(*reinterpret_cast<__half2 *>(&b), bias);
+    lo = *reinterpret_cast<const uint32_t *>(&x);
+    hi = *reinterpret_cast<const uint32_t *>(&y);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// a and b as f16 pairs hi + lo (22 bits).
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32_t &lo)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = pack_f16(a - f.x, b - f.y);
+}
+
+// A sequence of the batch as work: `chunks` row chunks x key heads x `tiles`.
+struct SeqWork {
     SeqInfo q;
-    int slot;
-    if (!seq_info(p.b, lo, q) || row < q.row0 || row >= q.row0 + q.n || !seq_in_cache(c, p.b, lo, q, slot)) return;
-    constexpr int N = D / 32;
-    const int pos = q.past + row - q.row0, kvh = head / (p.rows.q_heads / c.heads);
-    const T *x = static_cast<const T *>(p.rows.q) + row * p.rows.q_stride + head * D;
-    float qv[N], o[N], m = -INFINITY, l = 0.0f;
-    if (p.use_rope) {
-        norm_rope_head<D>(x, p.rope.q_norm, p.rope, pos, s_q[warp], lane);
-#pragma unroll
-        for (int i = 0; i < N; i++) qv[i] = s_q[warp][lane * N + i];
-    } else {
-        load_vals<N>(x + lane * N, qv);
-    }
-#pragma unroll
-    for (int i = 0; i < N; i++) o[i] = 0.0f;
-    const int first = p.window ? max(0, pos - p.window + 1) : 0;
-    for (int blk = first / kKvBlock; blk <= pos / kKvBlock; blk++) {
-        const int64_t at = block_index(c, slot, blk, kvh);
-        if (at < 0) {
-            if (lane == 0) kv_error(p.err);
-            continue;
+    int slot, tile0, tiles, chunks;
+};
+
+__device__ __forceinline__ int64_t seq_work(const AttnParams &p, int s, int g, int chunk_rows, SeqWork &w, bool &bad)
+{
+    bad = !seq_info(p.b, s, w.q) || !seq_in_cache(p.c, p.b, s, w.q, w.slot);
+    if (bad || w.q.n == 0) return 0;
+    w.tile0 = p.window ? max(0, w.q.past - p.window + 1) / kTile : 0;
+    w.tiles = (w.q.past + w.q.n - 1) / kTile + 1 - w.tile0;
+    w.chunks = (w.q.n * g + chunk_rows - 1) / chunk_rows;
+    return (int64_t)w.tiles * w.chunks * p.c.heads;
+}
+
+// A part of a CTA's run: tiles t0 .. t1 - 1 of one (sequence, chunk, key head).
+struct Segment {
+    SeqWork w;
+    int chunk, head, t0, t1;
+    int rows, row_first;       // rows of the chunk, its first flat row
+    int pos_first, pos_last;   // positions of its first and last row
+    int64_t unit;              // index of the segment's tile 0 in the batch's list
+};
+
+template <int D, typename T, bool SPLIT>
+struct Shape {
+    static constexpr int kRows = SPLIT ? 8 : 16;                 // rows of a row tile
+    static constexpr int kBlk = kKvBlock * D;                    // bytes of a block
+    static constexpr int kVBlk = kBlk + 32;                      // value blocks in shared memory: off the banks of each other
+    static constexpr int kQStride = D + 4;
+    static constexpr int kQBytes = kWarps * kRows * kQStride * 4;   // queries, then the warps' sums
+    static constexpr int kKBytes = kWarps * 4 * kBlk, kVBytes = kWarps * 4 * kVBlk;
+    static constexpr int kSmem = kKBytes + kVBytes + kQBytes;
+};
+
+template <int D, typename T, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid_constant__ AttnParams p, int group,
+                                                                    int *counters, float *partials)
+{
+    using Sh = Shape<D, T, SPLIT>;
+    constexpr int RR = Sh::kRows, NT = D / 8, KS = D / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ __align__(8) uint64_t s_full[2][kWarps], s_empty[2][kWarps];   // keys, values
+    __shared__ float s_m[kWarps][RR], s_l[kWarps][RR];
+    __shared__ int64_t s_scan[kWarps + 1];
+    __shared__ int s_b, s_last;
+    __shared__ int64_t s_base;
+    __shared__ int s_abort;
+    float *s_q = reinterpret_cast<float *>(smem + Sh::kKBytes + Sh::kVBytes);
+    const uint32_t kbase = smem_addr(smem), vbase = kbase + Sh::kKBytes;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, ln = lane / 4, lj = lane % 4;
+    const int streams = kWarps / group, stream = warp / group, rt = warp % group, depth = group;
+    const int g = p.rows.q_heads / p.c.heads, chunk_rows = group * RR, G = gridDim.x;
+    const bool leader = rt == 0;
+
+    if (tid == 0) {
+        for (int i = 0; i < kWarps; i++) {
+            mbar_init(&s_full[0][i], 1);
+            mbar_init(&s_full[1][i], 1);
+            mbar_init(&s_empty[0][i], group);
+            mbar_init(&s_empty[1][i], group);
         }
-        const float ks = __ldg(c.k_scale + at) * p.scale, vs = __ldg(c.v_scale + at);
-        const int8_t *kb = c.k + at * kKvBlock * D, *vb = c.v + at * kKvBlock * D;
-        for (int t = max(0, first - blk * kKvBlock); t <= min(kKvBlock - 1, pos - blk * kKvBlock); t++) {
-            float dot = 0.0f;
+        s_abort = 0;
+        s_b = -1;
+        fence_barrier_init();
+    }
+    pdl_wait();
+    fence_proxy_async_global();   // the cache as an append before this left it, to the bulk copies
+
+    // ---- this CTA's run of the batch's tiles
+    int64_t total = 0;
+    for (int s0 = 0; s0 < p.b.B; s0 += kThreads) {
+        SeqWork w;
+        bool bad = false;
+        int64_t n = s0 + tid < p.b.B ? seq_work(p, s0 + tid, g, chunk_rows, w, bad) : 0;
+        if (bad && blockIdx.x == 0) kv_error(p.err);
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int d = lane * N + i;
-                dot = fmaf(qv[i], (float)kb[d / 64 * 1024 + t * 64 + d % 64], dot);
+        for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+        if (lane == 0) s_scan[warp] = n;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kWarps; i++) total += s_scan[i];
+        __syncthreads();
+    }
+    if (total == 0) return;
+    const int ctas = (int)min((int64_t)G, (total + kMinTiles - 1) / kMinTiles), me = blockIdx.x;
+    if (me >= ctas) return;
+    const int64_t run0 = total * me / ctas, run1 = total * (me + 1) / ctas;
+    {
+        int64_t base = 0;
+        for (int s0 = 0; s0 < p.b.B; s0 += kThreads) {
+            SeqWork w;
+            bool bad;
+            const int64_t n = s0 + tid < p.b.B ? seq_work(p, s0 + tid, g, chunk_rows, w, bad) : 0;
+            int64_t incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            if (lane == 31) s_scan[warp] = incl;
+            __syncthreads();
+            int64_t before = base, sum = base;
+#pragma unroll
+            for (int i = 0; i < kWarps; i++) {
+                if (i == warp) before = sum;
+                sum += s_scan[i];
+            }
+            const int64_t first = before + incl - n;
+            if (n && first <= run0 && run0 < first + n) {
+                s_b = s0 + tid;
+                s_base = first;
+            }
+            __syncthreads();
+            if (s_b >= 0) break;
+            base = sum;
+        }
+    }
+
+    if (s_b < 0) return;
+    int b = s_b;
+    int64_t base = s_base, at = run0;
+    // The next segment of the run; false at its end.
+    auto next_segment = [&](Segment &sg) -> bool {
+        if (at >= run1) return false;
+        bool bad;
+        int64_t n = seq_work(p, b, g, chunk_rows, sg.w, bad);
+        while (at >= base + n) {
+            base += n;
+            if (b + 1 >= p.b.B) return false;
+            n = seq_work(p, ++b, g, chunk_rows, sg.w, bad);
+        }
+        const int64_t off = at - base;
+        const int idx = (int)(off / sg.w.tiles);
+        sg.t0 = (int)(off - (int64_t)idx * sg.w.tiles);
+        sg.t1 = (int)min((int64_t)sg.w.tiles, sg.t0 + (run1 - at));
+        sg.unit = at - sg.t0;
+        sg.chunk = idx / p.c.heads;
+        sg.head = idx - sg.chunk * p.c.heads;
+        sg.row_first = sg.chunk * chunk_rows;
+        sg.rows = min(chunk_rows, sg.w.q.n * g - sg.row_first);
+        sg.pos_first = sg.w.q.past + sg.row_first / g;
+        sg.pos_last = sg.w.q.past + (sg.row_first + sg.rows - 1) / g;
+        at += sg.t1 - sg.t0;
+        return true;
+    };
+    // Block of tile t that this lane (mod 4) looks after; -1: none of its tokens is seen, or a bad page.
+    auto lookup = [&](const Segment &sg, int t) -> int64_t {
+        if (t >= sg.t1) return -1;
+        const int blk = (sg.w.tile0 + t) * (kTile / kKvBlock) + lj, first = blk * kKvBlock;
+        if (first > sg.pos_last || (p.window && first + kKvBlock - 1 <= sg.pos_first - p.window)) return -1;
+        const int64_t i = block_index(p.c, sg.w.slot, blk, sg.head);
+        if (i < 0) kv_error(p.err);
+        return i;
+    };
+    // The leader warp loads tile t's keys or values into the stream's slot.
+    uint32_t issued[2] = {0, 0};
+    auto issue = [&](int which, int64_t blk) {
+        const uint32_t n = issued[which]++;
+        const int slot = stream * depth + (int)(n % depth);
+        uint64_t *full = &s_full[which][slot];
+        const unsigned have = __ballot_sync(0xffffffffu, blk >= 0) & 0xFu;
+        // the slot's last tile has been read by every warp of the group
+        if (n >= (uint32_t)depth) tc_spin_wait(&s_empty[which][slot], (n / depth - 1) & 1, &s_abort, p.err);
+        if (lane == 0) mbar_arrive_expect_tx(full, __popc(have) * Sh::kBlk);
+        __syncwarp();
+        if (lane < 4 && blk >= 0) {
+            const uint32_t dst = which ? vbase + (slot * 4 + lj) * Sh::kVBlk : kbase + (slot * 4 + lj) * Sh::kBlk;
+            bulk_load(dst, (which ? p.c.v : p.c.k) + blk * Sh::kBlk, Sh::kBlk, full);
+        }
+    };
+    auto issue_first = [&](const Segment &sg) {
+        if (!leader) return;
+        for (int i = 0; i < depth; i++) {
+            const int t = sg.t0 + stream + i * streams;
+            if (t >= sg.t1) break;
+            const int64_t blk = lookup(sg, t);
+            issue(0, blk);
+            issue(1, blk);
+        }
+    };
+
+    Segment sg;
+    if (!next_segment(sg)) return;
+    __syncthreads();
+    issue_first(sg);
+    uint32_t done = 0;   // tiles this stream has taken
+    const float log2e = 1.4426950408889634f;
+
+    for (;;) {
+        // ---- queries of the chunk to shared memory, in f32
+        for (int r = warp; r < sg.rows; r += kWarps) {
+            const int flat = sg.row_first + r, tok = flat / g;
+            const T *x = static_cast<const T *>(p.rows.q) + (int64_t)(sg.w.q.row0 + tok) * p.rows.q_stride +
+                         (sg.head * g + flat % g) * D;
+            float *y = s_q + r * Sh::kQStride;
+            if (p.use_rope) {
+                norm_rope_head<D>(x, p.rope.q_norm, p.rope, sg.w.q.past + tok, y, lane);
+            } else {
+                constexpr int N = D / 32;
+                float v[N];
+                load_vals<N>(x + lane * N, v);
+#pragma unroll
+                for (int i = 0; i < N; i++) y[lane * N + i] = v[i];
+            }
+        }
+        __syncthreads();
+
+        // ---- this warp's row tile as A fragments. Lane (ln, lj) holds the
+        // values 16 lj .. 16 lj + 15 of every 64 of its row, in the order in
+        // which a key's 16 bytes come out of one load.
+        uint32_t qa[KS][4];
+        float rf[SPLIT ? 1 : 2];        // per row: logit factor
+        int pos[SPLIT ? 1 : 2];
+        const int row_base = rt * RR;
+#pragma unroll
+        for (int u = 0; u < (SPLIT ? 1 : 2); u++) {
+            const int r = row_base + ln + 8 * u;
+            const bool live = r < sg.rows;
+            pos[u] = live ? sg.w.q.past + (sg.row_first + r) / g : -1;
+            const float *y = s_q + (live ? r : 0) * Sh::kQStride;
+            float amax = 0.0f;
+#pragma unroll
+            for (int h = 0; h < D / 64; h++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 v = *reinterpret_cast<const float4 *>(y + h * 64 + lj * 16 + i);
+                    amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                }
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            // largest value to [2^14, 2^15): f16 then holds values 2^-28 of it in full
+            const int e = max(-112, (__float_as_int(amax) >> 23) - 127);
+            const float up = __int_as_float((14 - e + 127) << 23);
+            rf[u] = __int_as_float((e - 14 + 127) << 23) * p.scale * log2e;
+#pragma unroll
+            for (int h = 0; h < D / 64; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float4 v = *reinterpret_cast<const float4 *>(y + h * 64 + lj * 16 + 4 * i);
+                    if (!live) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    uint32_t (&a)[4] = qa[h * 4 + i];
+                    if constexpr (SPLIT) {
+                        split_f16(v.x * up, v.y * up, a[0], a[1]);
+                        split_f16(v.z * up, v.w * up, a[2], a[3]);
+                    } else {
+                        a[u] = pack_f16(v.x * up, v.y * up);
+                        a[2 + u] = pack_f16(v.z * up, v.w * up);
+                    }
+                }
+        }
+        const int tile_pos0 = sg.w.q.past + (sg.row_first + min(row_base, sg.rows - 1)) / g;   // first row's position
+        const int tile_pos1 = sg.w.q.past + (sg.row_first + min(row_base + RR, sg.rows) - 1) / g;
+
+        float m[SPLIT ? 1 : 2], l[SPLIT ? 1 : 2], o[NT][4];
+#pragma unroll
+        for (int u = 0; u < (SPLIT ? 1 : 2); u++) {
+            m[u] = -INFINITY;
+            l[u] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+
+        // ---- the stream's tiles
+        for (int t = sg.t0 + stream; t < sg.t1; t += streams, done++) {
+            const int slot = stream * depth + (int)(done % depth);
+            const uint32_t ph = (done / depth) & 1;
+            const int64_t blk = lookup(sg, t);
+            const int64_t ahead = leader ? lookup(sg, t + depth * streams) : -1;
+            float sk = 0.0f, sv = 0.0f;
+            if (blk >= 0) {
+                sk = __ldg(p.c.k_scale + blk);
+                sv = __ldg(p.c.v_scale + blk);
+            }
+            float s[8][4];
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+            tc_spin_wait(&s_full[0][slot], ph, &s_abort, p.err);
+            // column c of the 8-token group i: token 16 (c / 2) + 2 i + (c & 1) of the
+            // tile, so that this lane's columns all lie in block lj
+            const uint32_t ka = kbase + (slot * 4 + ln / 2) * Sh::kBlk + (ln & 1) * 64 + lj * 16;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int h = 0; h < D / 64; h++) {
+                    const uint4 w = lds128(ka + h * 1024 + i * 128);
+                    uint32_t b0, b1;
+                    bytes_f16(w.x, b0, b1);
+                    mma16816(s[i], qa[h * 4], b0, b1);
+                    bytes_f16(w.y, b0, b1);
+                    mma16816(s[i], qa[h * 4 + 1], b0, b1);
+                    bytes_f16(w.z, b0, b1);
+                    mma16816(s[i], qa[h * 4 + 2], b0, b1);
+                    bytes_f16(w.w, b0, b1);
+                    mma16816(s[i], qa[h * 4 + 3], b0, b1);
+                }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_empty[0][slot]);
+            if (leader && t + depth * streams < sg.t1) issue(0, ahead);
+
+            // ---- weights
+            const float lsv = sv > 0.0f ? log2f(sv) : kNoScaleLog2, isv = sv > 0.0f ? 1.0f / sv : ex2(-kNoScaleLog2);
+            const int tok0 = (sg.w.tile0 + t) * kTile;
+            const bool clear = tok0 + kTile - 1 <= tile_pos0 && (!p.window || tok0 > tile_pos1 - p.window);
+            const bool whole = __all_sync(0xffffffffu, clear && blk >= 0);
+#pragma unroll
+            for (int u = 0; u < (SPLIT ? 1 : 2); u++) {
+                const float f = rf[u] * sk;
+                float mx = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        float v = SPLIT ? s[i][x] + s[i][2 + x] : s[i][2 * u + x];
+                        v = fmaf(v, f, lsv);
+                        if (!whole) {
+                            const int j = tok0 + lj * 16 + 2 * i + x;
+                            if (blk < 0 || j > pos[u] || (p.window && j <= pos[u] - p.window)) v = -INFINITY;
+                        }
+                        s[i][2 * u + x] = v;
+                        mx = fmaxf(mx, v);
+                    }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const float mn = fmaxf(m[u], mx), ms = mn == -INFINITY ? 0.0f : mn;
+                const float alpha = m[u] == mn ? 1.0f : ex2(m[u] - ms);
+                m[u] = mn;
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const float w = ex2(s[i][2 * u + x] - ms);
+                        s[i][2 * u + x] = w;
+                        sum += w;
+                    }
+                l[u] = fmaf(l[u], alpha, sum * isv);
+                if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        o[i][2 * u] *= alpha;
+                        o[i][2 * u + 1] *= alpha;
+                        if (SPLIT) {
+                            o[i][2] *= alpha;
+                            o[i][3] *= alpha;
+                        }
+                    }
+                }
+            }
+            // A fragments of the weights: k step q takes tokens 4 q .. 4 q + 3 of each lane's block
+            uint32_t pa[4][4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if constexpr (SPLIT) {
+                    split_f16(s[2 * q][0], s[2 * q][1], pa[q][0], pa[q][1]);
+                    split_f16(s[2 * q + 1][0], s[2 * q + 1][1], pa[q][2], pa[q][3]);
+                } else {
+                    pa[q][0] = pack_f16(s[2 * q][0], s[2 * q][1]);
+                    pa[q][1] = pack_f16(s[2 * q][2], s[2 * q][3]);
+                    pa[q][2] = pack_f16(s[2 * q + 1][0], s[2 * q + 1][1]);
+                    pa[q][3] = pack_f16(s[2 * q + 1][2], s[2 * q + 1][3]);
+                }
+            }
+            tc_spin_wait(&s_full[1][slot], ph, &s_abort, p.err);
+            const uint32_t va = vbase + (slot * 4 + lj) * Sh::kVBlk + ln * 16;
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                const uint4 w = lds128(va + i * 128);
+                uint32_t b0, b1;
+                bytes_f16(w.x, b0, b1);
+                mma16816(o[i], pa[0], b0, b1);
+                bytes_f16(w.y, b0, b1);
+                mma16816(o[i], pa[1], b0, b1);
+                bytes_f16(w.z, b0, b1);
+                mma16816(o[i], pa[2], b0, b1);
+                bytes_f16(w.w, b0, b1);
+                mma16816(o[i], pa[3], b0, b1);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_empty[1][slot]);
+            if (leader && t + depth * streams < sg.t1) issue(1, ahead);
+        }
+
+        // ---- the next segment's first tiles are on their way while this one is joined
+        const Segment cur = sg;
+        const bool more = next_segment(sg);
+        if (more) issue_first(sg);
+
+        const int taken = cur.t1 - cur.t0, used = min(streams, taken);
+        float *part = s_q + warp * RR * D;      // the queries are in registers by now
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < (SPLIT ? 1 : 2); u++) {
+            l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+            l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+            if (lj == 0) {
+                s_m[warp][ln + 8 * u] = m[u];
+                s_l[warp][ln + 8 * u] = l[u];
             }
 #pragma unroll
-            for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-            dot *= ks;
-            const float mn = fmaxf(m, dot), a = __expf(m - mn), w = __expf(dot - mn);
-            m = mn;
-            l = l * a + w;
-#pragma unroll
-            for (int i = 0; i < N; i++) o[i] = o[i] * a + w * vs * (float)vb[(lane * N + i) * kKvBlock + t];
+            for (int i = 0; i < NT; i++) {
+                const float a = SPLIT ? o[i][0] + o[i][2] : o[i][2 * u], c = SPLIT ? o[i][1] + o[i][3] : o[i][2 * u + 1];
+                *reinterpret_cast<float2 *>(part + (ln + 8 * u) * D + i * 8 + lj * 2) = make_float2(a, c);
+            }
         }
+        __syncthreads();
+        const bool whole_seq = taken == cur.w.tiles;
+        const int64_t last_unit = cur.unit + cur.w.tiles - 1;
+        const int c0 = (int)(((cur.unit + 1) * ctas - 1) / total), c1 = (int)(((last_unit + 1) * ctas - 1) / total);
+        float *mine = partials + (size_t)(me * 2 + (me == c0 ? 1 : 0)) * (kPartialBytes / 4);
+        auto write_out = [&](int r, int d, const float4 &acc, float den) {
+            const int flat = cur.row_first + r;
+            const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+            const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+            store_vals<4>(static_cast<T *>(p.out) + (int64_t)(cur.w.q.row0 + flat / g) * p.out_stride +
+                              (cur.head * g + flat % g) * D + d,
+                          v);
+        };
+        constexpr int Q4 = D / 4;
+        for (int e = tid; e < cur.rows * Q4; e += kThreads) {
+            const int r = e / Q4, d = e % Q4 * 4, w0 = r / RR, rr = r % RR;
+            float M = -INFINITY;
+            for (int i = 0; i < used; i++) M = fmaxf(M, s_m[i * group + w0][rr]);
+            const float Ms = M == -INFINITY ? 0.0f : M;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float den = 0.0f;
+            for (int i = 0; i < used; i++) {
+                const int w = i * group + w0;
+                const float a = ex2(s_m[w][rr] - Ms);
+                const float4 v = *reinterpret_cast<const float4 *>(s_q + (w * RR + rr) * D + d);
+                den = fmaf(s_l[w][rr], a, den);
+                acc.x = fmaf(v.x, a, acc.x);
+                acc.y = fmaf(v.y, a, acc.y);
+                acc.z = fmaf(v.z, a, acc.z);
+                acc.w = fmaf(v.w, a, acc.w);
+            }
+            if (whole_seq) {
+                write_out(r, d, acc, den);
+            } else {
+                *reinterpret_cast<float4 *>(mine + 2 * kMaxRows + r * D + d) = acc;
+                if (d == 0) *reinterpret_cast<float2 *>(mine + 2 * r) = make_float2(M, den);
+            }
+        }
+        if (!whole_seq) {
+            // the CTA that brings the last part joins them all, in their order
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const int n = atomicAdd(counters + c0, 1);
+                s_last = n == c1 - c0;
+                if (s_last) counters[c0] = 0;
+                __threadfence();
+            }
+            __syncthreads();
+            if (s_last) {
+                for (int e = tid; e < cur.rows * Q4; e += kThreads) {
+                    const int r = e / Q4, d = e % Q4 * 4;
+                    float M = -INFINITY;
+                    for (int c = c0; c <= c1; c++)
+                        M = fmaxf(M, __ldcg(partials + (size_t)(c * 2 + (c == c0)) * (kPartialBytes / 4) + 2 * r));
+                    const float Ms = M == -INFINITY ? 0.0f : M;
+                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    float den = 0.0f;
+#pragma unroll 4
+                    for (int c = c0; c <= c1; c++) {
+                        const float *src = partials + (size_t)(c * 2 + (c == c0)) * (kPartialBytes / 4);
+                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(src + 2 * r));
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(src + 2 * kMaxRows + r * D + d));
+                        const float a = ex2(ml.x - Ms);
+                        den = fmaf(ml.y, a, den);
+                        acc.x = fmaf(v.x, a, acc.x);
+                        acc.y = fmaf(v.y, a, acc.y);
+                        acc.z = fmaf(v.z, a, acc.z);
+                        acc.w = fmaf(v.w, a, acc.w);
+                    }
+                    write_out(r, d, acc, den);
+                }
+            }
+        }
+        if (!more) break;
+        __syncthreads();   // the sums are read before the next queries go there
     }
-#pragma unroll
-    for (int i = 0; i < N; i++) o[i] = l > 0.0f ? o[i] / l : 0.0f;
-    store_vals<N>(static_cast<T *>(p.out) + row * p.out_stride + head * D + lane * N, o);
+    // after a wait that ran out, copies may still be in flight
+    if (*(volatile int *)&s_abort && leader)
+        for (int which = 0; which < 2; which++)
+            for (uint32_t n = issued[which] > (uint32_t)depth ? issued[which] - depth : 0; n < issued[which]; n++)
+                drain_wait(&s_full[which][stream * depth + n % depth], (n / depth) & 1);
+}
+
+template <int D, typename T>
+cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
+{
+    constexpr bool kSplit = sizeof(T) == 4;
+    using Sh = Shape<D, T, kSplit>;
+    auto kern = attend_stream_kernel<D, T, kSplit>;
+    static bool set[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !set[dev]) {
+        if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem)) != cudaSuccess) return e;
+        if (dev < 64) set[dev] = true;
+    }
+    // warps that share a tile: one for each row tile, up to all eight
+    const int64_t rows = (int64_t)p.b.max_new * (p.rows.q_heads / p.c.heads);
+    int group = 1;
+    while (group < kWarps && (int64_t)group * Sh::kRows < rows) group *= 2;
+    uint8_t *ws = static_cast<uint8_t *>(p.ws);
+    return launch_dependent(kern, dim3(p.num_sms), dim3(kThreads), Sh::kSmem, st, p, group,
+                            reinterpret_cast<int *>(ws + kCounterOff), reinterpret_cast<float *>(ws + partial_off(p.num_sms)));
 }
 
 template <typename T>
 cudaError_t launch_t(const AttnParams &p, cudaStream_t st)
 {
-    const int64_t items = (int64_t)p.b.T * p.rows.q_heads;
-    const unsigned grid = (unsigned)((items + kSimpleWarps - 1) / kSimpleWarps);
-    if (p.c.D == 64) attention_simple_kernel<64, T><<<grid, kSimpleWarps * 32, 0, st>>>(p);
-    else attention_simple_kernel<128, T><<<grid, kSimpleWarps * 32, 0, st>>>(p);
-    return cudaGetLastError();
+    return p.c.D == 64 ? launch_stream<64, T>(p, st) : launch_stream<128, T>(p, st);
 }
 
 }  // namespace
 
-size_t attn_workspace_bytes(int) { return 256; }
+size_t attn_workspace_bytes(int num_sms) { return partial_off(num_sms) + (size_t)num_sms * 2 * kPartialBytes; }
 
 cudaError_t launch_attention(const AttnParams &p, cudaStream_t st)
 {
