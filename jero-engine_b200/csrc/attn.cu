@@ -55,13 +55,24 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
                  : "memory");
 }
 
+// c += a b, and c = a b.
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                  "{%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+
+__device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+__device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // Four signed bytes to f16 pairs: byte + 128 under the exponent of 1024, minus 1152.
 __device__ __forceinline__ void bytes_f16(uint32_t w, uint32_t &lo, uint32_t &hi)
@@ -344,14 +355,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
         const int tile_pos0 = sg.w.q.past + (sg.row_first + min(row_base, sg.rows - 1)) / g;   // first row's position
         const int tile_pos1 = sg.w.q.past + (sg.row_first + min(row_base + RR, sg.rows) - 1) / g;
 
-        float m[SPLIT ? 1 : 2], l[SPLIT ? 1 : 2], o[NT][4];
+        float m[SPLIT ? 1 : 2], l[SPLIT ? 1 : 2], o[NT][SPLIT ? 2 : 4];
 #pragma unroll
         for (int u = 0; u < (SPLIT ? 1 : 2); u++) {
             m[u] = -INFINITY;
             l[u] = 0.0f;
         }
 #pragma unroll
-        for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int x = 0; x < (SPLIT ? 2 : 4); x++) o[i][x] = 0.0f;
 
         // ---- the stream's tiles
         for (int t = sg.t0 + stream; t < sg.t1; t += streams, done++) {
@@ -365,26 +378,27 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
                 sv = __ldg(p.c.v_scale + blk);
             }
             float s[8][4];
-#pragma unroll
-            for (int i = 0; i < 8; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
             tc_spin_wait(&s_full[0][slot], ph, &s_abort, p.err);
             // column c of the 8-token group i: token 16 (c / 2) + 2 i + (c & 1) of the
             // tile, so that this lane's columns all lie in block lj
             const uint32_t ka = kbase + (slot * 4 + ln / 2) * Sh::kBlk + (ln & 1) * 64 + lj * 16;
+            // (four groups at a time: their accumulators do not wait for one another)
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+            for (int i0 = 0; i0 < 8; i0 += 4)
 #pragma unroll
                 for (int h = 0; h < D / 64; h++) {
-                    const uint4 w = lds128(ka + h * 1024 + i * 128);
-                    uint32_t b0, b1;
-                    bytes_f16(w.x, b0, b1);
-                    mma16816(s[i], qa[h * 4], b0, b1);
-                    bytes_f16(w.y, b0, b1);
-                    mma16816(s[i], qa[h * 4 + 1], b0, b1);
-                    bytes_f16(w.z, b0, b1);
-                    mma16816(s[i], qa[h * 4 + 2], b0, b1);
-                    bytes_f16(w.w, b0, b1);
-                    mma16816(s[i], qa[h * 4 + 3], b0, b1);
+                    uint4 w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) w[i] = lds128(ka + h * 1024 + (i0 + i) * 128);
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            uint32_t b0, b1;
+                            bytes_f16(word(w[i], q), b0, b1);
+                            if (h == 0 && q == 0) mma16816_first(s[i0 + i], qa[0], b0, b1);
+                            else mma16816(s[i0 + i], qa[h * 4 + q], b0, b1);
+                        }
                 }
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_empty[0][slot]);
@@ -395,6 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             const int tok0 = (sg.w.tile0 + t) * kTile;
             const bool clear = tok0 + kTile - 1 <= tile_pos0 && (!p.window || tok0 > tile_pos1 - p.window);
             const bool whole = __all_sync(0xffffffffu, clear && blk >= 0);
+            float alpha[SPLIT ? 1 : 2];
 #pragma unroll
             for (int u = 0; u < (SPLIT ? 1 : 2); u++) {
                 const float f = rf[u] * sk;
@@ -415,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const float mn = fmaxf(m[u], mx), ms = mn == -INFINITY ? 0.0f : mn;
-                const float alpha = m[u] == mn ? 1.0f : ex2(m[u] - ms);
+                alpha[u] = ex2(m[u] - ms);
                 m[u] = mn;
                 float sum = 0.0f;
 #pragma unroll
@@ -426,18 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
                         s[i][2 * u + x] = w;
                         sum += w;
                     }
-                l[u] = fmaf(l[u], alpha, sum * isv);
-                if (__any_sync(0xffffffffu, alpha != 1.0f)) {
-#pragma unroll
-                    for (int i = 0; i < NT; i++) {
-                        o[i][2 * u] *= alpha;
-                        o[i][2 * u + 1] *= alpha;
-                        if (SPLIT) {
-                            o[i][2] *= alpha;
-                            o[i][3] *= alpha;
-                        }
-                    }
-                }
+                l[u] = fmaf(l[u], alpha[u], sum * isv);
             }
             // A fragments of the weights: k step q takes tokens 4 q .. 4 q + 3 of each lane's block
             uint32_t pa[4][4];
@@ -455,18 +459,34 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             }
             tc_spin_wait(&s_full[1][slot], ph, &s_abort, p.err);
             const uint32_t va = vbase + (slot * 4 + lj) * Sh::kVBlk + ln * 16;
+            // a tile's sums start at zero and join the running ones in f32, rounded to
+            // nearest: the tensor cores' additions round towards zero
 #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                const uint4 w = lds128(va + i * 128);
-                uint32_t b0, b1;
-                bytes_f16(w.x, b0, b1);
-                mma16816(o[i], pa[0], b0, b1);
-                bytes_f16(w.y, b0, b1);
-                mma16816(o[i], pa[1], b0, b1);
-                bytes_f16(w.z, b0, b1);
-                mma16816(o[i], pa[2], b0, b1);
-                bytes_f16(w.w, b0, b1);
-                mma16816(o[i], pa[3], b0, b1);
+            for (int i0 = 0; i0 < NT; i0 += 4) {
+                uint4 w[4];
+                float c[4][4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = lds128(va + (i0 + i) * 128);
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t b0, b1;
+                        bytes_f16(word(w[i], q), b0, b1);
+                        if (q == 0) mma16816_first(c[i], pa[0], b0, b1);
+                        else mma16816(c[i], pa[q], b0, b1);
+                    }
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        if constexpr (SPLIT) {
+                            o[i0 + i][x] = fmaf(o[i0 + i][x], alpha[0], c[i][x] + c[i][2 + x]);
+                        } else {
+                            o[i0 + i][x] = fmaf(o[i0 + i][x], alpha[0], c[i][x]);
+                            o[i0 + i][2 + x] = fmaf(o[i0 + i][2 + x], alpha[1], c[i][2 + x]);
+                        }
+                    }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_empty[1][slot]);
@@ -491,8 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             }
 #pragma unroll
             for (int i = 0; i < NT; i++) {
-                const float a = SPLIT ? o[i][0] + o[i][2] : o[i][2 * u], c = SPLIT ? o[i][1] + o[i][3] : o[i][2 * u + 1];
-                *reinterpret_cast<float2 *>(part + (ln + 8 * u) * D + i * 8 + lj * 2) = make_float2(a, c);
+                *reinterpret_cast<float2 *>(part + (ln + 8 * u) * D + i * 8 + lj * 2) = make_float2(o[i][2 * u], o[i][2 * u + 1]);
             }
         }
         __syncthreads();
@@ -579,12 +598,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
                 drain_wait(&s_full[which][stream * depth + n % depth], (n / depth) & 1);
 }
 
-template <int D, typename T>
+template <int D, typename T, bool SPLIT>
 cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
 {
-    constexpr bool kSplit = sizeof(T) == 4;
-    using Sh = Shape<D, T, kSplit>;
-    auto kern = attend_stream_kernel<D, T, kSplit>;
+    using Sh = Shape<D, T, SPLIT>;
+    auto kern = attend_stream_kernel<D, T, SPLIT>;
     static bool set[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -605,7 +623,12 @@ cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
 template <typename T>
 cudaError_t launch_t(const AttnParams &p, cudaStream_t st)
 {
-    return p.c.D == 64 ? launch_stream<64, T>(p, st) : launch_stream<128, T>(p, st);
+    // eight rows at a time where no sequence has more (half the registers), or for 22 bits
+    if (sizeof(T) == 4 || (int64_t)p.b.max_new * (p.rows.q_heads / p.c.heads) <= 8)
+        return p.c.D == 64 ? launch_stream<64, T, true>(p, st) : launch_stream<128, T, true>(p, st);
+    if constexpr (sizeof(T) == 2)
+        return p.c.D == 64 ? launch_stream<64, T, false>(p, st) : launch_stream<128, T, false>(p, st);
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace
