@@ -48,6 +48,20 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
+__device__ __forceinline__ float warp_max_f(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+__device__ __forceinline__ float warp_sum_f(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar)
 {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -100,6 +114,23 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32
     lo = pack_f16(a - f.x, b - f.y);
 }
 
+// Quotients of numbers that nearly always fit in 32 bits.
+__device__ __forceinline__ int64_t div64(int64_t a, int64_t b)
+{
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// The batch's `total` tiles over `ctas` runs, the first `more` of them one tile longer.
+struct Runs {
+    int64_t each, more, edge;    // edge: first tile of the shorter runs
+    __device__ Runs(int64_t total, int ctas) : each(div64(total, ctas)), more(total - each * ctas), edge(more * (each + 1)) {}
+    __device__ int64_t first(int cta) const { return cta < more ? cta * (each + 1) : edge + (cta - more) * each; }
+    __device__ int of(int64_t tile) const
+    {
+        return (int)(tile < edge ? div64(tile, each + 1) : more + div64(tile - edge, each));
+    }
+};
+
 // A sequence of the batch as work: `chunks` row chunks x key heads x `tiles`.
 struct SeqWork {
     SeqInfo q;
@@ -108,11 +139,12 @@ struct SeqWork {
 
 __device__ __forceinline__ int64_t seq_work(const AttnParams &p, int s, int g, int chunk_rows, SeqWork &w, bool &bad)
 {
-    bad = !seq_info(p.b, s, w.q) || !seq_in_cache(p.c, p.b, s, w.q, w.slot);
+    const bool listed = seq_info(p.b, s, w.q), cached = seq_in_cache(p.c, p.b, s, w.q, w.slot);
+    bad = !listed || !cached;
     if (bad || w.q.n == 0) return 0;
     w.tile0 = p.window ? max(0, w.q.past - p.window + 1) / kTile : 0;
     w.tiles = (w.q.past + w.q.n - 1) / kTile + 1 - w.tile0;
-    w.chunks = (w.q.n * g + chunk_rows - 1) / chunk_rows;
+    w.chunks = w.q.n * g <= chunk_rows ? 1 : (w.q.n * g + chunk_rows - 1) / chunk_rows;
     return (int64_t)w.tiles * w.chunks * p.c.heads;
 }
 
@@ -121,6 +153,7 @@ struct Segment {
     SeqWork w;
     int chunk, head, t0, t1;
     int rows, row_first;       // rows of the chunk, its first flat row
+    int tok, rem;              // that row's token and its query head of the group
     int pos_first, pos_last;   // positions of its first and last row
     int64_t unit;              // index of the segment's tile 0 in the batch's list
 };
@@ -138,17 +171,14 @@ struct Shape {
 
 template <int D, typename T, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid_constant__ AttnParams p, int group,
-                                                                    int *counters, float *partials)
+                                                                    uint32_t g_mul, int *counters, float *partials)
 {
     using Sh = Shape<D, T, SPLIT>;
     constexpr int RR = Sh::kRows, NT = D / 8, KS = D / 16;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t s_full[2][kWarps], s_empty[2][kWarps];   // keys, values
     __shared__ float s_m[kWarps][RR], s_l[kWarps][RR];
-    __shared__ int64_t s_scan[kWarps + 1];
-    __shared__ int s_b, s_last;
-    __shared__ int64_t s_base;
-    __shared__ int s_abort;
+    __shared__ int s_last, s_abort;
     float *s_q = reinterpret_cast<float *>(smem + Sh::kKBytes + Sh::kVBytes);
     const uint32_t kbase = smem_addr(smem), vbase = kbase + Sh::kKBytes;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, ln = lane / 4, lj = lane % 4;
@@ -164,65 +194,55 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             mbar_init(&s_empty[1][i], group);
         }
         s_abort = 0;
-        s_b = -1;
         fence_barrier_init();
     }
     pdl_wait();
     fence_proxy_async_global();   // the cache as an append before this left it, to the bulk copies
 
-    // ---- this CTA's run of the batch's tiles
-    int64_t total = 0;
-    for (int s0 = 0; s0 < p.b.B; s0 += kThreads) {
+    // (flat row of a chunk's first token on) / g, for numbers below 2^32 / g
+    auto over_g = [&](int n) -> int { return g == 1 ? n : (int)__umulhi((uint32_t)n, g_mul); };
+
+    // ---- this CTA's run of the batch's tiles; each warp finds it on its own
+    SeqWork w0;
+    bool bad0 = false;
+    const int64_t n0 = lane < p.b.B ? seq_work(p, lane, g, chunk_rows, w0, bad0) : 0;
+    int64_t total = n0;
+    bool any_bad = bad0;
+    for (int s = 32 + lane; s < p.b.B; s += 32) {
         SeqWork w;
-        bool bad = false;
-        int64_t n = s0 + tid < p.b.B ? seq_work(p, s0 + tid, g, chunk_rows, w, bad) : 0;
-        if (bad && blockIdx.x == 0) kv_error(p.err);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-        if (lane == 0) s_scan[warp] = n;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kWarps; i++) total += s_scan[i];
-        __syncthreads();
+        total += seq_work(p, s, g, chunk_rows, w, bad0);
+        any_bad |= bad0;
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (any_bad && blockIdx.x == 0) kv_error(p.err);
     if (total == 0) return;
     const int ctas = (int)min((int64_t)G, (total + kMinTiles - 1) / kMinTiles), me = blockIdx.x;
     if (me >= ctas) return;
-    const int64_t run0 = total * me / ctas, run1 = total * (me + 1) / ctas;
-    {
-        int64_t base = 0;
-        for (int s0 = 0; s0 < p.b.B; s0 += kThreads) {
-            SeqWork w;
-            bool bad;
-            const int64_t n = s0 + tid < p.b.B ? seq_work(p, s0 + tid, g, chunk_rows, w, bad) : 0;
-            int64_t incl = n;
+    const Runs runs(total, ctas);
+    const int64_t run0 = runs.first(me), run1 = runs.first(me + 1);
+    int b = -1;
+    int64_t base = 0, at = run0;
+    for (int s0 = 0; s0 < p.b.B && b < 0; s0 += 32) {
+        SeqWork w;
+        const int64_t n = s0 == 0 ? n0 : s0 + lane < p.b.B ? seq_work(p, s0 + lane, g, chunk_rows, w, bad0) : 0;
+        int64_t end = n;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += v;
-            }
-            if (lane == 31) s_scan[warp] = incl;
-            __syncthreads();
-            int64_t before = base, sum = base;
-#pragma unroll
-            for (int i = 0; i < kWarps; i++) {
-                if (i == warp) before = sum;
-                sum += s_scan[i];
-            }
-            const int64_t first = before + incl - n;
-            if (n && first <= run0 && run0 < first + n) {
-                s_b = s0 + tid;
-                s_base = first;
-            }
-            __syncthreads();
-            if (s_b >= 0) break;
-            base = sum;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end += v;
+        }
+        end += base;
+        const unsigned hit = __ballot_sync(0xffffffffu, n && end - n <= run0 && run0 < end);
+        if (hit) {
+            b = s0 + __ffs(hit) - 1;
+            base = __shfl_sync(0xffffffffu, end - n, __ffs(hit) - 1);
+        } else {
+            base = __shfl_sync(0xffffffffu, end, 31);
         }
     }
+    if (b < 0) return;
 
-    if (s_b < 0) return;
-    int b = s_b;
-    int64_t base = s_base, at = run0;
     // The next segment of the run; false at its end.
     auto next_segment = [&](Segment &sg) -> bool {
         if (at >= run1) return false;
@@ -234,16 +254,18 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             n = seq_work(p, ++b, g, chunk_rows, sg.w, bad);
         }
         const int64_t off = at - base;
-        const int idx = (int)(off / sg.w.tiles);
+        const int idx = (int)div64(off, sg.w.tiles);
         sg.t0 = (int)(off - (int64_t)idx * sg.w.tiles);
         sg.t1 = (int)min((int64_t)sg.w.tiles, sg.t0 + (run1 - at));
         sg.unit = at - sg.t0;
-        sg.chunk = idx / p.c.heads;
+        sg.chunk = idx < p.c.heads ? 0 : idx / p.c.heads;
         sg.head = idx - sg.chunk * p.c.heads;
         sg.row_first = sg.chunk * chunk_rows;
         sg.rows = min(chunk_rows, sg.w.q.n * g - sg.row_first);
-        sg.pos_first = sg.w.q.past + sg.row_first / g;
-        sg.pos_last = sg.w.q.past + (sg.row_first + sg.rows - 1) / g;
+        sg.tok = sg.chunk ? sg.row_first / g : 0;
+        sg.rem = sg.row_first - sg.tok * g;
+        sg.pos_first = sg.w.q.past + sg.tok;
+        sg.pos_last = sg.pos_first + over_g(sg.rem + sg.rows - 1);
         at += sg.t1 - sg.t0;
         return true;
     };
@@ -272,39 +294,58 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             bulk_load(dst, (which ? p.c.v : p.c.k) + blk * Sh::kBlk, Sh::kBlk, full);
         }
     };
-    auto issue_first = [&](const Segment &sg) {
-        if (!leader) return;
-        for (int i = 0; i < depth; i++) {
-            const int t = sg.t0 + stream + i * streams;
-            if (t >= sg.t1) break;
-            const int64_t blk = lookup(sg, t);
-            issue(0, blk);
-            issue(1, blk);
+    // A segment's beginning: this warp's first query row and block scales are
+    // asked for, then the stream's first tiles.
+    constexpr int N = D / 32;
+    float qv[N], sk = 0.0f, sv = 0.0f;
+    int64_t blk = -1;
+    auto row_ptr = [&](const Segment &sg, int r, int &tok) -> const T * {
+        const int t = over_g(sg.rem + r);
+        tok = sg.tok + t;
+        return static_cast<const T *>(p.rows.q) + (int64_t)(sg.w.q.row0 + tok) * p.rows.q_stride +
+               (sg.head * g + sg.rem + r - t * g) * D;
+    };
+    auto scales = [&](int64_t i, float &k, float &v) {
+        k = v = 0.0f;
+        if (i >= 0) {
+            k = __ldg(p.c.k_scale + i);
+            v = __ldg(p.c.v_scale + i);
         }
+    };
+    auto begin = [&](const Segment &sg) {
+        int tok;
+        if (warp < sg.rows) load_vals<N>(row_ptr(sg, warp, tok) + lane * N, qv);
+        blk = lookup(sg, sg.t0 + stream);
+        if (leader)
+            for (int i = 0; i < depth; i++) {
+                const int t = sg.t0 + stream + i * streams;
+                if (t >= sg.t1) break;
+                const int64_t first = i ? lookup(sg, t) : blk;
+                issue(0, first);
+                issue(1, first);
+            }
+        scales(blk, sk, sv);
     };
 
     Segment sg;
     if (!next_segment(sg)) return;
     __syncthreads();
-    issue_first(sg);
+    begin(sg);
     uint32_t done = 0;   // tiles this stream has taken
     const float log2e = 1.4426950408889634f;
 
     for (;;) {
         // ---- queries of the chunk to shared memory, in f32
         for (int r = warp; r < sg.rows; r += kWarps) {
-            const int flat = sg.row_first + r, tok = flat / g;
-            const T *x = static_cast<const T *>(p.rows.q) + (int64_t)(sg.w.q.row0 + tok) * p.rows.q_stride +
-                         (sg.head * g + flat % g) * D;
+            int tok;
+            const T *x = row_ptr(sg, r, tok);
+            if (r != warp) load_vals<N>(x + lane * N, qv);
             float *y = s_q + r * Sh::kQStride;
             if (p.use_rope) {
-                norm_rope_head<D>(x, p.rope.q_norm, p.rope, sg.w.q.past + tok, y, lane);
+                norm_rope_vals<D>(qv, p.rope.q_norm, p.rope, sg.w.q.past + tok, y, lane);
             } else {
-                constexpr int N = D / 32;
-                float v[N];
-                load_vals<N>(x + lane * N, v);
 #pragma unroll
-                for (int i = 0; i < N; i++) y[lane * N + i] = v[i];
+                for (int i = 0; i < N; i++) y[lane * N + i] = qv[i];
             }
         }
         __syncthreads();
@@ -320,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
         for (int u = 0; u < (SPLIT ? 1 : 2); u++) {
             const int r = row_base + ln + 8 * u;
             const bool live = r < sg.rows;
-            pos[u] = live ? sg.w.q.past + (sg.row_first + r) / g : -1;
+            pos[u] = live ? sg.pos_first + over_g(sg.rem + r) : -1;
             const float *y = s_q + (live ? r : 0) * Sh::kQStride;
             float amax = 0.0f;
 #pragma unroll
@@ -352,8 +393,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
                     }
                 }
         }
-        const int tile_pos0 = sg.w.q.past + (sg.row_first + min(row_base, sg.rows - 1)) / g;   // first row's position
-        const int tile_pos1 = sg.w.q.past + (sg.row_first + min(row_base + RR, sg.rows) - 1) / g;
+        const int tile_pos0 = sg.pos_first + over_g(sg.rem + min(row_base, sg.rows - 1));   // of the first row
+        const int tile_pos1 = sg.pos_first + over_g(sg.rem + min(row_base + RR, sg.rows) - 1);
 
         float m[SPLIT ? 1 : 2], l[SPLIT ? 1 : 2], o[NT][SPLIT ? 2 : 4];
 #pragma unroll
@@ -370,13 +411,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
         for (int t = sg.t0 + stream; t < sg.t1; t += streams, done++) {
             const int slot = stream * depth + (int)(done % depth);
             const uint32_t ph = (done / depth) & 1;
-            const int64_t blk = lookup(sg, t);
-            const int64_t ahead = leader ? lookup(sg, t + depth * streams) : -1;
-            float sk = 0.0f, sv = 0.0f;
-            if (blk >= 0) {
-                sk = __ldg(p.c.k_scale + blk);
-                sv = __ldg(p.c.v_scale + blk);
-            }
+            const int64_t next = lookup(sg, t + streams);
+            const int64_t ahead = depth == 1 ? next : leader ? lookup(sg, t + depth * streams) : -1;
             float s[8][4];
             tc_spin_wait(&s_full[0][slot], ph, &s_abort, p.err);
             // column c of the 8-token group i: token 16 (c / 2) + 2 i + (c & 1) of the
@@ -403,6 +439,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_empty[0][slot]);
             if (leader && t + depth * streams < sg.t1) issue(0, ahead);
+            float sk_next, sv_next;
+            scales(next, sk_next, sv_next);
 
             // ---- weights
             const float lsv = sv > 0.0f ? log2f(sv) : kNoScaleLog2, isv = sv > 0.0f ? 1.0f / sv : ex2(-kNoScaleLog2);
@@ -491,12 +529,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_empty[1][slot]);
             if (leader && t + depth * streams < sg.t1) issue(1, ahead);
+            blk = next;
+            sk = sk_next;
+            sv = sv_next;
         }
 
         // ---- the next segment's first tiles are on their way while this one is joined
         const Segment cur = sg;
         const bool more = next_segment(sg);
-        if (more) issue_first(sg);
+        if (more) begin(sg);
 
         const int taken = cur.t1 - cur.t0, used = min(streams, taken);
         float *part = s_q + warp * RR * D;      // the queries are in registers by now
@@ -517,14 +558,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
         __syncthreads();
         const bool whole_seq = taken == cur.w.tiles;
         const int64_t last_unit = cur.unit + cur.w.tiles - 1;
-        const int c0 = (int)(((cur.unit + 1) * ctas - 1) / total), c1 = (int)(((last_unit + 1) * ctas - 1) / total);
+        const int c0 = cur.t0 == 0 ? me : runs.of(cur.unit), c1 = cur.t1 == cur.w.tiles ? me : runs.of(last_unit);
         float *mine = partials + (size_t)(me * 2 + (me == c0 ? 1 : 0)) * (kPartialBytes / 4);
-        auto write_out = [&](int r, int d, const float4 &acc, float den) {
-            const int flat = cur.row_first + r;
+        auto write_out = [&](int r, int d, auto &acc, float den) {
+            constexpr int V = sizeof(acc) / 4;
+            const int t = over_g(cur.rem + r);
             const float inv = den > 0.0f ? 1.0f / den : 0.0f;
-            const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-            store_vals<4>(static_cast<T *>(p.out) + (int64_t)(cur.w.q.row0 + flat / g) * p.out_stride +
-                              (cur.head * g + flat % g) * D + d,
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) v[i] = acc[i] * inv;
+            store_vals<V>(static_cast<T *>(p.out) + (int64_t)(cur.w.q.row0 + cur.tok + t) * p.out_stride +
+                              (cur.head * g + cur.rem + r - t * g) * D + d,
                           v);
         };
         constexpr int Q4 = D / 4;
@@ -533,30 +577,30 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             float M = -INFINITY;
             for (int i = 0; i < used; i++) M = fmaxf(M, s_m[i * group + w0][rr]);
             const float Ms = M == -INFINITY ? 0.0f : M;
-            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float den = 0.0f;
+            float acc[4] = {}, den = 0.0f;
             for (int i = 0; i < used; i++) {
                 const int w = i * group + w0;
                 const float a = ex2(s_m[w][rr] - Ms);
                 const float4 v = *reinterpret_cast<const float4 *>(s_q + (w * RR + rr) * D + d);
                 den = fmaf(s_l[w][rr], a, den);
-                acc.x = fmaf(v.x, a, acc.x);
-                acc.y = fmaf(v.y, a, acc.y);
-                acc.z = fmaf(v.z, a, acc.z);
-                acc.w = fmaf(v.w, a, acc.w);
+                acc[0] = fmaf(v.x, a, acc[0]);
+                acc[1] = fmaf(v.y, a, acc[1]);
+                acc[2] = fmaf(v.z, a, acc[2]);
+                acc[3] = fmaf(v.w, a, acc[3]);
             }
             if (whole_seq) {
                 write_out(r, d, acc, den);
             } else {
-                *reinterpret_cast<float4 *>(mine + 2 * kMaxRows + r * D + d) = acc;
+                *reinterpret_cast<float4 *>(mine + 2 * kMaxRows + r * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
                 if (d == 0) *reinterpret_cast<float2 *>(mine + 2 * r) = make_float2(M, den);
             }
         }
         if (!whole_seq) {
-            // the CTA that brings the last part joins them all, in their order
-            __threadfence();
+            // the CTA that brings the last part joins them all, in their order: a
+            // warp per row, lanes over the parts for the maximum, then over the values
             __syncthreads();
             if (tid == 0) {
+                __threadfence();
                 const int n = atomicAdd(counters + c0, 1);
                 s_last = n == c1 - c0;
                 if (s_last) counters[c0] = 0;
@@ -564,27 +608,42 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             }
             __syncthreads();
             if (s_last) {
-                for (int e = tid; e < cur.rows * Q4; e += kThreads) {
-                    const int r = e / Q4, d = e % Q4 * 4;
+                auto part_of = [&](int c) { return partials + (size_t)(c * 2 + (c == c0)) * (kPartialBytes / 4); };
+                for (int r = warp; r < cur.rows; r += kWarps) {
                     float M = -INFINITY;
-                    for (int c = c0; c <= c1; c++)
-                        M = fmaxf(M, __ldcg(partials + (size_t)(c * 2 + (c == c0)) * (kPartialBytes / 4) + 2 * r));
+                    for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, __ldcg(part_of(c) + 2 * r));
+                    M = warp_max_f(M);
                     const float Ms = M == -INFINITY ? 0.0f : M;
-                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    float den = 0.0f;
-#pragma unroll 4
-                    for (int c = c0; c <= c1; c++) {
-                        const float *src = partials + (size_t)(c * 2 + (c == c0)) * (kPartialBytes / 4);
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(src + 2 * r));
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(src + 2 * kMaxRows + r * D + d));
-                        const float a = ex2(ml.x - Ms);
-                        den = fmaf(ml.y, a, den);
-                        acc.x = fmaf(v.x, a, acc.x);
-                        acc.y = fmaf(v.y, a, acc.y);
-                        acc.z = fmaf(v.z, a, acc.z);
-                        acc.w = fmaf(v.w, a, acc.w);
+                    constexpr int V = D / 32;
+                    float acc[V], den = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < V; i++) acc[i] = 0.0f;
+                    for (int cb = c0; cb <= c1; cb += 32) {
+                        float a = 0.0f;
+                        if (cb + lane <= c1) {
+                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(cb + lane) + 2 * r));
+                            a = ex2(ml.x - Ms);
+                            den = fmaf(ml.y, a, den);
+                        }
+                        const int n = min(32, c1 - cb + 1);
+#pragma unroll 8
+                        for (int i = 0; i < n; i++) {
+                            const float *src = part_of(cb + i) + 2 * kMaxRows + r * D + lane * V;
+                            float v[V];
+                            if constexpr (V == 4) {
+                                const float4 x = __ldcg(reinterpret_cast<const float4 *>(src));
+                                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+                            } else {
+                                const float2 x = __ldcg(reinterpret_cast<const float2 *>(src));
+                                v[0] = x.x; v[1] = x.y;
+                            }
+                            const float ai = __shfl_sync(0xffffffffu, a, i);
+#pragma unroll
+                            for (int k = 0; k < V; k++) acc[k] = fmaf(v[k], ai, acc[k]);
+                        }
                     }
-                    write_out(r, d, acc, den);
+                    den = warp_sum_f(den);
+                    write_out(r, lane * V, acc, den);
                 }
             }
         }
@@ -612,11 +671,12 @@ cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
         if (dev < 64) set[dev] = true;
     }
     // warps that share a tile: one for each row tile, up to all eight
-    const int64_t rows = (int64_t)p.b.max_new * (p.rows.q_heads / p.c.heads);
+    const int g = p.rows.q_heads / p.c.heads;
+    const int64_t rows = (int64_t)p.b.max_new * g;
     int group = 1;
     while (group < kWarps && (int64_t)group * Sh::kRows < rows) group *= 2;
     uint8_t *ws = static_cast<uint8_t *>(p.ws);
-    return launch_dependent(kern, dim3(p.num_sms), dim3(kThreads), Sh::kSmem, st, p, group,
+    return launch_dependent(kern, dim3(p.num_sms), dim3(kThreads), Sh::kSmem, st, p, group, g > 1 ? (uint32_t)((1ull << 32) / g + 1) : 0u,
                             reinterpret_cast<int *>(ws + kCounterOff), reinterpret_cast<float *>(ws + partial_off(p.num_sms)));
 }
 

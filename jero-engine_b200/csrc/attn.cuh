@@ -110,14 +110,13 @@ __device__ __forceinline__ int2 rope_pair(const RopeDev &r, int i)
     return r.interleaved ? make_int2(2 * i, 2 * i + 1) : make_int2(i, i + r.R / 2);
 }
 
-// One warp: head row x[D] normed (w != nullptr) and rotated at position pos
-// into y[D] (shared memory), all in f32 but the angles.
-template <int D, typename T>
-__device__ __forceinline__ void norm_rope_head(const T *x, const float *w, const RopeDev &r, int pos, float *y, int lane)
+// One warp: a head row of D values, D / 32 consecutive ones in each lane's v,
+// normed (w != nullptr) and rotated at position pos into y[D] (shared memory),
+// all in f32 but the angles.
+template <int D>
+__device__ __forceinline__ void norm_rope_vals(float (&v)[D / 32], const float *w, const RopeDev &r, int pos, float *y, int lane)
 {
     constexpr int N = D / 32;
-    float v[N];
-    load_vals<N>(x + lane * N, v);
     if (w) {
         float ss = 0.0f;
 #pragma unroll
@@ -143,6 +142,14 @@ __device__ __forceinline__ void norm_rope_head(const T *x, const float *w, const
         y[ab.y] = b * c + a * s;
     }
     __syncwarp();
+}
+
+template <int D, typename T>
+__device__ __forceinline__ void norm_rope_head(const T *x, const float *w, const RopeDev &r, int pos, float *y, int lane)
+{
+    float v[D / 32];
+    load_vals<D / 32>(x + lane * (D / 32), v);
+    norm_rope_vals<D>(v, w, r, pos, y, lane);
 }
 
 }  // namespace jmoe
