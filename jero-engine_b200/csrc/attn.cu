@@ -19,6 +19,8 @@
 // The value scale sv of a block enters as a term of the exponent: the weights
 // w = exp2(s + log2 sv - m) stay in (0, 1] whatever the scales, and p = w / sv
 // is summed for the denominator.
+#include <algorithm>
+
 #include "attn.cuh"
 #include "kernels.h"
 #include "tc_common.cuh"
@@ -26,15 +28,21 @@
 namespace jmoe {
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kCtasPerSm = 2;                // one joins its parts while the other streams
 constexpr int kTile = 64;                    // tokens of a tile: 4 blocks
-constexpr int kMaxRows = 128;                // rows of a chunk (8 warps x 16)
+constexpr int kMaxRows = kWarps * 16;        // rows of a chunk
 // A run has at least this many tiles: fewer CTAs share a short sequence.
 constexpr int kMinTiles = 2;
+// What beginning and joining one more segment costs a CTA, in tiles.
+constexpr int kSegmentTiles = 8;
 
-// Workspace: status word | arrival counters [ctas] | partials [ctas][2].
+// A segment's parts are joined in groups of this many CTAs, then the groups.
+constexpr int kJoin = 16;
+
+// Workspace: status word | arrival counters [2][ctas][2] | partials [ctas][2].
 constexpr size_t kCounterOff = 256;
-size_t partial_off(int ctas) { return kCounterOff + ((size_t)ctas * 4 + 255) / 256 * 256; }
+size_t partial_off(int ctas) { return kCounterOff + ((size_t)ctas * 16 + 255) / 256 * 256; }
 constexpr size_t kPartialBytes = (size_t)kMaxRows * (kMaxHeadDim + 2) * 4;
 
 // Values of a sequence without a scale (an all-zero block): far below any real
@@ -46,6 +54,22 @@ __device__ __forceinline__ float ex2(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ float lg2(float x)
+{
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Adds with acquire and release at GPU scope: what the CTA wrote before its
+// last barrier is seen by whoever counts after it.
+__device__ __forceinline__ int atom_add_acq_rel(int *p, int v)
+{
+    int old;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+    return old;
 }
 
 __device__ __forceinline__ float warp_max_f(float v)
@@ -114,77 +138,89 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32
     lo = pack_f16(a - f.x, b - f.y);
 }
 
-// Quotients of numbers that nearly always fit in 32 bits.
-__device__ __forceinline__ int64_t div64(int64_t a, int64_t b)
+// x / d for 0 <= x < 2^24, inv about 1 / d.
+__device__ __forceinline__ int quot(int x, int d, float inv)
 {
-    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+    int q = (int)((float)x * inv);
+    q -= q * d > x;
+    return q + ((q + 1) * d <= x);
 }
 
-// The batch's `total` tiles over `ctas` runs, the first `more` of them one tile longer.
+// `total` tiles over `ctas` runs, the first `more` of them one tile longer.
 struct Runs {
-    int64_t each, more, edge;    // edge: first tile of the shorter runs
-    __device__ Runs(int64_t total, int ctas) : each(div64(total, ctas)), more(total - each * ctas), edge(more * (each + 1)) {}
-    __device__ int64_t first(int cta) const { return cta < more ? cta * (each + 1) : edge + (cta - more) * each; }
-    __device__ int of(int64_t tile) const
+    int each, more, edge;    // edge: first tile of the shorter runs
+    __device__ void set(int total, int ctas)
     {
-        return (int)(tile < edge ? div64(tile, each + 1) : more + div64(tile - edge, each));
+        each = total / ctas;
+        more = total - each * ctas;
+        edge = more * (each + 1);
     }
+    __device__ int first(int cta) const { return cta < more ? cta * (each + 1) : edge + (cta - more) * each; }
+    __device__ int of(int tile) const { return tile < edge ? tile / (each + 1) : more + (tile - edge) / each; }
 };
 
-// A sequence of the batch as work: `chunks` row chunks x key heads x `tiles`.
+// A sequence of the batch as work: `segs` segments (row chunk x key head) of
+// `tiles` tiles each.
 struct SeqWork {
     SeqInfo q;
-    int slot, tile0, tiles, chunks;
+    int slot, tile0, tiles, segs;
 };
 
-__device__ __forceinline__ int64_t seq_work(const AttnParams &p, int s, int g, int chunk_rows, SeqWork &w, bool &bad)
+__device__ __forceinline__ void seq_work(const AttnParams &p, int s, int g, int chunk_rows, SeqWork &w, bool &bad)
 {
     const bool listed = seq_info(p.b, s, w.q), cached = seq_in_cache(p.c, p.b, s, w.q, w.slot);
     bad = !listed || !cached;
-    if (bad || w.q.n == 0) return 0;
+    w.tile0 = w.tiles = w.segs = 0;
+    if (bad || w.q.n == 0) return;
     w.tile0 = p.window ? max(0, w.q.past - p.window + 1) / kTile : 0;
     w.tiles = (w.q.past + w.q.n - 1) / kTile + 1 - w.tile0;
-    w.chunks = w.q.n * g <= chunk_rows ? 1 : (w.q.n * g + chunk_rows - 1) / chunk_rows;
-    return (int64_t)w.tiles * w.chunks * p.c.heads;
+    w.segs = p.c.heads;
+    if (w.q.n * g > chunk_rows) w.segs *= (w.q.n * g + chunk_rows - 1) / chunk_rows;
 }
 
-// A part of a CTA's run: tiles t0 .. t1 - 1 of one (sequence, chunk, key head).
+// A part of a CTA's run: tiles t0 .. t1 - 1 of one segment.
 struct Segment {
-    SeqWork w;
-    int chunk, head, t0, t1;
-    int rows, row_first;       // rows of the chunk, its first flat row
-    int tok, rem;              // that row's token and its query head of the group
+    SeqInfo q;
+    int slot, tile0, tiles, head, t0, t1;
+    int tok, rem;              // token and query head of the group of the chunk's first row
+    int rows;                  // rows of the chunk
     int pos_first, pos_last;   // positions of its first and last row
-    int64_t unit;              // index of the segment's tile 0 in the batch's list
+    int cta0, cta1;            // CTAs that share the segment
 };
 
-template <int D, typename T, bool SPLIT>
+template <int D, bool SPLIT>
 struct Shape {
     static constexpr int kRows = SPLIT ? 8 : 16;                 // rows of a row tile
     static constexpr int kBlk = kKvBlock * D;                    // bytes of a block
     static constexpr int kVBlk = kBlk + 32;                      // value blocks in shared memory: off the banks of each other
-    static constexpr int kQStride = D + 4;
-    static constexpr int kQBytes = kWarps * kRows * kQStride * 4;   // queries, then the warps' sums
+    static constexpr int kQRow = D * 2 + 16;                     // bytes of a query row in f16
     static constexpr int kKBytes = kWarps * 4 * kBlk, kVBytes = kWarps * 4 * kVBlk;
-    static constexpr int kSmem = kKBytes + kVBytes + kQBytes;
+    static constexpr int kQBytes = kWarps * kRows * kQRow * (SPLIT ? 2 : 1);
+    static constexpr int kSumBytes = kWarps * kRows * D * 4;     // the warps' sums, where the queries were
+    static constexpr int kRowOff = kKBytes + kVBytes + (kQBytes > kSumBytes ? kQBytes : kSumBytes);
+    static constexpr int kSmem = kRowOff + kWarps * D * 4;       // a head row of each warp while it is rotated
 };
 
 template <int D, typename T, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid_constant__ AttnParams p, int group,
-                                                                    uint32_t g_mul, int *counters, float *partials)
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+    attend_stream_kernel(const __grid_constant__ AttnParams p, int seq0, int seq1, int group, uint32_t g_mul, int *counters,
+                         float *partials)
 {
-    using Sh = Shape<D, T, SPLIT>;
-    constexpr int RR = Sh::kRows, NT = D / 8, KS = D / 16;
+    using Sh = Shape<D, SPLIT>;
+    constexpr int RR = Sh::kRows, U = SPLIT ? 1 : 2, NT = D / 8, KS = D / 16, N = D / 32;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t s_full[2][kWarps], s_empty[2][kWarps];   // keys, values
-    __shared__ float s_m[kWarps][RR], s_l[kWarps][RR];
+    __shared__ float s_m[kWarps][RR], s_l[kWarps][RR], s_rf[kMaxRows];
     __shared__ int s_last, s_abort;
-    float *s_q = reinterpret_cast<float *>(smem + Sh::kKBytes + Sh::kVBytes);
+    uint8_t *s_q = smem + Sh::kKBytes + Sh::kVBytes;          // queries: f16 rows, with SPLIT the lower halves behind them
+    float *s_sum = reinterpret_cast<float *>(s_q);
     const uint32_t kbase = smem_addr(smem), vbase = kbase + Sh::kKBytes;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, ln = lane / 4, lj = lane % 4;
     const int streams = kWarps / group, stream = warp / group, rt = warp % group, depth = group;
-    const int g = p.rows.q_heads / p.c.heads, chunk_rows = group * RR, G = gridDim.x;
+    const int g = p.rows.q_heads / p.c.heads, chunk_rows = group * RR, me = blockIdx.x;
     const bool leader = rt == 0;
+    // n / g for numbers below 2^32 / g
+    auto over_g = [&](int n) -> int { return g == 1 ? n : (int)__umulhi((uint32_t)n, g_mul); };
 
     if (tid == 0) {
         for (int i = 0; i < kWarps; i++) {
@@ -197,92 +233,128 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
         fence_barrier_init();
     }
     pdl_wait();
+    pdl_trigger();
     fence_proxy_async_global();   // the cache as an append before this left it, to the bulk copies
 
-    // (flat row of a chunk's first token on) / g, for numbers below 2^32 / g
-    auto over_g = [&](int n) -> int { return g == 1 ? n : (int)__umulhi((uint32_t)n, g_mul); };
-
-    // ---- this CTA's run of the batch's tiles; each warp finds it on its own
-    SeqWork w0;
-    bool bad0 = false;
-    const int64_t n0 = lane < p.b.B ? seq_work(p, lane, g, chunk_rows, w0, bad0) : 0;
-    int64_t total = n0;
-    bool any_bad = bad0;
-    for (int s = 32 + lane; s < p.b.B; s += 32) {
-        SeqWork w;
-        total += seq_work(p, s, g, chunk_rows, w, bad0);
-        any_bad |= bad0;
+    // ---- this CTA's run of the batch's tiles; each warp finds it on its own, a
+    // sequence per lane
+    SeqWork w;
+    bool bad = false;
+    w.tiles = w.segs = 0;
+    if (seq0 + lane < seq1) seq_work(p, seq0 + lane, g, chunk_rows, w, bad);
+    const SeqWork w0 = w;
+    int total = w.tiles * w.segs, segs = w.segs;
+    for (int s = seq0 + 32 + lane; s < seq1; s += 32) {
+        bool worse;
+        seq_work(p, s, g, chunk_rows, w, worse);
+        total += w.tiles * w.segs;
+        segs += w.segs;
+        bad |= worse;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (any_bad && blockIdx.x == 0) kv_error(p.err);
+    if (bad && me == 0) kv_error(p.err);
+    total = __reduce_add_sync(0xffffffffu, total);
+    segs = __reduce_add_sync(0xffffffffu, segs);
     if (total == 0) return;
-    const int ctas = (int)min((int64_t)G, (total + kMinTiles - 1) / kMinTiles), me = blockIdx.x;
-    if (me >= ctas) return;
-    const Runs runs(total, ctas);
-    const int64_t run0 = runs.first(me), run1 = runs.first(me + 1);
-    int b = -1;
-    int64_t base = 0, at = run0;
-    for (int s0 = 0; s0 < p.b.B && b < 0; s0 += 32) {
-        SeqWork w;
-        const int64_t n = s0 == 0 ? n0 : s0 + lane < p.b.B ? seq_work(p, s0 + lane, g, chunk_rows, w, bad0) : 0;
-        int64_t end = n;
+    // Runs of `cut` tiles that end with their segment, where the CTAs suffice for
+    // that without much longer runs; else equal runs across segments.
+    const int ctas = min((int)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
+    int cut = 0;
+    if (segs < (int)gridDim.x) {
+        cut = max(kMinTiles, (int)__fdividef((float)total, (float)((int)gridDim.x - segs)) + 1);
+        if (cut > (int)__fdividef((float)total, (float)ctas) + kSegmentTiles) cut = 0;
+    }
+    const float inv_cut = cut ? __fdividef(1.0f, (float)cut) : 1.0f;
+    if (!cut && me >= ctas) return;
+    Runs runs;
+    int at = me, end = me + 1;
+    if (!cut) {
+        runs.set(total, ctas);
+        at = runs.first(me);
+        end = runs.first(me + 1);
+    }
+    int b = -1, base = 0;      // the sequence, and the list's units before it
+    for (int s0 = seq0; s0 < seq1 && b < 0; s0 += 32) {
+        w = w0;
+        if (s0 != seq0) {
+            w.tiles = w.segs = 0;
+            if (s0 + lane < seq1) seq_work(p, s0 + lane, g, chunk_rows, w, bad);
+        }
+        const int n = w.segs * (cut ? quot(w.tiles + cut - 1, cut, inv_cut) : w.tiles);
+        int last = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t v = __shfl_up_sync(0xffffffffu, end, o);
-            if (lane >= o) end += v;
+            const int v = __shfl_up_sync(0xffffffffu, last, o);
+            if (lane >= o) last += v;
         }
-        end += base;
-        const unsigned hit = __ballot_sync(0xffffffffu, n && end - n <= run0 && run0 < end);
-        if (hit) {
-            b = s0 + __ffs(hit) - 1;
-            base = __shfl_sync(0xffffffffu, end - n, __ffs(hit) - 1);
-        } else {
-            base = __shfl_sync(0xffffffffu, end, 31);
-        }
+        last += base;
+        const unsigned hit = __ballot_sync(0xffffffffu, n && last - n <= at && at < last);
+        b = hit ? s0 + __ffs(hit) - 1 : -1;
+        base = __shfl_sync(0xffffffffu, hit ? last - n : last, hit ? __ffs(hit) - 1 : 31);
     }
-    if (b < 0) return;
+    if (b < 0) return;         // fewer runs than CTAs
 
     // The next segment of the run; false at its end.
     auto next_segment = [&](Segment &sg) -> bool {
-        if (at >= run1) return false;
-        bool bad;
-        int64_t n = seq_work(p, b, g, chunk_rows, sg.w, bad);
-        while (at >= base + n) {
-            base += n;
-            if (b + 1 >= p.b.B) return false;
-            n = seq_work(p, ++b, g, chunk_rows, sg.w, bad);
+        if (at >= end) return false;
+        int per;                                   // units of a segment
+        for (;;) {
+            const int i = b - seq0;
+            if (i < 32) {
+                w.q.past = __shfl_sync(0xffffffffu, w0.q.past, i);
+                w.q.row0 = __shfl_sync(0xffffffffu, w0.q.row0, i);
+                w.q.n = __shfl_sync(0xffffffffu, w0.q.n, i);
+                w.slot = __shfl_sync(0xffffffffu, w0.slot, i);
+                w.tile0 = __shfl_sync(0xffffffffu, w0.tile0, i);
+                w.tiles = __shfl_sync(0xffffffffu, w0.tiles, i);
+                w.segs = __shfl_sync(0xffffffffu, w0.segs, i);
+            } else {
+                seq_work(p, b, g, chunk_rows, w, bad);
+            }
+            per = cut ? quot(w.tiles + cut - 1, cut, inv_cut) : w.tiles;
+            if (at < base + w.segs * per) break;
+            base += w.segs * per;
+            if (++b >= seq1) return false;
         }
-        const int64_t off = at - base;
-        const int idx = (int)div64(off, sg.w.tiles);
-        sg.t0 = (int)(off - (int64_t)idx * sg.w.tiles);
-        sg.t1 = (int)min((int64_t)sg.w.tiles, sg.t0 + (run1 - at));
-        sg.unit = at - sg.t0;
-        sg.chunk = idx < p.c.heads ? 0 : idx / p.c.heads;
-        sg.head = idx - sg.chunk * p.c.heads;
-        sg.row_first = sg.chunk * chunk_rows;
-        sg.rows = min(chunk_rows, sg.w.q.n * g - sg.row_first);
-        sg.tok = sg.chunk ? sg.row_first / g : 0;
-        sg.rem = sg.row_first - sg.tok * g;
-        sg.pos_first = sg.w.q.past + sg.tok;
+        const int idx = at - base < per ? 0 : (at - base) / per, off = at - base - idx * per;
+        sg.q = w.q;
+        sg.slot = w.slot;
+        sg.tile0 = w.tile0;
+        sg.tiles = w.tiles;
+        if (cut) {
+            sg.t0 = off * cut;
+            sg.t1 = min(w.tiles, sg.t0 + cut);
+            sg.cta0 = me - off;
+            sg.cta1 = sg.cta0 + per - 1;
+            at++;
+        } else {
+            sg.t0 = off;
+            sg.t1 = min(w.tiles, off + end - at);
+            sg.cta0 = off == 0 ? me : runs.of(at - off);
+            sg.cta1 = sg.t1 == w.tiles ? me : runs.of(at - off + w.tiles - 1);
+            at += sg.t1 - off;
+        }
+        const int chunk = idx < p.c.heads ? 0 : idx / p.c.heads;
+        sg.head = idx - chunk * p.c.heads;
+        sg.rows = min(chunk_rows, w.q.n * g - chunk * chunk_rows);
+        sg.tok = chunk ? chunk * chunk_rows / g : 0;
+        sg.rem = chunk * chunk_rows - sg.tok * g;
+        sg.pos_first = w.q.past + sg.tok;
         sg.pos_last = sg.pos_first + over_g(sg.rem + sg.rows - 1);
-        at += sg.t1 - sg.t0;
         return true;
     };
     // Block of tile t that this lane (mod 4) looks after; -1: none of its tokens is seen, or a bad page.
     auto lookup = [&](const Segment &sg, int t) -> int64_t {
         if (t >= sg.t1) return -1;
-        const int blk = (sg.w.tile0 + t) * (kTile / kKvBlock) + lj, first = blk * kKvBlock;
+        const int blk = (sg.tile0 + t) * (kTile / kKvBlock) + lj, first = blk * kKvBlock;
         if (first > sg.pos_last || (p.window && first + kKvBlock - 1 <= sg.pos_first - p.window)) return -1;
-        const int64_t i = block_index(p.c, sg.w.slot, blk, sg.head);
+        const int64_t i = block_index(p.c, sg.slot, blk, sg.head);
         if (i < 0) kv_error(p.err);
         return i;
     };
-    // The leader warp loads tile t's keys or values into the stream's slot.
-    uint32_t issued[2] = {0, 0};
-    auto issue = [&](int which, int64_t blk) {
-        const uint32_t n = issued[which]++;
-        const int slot = stream * depth + (int)(n % depth);
+    // The leader warp loads a tile's keys (0) or values (1) into the stream's next slot.
+    // n: tiles that the stream was given before it.
+    auto issue = [&](int which, int64_t blk, uint32_t n) {
+        const int slot = stream * depth + (int)(n & (depth - 1));
         uint64_t *full = &s_full[which][slot];
         const unsigned have = __ballot_sync(0xffffffffu, blk >= 0) & 0xFu;
         // the slot's last tile has been read by every warp of the group
@@ -294,17 +366,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             bulk_load(dst, (which ? p.c.v : p.c.k) + blk * Sh::kBlk, Sh::kBlk, full);
         }
     };
-    // A segment's beginning: this warp's first query row and block scales are
-    // asked for, then the stream's first tiles.
-    constexpr int N = D / 32;
-    float qv[N], sk = 0.0f, sv = 0.0f;
-    int64_t blk = -1;
-    auto row_ptr = [&](const Segment &sg, int r, int &tok) -> const T * {
-        const int t = over_g(sg.rem + r);
-        tok = sg.tok + t;
-        return static_cast<const T *>(p.rows.q) + (int64_t)(sg.w.q.row0 + tok) * p.rows.q_stride +
-               (sg.head * g + sg.rem + r - t * g) * D;
-    };
     auto scales = [&](int64_t i, float &k, float &v) {
         k = v = 0.0f;
         if (i >= 0) {
@@ -312,93 +373,282 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             v = __ldg(p.c.v_scale + i);
         }
     };
-    auto begin = [&](const Segment &sg) {
-        int tok;
-        if (warp < sg.rows) load_vals<N>(row_ptr(sg, warp, tok) + lane * N, qv);
-        blk = lookup(sg, sg.t0 + stream);
-        if (leader)
-            for (int i = 0; i < depth; i++) {
-                const int t = sg.t0 + stream + i * streams;
-                if (t >= sg.t1) break;
-                const int64_t first = i ? lookup(sg, t) : blk;
-                issue(0, first);
-                issue(1, first);
-            }
-        scales(blk, sk, sv);
+    auto row_ptr = [&](const Segment &sg, int r, int &tok) -> const T * {
+        const int t = over_g(sg.rem + r);
+        tok = sg.tok + t;
+        return static_cast<const T *>(p.rows.q) + (int64_t)(sg.q.row0 + tok) * p.rows.q_stride +
+               (sg.head * g + sg.rem + r - t * g) * D + lane * N;
     };
 
-    Segment sg;
-    if (!next_segment(sg)) return;
+    Segment cur, sg;
+    bool joining = false;      // cur's tiles are done, its parts not yet joined
+    uint32_t done = 0;         // tiles this stream has taken
+    float m[U], l[U], o[NT][SPLIT ? 2 : 4];
     __syncthreads();
-    begin(sg);
-    uint32_t done = 0;   // tiles this stream has taken
-    const float log2e = 1.4426950408889634f;
-
     for (;;) {
-        // ---- queries of the chunk to shared memory, in f32
-        for (int r = warp; r < sg.rows; r += kWarps) {
+        // ---- a segment's beginning: its first loads are on their way while the one
+        // before is joined
+        const bool more = next_segment(sg);
+        constexpr int kAhead = 2;             // query rows a warp asks for at once
+        float qv[kAhead][N], sk = 0.0f, sv = 0.0f;
+        int64_t blk = -1;
+        if (more) {
             int tok;
-            const T *x = row_ptr(sg, r, tok);
-            if (r != warp) load_vals<N>(x + lane * N, qv);
-            float *y = s_q + r * Sh::kQStride;
-            if (p.use_rope) {
-                norm_rope_vals<D>(qv, p.rope.q_norm, p.rope, sg.w.q.past + tok, y, lane);
-            } else {
 #pragma unroll
-                for (int i = 0; i < N; i++) y[lane * N + i] = qv[i];
+            for (int i = 0; i < kAhead; i++)
+                if (warp + i * kWarps < sg.rows) load_vals<N>(row_ptr(sg, warp + i * kWarps, tok), qv[i]);
+            blk = lookup(sg, sg.t0 + stream);
+            if (leader)
+                for (int i = 0; i < depth; i++) {
+                    const int t = sg.t0 + stream + i * streams;
+                    if (t >= sg.t1) break;
+                    const int64_t first = i ? lookup(sg, t) : blk;
+#pragma unroll 1
+                    for (int which = 0; which < 2; which++) issue(which, first, done + i);
+                }
+            scales(blk, sk, sv);
+        }
+
+        // ---- the warps' parts of the segment before, and the CTAs'
+        if (joining) {
+            const int taken = cur.t1 - cur.t0, used = min(streams, taken);
+            float *part = s_sum + warp * RR * D;      // the queries are in registers by now
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+                l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+                if (lj == 0) {
+                    s_m[warp][ln + 8 * u] = m[u];
+                    s_l[warp][ln + 8 * u] = l[u];
+                }
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+                    *reinterpret_cast<float2 *>(part + (ln + 8 * u) * D + i * 8 + lj * 2) = make_float2(o[i][2 * u], o[i][2 * u + 1]);
+            }
+            __syncthreads();
+            const bool whole_seg = taken == cur.tiles;
+            auto part_of = [&](int c) { return partials + (size_t)(c * 2 + (c == cur.cta0)) * (kPartialBytes / 4); };
+            float *mine = part_of(me);
+            auto write_out = [&](int r, int d, auto &acc, float den) {
+                constexpr int V = sizeof(acc) / 4;
+                const int t = over_g(cur.rem + r);
+                const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+                float v[V];
+#pragma unroll
+                for (int i = 0; i < V; i++) v[i] = acc[i] * inv;
+                store_vals<V>(static_cast<T *>(p.out) + (int64_t)(cur.q.row0 + cur.tok + t) * p.out_stride +
+                                  (cur.head * g + cur.rem + r - t * g) * D + d,
+                              v);
+            };
+            // Counts the CTA in; whether it is the last of n. (Thread 0's release covers what
+            // the CTA wrote before the barrier.)
+            auto arrive = [&](int *counter, int n) -> bool {
+                __syncthreads();
+                if (tid == 0) {
+                    s_last = atom_add_acq_rel(counter, 1) == n - 1;
+                    if (s_last) *counter = 0;
+                }
+                __syncthreads();
+                return s_last;
+            };
+            // Joins the parts of n CTAs, c, c + step, ...: into the output, or into the
+            // first one's part. A warp takes two rows at a time, a lane D / 32 values
+            // and a part's maximum and sum; all loads are under way before the first is used.
+            auto join = [&](int c, int step, int n, bool finish) {
+                for (int r0 = warp * 2; r0 < cur.rows; r0 += 2 * kWarps) {
+                    float M[2], a[2], den[2], acc[2][N];
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        M[k] = -INFINITY;
+                        den[k] = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < N; i++) acc[k][i] = 0.0f;
+                    }
+                    for (int i0 = 0; i0 < n; i0 += kJoin) {
+                        const int cn = min(kJoin, n - i0);
+                        float2 ml[2];
+                        float v[2][kJoin][N];
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const int r = min(r0 + k, cur.rows - 1);
+                            ml[k] = lane < cn ? __ldcg(reinterpret_cast<const float2 *>(part_of(c + (i0 + lane) * step) + 2 * r))
+                                              : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                            for (int i = 0; i < kJoin; i++) {
+                                if (i < cn) {
+                                    const float *src = part_of(c + (i0 + i) * step) + 2 * kMaxRows + r * D + lane * N;
+                                    if constexpr (N == 4) {
+                                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(src));
+                                        v[k][i][0] = x.x; v[k][i][1] = x.y; v[k][i][2] = x.z; v[k][i][3] = x.w;
+                                    } else {
+                                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(src));
+                                        v[k][i][0] = x.x; v[k][i][1] = x.y;
+                                    }
+                                } else {
+#pragma unroll
+                                    for (int j = 0; j < N; j++) v[k][i][j] = 0.0f;
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const float top = fmaxf(M[k], warp_max_f(ml[k].x)), ms = top == -INFINITY ? 0.0f : top;
+                            const float before = ex2(M[k] - ms);
+                            M[k] = top;
+                            a[k] = ex2(ml[k].x - ms);
+                            den[k] = fmaf(den[k], before, warp_sum_f(ml[k].y * a[k]));
+#pragma unroll
+                            for (int j = 0; j < N; j++) acc[k][j] *= before;
+#pragma unroll
+                            for (int i = 0; i < kJoin; i++) {
+                                const float ai = __shfl_sync(0xffffffffu, a[k], i);
+#pragma unroll
+                                for (int j = 0; j < N; j++) acc[k][j] = fmaf(v[k][i][j], ai, acc[k][j]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const int r = r0 + k;
+                        if (r >= cur.rows) break;
+                        if (finish) {
+                            write_out(r, lane * N, acc[k], den[k]);
+                        } else {
+                            float *dst = part_of(c);
+                            __syncwarp();          // its maximum and sum have been read
+#pragma unroll
+                            for (int j = 0; j < N; j++) dst[2 * kMaxRows + r * D + lane * N + j] = acc[k][j];
+                            if (lane == 0) *reinterpret_cast<float2 *>(dst + 2 * r) = make_float2(M[k], den[k]);
+                        }
+                    }
+                }
+            };
+            constexpr int Q4 = D / 4;
+            for (int e = tid; e < cur.rows * Q4; e += kThreads) {
+                const int r = e / Q4, d = e % Q4 * 4, wr = r / RR, rr = r % RR;
+                float M = -INFINITY;
+                for (int i = 0; i < used; i++) M = fmaxf(M, s_m[i * group + wr][rr]);
+                const float Ms = M == -INFINITY ? 0.0f : M;
+                float acc[4] = {}, den = 0.0f;
+                for (int i = 0; i < used; i++) {
+                    const int w = i * group + wr;
+                    const float a = ex2(s_m[w][rr] - Ms);
+                    const float4 v = *reinterpret_cast<const float4 *>(s_sum + (w * RR + rr) * D + d);
+                    den = fmaf(s_l[w][rr], a, den);
+                    acc[0] = fmaf(v.x, a, acc[0]);
+                    acc[1] = fmaf(v.y, a, acc[1]);
+                    acc[2] = fmaf(v.z, a, acc[2]);
+                    acc[3] = fmaf(v.w, a, acc[3]);
+                }
+                if (whole_seg) {
+                    write_out(r, d, acc, den);
+                } else {
+                    *reinterpret_cast<float4 *>(mine + 2 * kMaxRows + r * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                    if (d == 0) *reinterpret_cast<float2 *>(mine + 2 * r) = make_float2(M, den);
+                }
+            }
+            __syncthreads();   // the sums are read before the next queries go there
+            if (!whole_seg) {
+                // Whichever CTA brings a group's last part joins the group, in order;
+                // whichever brings the last group joins the groups.
+                const int first = cur.cta0 + (me - cur.cta0) / kJoin * kJoin, parts = cur.cta1 - cur.cta0 + 1;
+                bool last = arrive(counters + first * 2 + (first == cur.cta0), min(kJoin, cur.cta1 - first + 1));
+                const int groups = (parts + kJoin - 1) / kJoin;
+                if (last) join(first, 1, min(kJoin, cur.cta1 - first + 1), groups == 1);
+                if (last && groups > 1) {
+                    last = arrive(counters + 2 * gridDim.x + cur.cta0 * 2, groups);
+                    if (last) join(cur.cta0, kJoin, groups, true);
+                }
+            }
+        }
+        if (!more) break;
+
+        // ---- queries of the chunk to shared memory as f16, scaled per row by a power
+        // of two that takes the largest value to [2^14, 2^15): what is 2^-28 of it is still held in full
+#pragma unroll 1
+        for (int r0 = warp; r0 < sg.rows; r0 += kAhead * kWarps) {
+            float amax[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                const int r = min(r0 + k * kWarps, sg.rows - 1);     // (a last odd row goes twice)
+                int tok;
+                const T *x = row_ptr(sg, r, tok);
+                float (&v)[N] = qv[k];
+                if (r0 != warp || r != r0 + k * kWarps) load_vals<N>(x, v);
+                if (p.use_rope) {
+                    float *y = reinterpret_cast<float *>(smem + Sh::kRowOff) + warp * D;
+                    norm_rope_vals<D>(v, p.rope.q_norm, p.rope, sg.q.past + tok, y, lane);
+#pragma unroll
+                    for (int i = 0; i < N; i++) v[i] = y[lane * N + i];
+                    __syncwarp();
+                }
+                amax[k] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < N; i++) amax[k] = fmaxf(amax[k], fabsf(v[i]));
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) amax[k] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax[k])));
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                const int r = min(r0 + k * kWarps, sg.rows - 1);
+                const float (&v)[N] = qv[k];
+                const int e = max(-112, (int)(__float_as_uint(amax[k]) >> 23) - 127);
+                const float up = __int_as_float((14 - e + 127) << 23);
+                if (lane == 0) s_rf[r] = __int_as_float((e - 14 + 127) << 23) * p.scale * 1.4426950408889634f;
+                uint32_t hi[N / 2], lo[N / 2];
+#pragma unroll
+                for (int i = 0; i < N / 2; i++) {
+                    if constexpr (SPLIT) split_f16(v[2 * i] * up, v[2 * i + 1] * up, hi[i], lo[i]);
+                    else hi[i] = pack_f16(v[2 * i] * up, v[2 * i + 1] * up);
+                }
+                uint32_t *y = reinterpret_cast<uint32_t *>(s_q + r * Sh::kQRow) + lane * (N / 2);
+#pragma unroll
+                for (int i = 0; i < N / 2; i++) {
+                    y[i] = hi[i];
+                    if (SPLIT) y[i + kWarps * RR * Sh::kQRow / 4] = lo[i];
+                }
             }
         }
         __syncthreads();
 
-        // ---- this warp's row tile as A fragments. Lane (ln, lj) holds the
-        // values 16 lj .. 16 lj + 15 of every 64 of its row, in the order in
-        // which a key's 16 bytes come out of one load.
+        // ---- this warp's row tile as A fragments. Lane (ln, lj) holds the values
+        // 16 lj .. 16 lj + 15 of every 64 of its row, in the order in which a key's
+        // 16 bytes come out of one load.
         uint32_t qa[KS][4];
-        float rf[SPLIT ? 1 : 2];        // per row: logit factor
-        int pos[SPLIT ? 1 : 2];
+        float rf[U];
+        int pos[U];
         const int row_base = rt * RR;
 #pragma unroll
-        for (int u = 0; u < (SPLIT ? 1 : 2); u++) {
+        for (int u = 0; u < U; u++) {
             const int r = row_base + ln + 8 * u;
             const bool live = r < sg.rows;
             pos[u] = live ? sg.pos_first + over_g(sg.rem + r) : -1;
-            const float *y = s_q + (live ? r : 0) * Sh::kQStride;
-            float amax = 0.0f;
+            rf[u] = live ? s_rf[r] : 0.0f;
+            const uint4 *y = reinterpret_cast<const uint4 *>(s_q + (live ? r : 0) * Sh::kQRow + lj * 32);
 #pragma unroll
             for (int h = 0; h < D / 64; h++)
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const float4 v = *reinterpret_cast<const float4 *>(y + h * 64 + lj * 16 + i);
-                    amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-                }
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            // largest value to [2^14, 2^15): f16 then holds values 2^-28 of it in full
-            const int e = max(-112, (__float_as_int(amax) >> 23) - 127);
-            const float up = __int_as_float((14 - e + 127) << 23);
-            rf[u] = __int_as_float((e - 14 + 127) << 23) * p.scale * log2e;
-#pragma unroll
-            for (int h = 0; h < D / 64; h++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float4 v = *reinterpret_cast<const float4 *>(y + h * 64 + lj * 16 + 4 * i);
-                    if (!live) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    uint32_t (&a)[4] = qa[h * 4 + i];
+                for (int i = 0; i < 2; i++) {
+                    const uint4 a = y[h * 8 + i];
+                    uint32_t (&x)[4] = qa[h * 4 + 2 * i], (&z)[4] = qa[h * 4 + 2 * i + 1];
+                    x[u] = a.x;
+                    x[2 + u] = a.y;
+                    z[u] = a.z;
+                    z[2 + u] = a.w;
                     if constexpr (SPLIT) {
-                        split_f16(v.x * up, v.y * up, a[0], a[1]);
-                        split_f16(v.z * up, v.w * up, a[2], a[3]);
-                    } else {
-                        a[u] = pack_f16(v.x * up, v.y * up);
-                        a[2 + u] = pack_f16(v.z * up, v.w * up);
+                        const uint4 c = y[kWarps * RR * Sh::kQRow / 16 + h * 8 + i];
+                        x[1] = c.x;
+                        x[3] = c.y;
+                        z[1] = c.z;
+                        z[3] = c.w;
                     }
                 }
         }
         const int tile_pos0 = sg.pos_first + over_g(sg.rem + min(row_base, sg.rows - 1));   // of the first row
         const int tile_pos1 = sg.pos_first + over_g(sg.rem + min(row_base + RR, sg.rows) - 1);
-
-        float m[SPLIT ? 1 : 2], l[SPLIT ? 1 : 2], o[NT][SPLIT ? 2 : 4];
 #pragma unroll
-        for (int u = 0; u < (SPLIT ? 1 : 2); u++) {
+        for (int u = 0; u < U; u++) {
             m[u] = -INFINITY;
             l[u] = 0.0f;
         }
@@ -409,49 +659,50 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
 
         // ---- the stream's tiles
         for (int t = sg.t0 + stream; t < sg.t1; t += streams, done++) {
-            const int slot = stream * depth + (int)(done % depth);
+            const int slot = stream * depth + (int)(done & (depth - 1));
             const uint32_t ph = (done / depth) & 1;
             const int64_t next = lookup(sg, t + streams);
             const int64_t ahead = depth == 1 ? next : leader ? lookup(sg, t + depth * streams) : -1;
             float s[8][4];
             tc_spin_wait(&s_full[0][slot], ph, &s_abort, p.err);
             // column c of the 8-token group i: token 16 (c / 2) + 2 i + (c & 1) of the
-            // tile, so that this lane's columns all lie in block lj
+            // tile, so that this lane's columns all lie in block lj (four groups at a
+            // time: their accumulators do not wait for one another)
             const uint32_t ka = kbase + (slot * 4 + ln / 2) * Sh::kBlk + (ln & 1) * 64 + lj * 16;
-            // (four groups at a time: their accumulators do not wait for one another)
 #pragma unroll
             for (int i0 = 0; i0 < 8; i0 += 4)
 #pragma unroll
                 for (int h = 0; h < D / 64; h++) {
-                    uint4 w[4];
+                    uint4 kw[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) w[i] = lds128(ka + h * 1024 + (i0 + i) * 128);
+                    for (int i = 0; i < 4; i++) kw[i] = lds128(ka + h * 1024 + (i0 + i) * 128);
 #pragma unroll
                     for (int q = 0; q < 4; q++)
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             uint32_t b0, b1;
-                            bytes_f16(word(w[i], q), b0, b1);
+                            bytes_f16(word(kw[i], q), b0, b1);
                             if (h == 0 && q == 0) mma16816_first(s[i0 + i], qa[0], b0, b1);
                             else mma16816(s[i0 + i], qa[h * 4 + q], b0, b1);
                         }
                 }
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_empty[0][slot]);
-            if (leader && t + depth * streams < sg.t1) issue(0, ahead);
+            const bool reload = leader && t + depth * streams < sg.t1;
+            if (reload) issue(0, ahead, done + depth);
             float sk_next, sv_next;
             scales(next, sk_next, sv_next);
 
             // ---- weights
-            const float lsv = sv > 0.0f ? log2f(sv) : kNoScaleLog2, isv = sv > 0.0f ? 1.0f / sv : ex2(-kNoScaleLog2);
-            const int tok0 = (sg.w.tile0 + t) * kTile;
+            const float lsv = sv > 0.0f ? lg2(sv) : kNoScaleLog2, isv = ex2(-lsv);
+            const int tok0 = (sg.tile0 + t) * kTile;
             const bool clear = tok0 + kTile - 1 <= tile_pos0 && (!p.window || tok0 > tile_pos1 - p.window);
             const bool whole = __all_sync(0xffffffffu, clear && blk >= 0);
-            float alpha[SPLIT ? 1 : 2];
+            float alpha[U];
 #pragma unroll
-            for (int u = 0; u < (SPLIT ? 1 : 2); u++) {
+            for (int u = 0; u < U; u++) {
                 const float f = rf[u] * sk;
-                float mx = -INFINITY;
+                float mx[4];
 #pragma unroll
                 for (int i = 0; i < 8; i++)
 #pragma unroll
@@ -463,23 +714,24 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
                             if (blk < 0 || j > pos[u] || (p.window && j <= pos[u] - p.window)) v = -INFINITY;
                         }
                         s[i][2 * u + x] = v;
-                        mx = fmaxf(mx, v);
+                        mx[i % 4] = i < 4 && x == 0 ? v : fmaxf(mx[i % 4], v);
                     }
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float mn = fmaxf(m[u], mx), ms = mn == -INFINITY ? 0.0f : mn;
+                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float mn = fmaxf(m[u], top), ms = mn == -INFINITY ? 0.0f : mn;
                 alpha[u] = ex2(m[u] - ms);
                 m[u] = mn;
-                float sum = 0.0f;
+                float sum[4];
 #pragma unroll
                 for (int i = 0; i < 8; i++)
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const float w = ex2(s[i][2 * u + x] - ms);
-                        s[i][2 * u + x] = w;
-                        sum += w;
+                        const float e = ex2(s[i][2 * u + x] - ms);
+                        s[i][2 * u + x] = e;
+                        sum[i % 4] = i < 4 && x == 0 ? e : sum[i % 4] + e;
                     }
-                l[u] = fmaf(l[u], alpha[u], sum * isv);
+                l[u] = fmaf(l[u], alpha[u], ((sum[0] + sum[1]) + (sum[2] + sum[3])) * isv);
             }
             // A fragments of the weights: k step q takes tokens 4 q .. 4 q + 3 of each lane's block
             uint32_t pa[4][4];
@@ -499,168 +751,55 @@ __global__ void __launch_bounds__(kThreads, 1) attend_stream_kernel(const __grid
             const uint32_t va = vbase + (slot * 4 + lj) * Sh::kVBlk + ln * 16;
             // a tile's sums start at zero and join the running ones in f32, rounded to
             // nearest: the tensor cores' additions round towards zero
+            constexpr int PV = SPLIT ? 8 : 4;
 #pragma unroll
-            for (int i0 = 0; i0 < NT; i0 += 4) {
-                uint4 w[4];
-                float c[4][4];
+            for (int i0 = 0; i0 < NT; i0 += PV) {
+                uint4 vw[PV];
+                float c[PV][4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = lds128(va + (i0 + i) * 128);
+                for (int i = 0; i < PV; i++) vw[i] = lds128(va + (i0 + i) * 128);
 #pragma unroll
                 for (int q = 0; q < 4; q++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
+                    for (int i = 0; i < PV; i++) {
                         uint32_t b0, b1;
-                        bytes_f16(word(w[i], q), b0, b1);
+                        bytes_f16(word(vw[i], q), b0, b1);
                         if (q == 0) mma16816_first(c[i], pa[0], b0, b1);
                         else mma16816(c[i], pa[q], b0, b1);
                     }
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int i = 0; i < PV; i++)
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
                         if constexpr (SPLIT) {
                             o[i0 + i][x] = fmaf(o[i0 + i][x], alpha[0], c[i][x] + c[i][2 + x]);
                         } else {
                             o[i0 + i][x] = fmaf(o[i0 + i][x], alpha[0], c[i][x]);
-                            o[i0 + i][2 + x] = fmaf(o[i0 + i][2 + x], alpha[1], c[i][2 + x]);
+                            o[i0 + i][2 + x] = fmaf(o[i0 + i][2 + x], alpha[U - 1], c[i][2 + x]);
                         }
                     }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_empty[1][slot]);
-            if (leader && t + depth * streams < sg.t1) issue(1, ahead);
+            if (reload) issue(1, ahead, done + depth);
             blk = next;
             sk = sk_next;
             sv = sv_next;
         }
-
-        // ---- the next segment's first tiles are on their way while this one is joined
-        const Segment cur = sg;
-        const bool more = next_segment(sg);
-        if (more) begin(sg);
-
-        const int taken = cur.t1 - cur.t0, used = min(streams, taken);
-        float *part = s_q + warp * RR * D;      // the queries are in registers by now
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < (SPLIT ? 1 : 2); u++) {
-            l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-            l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-            if (lj == 0) {
-                s_m[warp][ln + 8 * u] = m[u];
-                s_l[warp][ln + 8 * u] = l[u];
-            }
-#pragma unroll
-            for (int i = 0; i < NT; i++) {
-                *reinterpret_cast<float2 *>(part + (ln + 8 * u) * D + i * 8 + lj * 2) = make_float2(o[i][2 * u], o[i][2 * u + 1]);
-            }
-        }
-        __syncthreads();
-        const bool whole_seq = taken == cur.w.tiles;
-        const int64_t last_unit = cur.unit + cur.w.tiles - 1;
-        const int c0 = cur.t0 == 0 ? me : runs.of(cur.unit), c1 = cur.t1 == cur.w.tiles ? me : runs.of(last_unit);
-        float *mine = partials + (size_t)(me * 2 + (me == c0 ? 1 : 0)) * (kPartialBytes / 4);
-        auto write_out = [&](int r, int d, auto &acc, float den) {
-            constexpr int V = sizeof(acc) / 4;
-            const int t = over_g(cur.rem + r);
-            const float inv = den > 0.0f ? 1.0f / den : 0.0f;
-            float v[V];
-#pragma unroll
-            for (int i = 0; i < V; i++) v[i] = acc[i] * inv;
-            store_vals<V>(static_cast<T *>(p.out) + (int64_t)(cur.w.q.row0 + cur.tok + t) * p.out_stride +
-                              (cur.head * g + cur.rem + r - t * g) * D + d,
-                          v);
-        };
-        constexpr int Q4 = D / 4;
-        for (int e = tid; e < cur.rows * Q4; e += kThreads) {
-            const int r = e / Q4, d = e % Q4 * 4, w0 = r / RR, rr = r % RR;
-            float M = -INFINITY;
-            for (int i = 0; i < used; i++) M = fmaxf(M, s_m[i * group + w0][rr]);
-            const float Ms = M == -INFINITY ? 0.0f : M;
-            float acc[4] = {}, den = 0.0f;
-            for (int i = 0; i < used; i++) {
-                const int w = i * group + w0;
-                const float a = ex2(s_m[w][rr] - Ms);
-                const float4 v = *reinterpret_cast<const float4 *>(s_q + (w * RR + rr) * D + d);
-                den = fmaf(s_l[w][rr], a, den);
-                acc[0] = fmaf(v.x, a, acc[0]);
-                acc[1] = fmaf(v.y, a, acc[1]);
-                acc[2] = fmaf(v.z, a, acc[2]);
-                acc[3] = fmaf(v.w, a, acc[3]);
-            }
-            if (whole_seq) {
-                write_out(r, d, acc, den);
-            } else {
-                *reinterpret_cast<float4 *>(mine + 2 * kMaxRows + r * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                if (d == 0) *reinterpret_cast<float2 *>(mine + 2 * r) = make_float2(M, den);
-            }
-        }
-        if (!whole_seq) {
-            // the CTA that brings the last part joins them all, in their order: a
-            // warp per row, lanes over the parts for the maximum, then over the values
-            __syncthreads();
-            if (tid == 0) {
-                __threadfence();
-                const int n = atomicAdd(counters + c0, 1);
-                s_last = n == c1 - c0;
-                if (s_last) counters[c0] = 0;
-                __threadfence();
-            }
-            __syncthreads();
-            if (s_last) {
-                auto part_of = [&](int c) { return partials + (size_t)(c * 2 + (c == c0)) * (kPartialBytes / 4); };
-                for (int r = warp; r < cur.rows; r += kWarps) {
-                    float M = -INFINITY;
-                    for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, __ldcg(part_of(c) + 2 * r));
-                    M = warp_max_f(M);
-                    const float Ms = M == -INFINITY ? 0.0f : M;
-                    constexpr int V = D / 32;
-                    float acc[V], den = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < V; i++) acc[i] = 0.0f;
-                    for (int cb = c0; cb <= c1; cb += 32) {
-                        float a = 0.0f;
-                        if (cb + lane <= c1) {
-                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(cb + lane) + 2 * r));
-                            a = ex2(ml.x - Ms);
-                            den = fmaf(ml.y, a, den);
-                        }
-                        const int n = min(32, c1 - cb + 1);
-#pragma unroll 8
-                        for (int i = 0; i < n; i++) {
-                            const float *src = part_of(cb + i) + 2 * kMaxRows + r * D + lane * V;
-                            float v[V];
-                            if constexpr (V == 4) {
-                                const float4 x = __ldcg(reinterpret_cast<const float4 *>(src));
-                                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-                            } else {
-                                const float2 x = __ldcg(reinterpret_cast<const float2 *>(src));
-                                v[0] = x.x; v[1] = x.y;
-                            }
-                            const float ai = __shfl_sync(0xffffffffu, a, i);
-#pragma unroll
-                            for (int k = 0; k < V; k++) acc[k] = fmaf(v[k], ai, acc[k]);
-                        }
-                    }
-                    den = warp_sum_f(den);
-                    write_out(r, lane * V, acc, den);
-                }
-            }
-        }
-        if (!more) break;
-        __syncthreads();   // the sums are read before the next queries go there
+        cur = sg;
+        joining = true;
     }
     // after a wait that ran out, copies may still be in flight
     if (*(volatile int *)&s_abort && leader)
         for (int which = 0; which < 2; which++)
-            for (uint32_t n = issued[which] > (uint32_t)depth ? issued[which] - depth : 0; n < issued[which]; n++)
+            for (uint32_t n = done > (uint32_t)depth ? done - depth : 0; n < done; n++)
                 drain_wait(&s_full[which][stream * depth + n % depth], (n / depth) & 1);
 }
 
 template <int D, typename T, bool SPLIT>
 cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
 {
-    using Sh = Shape<D, T, SPLIT>;
+    using Sh = Shape<D, SPLIT>;
     auto kern = attend_stream_kernel<D, T, SPLIT>;
     static bool set[64] = {};
     int dev = 0;
@@ -676,8 +815,18 @@ cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
     int group = 1;
     while (group < kWarps && (int64_t)group * Sh::kRows < rows) group *= 2;
     uint8_t *ws = static_cast<uint8_t *>(p.ws);
-    return launch_dependent(kern, dim3(p.num_sms), dim3(kThreads), Sh::kSmem, st, p, group, g > 1 ? (uint32_t)((1ull << 32) / g + 1) : 0u,
-                            reinterpret_cast<int *>(ws + kCounterOff), reinterpret_cast<float *>(ws + partial_off(p.num_sms)));
+    const int ctas = p.num_sms * kCtasPerSm;
+    // a launch's tiles are counted in 32 bits: sequences that could have more go in several
+    const int64_t most = (((int64_t)p.c.table_stride * kKvBlock << p.c.page_shift) / kTile + 2) * p.c.heads *
+                         ((rows + group * Sh::kRows - 1) / (group * Sh::kRows));
+    const int step = (int)std::max<int64_t>(1, std::min<int64_t>(p.b.B, (int64_t)INT_MAX / most));
+    for (int s = 0; s < p.b.B; s += step) {
+        e = launch_dependent(kern, dim3(ctas), dim3(kThreads), Sh::kSmem, st, p, s, std::min(p.b.B, s + step), group,
+                             g > 1 ? (uint32_t)((1ull << 32) / g + 1) : 0u, reinterpret_cast<int *>(ws + kCounterOff),
+                             reinterpret_cast<float *>(ws + partial_off(ctas)));
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 template <typename T>
@@ -693,7 +842,11 @@ cudaError_t launch_t(const AttnParams &p, cudaStream_t st)
 
 }  // namespace
 
-size_t attn_workspace_bytes(int num_sms) { return partial_off(num_sms) + (size_t)num_sms * 2 * kPartialBytes; }
+size_t attn_workspace_bytes(int num_sms)
+{
+    const int ctas = num_sms * kCtasPerSm;
+    return partial_off(ctas) + (size_t)ctas * 2 * kPartialBytes;
+}
 
 cudaError_t launch_attention(const AttnParams &p, cudaStream_t st)
 {
