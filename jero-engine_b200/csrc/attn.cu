@@ -34,6 +34,8 @@ constexpr int kTile = 64;                    // tokens of a tile: 4 blocks
 constexpr int kMaxRows = kWarps * 16;        // rows of a chunk
 // A run has at least this many tiles: fewer CTAs share a short sequence.
 constexpr int kMinTiles = 2;
+// Sequences with more rows (new tokens times query heads of a key head) go to attn_tiles.cu.
+constexpr int kFewRows = 64;
 // What beginning and joining one more segment costs a CTA, in tiles.
 constexpr int kSegmentTiles = 8;
 
@@ -44,6 +46,10 @@ constexpr int kJoin = 16;
 constexpr size_t kCounterOff = 256;
 size_t partial_off(int ctas) { return kCounterOff + ((size_t)ctas * 16 + 255) / 256 * 256; }
 constexpr size_t kPartialBytes = (size_t)kMaxRows * (kMaxHeadDim + 2) * 4;
+
+// Behind them the queries of attn_tiles.cu, a slice of the rows at a time.
+constexpr size_t kTilesBytes = (size_t)80 << 20;
+size_t tiles_off(int num_sms) { return partial_off(num_sms * kCtasPerSm) + (size_t)num_sms * kCtasPerSm * 2 * kPartialBytes; }
 
 // Values of a sequence without a scale (an all-zero block): far below any real
 // scale (>= 2^-74), so its weights stay small and its sums in range.
@@ -171,7 +177,7 @@ __device__ __forceinline__ void seq_work(const AttnParams &p, int s, int g, int 
     const bool listed = seq_info(p.b, s, w.q), cached = seq_in_cache(p.c, p.b, s, w.q, w.slot);
     bad = !listed || !cached;
     w.tile0 = w.tiles = w.segs = 0;
-    if (bad || w.q.n == 0) return;
+    if (bad || w.q.n == 0 || w.q.n * g > kFewRows) return;
     w.tile0 = p.window ? max(0, w.q.past - p.window + 1) / kTile : 0;
     w.tiles = (w.q.past + w.q.n - 1) / kTile + 1 - w.tile0;
     w.segs = p.c.heads;
@@ -811,7 +817,9 @@ cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
     }
     // warps that share a tile: one for each row tile, up to all eight
     const int g = p.rows.q_heads / p.c.heads;
-    const int64_t rows = (int64_t)p.b.max_new * g;
+    int64_t rows = (int64_t)p.b.max_new * g;
+    const bool prompts = rows > kFewRows;
+    if (prompts) rows = kFewRows;
     int group = 1;
     while (group < kWarps && (int64_t)group * Sh::kRows < rows) group *= 2;
     uint8_t *ws = static_cast<uint8_t *>(p.ws);
@@ -826,6 +834,7 @@ cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
                              reinterpret_cast<float *>(ws + partial_off(ctas)));
         if (e != cudaSuccess) return e;
     }
+    if (prompts) return launch_attention_tiles(p, kFewRows, ws + tiles_off(p.num_sms), kTilesBytes, st);
     return cudaSuccess;
 }
 
@@ -842,11 +851,7 @@ cudaError_t launch_t(const AttnParams &p, cudaStream_t st)
 
 }  // namespace
 
-size_t attn_workspace_bytes(int num_sms)
-{
-    const int ctas = num_sms * kCtasPerSm;
-    return partial_off(ctas) + (size_t)ctas * 2 * kPartialBytes;
-}
+size_t attn_workspace_bytes(int num_sms) { return tiles_off(num_sms) + kTilesBytes; }
 
 cudaError_t launch_attention(const AttnParams &p, cudaStream_t st)
 {

@@ -110,6 +110,61 @@ __device__ __forceinline__ int2 rope_pair(const RopeDev &r, int i)
     return r.interleaved ? make_int2(2 * i, 2 * i + 1) : make_int2(i, i + r.R / 2);
 }
 
+// A warp: the sequence whose rows hold `row` (row_start ascending), -1 for none.
+__device__ __forceinline__ int seq_of_row_warp(const KvBatchDev &b, int row, int lane)
+{
+    if (!b.row_start) return row < b.B ? row : -1;
+    int n = 0;
+    for (int s = lane; s < b.B; s += 32) n += __ldg(b.row_start + s) <= row;
+    return __reduce_add_sync(0xffffffffu, n) - 1;
+}
+
+// cos and sin of a position's R / 2 angles, times mscale, by n threads.
+__device__ __forceinline__ void rope_table(const RopeDev &r, int pos, float2 *turn, int tid, int n)
+{
+    for (int i = tid; i < r.R / 2; i += n) {
+        float c, s;
+        turn_f32((double)pos * r.inv[i], c, s);
+        turn[i] = make_float2(c * (float)r.mscale, s * (float)r.mscale);
+    }
+}
+
+// One warp: a head row, D / 32 consecutive values in each lane's v, normed
+// (w != nullptr) and turned by the table's angles, in f32. y: D floats of
+// shared memory of the warp's own.
+template <int D>
+__device__ __forceinline__ void turn_head(float (&v)[D / 32], const float *w, const RopeDev &r, const float2 *turn, float *y, int lane)
+{
+    constexpr int N = D / 32;
+    if (w) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; i++) ss = fmaf(v[i], v[i], ss);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = 1.0f / sqrtf(ss * (1.0f / D) + (float)r.eps);
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = v[i] * inv * __ldg(w + lane * N + i);
+    }
+    if (r.R == 0) return;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < N; i++) y[lane * N + i] = v[i];
+    __syncwarp();
+    // each value with its partner: a cos - b sin for the first of a pair, b cos + a sin for the second
+    const int half = r.R / 2;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int d = lane * N + i;
+        if (d < r.R) {
+            const bool second = r.interleaved ? d & 1 : d >= half;
+            const float2 t = turn[r.interleaved ? d / 2 : second ? d - half : d];
+            const float other = y[r.interleaved ? d ^ 1 : second ? d - half : d + half];
+            v[i] = second ? v[i] * t.x + other * t.y : v[i] * t.x - other * t.y;
+        }
+    }
+}
+
 // One warp: a head row of D values, D / 32 consecutive ones in each lane's v,
 // normed (w != nullptr) and rotated at position pos into y[D] (shared memory),
 // all in f32 but the angles.

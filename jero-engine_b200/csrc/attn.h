@@ -59,6 +59,10 @@ struct AttnParams {
 // Bytes of a context's attention workspace.
 size_t attn_workspace_bytes(int num_sms);
 
+// Attention of the sequences with more than few_rows rows (tokens times query
+// heads of a key head) on tcgen05; the others' rows are left alone.
+cudaError_t launch_attention_tiles(const AttnParams &p, int few_rows, void *ws, size_t ws_bytes, cudaStream_t st);
+
 cudaError_t launch_qk_norm_rope(const KvBatchDev &b, const RopeDev &rope, const AttnRows &in, const AttnRows &out, int D,
                                 int *err, cudaStream_t st);
 cudaError_t launch_kv_append(const KvCacheDev &c, const KvBatchDev &b, const RopeDev *rope, const AttnRows &rows, int *err,
