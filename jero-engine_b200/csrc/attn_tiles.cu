@@ -19,6 +19,7 @@
 // weights take 1024 cycles of the 16 a cycle that the SM gives, the two
 // products of a row tile 2 x 512.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn.cuh"
 #include "kernels.h"
@@ -479,27 +480,48 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int hi = pos - tok0, lo = p.window ? pos - p.window - tok0 : INT_MIN;   // seen: lo < column <= hi
                 const uint32_t okm = s_ok[rr];
                 const bool whole = __all_sync(0xffffffffu, hi >= kKv - 1 && (!live || lo < 0)) && okm == 0xFFu;
-                auto seen = [&](int c) -> bool { return c <= hi && c > lo && ((okm >> (c / kKvBlock)) & 1); };
-                // ---- the row's maximum
+                // bit i: column 32 c + i is seen
+                auto seen = [&](int c) -> uint32_t {
+                    const int up = hi - 32 * c, down = lo - 32 * c;
+                    uint32_t mask = up < 0 ? 0u : up >= 31 ? ~0u : (2u << up) - 1;
+                    if (down >= 0) mask &= down >= 31 ? 0u : ~((2u << down) - 1);
+                    const uint32_t ok2 = okm >> (2 * c);
+                    return mask & ((ok2 & 1 ? 0xFFFFu : 0u) | (ok2 & 2 ? 0xFFFF0000u : 0u));
+                };
+                // ---- the row's maximum, over two quarters of the tile at a time
                 float top = -INFINITY;
+                auto maxima = [&](auto kind) {
+                    constexpr bool masked = decltype(kind)::value;
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t s[32];
-                    tmem_ld32(ts + c * 32, s);
-                    tmem_ld_wait();
+                    for (int c0 = 0; c0 < 4; c0 += 2) {
+                        uint32_t s[2][32];
+                        tmem_ld32(ts + c0 * 32, s[0]);
+                        tmem_ld32(ts + c0 * 32 + 32, s[1]);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        float x = -INFINITY;
+                        for (int c = 0; c < 2; c++) {
+                            const uint32_t mask = masked ? seen(c0 + c) : ~0u;
+                            const float2 sk = *reinterpret_cast<const float2 *>(&s_sk[rr][(c0 + c) * 2]);
+                            const float2 ls = *reinterpret_cast<const float2 *>(&s_lsv[rr][(c0 + c) * 2]);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const float v = __uint_as_float(s[b * 16 + i]);
-                            x = fmaxf(x, whole || seen(c * 32 + b * 16 + i) ? v : -INFINITY);
+                            for (int b = 0; b < 2; b++) {
+                                float x[4];
+#pragma unroll
+                                for (int i = 0; i < 16; i++) {
+                                    float v = __uint_as_float(s[c][b * 16 + i]);
+                                    if (masked) v = mask >> (b * 16 + i) & 1 ? v : -INFINITY;
+                                    x[i % 4] = i < 4 ? v : fmaxf(x[i % 4], v);
+                                }
+                                const float y = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                                const float u = fmaf(y, rf * (b ? sk.y : sk.x), b ? ls.y : ls.x);
+                                // (a block unseen stays at -inf whatever its factor)
+                                top = fmaxf(top, masked && y == -INFINITY ? -INFINITY : u);
+                            }
                         }
-                        // (a block unseen stays at -inf whatever its factor)
-                        const float u = fmaf(x, rf * s_sk[rr][c * 2 + b], s_lsv[rr][c * 2 + b]);
-                        top = fmaxf(top, x == -INFINITY ? -INFINITY : u);
                     }
-                }
+                };
+                if (whole) maxima(std::false_type{});
+                else maxima(std::true_type{});
                 const bool grow = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float a = grow ? ex2(m - top) : 1.0f;
@@ -520,36 +542,51 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 // ---- the weights, over the logits they come from
                 const float ms = m == -INFINITY ? 0.0f : m;
+                auto weights = [&](auto kind) {
+                    constexpr bool masked = decltype(kind)::value;
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t s[32], ph[16], pl[16];
-                    tmem_ld32(ts + c * 32, s);
-                    tmem_ld_wait();
+                    for (int c0 = 0; c0 < 4; c0 += 2) {
+                        uint32_t s[2][32];
+                        tmem_ld32(ts + c0 * 32, s[0]);
+                        tmem_ld32(ts + c0 * 32 + 32, s[1]);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        const float f = rf * s_sk[rr][c * 2 + b], z = s_lsv[rr][c * 2 + b] - ms;
-                        float sum[2] = {0.0f, 0.0f};
+                        for (int c = 0; c < 2; c++) {
+                            uint32_t ph[16];
+                            [[maybe_unused]] uint32_t pl[16];
+                            const uint32_t mask = masked ? seen(c0 + c) : ~0u;
+                            const float2 sk = *reinterpret_cast<const float2 *>(&s_sk[rr][(c0 + c) * 2]);
+                            const float2 ls = *reinterpret_cast<const float2 *>(&s_lsv[rr][(c0 + c) * 2]);
+                            const float2 is = *reinterpret_cast<const float2 *>(&s_isv[rr][(c0 + c) * 2]);
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            float x = ex2(fmaf(__uint_as_float(s[b * 16 + i]), f, z));
-                            float y = ex2(fmaf(__uint_as_float(s[b * 16 + i + 1]), f, z));
-                            if (!whole) {
-                                x = seen(c * 32 + b * 16 + i) ? x : 0.0f;
-                                y = seen(c * 32 + b * 16 + i + 1) ? y : 0.0f;
+                            for (int b = 0; b < 2; b++) {
+                                const float f = rf * (b ? sk.y : sk.x), z = (b ? ls.y : ls.x) - ms;
+                                float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                                for (int i = 0; i < 16; i += 2) {
+                                    float x = ex2(fmaf(__uint_as_float(s[c][b * 16 + i]), f, z));
+                                    float y = ex2(fmaf(__uint_as_float(s[c][b * 16 + i + 1]), f, z));
+                                    if (masked) {
+                                        x = mask >> (b * 16 + i) & 1 ? x : 0.0f;
+                                        y = mask >> (b * 16 + i + 1) & 1 ? y : 0.0f;
+                                    }
+                                    sum[0] += x;
+                                    sum[1] += y;
+                                    ph[b * 8 + i / 2] = pack_f16(x, y);
+                                    if constexpr (SPLIT) {
+                                        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&ph[b * 8 + i / 2]));
+                                        pl[b * 8 + i / 2] = pack_f16(x - h.x, y - h.y);
+                                    }
+                                }
+                                l = fmaf(sum[0] + sum[1], b ? is.y : is.x, l);
                             }
-                            sum[0] += x;
-                            sum[1] += y;
-                            ph[b * 8 + i / 2] = pack_f16(x, y);
-                            if constexpr (SPLIT) {
-                                const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&ph[b * 8 + i / 2]));
-                                pl[b * 8 + i / 2] = pack_f16(x - h.x, y - h.y);
-                            }
+                            tmem_st16(ts + (c0 + c) * 32, ph);
+                            if constexpr (SPLIT) tmem_st16(ts + (c0 + c) * 32 + 16, pl);
                         }
-                        l = fmaf(sum[0] + sum[1], s_isv[rr][c * 2 + b], l);
                     }
-                    tmem_st16(ts + c * 32, ph);
-                    if constexpr (SPLIT) tmem_st16(ts + c * 32 + 16, pl);
-                }
+                };
+                if (whole) weights(std::false_type{});
+                else weights(std::true_type{});
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
