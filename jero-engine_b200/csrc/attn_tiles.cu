@@ -34,6 +34,7 @@ constexpr int kThreads = 16 * 32;    // whole warpgroups: three warps beside the
 // Registers a thread after the split: 2 x 152 + 2 x 104 = 4 x the launch's 128.
 constexpr int kSoftRegs = 152, kOtherRegs = 104;
 constexpr float kNoScaleLog2 = -80.0f;
+constexpr int kCubic = 4;            // one pair of weights in this many takes the cubic
 constexpr float kLazy = 8.0f;        // growth of a row's maximum (log2) that its sums are left unscaled for
 
 __device__ __forceinline__ float ex2(float x)
@@ -71,6 +72,54 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b)
 {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Two f32 at a time.
+using f32x2 = uint64_t;
+__device__ __forceinline__ f32x2 pair(float a, float b)
+{
+    f32x2 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 unpair(f32x2 a)
+{
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(a));
+    return v;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c)
+{
+    f32x2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
+{
+    f32x2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// 2^x of a pair on the multiply-add pipes, which have room where the
+// exponential's own is full: x = n + f with n its nearest integer (the low bits
+// of x + 1.5 * 2^23), and a cubic for 2^f on [-1/2, 1/2] with the smallest
+// largest relative error, 7.5e-5 (2^-13.7), below the 2^-12 that the weights'
+// rounding to f16 brings.
+__device__ __forceinline__ float2 ex2_cubic(f32x2 x)
+{
+    float2 v = unpair(x);
+    v.x = fmaxf(v.x, -126.0f);
+    v.y = fmaxf(v.y, -126.0f);
+    x = pair(v.x, v.y);
+    const f32x2 t = add2(x, pair(12582912.0f, 12582912.0f));
+    const f32x2 f = fma2(add2(t, pair(-12582912.0f, -12582912.0f)), pair(-1.0f, -1.0f), x);
+    f32x2 y = fma2(f, pair(0.0551716685f, 0.0551716685f), pair(0.2426111251f, 0.2426111251f));
+    y = fma2(y, f, pair(0.6932609677f, 0.6932609677f));
+    y = fma2(y, f, pair(0.9999280572f, 0.9999280572f));
+    const float2 n = unpair(t), z = unpair(y);
+    return make_float2(__int_as_float(__float_as_int(z.x) + (__float_as_int(n.x) << 23)),
+                       __int_as_float(__float_as_int(z.y) + (__float_as_int(n.y) << 23)));
 }
 
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -312,9 +361,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint8_t *dst = sm_k + buf * Sh::kOperand + slab * (kKv * 128) + tok * 128;
                     const uint32_t src = smem_addr(sm_st) + ct * 16, x = smem_addr(dst) + ((c ^ (tok & 7)) * 16),
                                    y = smem_addr(dst) + (((c + 1) ^ (tok & 7)) * 16);
+                    uint4 in[8 * D / 128];
+#pragma unroll
+                    for (int i = 0; i < 8 * D / 128; i++) in[i] = lds128(src + i * 2048);
 #pragma unroll
                     for (int i = 0; i < 8 * D / 128; i++) {
-                        const uint4 w = lds128(src + i * 2048);
+                        const uint4 w = in[i];
                         uint4 a, b;
                         bytes_f16(w.x, a.x, a.y);
                         bytes_f16(w.y, a.z, a.w);
@@ -336,9 +388,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int d = ct % D, sub = ct / D;
                     uint8_t *dst = sm_v + buf * Sh::kOperand + d * 128;
                     const uint32_t src = smem_addr(sm_st + Sh::kStage) + ct * 16, base = smem_addr(dst);
+                    uint4 in[8 * D / 128];
+#pragma unroll
+                    for (int i = 0; i < 8 * D / 128; i++) in[i] = lds128(src + i * 2048);
 #pragma unroll
                     for (int i = 0; i < 8 * D / 128; i++) {
-                        const uint4 w = lds128(src + i * 2048);
+                        const uint4 w = in[i];
                         uint4 a, b;
                         bytes_f16(w.x, a.x, a.y);
                         bytes_f16(w.y, a.z, a.w);
@@ -477,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = warp_wait(&s_full[w], turns & 1, abort_flag, p.err))) break;
                 tc_fence_after();
                 const int rr = done & 3, tok0 = (it.tile0 + t) * kKv;
-                const int hi = pos - tok0, lo = p.window ? pos - p.window - tok0 : INT_MIN;   // seen: lo < column <= hi
+                const int hi = pos - tok0, lo = p.window ? max(-1, pos - p.window - tok0) : -1;   // seen: lo < column <= hi
                 const uint32_t okm = s_ok[rr];
                 const bool whole = __all_sync(0xffffffffu, hi >= kKv - 1 && (!live || lo < 0)) && okm == 0xFFu;
                 // bit i: column 32 c + i is seen
@@ -488,37 +543,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t ok2 = okm >> (2 * c);
                     return mask & ((ok2 & 1 ? 0xFFFFu : 0u) | (ok2 & 2 ? 0xFFFF0000u : 0u));
                 };
-                // ---- the row's maximum, over two quarters of the tile at a time
+                // The tile's logits by halves, in two quarters. (Rolled: unrolled, the two
+                // passes outgrow the instruction caches.)
+                auto quarters = [&](auto &&take) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; c += 2) {
+                        uint32_t x[32], y[32];
+                        tmem_ld32(ts + c * 32, x);
+                        tmem_ld32(ts + c * 32 + 32, y);
+                        tmem_ld_wait();
+                        take(c, x);
+                        take(c + 1, y);
+                    }
+                };
+                // ---- the row's maximum
                 float top = -INFINITY;
                 auto maxima = [&](auto kind) {
-                    constexpr bool masked = decltype(kind)::value;
+                    quarters([&](int c, uint32_t (&s)[32]) {
+                        constexpr bool masked = decltype(kind)::value;
+                        const uint32_t mask = masked ? seen(c) : ~0u;
+                        const float2 sk = *reinterpret_cast<const float2 *>(&s_sk[rr][c * 2]);
+                        const float2 ls = *reinterpret_cast<const float2 *>(&s_lsv[rr][c * 2]);
 #pragma unroll
-                    for (int c0 = 0; c0 < 4; c0 += 2) {
-                        uint32_t s[2][32];
-                        tmem_ld32(ts + c0 * 32, s[0]);
-                        tmem_ld32(ts + c0 * 32 + 32, s[1]);
-                        tmem_ld_wait();
+                        for (int b = 0; b < 2; b++) {
+                            float x[4];
 #pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            const uint32_t mask = masked ? seen(c0 + c) : ~0u;
-                            const float2 sk = *reinterpret_cast<const float2 *>(&s_sk[rr][(c0 + c) * 2]);
-                            const float2 ls = *reinterpret_cast<const float2 *>(&s_lsv[rr][(c0 + c) * 2]);
-#pragma unroll
-                            for (int b = 0; b < 2; b++) {
-                                float x[4];
-#pragma unroll
-                                for (int i = 0; i < 16; i++) {
-                                    float v = __uint_as_float(s[c][b * 16 + i]);
-                                    if (masked) v = mask >> (b * 16 + i) & 1 ? v : -INFINITY;
-                                    x[i % 4] = i < 4 ? v : fmaxf(x[i % 4], v);
-                                }
-                                const float y = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                                const float u = fmaf(y, rf * (b ? sk.y : sk.x), b ? ls.y : ls.x);
-                                // (a block unseen stays at -inf whatever its factor)
-                                top = fmaxf(top, masked && y == -INFINITY ? -INFINITY : u);
+                            for (int i = 0; i < 16; i++) {
+                                float v = __uint_as_float(s[b * 16 + i]);
+                                if (masked) v = mask >> (b * 16 + i) & 1 ? v : -INFINITY;
+                                x[i % 4] = i < 4 ? v : fmaxf(x[i % 4], v);
                             }
+                            const float y = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                            const float u = fmaf(y, rf * (b ? sk.y : sk.x), b ? ls.y : ls.x);
+                            // (a block unseen stays at -inf whatever its factor)
+                            top = fmaxf(top, masked && y == -INFINITY ? -INFINITY : u);
                         }
-                    }
+                    });
                 };
                 if (whole) maxima(std::false_type{});
                 else maxima(std::true_type{});
@@ -528,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (grow) m = top;
                     l *= a;
                     if (t > 0) {
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D / 32; c++) {
                             uint32_t o[32];
                             tmem_ld32(to + c * 32, o);
@@ -543,47 +603,41 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // ---- the weights, over the logits they come from
                 const float ms = m == -INFINITY ? 0.0f : m;
                 auto weights = [&](auto kind) {
-                    constexpr bool masked = decltype(kind)::value;
+                    quarters([&](int c, uint32_t (&s)[32]) {
+                        constexpr bool masked = decltype(kind)::value;
+                        uint32_t hi16[16];
+                        [[maybe_unused]] uint32_t lo16[16];
+                        const uint32_t mask = masked ? seen(c) : ~0u;
+                        const float2 sk = *reinterpret_cast<const float2 *>(&s_sk[rr][c * 2]);
+                        const float2 ls = *reinterpret_cast<const float2 *>(&s_lsv[rr][c * 2]);
+                        const float2 is = *reinterpret_cast<const float2 *>(&s_isv[rr][c * 2]);
 #pragma unroll
-                    for (int c0 = 0; c0 < 4; c0 += 2) {
-                        uint32_t s[2][32];
-                        tmem_ld32(ts + c0 * 32, s[0]);
-                        tmem_ld32(ts + c0 * 32 + 32, s[1]);
-                        tmem_ld_wait();
+                        for (int b = 0; b < 2; b++) {
+                            const float f = rf * (b ? sk.y : sk.x), z = (b ? ls.y : ls.x) - ms;
+                            const f32x2 f2 = pair(f, f), z2 = pair(z, z);
+                            f32x2 add = pair(0.0f, 0.0f);
 #pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            uint32_t ph[16];
-                            [[maybe_unused]] uint32_t pl[16];
-                            const uint32_t mask = masked ? seen(c0 + c) : ~0u;
-                            const float2 sk = *reinterpret_cast<const float2 *>(&s_sk[rr][(c0 + c) * 2]);
-                            const float2 ls = *reinterpret_cast<const float2 *>(&s_lsv[rr][(c0 + c) * 2]);
-                            const float2 is = *reinterpret_cast<const float2 *>(&s_isv[rr][(c0 + c) * 2]);
-#pragma unroll
-                            for (int b = 0; b < 2; b++) {
-                                const float f = rf * (b ? sk.y : sk.x), z = (b ? ls.y : ls.x) - ms;
-                                float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-                                for (int i = 0; i < 16; i += 2) {
-                                    float x = ex2(fmaf(__uint_as_float(s[c][b * 16 + i]), f, z));
-                                    float y = ex2(fmaf(__uint_as_float(s[c][b * 16 + i + 1]), f, z));
-                                    if (masked) {
-                                        x = mask >> (b * 16 + i) & 1 ? x : 0.0f;
-                                        y = mask >> (b * 16 + i + 1) & 1 ? y : 0.0f;
-                                    }
-                                    sum[0] += x;
-                                    sum[1] += y;
-                                    ph[b * 8 + i / 2] = pack_f16(x, y);
-                                    if constexpr (SPLIT) {
-                                        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&ph[b * 8 + i / 2]));
-                                        pl[b * 8 + i / 2] = pack_f16(x - h.x, y - h.y);
-                                    }
+                            for (int i = 0; i < 16; i += 2) {
+                                const f32x2 u = fma2(pair(__uint_as_float(s[b * 16 + i]), __uint_as_float(s[b * 16 + i + 1])), f2, z2);
+                                float2 e;
+                                if (!SPLIT && i / 2 % kCubic == kCubic - 1) e = ex2_cubic(u);
+                                else e = make_float2(ex2(unpair(u).x), ex2(unpair(u).y));
+                                if (masked) {
+                                    e.x = mask >> (b * 16 + i) & 1 ? e.x : 0.0f;
+                                    e.y = mask >> (b * 16 + i + 1) & 1 ? e.y : 0.0f;
                                 }
-                                l = fmaf(sum[0] + sum[1], b ? is.y : is.x, l);
+                                add = add2(add, pair(e.x, e.y));
+                                hi16[b * 8 + i / 2] = pack_f16(e.x, e.y);
+                                if constexpr (SPLIT) {
+                                    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi16[b * 8 + i / 2]));
+                                    lo16[b * 8 + i / 2] = pack_f16(e.x - h.x, e.y - h.y);
+                                }
                             }
-                            tmem_st16(ts + (c0 + c) * 32, ph);
-                            if constexpr (SPLIT) tmem_st16(ts + (c0 + c) * 32 + 16, pl);
+                            l = fmaf(unpair(add).x + unpair(add).y, b ? is.y : is.x, l);
                         }
-                    }
+                        tmem_st16(ts + c * 32, hi16);
+                        if constexpr (SPLIT) tmem_st16(ts + c * 32 + 16, lo16);
+                    });
                 };
                 if (whole) weights(std::false_type{});
                 else weights(std::true_type{});
