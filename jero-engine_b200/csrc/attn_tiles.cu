@@ -5,10 +5,14 @@
 // Per 128 cached tokens: four conversion warps turn the cache's bytes into f16
 // operands in shared memory (exact; K-major, 128-byte swizzle: a value block
 // lies as [D][16 tokens] in the cache, so neither keys nor values are
-// transposed), one thread issues S = Q K^T (tcgen05.mma, M 128, N 128) and
+// transposed), one thread issues S = Q K^T (tcgen05.mma, M 128, N 64) and
 // O += P V (N = D, the weights P read from TMEM), and a warpgroup for each row
-// tile does its softmax: a thread holds a row. TMEM: S0, S1 (128 columns each,
-// P over S once S has been read) and O0, O1 (D columns each).
+// tile does its softmax: a thread holds a row. TMEM: for each row tile S in two
+// halves of 64 tokens (P over S once S has been read) and O (D columns). While
+// a warpgroup weighs one half, the tensor cores add the other half's weights
+// and refill it: with one S of 128 columns a row tile the two waited for one
+// another, and the same work took 561 us instead of @@ (4096 rows of 32 heads
+// over 4096 + 4096 tokens, bf16).
 //
 // The sums O are scaled down only when a row's maximum has grown by more than
 // 2^8 since they were last: the weights then reach 2^8 instead of 1, which f16
@@ -28,7 +32,7 @@
 namespace jmoe {
 namespace {
 
-constexpr int kRowsTile = 128, kRowsItem = 256, kKv = 128;
+constexpr int kRowsTile = 128, kRowsItem = 256, kKv = 128, kHalf = 64;
 constexpr int kSoftWarps = 8, kConvWarps = 4, kMmaWarp = kSoftWarps + kConvWarps;
 constexpr int kThreads = 16 * 32;    // whole warpgroups: three warps beside the product warp only lend registers
 // Registers a thread after the split: 2 x 152 + 2 x 104 = 4 x the launch's 128.
@@ -120,6 +124,38 @@ __device__ __forceinline__ float2 ex2_cubic(f32x2 x)
     const float2 n = unpair(t), z = unpair(y);
     return make_float2(__int_as_float(__float_as_int(z.x) + (__float_as_int(n.x) << 23)),
                        __int_as_float(__float_as_int(z.y) + (__float_as_int(n.y) << 23)));
+}
+
+// tcgen05.mma and commit by one lane of a converged warp: with everything
+// around them uniform the descriptors stay in uniform registers (issued under
+// "if (lane == 0)" each product took 70 to 100 cycles to issue).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0)
+        : "memory");
+}
+__device__ __forceinline__ void commit_one(uint64_t *bar)
+{
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
+        : "memory");
 }
 
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -246,8 +282,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     using Sh = TileShape<D, SPLIT>;
     constexpr int NB = Sh::kBufs, SL = Sh::kSlabs;
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ __align__(8) uint64_t q_full, q_free, k_full[NB], k_empty[NB], v_full[NB], v_empty[NB], st_full[2], s_full[2],
-        p_full[2], o_done[2], drained;
+    __shared__ __align__(8) uint64_t q_full[2], q_free[2], k_full[NB], k_empty[NB], v_full[NB], v_empty[NB], st_full[2], s_full[2][2],
+        p_full[2][2], o_sum[2], o_done[2], drained[2];
     __shared__ __align__(16) float s_sk[4][8], s_lsv[4][8], s_isv[4][8];
     __shared__ uint32_t s_ok[4];
     __shared__ uint32_t s_tmem;
@@ -257,20 +293,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int g = p.rows.q_heads / p.c.heads;
 
     if (tid == 0) {
-        mbar_init(&q_full, 1);
-        mbar_init(&q_free, 1);
-        mbar_init(&drained, 1);
         for (int i = 0; i < NB; i++) {
             mbar_init(&k_full[i], kConvWarps);
             mbar_init(&v_full[i], kConvWarps);
-            mbar_init(&k_empty[i], 1);
-            mbar_init(&v_empty[i], 1);
+            mbar_init(&k_empty[i], 2);
+            mbar_init(&v_empty[i], 2);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&st_full[i], 1);
-            mbar_init(&s_full[i], 2);      // the products' end, and what the product thread has seen
-            mbar_init(&p_full[i], 4);
+            for (int h = 0; h < 2; h++) {
+                mbar_init(&s_full[i][h], 2);      // the products' end, and what the product thread has seen
+                mbar_init(&p_full[i][h], 4);
+            }
+            mbar_init(&o_sum[i], 1);
             mbar_init(&o_done[i], 1);
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_free[i], 1);
+            mbar_init(&drained[i], 1);
         }
         s_abort = 0;
         fence_barrier_init();
@@ -419,94 +458,99 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (staged) drain_wait(&st_full[w], (staged - 1) & 1);
     } else if (warp >= kMmaWarp) {
         regs_down<kOtherRegs>();
-        if (warp == kMmaWarp) {
-            // ============ products
+        if (warp < kMmaWarp + 2) {
+            // ============ products: a warp for each row tile
             fence_proxy_async_global();       // the queries as the kernel before left them
-            const uint32_t id_s = (1u << 4) | ((uint32_t)(kKv >> 3) << 17) | ((uint32_t)(kRowsTile >> 4) << 24);
+            const int i = warp - kMmaWarp;
+            const uint32_t id_s = (1u << 4) | ((uint32_t)(kHalf >> 3) << 17) | ((uint32_t)(kRowsTile >> 4) << 24);
             const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kRowsTile >> 4) << 24);
-            const uint64_t dq = umma_desc_sw128(smem_addr(sm_q)), dk = umma_desc_sw128(smem_addr(sm_k)), dv = umma_desc_sw128(smem_addr(sm_v));
-            uint32_t done = 0, items = 0, turns[2] = {0, 0};     // tiles and items of the CTA, tiles of each row tile
+            const uint64_t dq = umma_desc_sw128(smem_addr(sm_q + i * Sh::kQTile)), dk = umma_desc_sw128(smem_addr(sm_k)),
+                           dv = umma_desc_sw128(smem_addr(sm_v));
+            const uint32_t ts = tmem + i * kKv, to = tmem + 2 * kKv + i * D;
+            // S of half h from the keys in buffer buf
+            auto scores = [&](int h, int buf) {
+                if (lane == 0) mbar_arrive(&s_full[i][h]);      // with the scales that the keys came with
+                const uint64_t b = dk + ((buf * Sh::kOperand + h * kHalf * 128) >> 4);
+#pragma unroll
+                for (int half = 0; half < (SPLIT ? 2 : 1); half++)
+#pragma unroll
+                    for (int s = 0; s < SL; s++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            mma_ss(ts + h * kHalf, dq + ((half * SL + s) * kRowsTile * 128 >> 4) + 2 * k, b + (s * kKv * 128 >> 4) + 2 * k,
+                                   id_s, half + s + k != 0);
+                commit_one(&s_full[i][h]);
+            };
+            // O: the weights of half h times the values in buffer buf
+            auto sums = [&](int h, int buf, uint32_t acc) {
+                const uint64_t b = dv + ((buf * Sh::kOperand + h * D * 128) >> 4);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int half = 0; half < (SPLIT ? 2 : 1); half++)
+                        mma_ts(to, ts + h * kHalf + k / 2 * 32 + k % 2 * 8 + half * 16, b + 2 * k, id_o, half + k != 0 ? 1u : acc);
+                commit_one(&o_sum[i]);
+            };
+            uint32_t done = 0, items = 0, turns = 0;     // tiles of the CTA, items and tiles of this row tile
             bool ok = true, loading = false;
+            auto wait = [&](uint64_t *bar, uint32_t phase) -> bool { return ok = warp_wait(bar, phase & 1, abort_flag, p.err); };
             for (int j = 0, have; ok && (have = item(j)) >= 0; j++) {
                 if (!have) continue;
-                if (lane == 0) {
-                    const int mt = it.rows > kRowsTile ? 2 : 1;
-                    auto scores = [&](int i, int buf) {
-                        uint32_t acc = 0;
-                        mbar_arrive(&s_full[i]);      // with the scales that the keys came with
-#pragma unroll
-                        for (int half = 0; half < (SPLIT ? 2 : 1); half++)
-#pragma unroll
-                            for (int s = 0; s < SL; s++)
-#pragma unroll
-                                for (int k = 0; k < 4; k++) {
-                                    tc_mma_f16(tmem + i * kKv, dq + ((i * Sh::kQTile + (half * SL + s) * kRowsTile * 128) >> 4) + 2 * k,
-                                               dk + ((buf * Sh::kOperand + s * kKv * 128) >> 4) + 2 * k, id_s, acc);
-                                    acc = 1;
-                                }
-                        tc_commit(&s_full[i]);
-                    };
-                    auto sums = [&](int i, int buf, uint32_t acc) {
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-#pragma unroll
-                            for (int half = 0; half < (SPLIT ? 2 : 1); half++) {
-                                tc_mma_f16_ts(tmem + 2 * kKv + i * D, tmem + i * kKv + k / 2 * 32 + k % 2 * 8 + half * 16,
-                                              dv + ((buf * Sh::kOperand + k / 4 * D * 128) >> 4) + 2 * (k % 4), id_o, acc);
-                                acc = 1;
-                            }
-                    };
-                    do {
-                        if (items && !(ok = tc_spin_wait(&q_free, (items - 1) & 1, abort_flag, p.err))) break;
-                        mbar_arrive_expect_tx(&q_full, mt * Sh::kQTile);
-                        bulk_load(smem_addr(sm_q), images + (int64_t)image * Sh::kImage, mt * Sh::kQTile, &q_full);
-                        loading = true;
-                        if (!(ok = tc_spin_wait(&q_full, items & 1, abort_flag, p.err))) break;
-                        loading = false;
-                        if (!(ok = tc_spin_wait(&k_full[done % NB], (done / NB) & 1, abort_flag, p.err))) break;
-                        tc_fence_after();
-                        for (int i = 0; i < mt; i++) scores(i, done % NB);
-                        tc_commit(&k_empty[done % NB]);
-                        if (it.tiles == 1) tc_commit(&q_free);
-                        for (int t = 0; t < it.tiles; t++, done++) {
-                            const bool last = t + 1 == it.tiles;
-                            const int buf = done % NB, nbuf = (done + 1) % NB;
-                            if (!(ok = tc_spin_wait(&v_full[buf], (done / NB) & 1, abort_flag, p.err))) break;
-                            for (int i = 0; i < mt; i++) {
-                                const uint32_t turn = i ? turns[1]++ : turns[0]++;
-                                if (!(ok = tc_spin_wait(&p_full[i], turn & 1, abort_flag, p.err))) break;
-                                tc_fence_after();
-                                sums(i, buf, t > 0);
-                                if (i == mt - 1) tc_commit(&v_empty[buf]);
-                                if (last) {
-                                    tc_commit(&o_done[i]);
-                                    continue;
-                                }
-                                if (i == 0) {
-                                    if (!(ok = tc_spin_wait(&k_full[nbuf], ((done + 1) / NB) & 1, abort_flag, p.err))) break;
-                                    tc_fence_after();
-                                }
-                                // (issued behind the product that reads the weights it overwrites: one
-                                // thread's tcgen05.mma run in the order of their issue)
-                                scores(i, nbuf);
-                                if (i == mt - 1) {
-                                    tc_commit(&k_empty[nbuf]);
-                                    if (t + 2 == it.tiles) tc_commit(&q_free);
-                                }
-                            }
-                            if (!ok) break;
-                        }
-                        items++;
-                    } while (0);
+                if (it.rows <= i * kRowsTile) {       // nothing here: the buffers pass by
+                    for (int t = 0; t < it.tiles; t++, done++) {
+                        if (!wait(&k_full[done % NB], done / NB)) break;
+                        if (lane == 0) mbar_arrive(&k_empty[done % NB]);
+                        if (!wait(&v_full[done % NB], done / NB)) break;
+                        if (lane == 0) mbar_arrive(&v_empty[done % NB]);
+                    }
+                    continue;
                 }
-                ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-                done = __shfl_sync(0xffffffffu, done, 0);
-                items = __shfl_sync(0xffffffffu, items, 0);
+                if (items && !wait(&q_free[i], items - 1)) break;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&q_full[i], Sh::kQTile);
+                    bulk_load(smem_addr(sm_q + i * Sh::kQTile), images + (int64_t)image * Sh::kImage + i * Sh::kQTile, Sh::kQTile, &q_full[i]);
+                }
+                loading = true;
+                if (!wait(&q_full[i], items)) break;
+                loading = false;
+                if (!wait(&k_full[done % NB], done / NB)) break;
+                tc_fence_after();
+                scores(0, done % NB);
+                scores(1, done % NB);
+                commit_one(&k_empty[done % NB]);
+                if (it.tiles == 1) commit_one(&q_free[i]);
+                for (int t = 0; t < it.tiles; t++, done++, turns++) {
+                    const bool last = t + 1 == it.tiles;
+                    const int buf = done % NB, nbuf = (done + 1) % NB;
+                    if (!wait(&v_full[buf], done / NB)) break;
+#pragma unroll 1
+                    for (int h = 0; h < 2; h++) {
+                        if (!wait(&p_full[i][h], turns)) break;
+                        tc_fence_after();
+                        sums(h, buf, t > 0 || h > 0);
+                        if (h) commit_one(&v_empty[buf]);
+                        if (last) continue;
+                        if (h == 0) {
+                            if (!wait(&k_full[nbuf], (done + 1) / NB)) break;
+                            tc_fence_after();
+                        }
+                        // (issued behind the product that reads the weights it overwrites: one
+                        // thread's tcgen05.mma run in the order of their issue)
+                        scores(h, nbuf);
+                        if (h) {
+                            commit_one(&k_empty[nbuf]);
+                            if (t + 2 == it.tiles) commit_one(&q_free[i]);
+                        }
+                    }
+                    if (!ok) break;
+                    if (last) commit_one(&o_done[i]);
+                }
+                items++;
             }
-            if (lane == 0 && !ok) {
-                if (loading) drain_wait(&q_full, items & 1);
-                tc_commit(&drained);
-                drain_wait(&drained, 0);
+            if (!ok) {
+                if (loading) drain_wait(&q_full[i], items & 1);
+                commit_one(&drained[i]);
+                drain_wait(&drained[i], 0);
             }
             __syncwarp();
         }
@@ -528,66 +572,59 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int pos = live ? it.q.past + tok : INT_MAX;
             const float rf = live ? __ldg(factors + (int64_t)image * kRowsItem + r) : 0.0f;
             float m = -INFINITY, l = 0.0f;
-            for (int t = 0; t < it.tiles; t++, done++, turns++) {
-                if (!(ok = warp_wait(&s_full[w], turns & 1, abort_flag, p.err))) break;
+            for (int u = 0; u < 2 * it.tiles; u++) {
+                // ---- half u & 1 of tile u / 2
+                const int h = u & 1, rr = done & 3, tok0 = (it.tile0 + u / 2) * kKv + h * kHalf;
+                if (!(ok = warp_wait(&s_full[w][h], turns & 1, abort_flag, p.err))) break;
                 tc_fence_after();
-                const int rr = done & 3, tok0 = (it.tile0 + t) * kKv;
+                uint32_t s[kHalf];
+                tmem_ld32(ts + h * kHalf, reinterpret_cast<uint32_t (&)[32]>(s[0]));
+                tmem_ld32(ts + h * kHalf + 32, reinterpret_cast<uint32_t (&)[32]>(s[32]));
+                // factors and offsets of the half's four blocks
+                const float4 sk = *reinterpret_cast<const float4 *>(&s_sk[rr][4 * h]), ls = *reinterpret_cast<const float4 *>(&s_lsv[rr][4 * h]),
+                             is = *reinterpret_cast<const float4 *>(&s_isv[rr][4 * h]);
+                const float f[4] = {rf * sk.x, rf * sk.y, rf * sk.z, rf * sk.w}, off[4] = {ls.x, ls.y, ls.z, ls.w},
+                            isv[4] = {is.x, is.y, is.z, is.w};
                 const int hi = pos - tok0, lo = p.window ? max(-1, pos - p.window - tok0) : -1;   // seen: lo < column <= hi
-                const uint32_t okm = s_ok[rr];
-                const bool whole = __all_sync(0xffffffffu, hi >= kKv - 1 && (!live || lo < 0)) && okm == 0xFFu;
-                // bit i: column 32 c + i is seen
-                auto seen = [&](int c) -> uint32_t {
-                    const int up = hi - 32 * c, down = lo - 32 * c;
-                    uint32_t mask = up < 0 ? 0u : up >= 31 ? ~0u : (2u << up) - 1;
-                    if (down >= 0) mask &= down >= 31 ? 0u : ~((2u << down) - 1);
-                    const uint32_t ok2 = okm >> (2 * c);
-                    return mask & ((ok2 & 1 ? 0xFFFFu : 0u) | (ok2 & 2 ? 0xFFFF0000u : 0u));
-                };
-                // The tile's logits by halves, in two quarters. (Rolled: unrolled, the two
-                // passes outgrow the instruction caches.)
-                auto quarters = [&](auto &&take) {
-#pragma unroll 1
-                    for (int c = 0; c < 4; c += 2) {
-                        uint32_t x[32], y[32];
-                        tmem_ld32(ts + c * 32, x);
-                        tmem_ld32(ts + c * 32 + 32, y);
-                        tmem_ld_wait();
-                        take(c, x);
-                        take(c + 1, y);
+                const uint32_t okm = s_ok[rr] >> (4 * h) & 0xFu;
+                const bool whole = __all_sync(0xffffffffu, hi >= kHalf - 1 && (!live || lo < 0)) && okm == 0xFu;
+                tmem_ld_wait();
+                if (!whole) {
+                    // unseen columns to -inf (the other values are finite: cache bytes times f16)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const int up = hi - 32 * c, down = lo - 32 * c;
+                        uint32_t mask = up < 0 ? 0u : up >= 31 ? ~0u : (2u << up) - 1;
+                        if (down >= 0) mask &= down >= 31 ? 0u : ~((2u << down) - 1);
+                        mask &= (okm >> (2 * c) & 1 ? 0xFFFFu : 0u) | (okm >> (2 * c) & 2 ? 0xFFFF0000u : 0u);
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (!(mask >> i & 1)) s[32 * c + i] = 0xFF800000u;
                     }
-                };
+                }
                 // ---- the row's maximum
                 float top = -INFINITY;
-                auto maxima = [&](auto kind) {
-                    quarters([&](int c, uint32_t (&s)[32]) {
-                        constexpr bool masked = decltype(kind)::value;
-                        const uint32_t mask = masked ? seen(c) : ~0u;
-                        const float2 sk = *reinterpret_cast<const float2 *>(&s_sk[rr][c * 2]);
-                        const float2 ls = *reinterpret_cast<const float2 *>(&s_lsv[rr][c * 2]);
 #pragma unroll
-                        for (int b = 0; b < 2; b++) {
-                            float x[4];
+                for (int b = 0; b < 4; b++) {
+                    float x[4];
 #pragma unroll
-                            for (int i = 0; i < 16; i++) {
-                                float v = __uint_as_float(s[b * 16 + i]);
-                                if (masked) v = mask >> (b * 16 + i) & 1 ? v : -INFINITY;
-                                x[i % 4] = i < 4 ? v : fmaxf(x[i % 4], v);
-                            }
-                            const float y = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                            const float u = fmaf(y, rf * (b ? sk.y : sk.x), b ? ls.y : ls.x);
-                            // (a block unseen stays at -inf whatever its factor)
-                            top = fmaxf(top, masked && y == -INFINITY ? -INFINITY : u);
-                        }
-                    });
-                };
-                if (whole) maxima(std::false_type{});
-                else maxima(std::true_type{});
+                    for (int i = 0; i < 16; i++) {
+                        const float v = __uint_as_float(s[b * 16 + i]);
+                        x[i % 4] = i < 4 ? v : fmaxf(x[i % 4], v);
+                    }
+                    const float y = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                    top = fmaxf(top, y == -INFINITY ? -INFINITY : fmaf(y, f[b], off[b]));     // (0 * -inf)
+                }
                 const bool grow = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float a = grow ? ex2(m - top) : 1.0f;
                     if (grow) m = top;
                     l *= a;
-                    if (t > 0) {
+                    if (u > 0) {
+                        // the sums so far, the other half's product among them (the one before
+                        // that is done: these logits came after it)
+                        if (!(ok = warp_wait(&o_sum[w], (2 * turns + h - 1) & 1, abort_flag, p.err))) break;
+                        tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < D / 32; c++) {
                             uint32_t o[32];
@@ -602,49 +639,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 // ---- the weights, over the logits they come from
                 const float ms = m == -INFINITY ? 0.0f : m;
-                auto weights = [&](auto kind) {
-                    quarters([&](int c, uint32_t (&s)[32]) {
-                        constexpr bool masked = decltype(kind)::value;
-                        uint32_t hi16[16];
-                        [[maybe_unused]] uint32_t lo16[16];
-                        const uint32_t mask = masked ? seen(c) : ~0u;
-                        const float2 sk = *reinterpret_cast<const float2 *>(&s_sk[rr][c * 2]);
-                        const float2 ls = *reinterpret_cast<const float2 *>(&s_lsv[rr][c * 2]);
-                        const float2 is = *reinterpret_cast<const float2 *>(&s_isv[rr][c * 2]);
 #pragma unroll
-                        for (int b = 0; b < 2; b++) {
-                            const float f = rf * (b ? sk.y : sk.x), z = (b ? ls.y : ls.x) - ms;
-                            const f32x2 f2 = pair(f, f), z2 = pair(z, z);
-                            f32x2 add = pair(0.0f, 0.0f);
+                for (int c = 0; c < 2; c++) {
+                    uint32_t hi16[16];
+                    [[maybe_unused]] uint32_t lo16[16];
 #pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                const f32x2 u = fma2(pair(__uint_as_float(s[b * 16 + i]), __uint_as_float(s[b * 16 + i + 1])), f2, z2);
-                                float2 e;
-                                if (!SPLIT && i / 2 % kCubic == kCubic - 1) e = ex2_cubic(u);
-                                else e = make_float2(ex2(unpair(u).x), ex2(unpair(u).y));
-                                if (masked) {
-                                    e.x = mask >> (b * 16 + i) & 1 ? e.x : 0.0f;
-                                    e.y = mask >> (b * 16 + i + 1) & 1 ? e.y : 0.0f;
-                                }
-                                add = add2(add, pair(e.x, e.y));
-                                hi16[b * 8 + i / 2] = pack_f16(e.x, e.y);
-                                if constexpr (SPLIT) {
-                                    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi16[b * 8 + i / 2]));
-                                    lo16[b * 8 + i / 2] = pack_f16(e.x - h.x, e.y - h.y);
-                                }
+                    for (int b = 0; b < 2; b++) {
+                        const float ff = whole ? f[2 * c + b] : fmaxf(f[2 * c + b], 1e-30f), z = off[2 * c + b] - ms;    // (0 * -inf)
+                        const f32x2 f2 = pair(ff, ff), z2 = pair(z, z);
+                        f32x2 add = pair(0.0f, 0.0f);
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            const int k = c * 32 + b * 16 + i;
+                            const f32x2 x = fma2(pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), f2, z2);
+                            float2 e;
+                            if (!SPLIT && i / 2 % kCubic == kCubic - 1) e = ex2_cubic(x);
+                            else e = make_float2(ex2(unpair(x).x), ex2(unpair(x).y));
+                            add = add2(add, pair(e.x, e.y));
+                            hi16[b * 8 + i / 2] = pack_f16(e.x, e.y);
+                            if constexpr (SPLIT) {
+                                const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&hi16[b * 8 + i / 2]));
+                                lo16[b * 8 + i / 2] = pack_f16(e.x - q.x, e.y - q.y);
                             }
-                            l = fmaf(unpair(add).x + unpair(add).y, b ? is.y : is.x, l);
                         }
-                        tmem_st16(ts + c * 32, hi16);
-                        if constexpr (SPLIT) tmem_st16(ts + c * 32 + 16, lo16);
-                    });
-                };
-                if (whole) weights(std::false_type{});
-                else weights(std::true_type{});
+                        l = fmaf(unpair(add).x + unpair(add).y, isv[2 * c + b], l);
+                    }
+                    tmem_st16(ts + h * kHalf + c * 32, hi16);
+                    if constexpr (SPLIT) tmem_st16(ts + h * kHalf + c * 32 + 16, lo16);
+                }
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[w]);
+                if (lane == 0) mbar_arrive(&p_full[w][h]);
+                if (h) {
+                    done++;
+                    turns++;
+                }
             }
             if (!ok || !(ok = warp_wait(&o_done[w], items & 1, abort_flag, p.err))) break;
             items++;
