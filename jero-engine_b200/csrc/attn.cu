@@ -375,8 +375,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     auto scales = [&](int64_t i, float &k, float &v) {
         k = v = 0.0f;
         if (i >= 0) {
-            k = __ldg(p.c.k_scale + i);
-            v = __ldg(p.c.v_scale + i);
+            k = ld_plain(p.c.k_scale + i);
+            v = ld_plain(p.c.v_scale + i);
         }
     };
     auto row_ptr = [&](const Segment &sg, int r, int &tok) -> const T * {

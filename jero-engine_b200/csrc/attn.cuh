@@ -25,6 +25,11 @@ __device__ __forceinline__ void from_f32(float &d, float v) { d = v; }
 __device__ __forceinline__ void from_f32(__half &d, float v) { d = __float2half_rn(v); }
 __device__ __forceinline__ void from_f32(__nv_bfloat16 &d, float v) { d = __float2bfloat16_rn(v); }
 
+// Loads of memory that a kernel before this one may have written: this kernel
+// may have been launched while that one ran, so none goes through the read-only path.
+template <typename T>
+__device__ __forceinline__ T ld_plain(const T *p) { return *p; }
+
 // N consecutive values (N * size a multiple of 8 bytes, so aligned) to and from f32.
 template <int N, typename T>
 __device__ __forceinline__ void load_vals(const T *p, float (&v)[N])
@@ -34,9 +39,9 @@ __device__ __forceinline__ void load_vals(const T *p, float (&v)[N])
     alignas(16) T t[N];
 #pragma unroll
     for (int i = 0; i < kBytes / kWord; i++) {
-        if (kWord == 16) reinterpret_cast<uint4 *>(t)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
-        else if (kWord == 8) reinterpret_cast<uint2 *>(t)[i] = __ldg(reinterpret_cast<const uint2 *>(p) + i);
-        else reinterpret_cast<uint32_t *>(t)[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
+        if (kWord == 16) reinterpret_cast<uint4 *>(t)[i] = ld_plain(reinterpret_cast<const uint4 *>(p) + i);
+        else if (kWord == 8) reinterpret_cast<uint2 *>(t)[i] = ld_plain(reinterpret_cast<const uint2 *>(p) + i);
+        else reinterpret_cast<uint32_t *>(t)[i] = ld_plain(reinterpret_cast<const uint32_t *>(p) + i);
     }
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = to_f32(t[i]);
@@ -60,7 +65,7 @@ __device__ __forceinline__ void store_vals(T *p, const float (&v)[N])
 
 __device__ __forceinline__ void kv_error(int *err) { atomicExch(err, kErrKvBounds); }
 
-__device__ __forceinline__ int row_of(const KvBatchDev &b, int s) { return b.row_start ? __ldg(b.row_start + s) : s; }
+__device__ __forceinline__ int row_of(const KvBatchDev &b, int s) { return b.row_start ? ld_plain(b.row_start + s) : s; }
 
 struct SeqInfo {
     int past, row0, n;
@@ -69,7 +74,7 @@ struct SeqInfo {
 // Sequence s of the batch; false where its entries are out of range.
 __device__ __forceinline__ bool seq_info(const KvBatchDev &b, int s, SeqInfo &q)
 {
-    q.past = __ldg(b.past + s);
+    q.past = ld_plain(b.past + s);
     q.row0 = row_of(b, s);
     const int end = row_of(b, s + 1);
     q.n = end - q.row0;
@@ -80,7 +85,7 @@ __device__ __forceinline__ bool seq_info(const KvBatchDev &b, int s, SeqInfo &q)
 // The same against a cache: the slot exists and its table holds the sequence's tokens.
 __device__ __forceinline__ bool seq_in_cache(const KvCacheDev &c, const KvBatchDev &b, int s, const SeqInfo &q, int &slot)
 {
-    slot = b.slot ? __ldg(b.slot + s) : s;
+    slot = b.slot ? ld_plain(b.slot + s) : s;
     return slot >= 0 && slot < c.n_slots &&
            ((int64_t)q.past + q.n + kKvBlock - 1) / kKvBlock <= ((int64_t)c.table_stride << c.page_shift);
 }
@@ -89,7 +94,7 @@ __device__ __forceinline__ bool seq_in_cache(const KvCacheDev &c, const KvBatchD
 // in units of blocks, with the head stride page_blocks; -1 for a bad page id.
 __device__ __forceinline__ int64_t block_index(const KvCacheDev &c, int slot, int blk, int head)
 {
-    const int page = __ldg(c.table + (int64_t)slot * c.table_stride + (blk >> c.page_shift));
+    const int page = ld_plain(c.table + (int64_t)slot * c.table_stride + (blk >> c.page_shift));
     if (page < 0 || page >= c.n_pages) return -1;
     return (((int64_t)page * c.heads + head) << c.page_shift) + (blk & ((1 << c.page_shift) - 1));
 }
@@ -115,7 +120,7 @@ __device__ __forceinline__ int seq_of_row_warp(const KvBatchDev &b, int row, int
 {
     if (!b.row_start) return row < b.B ? row : -1;
     int n = 0;
-    for (int s = lane; s < b.B; s += 32) n += __ldg(b.row_start + s) <= row;
+    for (int s = lane; s < b.B; s += 32) n += ld_plain(b.row_start + s) <= row;
     return __reduce_add_sync(0xffffffffu, n) - 1;
 }
 
@@ -144,7 +149,7 @@ __device__ __forceinline__ void turn_head(float (&v)[D / 32], const float *w, co
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const float inv = 1.0f / sqrtf(ss * (1.0f / D) + (float)r.eps);
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = v[i] * inv * __ldg(w + lane * N + i);
+        for (int i = 0; i < N; i++) v[i] = v[i] * inv * ld_plain(w + lane * N + i);
     }
     if (r.R == 0) return;
     __syncwarp();
@@ -180,7 +185,7 @@ __device__ __forceinline__ void norm_rope_vals(float (&v)[D / 32], const float *
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const float inv = 1.0f / sqrtf(ss * (1.0f / D) + (float)r.eps);
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = v[i] * inv * __ldg(w + lane * N + i);
+        for (int i = 0; i < N; i++) v[i] = v[i] * inv * ld_plain(w + lane * N + i);
     }
     __syncwarp();
 #pragma unroll

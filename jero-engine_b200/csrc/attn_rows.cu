@@ -13,48 +13,59 @@ namespace {
 
 constexpr int kRowWarps = 4;
 
-// Sequence whose rows hold `row` (row_start ascending), or -1.
-__device__ __forceinline__ int seq_of_row(const KvBatchDev &b, int row)
-{
-    int lo = 0, hi = b.B - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (row_of(b, mid) <= row) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
-}
+// Norms and rotation: one CTA per token and group of heads. The token's angles
+// are formed once for all its heads (the f64 products and reductions cost more
+// than a head's arithmetic); a warp takes kAhead heads at a time, all loaded
+// before the first is worked on.
+constexpr int kAhead = 4;
 
-// One warp per (row, head).
 template <int D, typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) qk_norm_rope_kernel(KvBatchDev b, const __grid_constant__ RopeDev rope,
-                                                                      AttnRows in, AttnRows out, int *err)
+                                                                      AttnRows in, AttnRows out, int group, int *err)
 {
+    constexpr int N = D / 32;
+    __shared__ float2 s_turn[D / 2];
     __shared__ float s_y[kRowWarps][D];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (blockIdx.x == 0)
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.x;
+    pdl_wait();
+    pdl_trigger();
+    if (row == 0 && blockIdx.y == 0)
         for (int s = threadIdx.x; s < b.B; s += blockDim.x) {
             SeqInfo q;
             if (!seq_info(b, s, q)) kv_error(err);
         }
-    const int heads = (in.q ? in.q_heads : 0) + (in.k ? in.kv_heads : 0);
-    const int64_t item = (int64_t)blockIdx.x * kRowWarps + warp;
-    const int row = (int)(item / heads);
-    int head = (int)(item - (int64_t)row * heads);
-    if (row >= b.T) return;
-    const int s = seq_of_row(b, row);
-    SeqInfo q;
-    if (!seq_info(b, s, q) || row < q.row0 || row >= q.row0 + q.n) return;
-    const bool is_q = in.q && head < in.q_heads;
-    if (in.q && !is_q) head -= in.q_heads;
-    const T *x = static_cast<const T *>(is_q ? in.q : in.k) + row * (is_q ? in.q_stride : in.k_stride) + head * D;
-    T *y = static_cast<T *>(const_cast<void *>(is_q ? out.q : out.k)) + row * (is_q ? out.q_stride : out.k_stride) + head * D;
-    norm_rope_head<D>(x, is_q ? rope.q_norm : rope.k_norm, rope, q.past + row - q.row0, s_y[warp], lane);
-    constexpr int N = D / 32;
-    float v[N];
+    const int q_heads = in.q ? in.q_heads : 0, heads = q_heads + (in.k ? in.kv_heads : 0);
+    const int head1 = min(heads, (int)(blockIdx.y + 1) * group);
+    const T *in_q = static_cast<const T *>(in.q) + row * in.q_stride, *in_k = static_cast<const T *>(in.k) + row * in.k_stride;
+    float v[kAhead][N];
+    auto load = [&](int h0) {
 #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = s_y[warp][lane * N + i];
-    store_vals<N>(y + lane * N, v);
+        for (int i = 0; i < kAhead; i++) {
+            const int h = h0 + i * kRowWarps;
+            if (h < head1) load_vals<N>((h < q_heads ? in_q + h * D : in_k + (h - q_heads) * D) + lane * N, v[i]);
+        }
+    };
+    int h0 = blockIdx.y * group + warp;
+    load(h0);
+    const int s = seq_of_row_warp(b, row, lane);
+    SeqInfo q;
+    if (s < 0 || !seq_info(b, s, q) || row < q.row0 || row >= q.row0 + q.n) return;
+    rope_table(rope, q.past + row - q.row0, s_turn, threadIdx.x, kRowWarps * 32);
+    __syncthreads();
+    T *out_q = static_cast<T *>(const_cast<void *>(out.q)) + row * out.q_stride,
+      *out_k = static_cast<T *>(const_cast<void *>(out.k)) + row * out.k_stride;
+    for (;;) {
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const int h = h0 + i * kRowWarps;
+            if (h >= head1) break;
+            turn_head<D>(v[i], h < q_heads ? rope.q_norm : rope.k_norm, rope, s_turn, s_y[warp], lane);
+            store_vals<N>((h < q_heads ? out_q + h * D : out_k + (h - q_heads) * D) + lane * N, v[i]);
+        }
+        h0 += kAhead * kRowWarps;
+        if (h0 >= head1) break;
+        load(h0);
+    }
 }
 
 // ------------------------------------------------------------------ append
@@ -111,7 +122,7 @@ __global__ void __launch_bounds__(128) kv_append_kernel(KvCacheDev c, KvBatchDev
     if (b.slot) {
         bool twice = false;
         for (int i = tid; i < s; i += blockDim.x)
-            twice |= __ldg(b.slot + i) == slot && row_of(b, i + 1) > row_of(b, i);
+            twice |= ld_plain(b.slot + i) == slot && row_of(b, i + 1) > row_of(b, i);
         if (__syncthreads_or(twice)) {
             if (tid == 0) kv_error(err);
             return;
@@ -171,14 +182,14 @@ __global__ void __launch_bounds__(128) kv_append_kernel(KvCacheDev c, KvBatchDev
                     sincos((double)(first + t) * rope.inv[i], &sn, &cs);
                     double va = x[ab.x] * inv, vb = x[ab.y] * inv;
                     if (rope.k_norm) {
-                        va *= __ldg(rope.k_norm + ab.x);
-                        vb *= __ldg(rope.k_norm + ab.y);
+                        va *= ld_plain(rope.k_norm + ab.x);
+                        vb *= ld_plain(rope.k_norm + ab.y);
                     }
                     x[ab.x] = (float)((va * cs - vb * sn) * rope.mscale);
                     x[ab.y] = (float)((vb * cs + va * sn) * rope.mscale);
                 } else if (rope.k_norm) {
                     const int d = rope.R + i - pairs;
-                    x[d] = (float)(x[d] * inv * __ldg(rope.k_norm + d));
+                    x[d] = (float)(x[d] * inv * ld_plain(rope.k_norm + d));
                 }
             }
             __syncthreads();
@@ -237,38 +248,47 @@ __global__ void __launch_bounds__(128) kv_append_kernel(KvCacheDev c, KvBatchDev
 
 // -------------------------------------------------------------------- read
 
-// One warp per (row, head).
+// One CTA per row: a warp a head, keys and values at a time. A value's 16 tokens
+// lie together, so a row's bytes are D sectors of which it needs one byte each:
+// rows that follow one another find them in the caches.
 template <int D, typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) kv_read_kernel(KvCacheDev c, KvBatchDev b, AttnRows out, int *err)
 {
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (blockIdx.x == 0)
+    constexpr int N = D / 32;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.x;
+    pdl_wait();
+    pdl_trigger();
+    if (row == 0)
         for (int s = threadIdx.x; s < b.B; s += blockDim.x) {
             SeqInfo q;
             int slot;
             if (!seq_info(b, s, q) || !seq_in_cache(c, b, s, q, slot)) kv_error(err);
         }
-    const int64_t item = (int64_t)blockIdx.x * kRowWarps + warp;
-    const int row = (int)(item / c.heads), head = (int)(item - (int64_t)row * c.heads);
-    if (row >= b.T) return;
-    const int s = seq_of_row(b, row);
+    const int s = seq_of_row_warp(b, row, lane);
+    if (s < 0) return;
     SeqInfo q;
     int slot;
     if (!seq_info(b, s, q) || row < q.row0 || row >= q.row0 + q.n || !seq_in_cache(c, b, s, q, slot)) return;
     const int pos = q.past + row - q.row0, t = pos % kKvBlock;
-    const int64_t at = block_index(c, slot, pos / kKvBlock, head);
-    if (at < 0 && lane == 0) kv_error(err);
-    constexpr int N = D / 32;
-    float kv[N], vv[N];
-    const float ks = at >= 0 ? __ldg(c.k_scale + at) : 0.0f, vs = at >= 0 ? __ldg(c.v_scale + at) : 0.0f;
+    for (int head = warp; head < c.heads; head += kRowWarps) {
+        const int64_t at = block_index(c, slot, pos / kKvBlock, head);
+        if (at < 0 && lane == 0) kv_error(err);
+        float kv[N], vv[N];
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int d = lane * N + i;
-        kv[i] = at >= 0 ? ks * (float)c.k[at * kKvBlock * D + d / 64 * 1024 + t * 64 + d % 64] : 0.0f;
-        vv[i] = at >= 0 ? vs * (float)c.v[at * kKvBlock * D + d * kKvBlock + t] : 0.0f;
+        for (int i = 0; i < N; i++) kv[i] = vv[i] = 0.0f;
+        if (at >= 0) {
+            const float ks = ld_plain(c.k_scale + at), vs = ld_plain(c.v_scale + at);
+            const int8_t *k = c.k + at * kKvBlock * D + lane * N / 64 * 1024 + t * 64 + lane * N % 64;
+            const int8_t *v = c.v + at * kKvBlock * D + lane * N * kKvBlock + t;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                kv[i] = ks * (float)k[i];
+                vv[i] = vs * (float)v[i * kKvBlock];
+            }
+        }
+        if (out.k) store_vals<N>(static_cast<T *>(const_cast<void *>(out.k)) + row * out.k_stride + head * D + lane * N, kv);
+        if (out.v) store_vals<N>(static_cast<T *>(const_cast<void *>(out.v)) + row * out.v_stride + head * D + lane * N, vv);
     }
-    if (out.k) store_vals<N>(static_cast<T *>(const_cast<void *>(out.k)) + row * out.k_stride + head * D + lane * N, kv);
-    if (out.v) store_vals<N>(static_cast<T *>(const_cast<void *>(out.v)) + row * out.v_stride + head * D + lane * N, vv);
 }
 
 template <typename F>
@@ -289,11 +309,11 @@ cudaError_t by_type(int act, int D, F &&f)
 cudaError_t launch_qk_norm_rope(const KvBatchDev &b, const RopeDev &rope, const AttnRows &in, const AttnRows &out, int D,
                                 int *err, cudaStream_t st)
 {
-    const int64_t items = (int64_t)b.T * ((in.q ? in.q_heads : 0) + (in.k ? in.kv_heads : 0));
-    const unsigned grid = (unsigned)((items + kRowWarps - 1) / kRowWarps);
+    // few tokens: a head a warp, for the shortest time; many: up to sixteen heads a CTA
+    const int heads = (in.q ? in.q_heads : 0) + (in.k ? in.kv_heads : 0), group = b.T <= 256 ? kRowWarps : kAhead * kRowWarps;
     return by_type(in.act, D, [&](auto d, auto t) {
-        qk_norm_rope_kernel<decltype(d)::value, decltype(t)><<<grid, kRowWarps * 32, 0, st>>>(b, rope, in, out, err);
-        return cudaGetLastError();
+        return launch_dependent(qk_norm_rope_kernel<decltype(d)::value, decltype(t)>, dim3(b.T, (heads + group - 1) / group),
+                                dim3(kRowWarps * 32), 0, st, b, rope, in, out, group, err);
     });
 }
 
@@ -311,11 +331,9 @@ cudaError_t launch_kv_append(const KvCacheDev &c, const KvBatchDev &b, const Rop
 
 cudaError_t launch_kv_read(const KvCacheDev &c, const KvBatchDev &b, const AttnRows &out, int *err, cudaStream_t st)
 {
-    const int64_t items = (int64_t)b.T * c.heads;
-    const unsigned grid = (unsigned)((items + kRowWarps - 1) / kRowWarps);
     return by_type(out.act, c.D, [&](auto d, auto t) {
-        kv_read_kernel<decltype(d)::value, decltype(t)><<<grid, kRowWarps * 32, 0, st>>>(c, b, out, err);
-        return cudaGetLastError();
+        return launch_dependent(kv_read_kernel<decltype(d)::value, decltype(t)>, dim3(b.T), dim3(kRowWarps * 32), 0, st, c, b, out,
+                                err);
     });
 }
 

@@ -11,7 +11,7 @@
 // halves of 64 tokens (P over S once S has been read) and O (D columns). While
 // a warpgroup weighs one half, the tensor cores add the other half's weights
 // and refill it: with one S of 128 columns a row tile the two waited for one
-// another, and the same work took 561 us instead of @@ (4096 rows of 32 heads
+// another, and the same work took 561 us instead of 504 (4096 rows of 32 heads
 // over 4096 + 4096 tokens, bf16).
 //
 // The sums O are scaled down only when a row's maximum has grown by more than
@@ -233,15 +233,24 @@ __global__ void __launch_bounds__(128) query_tiles_kernel(const __grid_constant_
     if (s < 0 || !seq_info(p.b, s, q) || row < q.row0 || row >= q.row0 + q.n || q.n * g <= few_rows) return;
     const int tok = row - q.row0, entry = first_entry(p.b, s, g);
     if (entry + (tok * g + g - 1) / kRowsItem < entry0 || entry + tok * g / kRowsItem >= entry1) return;
+    const T *src = static_cast<const T *>(p.rows.q) + (int64_t)row * p.rows.q_stride;
     if (p.use_rope) {
         rope_table(p.rope, q.past + tok, s_turn, tid, 128);
         __syncthreads();
     }
-    for (int h = blockIdx.y * 4 + warp; h < p.rows.q_heads; h += gridDim.y * 4) {
-        const int kvh = h / g, flat = tok * g + h - kvh * g, e = entry + flat / kRowsItem, r = flat % kRowsItem;
-        if (e < entry0 || e >= entry1) continue;
+    constexpr int kAhead = 4;      // heads of a warp that are loaded before the first is worked on
+    float vs[kAhead][N];
+    for (int h0 = blockIdx.y * 4 + warp, n = 0; h0 < p.rows.q_heads; n++, h0 += gridDim.y * 4) {
+        const int step = gridDim.y * 4;
+        if (n % kAhead == 0)
+#pragma unroll
+            for (int i = 0; i < kAhead; i++)
+                if (h0 + i * step < p.rows.q_heads) load_vals<N>(src + (h0 + i * step) * D + lane * N, vs[i]);
+        const int h = h0, kvh = h / g, flat = tok * g + h - kvh * g, e = entry + flat / kRowsItem, r = flat % kRowsItem;
         float v[N];
-        load_vals<N>(static_cast<const T *>(p.rows.q) + (int64_t)row * p.rows.q_stride + h * D + lane * N, v);
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = n % kAhead == 0 ? vs[0][i] : n % kAhead == 1 ? vs[1][i] : n % kAhead == 2 ? vs[2][i] : vs[3][i];
+        if (e < entry0 || e >= entry1) continue;
         if (p.use_rope) turn_head<D>(v, p.rope.q_norm, p.rope, s_turn, s_y[warp], lane);
         float amax = 0.0f;
 #pragma unroll
@@ -368,8 +377,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (which == 0) {
                     sk = sv = 0.0f;
                     if (at >= 0) {
-                        sk = __ldg(p.c.k_scale + at);
-                        sv = __ldg(p.c.v_scale + at);
+                        sk = ld_plain(p.c.k_scale + at);
+                        sv = ld_plain(p.c.v_scale + at);
                     }
                 }
             };
@@ -570,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool live = r < it.rows;
             const int tok = it.tok + (it.rem + r) / g;
             const int pos = live ? it.q.past + tok : INT_MAX;
-            const float rf = live ? __ldg(factors + (int64_t)image * kRowsItem + r) : 0.0f;
+            const float rf = live ? ld_plain(factors + (int64_t)image * kRowsItem + r) : 0.0f;
             float m = -INFINITY, l = 0.0f;
             for (int u = 0; u < 2 * it.tiles; u++) {
                 // ---- half u & 1 of tile u / 2
