@@ -30,7 +30,7 @@ __device__ __forceinline__ void from_f32(__nv_bfloat16 &d, float v) { d = __floa
 template <typename T>
 __device__ __forceinline__ T ld_plain(const T *p) { return *p; }
 
-// N consecutive values (N * size a multiple of 8 bytes, so aligned) to and from f32.
+// N consecutive values (N * size a multiple of 4 bytes, so aligned) to and from f32.
 template <int N, typename T>
 __device__ __forceinline__ void load_vals(const T *p, float (&v)[N])
 {
@@ -124,51 +124,105 @@ __device__ __forceinline__ int seq_of_row_warp(const KvBatchDev &b, int row, int
     return __reduce_add_sync(0xffffffffu, n) - 1;
 }
 
-// cos and sin of a position's R / 2 angles, times mscale, by n threads.
-__device__ __forceinline__ void rope_table(const RopeDev &r, int pos, float2 *turn, int tid, int n)
-{
-    for (int i = tid; i < r.R / 2; i += n) {
-        float c, s;
-        turn_f32((double)pos * r.inv[i], c, s);
-        turn[i] = make_float2(c * (float)r.mscale, s * (float)r.mscale);
-    }
-}
+// A token's heads by one warp, 16 bytes of a head to a lane: the lane's values
+// lie at the same place of every head, so its angles and norm weights are
+// fetched once for the token and stay in registers.
+template <int D, typename T>
+struct HeadLanes {
+    static constexpr int kVals = 16 / (int)sizeof(T);      // values of a lane
+    static constexpr int kLanes = D / kVals;               // lanes of a head
+    static constexpr int kHeads = 32 / kLanes;             // heads a warp takes at once
+    static constexpr int kScratch = D;                     // floats of shared memory of a warp's own (see begin and turn)
+    int lane, d0;               // first value of the lane
+    int half, shift;            // R / 2; lanes to the partner's (0: not a whole number of lanes)
+    bool inter, first, turns;   // interleaved pairs; the lane's values are first of their pairs; they turn
+    float c[kVals], s[kVals];
 
-// One warp: a head row, D / 32 consecutive values in each lane's v, normed
-// (w != nullptr) and turned by the table's angles, in f32. y: D floats of
-// shared memory of the warp's own.
-template <int D>
-__device__ __forceinline__ void turn_head(float (&v)[D / 32], const float *w, const RopeDev &r, const float2 *turn, float *y, int lane)
-{
-    constexpr int N = D / 32;
-    if (w) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; i++) ss = fmaf(v[i], v[i], ss);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = 1.0f / sqrtf(ss * (1.0f / D) + (float)r.eps);
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = v[i] * inv * ld_plain(w + lane * N + i);
-    }
-    if (r.R == 0) return;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < N; i++) y[lane * N + i] = v[i];
-    __syncwarp();
-    // each value with its partner: a cos - b sin for the first of a pair, b cos + a sin for the second
-    const int half = r.R / 2;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int d = lane * N + i;
-        if (d < r.R) {
-            const bool second = r.interleaved ? d & 1 : d >= half;
-            const float2 t = turn[r.interleaved ? d / 2 : second ? d - half : d];
-            const float other = y[r.interleaved ? d ^ 1 : second ? d - half : d + half];
-            v[i] = second ? v[i] * t.x + other * t.y : v[i] * t.x - other * t.y;
+    // Angles of a position: formed by the warp in y, each lane's kept.
+    __device__ __forceinline__ void begin(const RopeDev &r, int pos, float *y, int lane_)
+    {
+        lane = lane_;
+        d0 = lane % kLanes * kVals;
+        half = r.R / 2;
+        inter = r.interleaved || r.R == 2;
+        shift = half % kVals ? 0 : half / kVals;
+        first = d0 < half;
+        turns = r.R > 0;
+        if (!turns) return;
+        float2 *turn = reinterpret_cast<float2 *>(y);
+        for (int i = lane; i < half; i += 32) {
+            float cs, sn;
+            turn_f32((double)pos * r.inv[i], cs, sn);
+            turn[i] = make_float2(cs * (float)r.mscale, sn * (float)r.mscale);
         }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kVals; i++) {
+            const int d = d0 + i;
+            const float2 t = d < 2 * half ? turn[inter ? d / 2 : d < half ? d : d - half] : make_float2(1.0f, 0.0f);
+            // a cos - b sin for the first of a pair, b cos + a sin for the second
+            c[i] = t.x;
+            s[i] = (inter ? d & 1 : d >= half) ? t.y : -t.y;
+        }
+        __syncwarp();
     }
-}
+    // The lane's values of a norm's weights.
+    __device__ __forceinline__ void weights(const float *w, float (&v)[kVals]) const
+    {
+#pragma unroll
+        for (int i = 0; i < kVals; i++) v[i] = w ? ld_plain(w + d0 + i) : 1.0f;
+    }
+    __device__ __forceinline__ float head_max(float v) const
+    {
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
+    }
+    // v normed (norm) and turned, in f32; the whole warp, each kLanes a head.
+    __device__ __forceinline__ void turn(float (&v)[kVals], bool norm, const float (&w)[kVals], float eps, float *y) const
+    {
+        if (norm) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kVals; i++) ss = fmaf(v[i], v[i], ss);
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float inv = 1.0f / sqrtf(ss * (1.0f / D) + eps);
+#pragma unroll
+            for (int i = 0; i < kVals; i++) v[i] = v[i] * inv * w[i];
+        }
+        if (!turns) return;
+        float other[kVals];
+        if (inter) {
+#pragma unroll
+            for (int i = 0; i < kVals; i++) other[i] = v[i ^ 1];
+        } else if (shift) {
+            const int from = first ? lane + shift : lane - shift;
+#pragma unroll
+            for (int i = 0; i < kVals; i++) other[i] = __shfl_sync(0xffffffffu, v[i], from & 31);
+        } else {        // pairs that do not lie lane by lane: through shared memory, a head at a time
+#pragma unroll
+            for (int i = 0; i < kVals; i++) other[i] = 0.0f;
+            for (int h = 0; h < kHeads; h++) {
+                __syncwarp();
+                if (lane / kLanes == h)
+#pragma unroll
+                    for (int i = 0; i < kVals; i++) y[d0 + i] = v[i];
+                __syncwarp();
+                if (lane / kLanes == h)
+#pragma unroll
+                    for (int i = 0; i < kVals; i++) {
+                        const int d = d0 + i;
+                        if (d < 2 * half) other[i] = y[d < half ? d + half : d - half];
+                    }
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < kVals; i++)
+            if (d0 + i < 2 * half) v[i] = v[i] * c[i] + other[i] * s[i];
+    }
+};
 
 // One warp: a head row of D values, D / 32 consecutive ones in each lane's v,
 // normed (w != nullptr) and rotated at position pos into y[D] (shared memory),

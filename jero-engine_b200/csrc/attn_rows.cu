@@ -13,58 +13,68 @@ namespace {
 
 constexpr int kRowWarps = 4;
 
-// Norms and rotation: one CTA per token and group of heads. The token's angles
-// are formed once for all its heads (the f64 products and reductions cost more
-// than a head's arithmetic); a warp takes kAhead heads at a time, all loaded
-// before the first is worked on.
+// Norms and rotation: a warp takes a group of a token's heads, kAhead loads of
+// 16 bytes a lane under way before the first is worked on.
 constexpr int kAhead = 4;
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) qk_norm_rope_kernel(KvBatchDev b, const __grid_constant__ RopeDev rope,
-                                                                      AttnRows in, AttnRows out, int group, int *err)
+                                                                      AttnRows in, AttnRows out, int group, int groups, int *err)
 {
-    constexpr int N = D / 32;
-    __shared__ float2 s_turn[D / 2];
-    __shared__ float s_y[kRowWarps][D];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.x;
+    using L = HeadLanes<D, T>;
+    __shared__ __align__(16) float s_y[kRowWarps][L::kScratch];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     pdl_wait();
     pdl_trigger();
-    if (row == 0 && blockIdx.y == 0)
+    if (blockIdx.x == 0)
         for (int s = threadIdx.x; s < b.B; s += blockDim.x) {
             SeqInfo q;
             if (!seq_info(b, s, q)) kv_error(err);
         }
+    const int64_t item = (int64_t)blockIdx.x * kRowWarps + warp;
+    const int row = (int)(item / groups);
+    if (row >= b.T) return;
     const int q_heads = in.q ? in.q_heads : 0, heads = q_heads + (in.k ? in.kv_heads : 0);
-    const int head1 = min(heads, (int)(blockIdx.y + 1) * group);
-    const T *in_q = static_cast<const T *>(in.q) + row * in.q_stride, *in_k = static_cast<const T *>(in.k) + row * in.k_stride;
-    float v[kAhead][N];
-    auto load = [&](int h0) {
+    int h = (int)(item - (int64_t)row * groups) * group + lane / L::kLanes;
+    const int head1 = min(heads, h - lane / L::kLanes + group), d0 = lane % L::kLanes * L::kVals;
+    const T *in_q = static_cast<const T *>(in.q) + row * in.q_stride + d0, *in_k = static_cast<const T *>(in.k) + row * in.k_stride + d0;
+    T *out_q = static_cast<T *>(const_cast<void *>(out.q)) + row * out.q_stride + d0,
+      *out_k = static_cast<T *>(const_cast<void *>(out.k)) + row * out.k_stride + d0;
+    float v[kAhead][L::kVals];
+    auto load = [&](int h) {
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-            const int h = h0 + i * kRowWarps;
-            if (h < head1) load_vals<N>((h < q_heads ? in_q + h * D : in_k + (h - q_heads) * D) + lane * N, v[i]);
+            const int x = h + i * L::kHeads;
+            if (x < head1) load_vals<L::kVals>(x < q_heads ? in_q + x * D : in_k + (x - q_heads) * D, v[i]);
+            else
+#pragma unroll
+                for (int k = 0; k < L::kVals; k++) v[i][k] = 0.0f;
         }
     };
-    int h0 = blockIdx.y * group + warp;
-    load(h0);
+    load(h);
     const int s = seq_of_row_warp(b, row, lane);
     SeqInfo q;
     if (s < 0 || !seq_info(b, s, q) || row < q.row0 || row >= q.row0 + q.n) return;
-    rope_table(rope, q.past + row - q.row0, s_turn, threadIdx.x, kRowWarps * 32);
-    __syncthreads();
-    T *out_q = static_cast<T *>(const_cast<void *>(out.q)) + row * out.q_stride,
-      *out_k = static_cast<T *>(const_cast<void *>(out.k)) + row * out.k_stride;
+    L l;
+    l.begin(rope, q.past + row - q.row0, s_y[warp], lane);
+    float wq[L::kVals], wk[L::kVals];
+    l.weights(rope.q_norm, wq);
+    l.weights(rope.k_norm, wk);
     for (;;) {
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-            const int h = h0 + i * kRowWarps;
-            if (h >= head1) break;
-            turn_head<D>(v[i], h < q_heads ? rope.q_norm : rope.k_norm, rope, s_turn, s_y[warp], lane);
-            store_vals<N>((h < q_heads ? out_q + h * D : out_k + (h - q_heads) * D) + lane * N, v[i]);
+            const int x = h + i * L::kHeads;
+            if (x - lane / L::kLanes >= head1) break;
+            const bool is_q = x < q_heads;
+            float w[L::kVals];
+#pragma unroll
+            for (int k = 0; k < L::kVals; k++) w[k] = is_q ? wq[k] : wk[k];
+            l.turn(v[i], __any_sync(0xffffffffu, (is_q ? rope.q_norm : rope.k_norm) != nullptr), w, (float)rope.eps, s_y[warp]);
+            if (x < head1) store_vals<L::kVals>(is_q ? out_q + x * D : out_k + (x - q_heads) * D, v[i]);
         }
-        h0 += kAhead * kRowWarps;
-        if (h0 >= head1) break;
-        load(h0);
+        h += kAhead * L::kHeads;
+        if (h - lane / L::kLanes >= head1) break;
+        load(h);
     }
 }
 
@@ -309,11 +319,14 @@ cudaError_t by_type(int act, int D, F &&f)
 cudaError_t launch_qk_norm_rope(const KvBatchDev &b, const RopeDev &rope, const AttnRows &in, const AttnRows &out, int D,
                                 int *err, cudaStream_t st)
 {
-    // few tokens: a head a warp, for the shortest time; many: up to sixteen heads a CTA
-    const int heads = (in.q ? in.q_heads : 0) + (in.k ? in.kv_heads : 0), group = b.T <= 256 ? kRowWarps : kAhead * kRowWarps;
+    // few tokens: one load a warp, for the shortest time; many: a token's heads up to four loads' worth a turn
+    const int heads = (in.q ? in.q_heads : 0) + (in.k ? in.kv_heads : 0);
     return by_type(in.act, D, [&](auto d, auto t) {
-        return launch_dependent(qk_norm_rope_kernel<decltype(d)::value, decltype(t)>, dim3(b.T, (heads + group - 1) / group),
-                                dim3(kRowWarps * 32), 0, st, b, rope, in, out, group, err);
+        using L = HeadLanes<decltype(d)::value, decltype(t)>;
+        const int group = b.T <= 512 ? L::kHeads : kAhead * L::kHeads * 2, groups = (heads + group - 1) / group;
+        return launch_dependent(qk_norm_rope_kernel<decltype(d)::value, decltype(t)>,
+                                dim3((unsigned)(((int64_t)b.T * groups + kRowWarps - 1) / kRowWarps)), dim3(kRowWarps * 32), 0, st, b,
+                                rope, in, out, group, groups, err);
     });
 }
 

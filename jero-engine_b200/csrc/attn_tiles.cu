@@ -215,69 +215,93 @@ struct TileShape {
 
 // Queries as the item's shared-memory image: f16 rows scaled by a power of two
 // that takes the largest value to [2^14, 2^15), and the factor that a row's
-// logits then need. One CTA per token, heads over its warps.
+// logits then need. A warp takes a group of a token's heads.
+constexpr int kQueryWarps = 4, kAhead = 4;
+
 template <int D, typename T, bool SPLIT>
-__global__ void __launch_bounds__(128) query_tiles_kernel(const __grid_constant__ AttnParams p, int entry0, int entry1,
-                                                          int few_rows, uint8_t *images, float *factors)
+__global__ void __launch_bounds__(kQueryWarps * 32)
+    query_tiles_kernel(const __grid_constant__ AttnParams p, int entry0, int entry1, int few_rows, int group, int groups,
+                       uint8_t *images, float *factors)
 {
     using Sh = TileShape<D, SPLIT>;
-    constexpr int N = D / 32;
-    __shared__ float2 s_turn[D / 2];
-    __shared__ float s_y[4][D];
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, row = blockIdx.x;
+    using L = HeadLanes<D, T>;
+    __shared__ __align__(16) float s_y[kQueryWarps][L::kScratch];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     pdl_wait();
     pdl_trigger();
-    const int g = p.rows.q_heads / p.c.heads;
+    const int64_t item = (int64_t)blockIdx.x * kQueryWarps + warp;
+    const int row = (int)(item / groups);
+    if (row >= p.b.T) return;
+    const int g = p.rows.q_heads / p.c.heads, sub = lane / L::kLanes;
+    int h = (int)(item - (int64_t)row * groups) * group + sub;
+    const int head1 = min(p.rows.q_heads, h - sub + group), d0 = lane % L::kLanes * L::kVals;
+    const T *src = static_cast<const T *>(p.rows.q) + row * p.rows.q_stride + d0;
+    float v[kAhead][L::kVals];
+    auto load = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const int x = h + i * L::kHeads;
+            if (x < head1) load_vals<L::kVals>(src + x * D, v[i]);
+            else
+#pragma unroll
+                for (int k = 0; k < L::kVals; k++) v[i][k] = 0.0f;
+        }
+    };
+    load(h);
     const int s = seq_of_row_warp(p.b, row, lane);
     SeqInfo q;
     if (s < 0 || !seq_info(p.b, s, q) || row < q.row0 || row >= q.row0 + q.n || q.n * g <= few_rows) return;
     const int tok = row - q.row0, entry = first_entry(p.b, s, g);
     if (entry + (tok * g + g - 1) / kRowsItem < entry0 || entry + tok * g / kRowsItem >= entry1) return;
-    const T *src = static_cast<const T *>(p.rows.q) + (int64_t)row * p.rows.q_stride;
+    L l;
+    float w[L::kVals];
     if (p.use_rope) {
-        rope_table(p.rope, q.past + tok, s_turn, tid, 128);
-        __syncthreads();
+        l.begin(p.rope, q.past + tok, s_y[warp], lane);
+        l.weights(p.rope.q_norm, w);
+    } else {
+        l.lane = lane;
     }
-    constexpr int kAhead = 4;      // heads of a warp that are loaded before the first is worked on
-    float vs[kAhead][N];
-    for (int h0 = blockIdx.y * 4 + warp, n = 0; h0 < p.rows.q_heads; n++, h0 += gridDim.y * 4) {
-        const int step = gridDim.y * 4;
-        if (n % kAhead == 0)
+    for (;;) {
 #pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (h0 + i * step < p.rows.q_heads) load_vals<N>(src + (h0 + i * step) * D + lane * N, vs[i]);
-        const int h = h0, kvh = h / g, flat = tok * g + h - kvh * g, e = entry + flat / kRowsItem, r = flat % kRowsItem;
-        float v[N];
+        for (int i = 0; i < kAhead; i++) {
+            const int x = h + i * L::kHeads;
+            if (x - sub >= head1) break;
+            float (&a)[L::kVals] = v[i];
+            if (p.use_rope) l.turn(a, p.rope.q_norm != nullptr, w, (float)p.rope.eps, s_y[warp]);
+            float amax = 0.0f;
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = n % kAhead == 0 ? vs[0][i] : n % kAhead == 1 ? vs[1][i] : n % kAhead == 2 ? vs[2][i] : vs[3][i];
-        if (e < entry0 || e >= entry1) continue;
-        if (p.use_rope) turn_head<D>(v, p.rope.q_norm, p.rope, s_turn, s_y[warp], lane);
-        float amax = 0.0f;
+            for (int k = 0; k < L::kVals; k++) amax = fmaxf(amax, fabsf(a[k]));
+            amax = l.head_max(amax);
+            const int kvh = x / g, flat = tok * g + x - kvh * g, e = entry + flat / kRowsItem, r = flat % kRowsItem;
+            if (x >= head1 || e < entry0 || e >= entry1) continue;
+            const int ex = max(-112, (int)(__float_as_uint(amax) >> 23) - 127);
+            float up = __int_as_float((14 - ex + 127) << 23);
+            const int64_t image = (int64_t)(e - entry0) * p.c.heads + kvh;
+            if (d0 == 0) factors[image * kRowsItem + r] = __int_as_float((ex - 14 + 127) << 23) * fabsf(p.scale) * 1.4426950408889634f;
+            if (p.scale < 0.0f) up = -up;      // the factors are not negative: maxima stay maxima
+            uint32_t hi[L::kVals / 2], lo[L::kVals / 2];
 #pragma unroll
-        for (int i = 0; i < N; i++) amax = fmaxf(amax, fabsf(v[i]));
-        const int x = max(-112, (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)) >> 23) - 127);
-        float up = __int_as_float((14 - x + 127) << 23);
-        const int64_t image = (int64_t)(e - entry0) * p.c.heads + kvh;
-        if (lane == 0) factors[image * kRowsItem + r] = __int_as_float((x - 14 + 127) << 23) * fabsf(p.scale) * 1.4426950408889634f;
-        if (p.scale < 0.0f) up = -up;      // the factors are not negative: maxima stay maxima
-        uint32_t hi[N / 2], lo[N / 2];
-#pragma unroll
-        for (int i = 0; i < N / 2; i++) {
-            const float a = v[2 * i] * up, b = v[2 * i + 1] * up;
-            hi[i] = pack_f16(a, b);
-            if constexpr (SPLIT) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
-                lo[i] = pack_f16(a - f.x, b - f.y);
+            for (int k = 0; k < L::kVals / 2; k++) {
+                const float y = a[2 * k] * up, z = a[2 * k + 1] * up;
+                hi[k] = pack_f16(y, z);
+                if constexpr (SPLIT) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[k]));
+                    lo[k] = pack_f16(y - f.x, z - f.y);
+                }
+            }
+            const int rt = r % kRowsTile;
+            uint8_t *dst = images + image * Sh::kImage + r / kRowsTile * Sh::kQTile + d0 / 64 * (kRowsTile * 128) + rt * 128 +
+                           (((d0 % 64) / 8) ^ (rt & 7)) * 16 + d0 % 8 * 2;
+            if constexpr (L::kVals == 8) {
+                *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            } else {
+                *reinterpret_cast<uint2 *>(dst) = make_uint2(hi[0], hi[1]);
+                if constexpr (SPLIT) *reinterpret_cast<uint2 *>(dst + Sh::kQTile / 2) = make_uint2(lo[0], lo[1]);
             }
         }
-        const int d = lane * N, rt = r % kRowsTile;
-        uint8_t *dst = images + image * Sh::kImage + r / kRowsTile * Sh::kQTile + d / 64 * (kRowsTile * 128) + rt * 128 +
-                       (((d % 64) / 8) ^ (rt & 7)) * 16 + d % 8 * 2;
-#pragma unroll
-        for (int i = 0; i < N / 2; i++) {
-            reinterpret_cast<uint32_t *>(dst)[i] = hi[i];
-            if constexpr (SPLIT) reinterpret_cast<uint32_t *>(dst + Sh::kQTile / 2)[i] = lo[i];
-        }
+        h += kAhead * L::kHeads;
+        if (h - sub >= head1) break;
+        load(h);
     }
 }
 
@@ -733,9 +757,11 @@ cudaError_t launch_tiles_d(const AttnParams &p, int few_rows, uint8_t *ws, size_
     for (int64_t e0 = 0; e0 < entries; e0 += slice) {
         const int e1 = (int)std::min(entries, e0 + slice);
         float *factors = reinterpret_cast<float *>(ws + (size_t)(e1 - e0) * p.c.heads * Sh::kImage);
-        const unsigned gy = p.b.T >= 512 ? 1 : (unsigned)((p.rows.q_heads + 3) / 4);
-        if ((e = launch_dependent(query_tiles_kernel<D, T, kSplit>, dim3(p.b.T, gy), dim3(128), 0, st, p, (int)e0, e1, few_rows, ws,
-                                  factors)) != cudaSuccess)
+        using L = HeadLanes<D, T>;
+        const int group = p.b.T <= 512 ? L::kHeads : kAhead * L::kHeads * 2, groups = (p.rows.q_heads + group - 1) / group;
+        if ((e = launch_dependent(query_tiles_kernel<D, T, kSplit>,
+                                  dim3((unsigned)(((int64_t)p.b.T * groups + kQueryWarps - 1) / kQueryWarps)), dim3(kQueryWarps * 32), 0,
+                                  st, p, (int)e0, e1, few_rows, group, groups, ws, factors)) != cudaSuccess)
             return e;
         const int grid = (int)std::min<int64_t>(p.num_sms, (e1 - e0) * p.c.heads);
         if ((e = launch_dependent(kern, dim3(grid), dim3(kThreads), Sh::kSmem, st, p, (int)e0, e1, few_rows, (const uint8_t *)ws,
