@@ -187,7 +187,7 @@ struct HeadLanes {
             for (int i = 0; i < kVals; i++) ss = fmaf(v[i], v[i], ss);
 #pragma unroll
             for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = 1.0f / sqrtf(ss * (1.0f / D) + eps);
+            const float inv = rsqrtf(ss * (1.0f / D) + eps);
 #pragma unroll
             for (int i = 0; i < kVals; i++) v[i] = v[i] * inv * w[i];
         }

@@ -5,6 +5,8 @@
 // All three touch each value once and are bound by memory (or, for a decode
 // step's few rows, by the launch): bytes per call = rows in + rows out, and for
 // the append the 8-bit blocks, their scales and the open blocks in f32.
+#include <algorithm>
+
 #include "attn.cuh"
 #include "kernels.h"
 
@@ -34,18 +36,21 @@ __global__ void __launch_bounds__(kRowWarps * 32) qk_norm_rope_kernel(KvBatchDev
     const int64_t item = (int64_t)blockIdx.x * kRowWarps + warp;
     const int row = (int)(item / groups);
     if (row >= b.T) return;
-    const int q_heads = in.q ? in.q_heads : 0, heads = q_heads + (in.k ? in.kv_heads : 0);
-    int h = (int)(item - (int64_t)row * groups) * group + lane / L::kLanes;
-    const int head1 = min(heads, h - lane / L::kLanes + group), d0 = lane % L::kLanes * L::kVals;
-    const T *in_q = static_cast<const T *>(in.q) + row * in.q_stride + d0, *in_k = static_cast<const T *>(in.k) + row * in.k_stride + d0;
-    T *out_q = static_cast<T *>(const_cast<void *>(out.q)) + row * out.q_stride + d0,
-      *out_k = static_cast<T *>(const_cast<void *>(out.k)) + row * out.k_stride + d0;
+    // groups of query heads, then of key heads
+    const int q_heads = in.q ? in.q_heads : 0, q_groups = (q_heads + group - 1) / group, gi = (int)(item - (int64_t)row * groups);
+    const bool is_q = gi < q_groups;
+    const int heads = is_q ? q_heads : in.kv_heads, sub = lane / L::kLanes, d0 = lane % L::kLanes * L::kVals;
+    int h = (is_q ? gi : gi - q_groups) * group + sub;
+    const int head1 = min(heads, h - sub + group);
+    const T *src = static_cast<const T *>(is_q ? in.q : in.k) + row * (is_q ? in.q_stride : in.k_stride) + d0;
+    T *dst = static_cast<T *>(const_cast<void *>(is_q ? out.q : out.k)) + row * (is_q ? out.q_stride : out.k_stride) + d0;
+    const float *norm = is_q ? rope.q_norm : rope.k_norm;
     float v[kAhead][L::kVals];
     auto load = [&](int h) {
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
             const int x = h + i * L::kHeads;
-            if (x < head1) load_vals<L::kVals>(x < q_heads ? in_q + x * D : in_k + (x - q_heads) * D, v[i]);
+            if (x < head1) load_vals<L::kVals>(src + x * D, v[i]);
             else
 #pragma unroll
                 for (int k = 0; k < L::kVals; k++) v[i][k] = 0.0f;
@@ -57,23 +62,18 @@ __global__ void __launch_bounds__(kRowWarps * 32) qk_norm_rope_kernel(KvBatchDev
     if (s < 0 || !seq_info(b, s, q) || row < q.row0 || row >= q.row0 + q.n) return;
     L l;
     l.begin(rope, q.past + row - q.row0, s_y[warp], lane);
-    float wq[L::kVals], wk[L::kVals];
-    l.weights(rope.q_norm, wq);
-    l.weights(rope.k_norm, wk);
+    float w[L::kVals];
+    l.weights(norm, w);
     for (;;) {
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
             const int x = h + i * L::kHeads;
-            if (x - lane / L::kLanes >= head1) break;
-            const bool is_q = x < q_heads;
-            float w[L::kVals];
-#pragma unroll
-            for (int k = 0; k < L::kVals; k++) w[k] = is_q ? wq[k] : wk[k];
-            l.turn(v[i], __any_sync(0xffffffffu, (is_q ? rope.q_norm : rope.k_norm) != nullptr), w, (float)rope.eps, s_y[warp]);
-            if (x < head1) store_vals<L::kVals>(is_q ? out_q + x * D : out_k + (x - q_heads) * D, v[i]);
+            if (x - sub >= head1) break;
+            l.turn(v[i], norm != nullptr, w, (float)rope.eps, s_y[warp]);
+            if (x < head1) store_vals<L::kVals>(dst + x * D, v[i]);
         }
         h += kAhead * L::kHeads;
-        if (h - lane / L::kLanes >= head1) break;
+        if (h - sub >= head1) break;
         load(h);
     }
 }
@@ -92,35 +92,116 @@ __device__ __forceinline__ int quantise(float x, float s, float inv)
     return (int)q;
 }
 
-// One CTA per (touched block, head). Flat block index u: sequence s owns the
-// indices from row_start[s] / 16 + 2 s on, at least as many as the blocks its
-// rows can touch (ceil((15 + n) / 16)), so no prefix sum is needed.
-template <int D, typename T>
-__global__ void __launch_bounds__(128) kv_append_kernel(KvCacheDev c, KvBatchDev b, const __grid_constant__ RopeDev rope,
-                                                        int use_rope, AttnRows rows, int *err)
+// The same for the values of a lane at once: x inv + 1.5 2^23 holds the rounded
+// quotient in its low bits, and the remainder shows whether it is the nearest
+// (all but always); where one is not, or lies half way, or is not finite, the
+// lane takes them one by one. by[i]: the byte in the low eight bits.
+template <int M>
+__device__ __forceinline__ void quantise_all(const float (&x)[M], float s, float inv, uint32_t (&by)[M])
 {
-    __shared__ float s_x[2][kKvBlock][D];      // keys, values
-    __shared__ double s_inv[kKvBlock];
-    __shared__ float s_amax[2];
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, head = blockIdx.y;
-    const int u = blockIdx.x;
-    int lo = 0, hi = b.B - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (row_of(b, mid) / kKvBlock + 2 * mid <= u) lo = mid;
-        else hi = mid - 1;
+    const float h = 0.5f * s;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < M; i++) {
+        const float t = fmaf(x[i], inv, 12582912.0f), r = fmaf(-(t - 12582912.0f), s, x[i]);
+        odd |= !(fabsf(r) < h);
+        by[i] = __float_as_uint(t);
     }
-    const int s = lo;
-    SeqInfo q;
-    int slot = -1;
-    const bool ok = seq_info(b, s, q) && seq_in_cache(c, b, s, q, slot);
-    if (blockIdx.x == 0 && head == 0)
+    if (odd) {
+#pragma unroll 1
+        for (int i = 0; i < M; i++) {
+            float v = x[0];
+#pragma unroll
+            for (int k = 1; k < M; k++) v = i == k ? x[k] : v;
+            const uint32_t q = s > 0.0f ? (uint32_t)quantise(v, s, inv) : 0u;
+#pragma unroll
+            for (int k = 0; k < M; k++) by[k] = i == k ? q : by[k];
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// cos and sin in f64: the angle less its whole quarter turns, then the Taylor
+// series up to x^14 and x^13 on [-pi/4, pi/4] (the next terms are below 2e-14;
+// the keys are rounded to f32 afterwards). A third of the library function's
+// work and no call, so that a lane's angles go side by side.
+__device__ __forceinline__ void turn_f64(double angle, double &c, double &s)
+{
+    const double n = rint(angle * 0.6366197723675814);       // 2 / pi
+    double x = fma(-n, 1.5707963267948966, angle);
+    x = fma(-n, 6.123233995736766e-17, x);                    // the rest of pi / 2
+    const double z = x * x;
+    double a = 1.0 / 6227020800.0, b = -1.0 / 87178291200.0;
+    a = fma(a, z, -1.0 / 39916800.0);
+    b = fma(b, z, 1.0 / 479001600.0);
+    a = fma(a, z, 1.0 / 362880.0);
+    b = fma(b, z, -1.0 / 3628800.0);
+    a = fma(a, z, -1.0 / 5040.0);
+    b = fma(b, z, 1.0 / 40320.0);
+    a = fma(a, z, 1.0 / 120.0);
+    b = fma(b, z, -1.0 / 720.0);
+    a = fma(a, z, -1.0 / 6.0);
+    b = fma(b, z, 1.0 / 24.0);
+    a = fma(a * z, x, x);
+    b = fma(b, z, -0.5);
+    b = fma(b, z, 1.0);
+    const int k = (int)(__double2ll_rn(n) & 3);
+    c = k & 1 ? a : b;
+    s = k & 1 ? b : a;
+    if (k == 1 || k == 2) c = -c;
+    if (k >= 2) s = -s;
+}
+
+// 1 / sqrt in f64 by one Newton step from f32's, which has 22 bits: 2^-43.
+__device__ __forceinline__ double root_f64(double x)
+{
+    if (!(x > 1e-30 && x < 1e30)) return 1.0 / sqrt(x);
+    const double y = (double)rsqrtf((float)x);
+    return y * fma(-0.5 * x * y, y, 1.5);
+}
+
+// One CTA per (touched block, group of heads): warp w has the block's tokens
+// 4 w .. 4 w + 3, a lane D / 32 of their values. The keys' angles are formed in
+// f64 once for the group, a token's from the one before by a turn of the
+// frequency (a few ulp of f64 after three of them).
+//
+// Flat block index u: sequence s owns the indices from row_start[s] / 16 + 2 s
+// on, at least as many as the blocks its rows can touch (ceil((15 + n) / 16)),
+// so no prefix sum is needed.
+template <int D, typename T>
+__global__ void __launch_bounds__(128, 5) kv_append_kernel(KvCacheDev c, KvBatchDev b, const __grid_constant__ RopeDev rope,
+                                                        int use_rope, AttnRows rows, int group, int *err)
+{
+    constexpr int N = D / 32;
+    __shared__ __align__(16) double2 s_turn[4][4 * N][32];     // [warp][token, value][lane]: cos, +- sin
+    __shared__ __align__(16) uint32_t s_v[2][4][D];            // a head's value bytes, four tokens (a warp's) to a word
+    __shared__ double s_row[4][D];                             // a row of pairs that do not lie lane by lane
+    __shared__ double s_inv[D / 2];
+    __shared__ unsigned s_amax[2][2];
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const int head0 = blockIdx.y * group, head1 = min(c.heads, head0 + group), half = rope.R / 2;
+    const int u = blockIdx.x;
+    if (tid < half) s_inv[tid] = rope.inv[tid];
+    if (tid < 4) s_amax[tid / 2][tid % 2] = 0u;
+    pdl_wait();
+    pdl_trigger();
+    // the sequence: the last whose indices start at or before u
+    int s = 0;
+    for (int i = lane; i < b.B; i += 32) s += row_of(b, i) / kKvBlock + 2 * i <= u;
+    s = __reduce_add_sync(0xffffffffu, s) - 1;
+    if (u == 0 && head0 == 0)
         for (int i = tid; i < b.B; i += blockDim.x) {
             SeqInfo qi;
             int sl;
             if (!seq_info(b, i, qi) || !seq_in_cache(c, b, i, qi, sl)) kv_error(err);
         }
-    if (!ok || q.n == 0) return;
+    SeqInfo q;
+    int slot = -1;
+    if (s < 0 || !seq_info(b, s, q) || !seq_in_cache(c, b, s, q, slot) || q.n == 0) return;
     const int total = q.past + q.n, blk0 = q.past / kKvBlock, blk_end = (total + kKvBlock - 1) / kKvBlock;
     const int blk1 = blk0 + (u - (q.row0 / kKvBlock + 2 * s));
     if (blk1 >= blk_end) return;
@@ -129,129 +210,197 @@ __global__ void __launch_bounds__(128) kv_append_kernel(KvCacheDev c, KvBatchDev
     const bool both = blk_end - 1 > blk0 && q.past % kKvBlock && total % kKvBlock;
     if (both && blk1 == blk_end - 1) return;
     // a slot that an earlier sequence of the batch appends to: refused
-    if (b.slot) {
-        bool twice = false;
-        for (int i = tid; i < s; i += blockDim.x)
-            twice |= ld_plain(b.slot + i) == slot && row_of(b, i + 1) > row_of(b, i);
-        if (__syncthreads_or(twice)) {
-            if (tid == 0) kv_error(err);
-            return;
-        }
+    bool twice = false;
+    if (b.slot)
+        for (int i = tid; i < s; i += blockDim.x) twice |= ld_plain(b.slot + i) == slot && row_of(b, i + 1) > row_of(b, i);
+    if (__syncthreads_or(twice)) {
+        if (tid == 0) kv_error(err);
+        return;
     }
-    constexpr int N = D / 32;
-    const int64_t open = ((int64_t)slot * c.heads + head) * kKvBlock * D;
+    const bool inter = rope.interleaved || rope.R == 2;
+    const int shift = half % N ? 0 : half / N, d0 = lane * N;
+    double w[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) w[i] = use_rope && rope.k_norm ? (double)ld_plain(rope.k_norm + d0 + i) : 1.0;
+
     for (int blk = blk1;; blk = blk_end - 1) {
-        const int first = blk * kKvBlock;                       // position of the block's first token
-        const int64_t at = block_index(c, slot, blk, head);
-        if (at < 0 && tid == 0) kv_error(err);
-        const int count = min(kKvBlock, total - first);
-        for (int t = warp; t < kKvBlock; t += 4) {
-            float kv[N], vv[N];
+        const int first = blk * kKvBlock + 4 * warp;            // position of this warp's first token
+        const int count = min(kKvBlock, total - blk * kKvBlock);
+        const int new0 = max(0, q.past - first), new1 = min(4, total - first);   // this warp's new tokens: new0 .. new1 - 1
+        float kx[4][N], vx[4][N];
+        auto load = [&](int head) {
+            const int64_t open = (((int64_t)slot * c.heads + head) * kKvBlock + 4 * warp) * D + d0;
 #pragma unroll
-            for (int i = 0; i < N; i++) kv[i] = vv[i] = 0.0f;
-            const int pos = first + t;
-            double inv = 0.0;
-            if (pos < q.past) {
+            for (int j = 0; j < 4; j++) {
+                if (j < new0 && j < new1) {
+                    load_vals<N>(c.open_k + open + j * D, kx[j]);
+                    load_vals<N>(c.open_v + open + j * D, vx[j]);
+                } else if (j < new1) {
+                    const int64_t row = q.row0 + first + j - q.past;
+                    load_vals<N>(static_cast<const T *>(rows.k) + row * rows.k_stride + head * D + d0, kx[j]);
+                    load_vals<N>(static_cast<const T *>(rows.v) + row * rows.v_stride + head * D + d0, vx[j]);
+                } else {
 #pragma unroll
-                for (int i = 0; i < N; i++) {
-                    kv[i] = c.open_k[open + t * D + lane * N + i];
-                    vv[i] = c.open_v[open + t * D + lane * N + i];
-                }
-            } else if (t < count) {
-                const int64_t row = q.row0 + pos - q.past;
-                load_vals<N>(static_cast<const T *>(rows.k) + row * rows.k_stride + head * D + lane * N, kv);
-                load_vals<N>(static_cast<const T *>(rows.v) + row * rows.v_stride + head * D + lane * N, vv);
-                if (use_rope && rope.k_norm) {
-                    double ss = 0.0;
-#pragma unroll
-                    for (int i = 0; i < N; i++) ss = fma((double)kv[i], (double)kv[i], ss);
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                    inv = 1.0 / sqrt(ss / D + rope.eps);
+                    for (int i = 0; i < N; i++) kx[j][i] = vx[j][i] = 0.0f;
                 }
             }
+        };
+        load(head0);
+        if (use_rope && half && new0 < new1) {
+            double cs[N], sn[N], cf[N], sf[N];
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                s_x[0][t][lane * N + i] = kv[i];
-                s_x[1][t][lane * N + i] = vv[i];
+                const int d = d0 + i;
+                const double f = d < 2 * half ? s_inv[inter ? d / 2 : d < half ? d : d - half] : 0.0;
+                turn_f64((double)(first + new0) * f, cs[i], sn[i]);
+                if (new1 - new0 > 1) turn_f64(f, cf[i], sf[i]);
             }
-            if (lane == 0) s_inv[t] = inv;
-        }
-        if (tid < 2) s_amax[tid] = 0.0f;
-        __syncthreads();
-        if (use_rope) {
-            // the new tokens' keys, in f64: pairs first, then the values that do not turn
-            const int t0 = max(0, q.past - first), pairs = rope.R / 2, units = pairs + (D - rope.R);
-            for (int e = tid; e < (count - t0) * units; e += blockDim.x) {
-                const int t = t0 + e / units, i = e % units;
-                float *x = s_x[0][t];
-                const double inv = rope.k_norm ? s_inv[t] : 1.0;
-                if (i < pairs) {
-                    const int2 ab = rope_pair(rope, i);
-                    double cs, sn;
-                    sincos((double)(first + t) * rope.inv[i], &sn, &cs);
-                    double va = x[ab.x] * inv, vb = x[ab.y] * inv;
-                    if (rope.k_norm) {
-                        va *= ld_plain(rope.k_norm + ab.x);
-                        vb *= ld_plain(rope.k_norm + ab.y);
-                    }
-                    x[ab.x] = (float)((va * cs - vb * sn) * rope.mscale);
-                    x[ab.y] = (float)((vb * cs + va * sn) * rope.mscale);
-                } else if (rope.k_norm) {
-                    const int d = rope.R + i - pairs;
-                    x[d] = (float)(x[d] * inv * ld_plain(rope.k_norm + d));
+            for (int j = new0;;) {
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    // a cos - b sin for the first of a pair, b cos + a sin for the second
+                    const double sign = (inter ? (d0 + i) & 1 : d0 + i >= half) ? rope.mscale : -rope.mscale;
+                    s_turn[warp][j * N + i][lane] = make_double2(cs[i] * rope.mscale, sn[i] * sign);
+                }
+                if (++j >= new1) break;
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const double x = cs[i] * cf[i] - sn[i] * sf[i];
+                    sn[i] = sn[i] * cf[i] + cs[i] * sf[i];
+                    cs[i] = x;
                 }
             }
-            __syncthreads();
         }
-        // scales
+        for (int head = head0; head < head1; head++) {
+            const int par = (head - head0) & 1;
+            const int64_t at = block_index(c, slot, blk, head);
+            if (at < 0 && tid == 0) kv_error(err);
+            if (use_rope) {
+                // ---- the new keys, in f64. The four tokens' sums of squares are halved
+                // together: after two exchanges a lane carries one token, after three
+                // more its sum, and one root serves all four.
+                double inv[4] = {1.0, 1.0, 1.0, 1.0};
+                if (rope.k_norm && new0 < new1) {
+                    double ss[4];
 #pragma unroll
-        for (int m = 0; m < 2; m++) {
-            float a = 0.0f;
-            for (int e = tid; e < kKvBlock * D; e += blockDim.x) {
-                const float x = fabsf((&s_x[m][0][0])[e]);
-                if (x <= 3.402823466e38f) a = fmaxf(a, x);
+                    for (int j = 0; j < 4; j++) {
+                        ss[j] = 0.0;
+#pragma unroll
+                        for (int i = 0; i < N; i++) ss[j] = fma((double)kx[j][i], (double)kx[j][i], ss[j]);
+                    }
+                    const bool up = lane & 16, mid = lane & 8;
+                    double a = up ? ss[2] : ss[0], e = up ? ss[3] : ss[1];
+                    a += __shfl_xor_sync(0xffffffffu, up ? ss[0] : ss[2], 16);
+                    e += __shfl_xor_sync(0xffffffffu, up ? ss[1] : ss[3], 16);
+                    double x = (mid ? e : a) + __shfl_xor_sync(0xffffffffu, mid ? a : e, 8);
+#pragma unroll
+                    for (int o = 4; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                    x = root_f64(x * (1.0 / D) + rope.eps);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) inv[j] = __shfl_sync(0xffffffffu, x, (j & 2) * 8 + (j & 1) * 8);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (j < new0 || j >= new1) continue;
+                    double x[N], other[N];
+#pragma unroll
+                    for (int i = 0; i < N; i++) x[i] = (double)kx[j][i] * (inv[j] * w[i]);
+                    if (half) {
+                        if (inter) {
+#pragma unroll
+                            for (int i = 0; i < N; i++) other[i] = x[i ^ 1];
+                        } else if (shift) {
+                            const int from = (d0 < half ? lane + shift : lane - shift) & 31;
+#pragma unroll
+                            for (int i = 0; i < N; i++) other[i] = __shfl_sync(0xffffffffu, x[i], from);
+                        } else {
+                            __syncwarp();
+#pragma unroll
+                            for (int i = 0; i < N; i++) s_row[warp][d0 + i] = x[i];
+                            __syncwarp();
+#pragma unroll
+                            for (int i = 0; i < N; i++) {
+                                const int d = d0 + i;
+                                other[i] = d < 2 * half ? s_row[warp][d < half ? d + half : d - half] : 0.0;
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < N; i++)
+                            if (d0 + i < 2 * half) {
+                                const double2 t = s_turn[warp][j * N + i][lane];
+                                x[i] = x[i] * t.x + other[i] * t.y;
+                            }
+                    }
+#pragma unroll
+                    for (int i = 0; i < N; i++) kx[j][i] = (float)x[i];
+                }
             }
+            // ---- the block's scales
+            float ka = 0.0f, va = 0.0f;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-            if (lane == 0) atomicMax(reinterpret_cast<int *>(&s_amax[m]), __float_as_int(a));   // a >= 0: ordered as integers
-        }
-        __syncthreads();
-        if (at >= 0) {
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const float x = fabsf(kx[j][i]), y = fabsf(vx[j][i]);
+                    ka = x <= 3.402823466e38f ? fmaxf(ka, x) : ka;
+                    va = y <= 3.402823466e38f ? fmaxf(va, y) : va;
+                }
+            const unsigned kb = __reduce_max_sync(0xffffffffu, __float_as_uint(ka)), vb = __reduce_max_sync(0xffffffffu, __float_as_uint(va));
+            if (lane == 0) {
+                atomicMax(&s_amax[par][0], kb);      // not negative: ordered as integers
+                atomicMax(&s_amax[par][1], vb);
+            }
+            __syncthreads();
             float sc[2], inv[2];
 #pragma unroll
             for (int m = 0; m < 2; m++) {
-                sc[m] = s_amax[m] >= kKvTiny ? __fdiv_rn(s_amax[m], 127.0f) : 0.0f;
+                const float amax = __uint_as_float(s_amax[par][m]);
+                sc[m] = amax >= kKvTiny ? __fdiv_rn(amax, 127.0f) : 0.0f;
                 inv[m] = sc[m] > 0.0f ? 1.0f / sc[m] : 0.0f;
             }
-            if (tid < 2) (tid ? c.v_scale : c.k_scale)[at] = sc[tid];
-            // four bytes at a time: keys [D/64][16][64], values [D][16]
-            uint32_t *ko = reinterpret_cast<uint32_t *>(c.k + at * kKvBlock * D);
-            uint32_t *vo = reinterpret_cast<uint32_t *>(c.v + at * kKvBlock * D);
-            for (int e = tid; e < kKvBlock * D / 4; e += blockDim.x) {
-                const int slab = e / (kKvBlock * 16), t = e / 16 % kKvBlock, d = slab * 64 + e % 16 * 4;
-                uint32_t w = 0, z = 0;
+            if (tid < 2) s_amax[par ^ 1][tid] = 0u;  // for the next head: read last before this barrier's head
+            // ---- bytes: keys [D/64][16][64] from the lanes, values [D][16] by way of shared memory
+            {
+                uint32_t by[4][N];
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    w |= (uint32_t)(uint8_t)(sc[0] > 0.0f ? quantise(s_x[0][t][d + i], sc[0], inv[0]) : 0) << (8 * i);
-                const int vd = e / 4, vt = e % 4 * 4;
+                for (int j = 0; j < 4; j++) {
+                    quantise_all<N>(kx[j], sc[0], inv[0], by[j]);
+                    if (at >= 0) {
+                        int8_t *k = c.k + at * kKvBlock * D + d0 / 64 * 1024 + (4 * warp + j) * 64 + d0 % 64;
+                        if constexpr (N == 4) *reinterpret_cast<uint32_t *>(k) = pack_bytes(by[j][0], by[j][1], by[j][2], by[j][3]);
+                        else *reinterpret_cast<uint16_t *>(k) = (uint16_t)__byte_perm(by[j][0], by[j][1], 0x0040);
+                    }
+                }
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    z |= (uint32_t)(uint8_t)(sc[1] > 0.0f ? quantise(s_x[1][vt + i][vd], sc[1], inv[1]) : 0) << (8 * i);
-                ko[e] = w;
-                vo[e] = z;
+                for (int j = 0; j < 4; j++) quantise_all<N>(vx[j], sc[1], inv[1], by[j]);
+                uint32_t vw[N];
+#pragma unroll
+                for (int i = 0; i < N; i++) vw[i] = pack_bytes(by[0][i], by[1][i], by[2][i], by[3][i]);
+                if constexpr (N == 4) *reinterpret_cast<uint4 *>(&s_v[par][warp][d0]) = make_uint4(vw[0], vw[1], vw[2], vw[3]);
+                else *reinterpret_cast<uint2 *>(&s_v[par][warp][d0]) = make_uint2(vw[0], vw[1]);
+            }
+            // ---- the rows of the block left open
+            if (count < kKvBlock) {
+                const int64_t open = (((int64_t)slot * c.heads + head) * kKvBlock + 4 * warp) * D + d0;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (j >= new0 && j < new1) {
+                        store_vals<N>(c.open_k + open + j * D, kx[j]);
+                        store_vals<N>(c.open_v + open + j * D, vx[j]);
+                    }
+            }
+            if (head + 1 < head1) load(head + 1);
+            __syncthreads();
+            if (at >= 0) {
+                if (tid < 2) (tid ? c.v_scale : c.k_scale)[at] = tid ? sc[1] : sc[0];
+                if (tid < D)
+                    reinterpret_cast<uint4 *>(c.v + at * kKvBlock * D)[tid] =
+                        make_uint4(s_v[par][0][tid], s_v[par][1][tid], s_v[par][2][tid], s_v[par][3][tid]);
             }
         }
-        // the rows of the block left open
-        if (count < kKvBlock)
-            for (int t = warp; t < count; t += 4)
-                if (first + t >= q.past)
-#pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        c.open_k[open + t * D + lane * N + i] = s_x[0][t][lane * N + i];
-                        c.open_v[open + t * D + lane * N + i] = s_x[1][t][lane * N + i];
-                    }
         if (!both || blk != blk0) break;
+        __syncthreads();       // the open rows have been read, and the next block's maxima start at zero
+        if (tid < 4) s_amax[tid / 2][tid % 2] = 0u;
         __syncthreads();
     }
 }
@@ -320,10 +469,10 @@ cudaError_t launch_qk_norm_rope(const KvBatchDev &b, const RopeDev &rope, const 
                                 int *err, cudaStream_t st)
 {
     // few tokens: one load a warp, for the shortest time; many: a token's heads up to four loads' worth a turn
-    const int heads = (in.q ? in.q_heads : 0) + (in.k ? in.kv_heads : 0);
     return by_type(in.act, D, [&](auto d, auto t) {
         using L = HeadLanes<decltype(d)::value, decltype(t)>;
-        const int group = b.T <= 512 ? L::kHeads : kAhead * L::kHeads * 2, groups = (heads + group - 1) / group;
+        const int group = b.T <= 512 ? L::kHeads : kAhead * L::kHeads * 2;
+        const int groups = (in.q ? (in.q_heads + group - 1) / group : 0) + (in.k ? (in.kv_heads + group - 1) / group : 0);
         return launch_dependent(qk_norm_rope_kernel<decltype(d)::value, decltype(t)>,
                                 dim3((unsigned)(((int64_t)b.T * groups + kRowWarps - 1) / kRowWarps)), dim3(kRowWarps * 32), 0, st, b,
                                 rope, in, out, group, groups, err);
@@ -333,12 +482,13 @@ cudaError_t launch_qk_norm_rope(const KvBatchDev &b, const RopeDev &rope, const 
 cudaError_t launch_kv_append(const KvCacheDev &c, const KvBatchDev &b, const RopeDev *rope, const AttnRows &rows, int *err,
                              cudaStream_t st)
 {
-    const dim3 grid((unsigned)(b.T / kKvBlock + 2 * b.B), (unsigned)c.heads);
+    // few blocks: a head a CTA, for the shortest time; many: the heads share the angles
+    const unsigned blocks = (unsigned)(b.T / kKvBlock + 2 * b.B);
+    const int group = blocks >= 512 ? std::min(c.heads, 4) : 1;
     const RopeDev none{};
     return by_type(rows.act, c.D, [&](auto d, auto t) {
-        kv_append_kernel<decltype(d)::value, decltype(t)><<<grid, 128, 0, st>>>(c, b, rope ? *rope : none, rope != nullptr,
-                                                                               rows, err);
-        return cudaGetLastError();
+        return launch_dependent(kv_append_kernel<decltype(d)::value, decltype(t)>, dim3(blocks, (c.heads + group - 1) / group), dim3(128),
+                                0, st, c, b, rope ? *rope : none, (int)(rope != nullptr), rows, group, err);
     });
 }
 
