@@ -29,7 +29,9 @@ namespace jmoe {
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kCtasPerSm = 2;                // one joins its parts while the other streams
+// CTAs of an SM: one joins its parts while the others stream. Three where eight
+// rows of queries are all that a CTA holds (shared memory), else two.
+constexpr int kMaxCtasPerSm = 3;
 constexpr int kTile = 64;                    // tokens of a tile: 4 blocks
 constexpr int kMaxRows = kWarps * 16;        // rows of a chunk
 // A run has at least this many tiles: fewer CTAs share a short sequence.
@@ -49,7 +51,10 @@ constexpr size_t kPartialBytes = (size_t)kMaxRows * (kMaxHeadDim + 2) * 4;
 
 // Behind them the queries of attn_tiles.cu, a slice of the rows at a time.
 constexpr size_t kTilesBytes = (size_t)80 << 20;
-size_t tiles_off(int num_sms) { return partial_off(num_sms * kCtasPerSm) + (size_t)num_sms * kCtasPerSm * 2 * kPartialBytes; }
+size_t tiles_off(int num_sms)
+{
+    return partial_off(num_sms * kMaxCtasPerSm) + (size_t)num_sms * kMaxCtasPerSm * 2 * kPartialBytes;
+}
 
 // Values of a sequence without a scale (an all-zero block): far below any real
 // scale (>= 2^-74), so its weights stay small and its sums in range.
@@ -201,14 +206,14 @@ struct Shape {
     static constexpr int kVBlk = kBlk + 32;                      // value blocks in shared memory: off the banks of each other
     static constexpr int kQRow = D * 2 + 16;                     // bytes of a query row in f16
     static constexpr int kKBytes = kWarps * 4 * kBlk, kVBytes = kWarps * 4 * kVBlk;
-    static constexpr int kQBytes = kWarps * kRows * kQRow * (SPLIT ? 2 : 1);
-    static constexpr int kSumBytes = kWarps * kRows * D * 4;     // the warps' sums, where the queries were
-    static constexpr int kRowOff = kKBytes + kVBytes + (kQBytes > kSumBytes ? kQBytes : kSumBytes);
-    static constexpr int kSmem = kRowOff + kWarps * D * 4;       // a head row of each warp while it is rotated
+    static constexpr int kRowOff = kKBytes + kVBytes;            // a head row of each warp while it is rotated
+    static constexpr int kQOff = kRowOff + kWarps * D * 4;       // queries, upper halves, then the lower ones
+    static constexpr int smem(int group) { return kQOff + group * kRows * kQRow * (SPLIT ? 2 : 1); }
+    static_assert(kWarps * kRows * D * 4 <= kKBytes + kVBytes, "the warps' sums lie where their tiles were");
 };
 
 template <int D, typename T, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+__global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
     attend_stream_kernel(const __grid_constant__ AttnParams p, int seq0, int seq1, int group, uint32_t g_mul, int *counters,
                          float *partials)
 {
@@ -218,13 +223,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     __shared__ __align__(8) uint64_t s_full[2][kWarps], s_empty[2][kWarps];   // keys, values
     __shared__ float s_m[kWarps][RR], s_l[kWarps][RR], s_rf[kMaxRows];
     __shared__ int s_last, s_abort;
-    uint8_t *s_q = smem + Sh::kKBytes + Sh::kVBytes;          // queries: f16 rows, with SPLIT the lower halves behind them
-    float *s_sum = reinterpret_cast<float *>(s_q);
+    uint8_t *s_q = smem + Sh::kQOff;                          // queries: f16 rows, with SPLIT the lower halves behind them
+    float *s_sum = reinterpret_cast<float *>(smem);           // the warps' sums of a finished segment
     const uint32_t kbase = smem_addr(smem), vbase = kbase + Sh::kKBytes;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, ln = lane / 4, lj = lane % 4;
     const int streams = kWarps / group, stream = warp / group, rt = warp % group, depth = group;
     const int g = p.rows.q_heads / p.c.heads, chunk_rows = group * RR, me = blockIdx.x;
     const bool leader = rt == 0;
+    const int q_lower = chunk_rows * Sh::kQRow;
     // n / g for numbers below 2^32 / g
     auto over_g = [&](int n) -> int { return g == 1 ? n : (int)__umulhi((uint32_t)n, g_mul); };
 
@@ -392,34 +398,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     float m[U], l[U], o[NT][SPLIT ? 2 : 4];
     __syncthreads();
     for (;;) {
-        // ---- a segment's beginning: its first loads are on their way while the one
-        // before is joined
-        const bool more = next_segment(sg);
-        constexpr int kAhead = 2;             // query rows a warp asks for at once
-        float qv[kAhead][N], sk = 0.0f, sv = 0.0f;
-        int64_t blk = -1;
-        if (more) {
-            int tok;
-#pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (warp + i * kWarps < sg.rows) load_vals<N>(row_ptr(sg, warp + i * kWarps, tok), qv[i]);
-            blk = lookup(sg, sg.t0 + stream);
-            if (leader)
-                for (int i = 0; i < depth; i++) {
-                    const int t = sg.t0 + stream + i * streams;
-                    if (t >= sg.t1) break;
-                    const int64_t first = i ? lookup(sg, t) : blk;
-#pragma unroll 1
-                    for (int which = 0; which < 2; which++) issue(which, first, done + i);
-                }
-            scales(blk, sk, sv);
-        }
-
         // ---- the warps' parts of the segment before, and the CTAs'
         if (joining) {
             const int taken = cur.t1 - cur.t0, used = min(streams, taken);
-            float *part = s_sum + warp * RR * D;      // the queries are in registers by now
-            __syncthreads();
+            float *part = s_sum + warp * RR * D;
+            __syncthreads();          // every warp is done with its tiles
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
@@ -459,74 +442,55 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 return s_last;
             };
             // Joins the parts of n CTAs, c, c + step, ...: into the output, or into the
-            // first one's part. A warp takes two rows at a time, a lane D / 32 values
-            // and a part's maximum and sum; all loads are under way before the first is used.
+            // first one's part. A warp takes a row at a time, a lane D / 32 values and a
+            // part's maximum and sum; all loads are under way before the first is used.
             auto join = [&](int c, int step, int n, bool finish) {
-                for (int r0 = warp * 2; r0 < cur.rows; r0 += 2 * kWarps) {
-                    float M[2], a[2], den[2], acc[2][N];
+                for (int r = warp; r < cur.rows; r += kWarps) {
+                    float M = -INFINITY, den = 0.0f, acc[N];
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        M[k] = -INFINITY;
-                        den[k] = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < N; i++) acc[k][i] = 0.0f;
-                    }
+                    for (int i = 0; i < N; i++) acc[i] = 0.0f;
                     for (int i0 = 0; i0 < n; i0 += kJoin) {
                         const int cn = min(kJoin, n - i0);
-                        float2 ml[2];
-                        float v[2][kJoin][N];
+                        float v[kJoin][N];
+                        const float2 ml = lane < cn ? __ldcg(reinterpret_cast<const float2 *>(part_of(c + (i0 + lane) * step) + 2 * r))
+                                                    : make_float2(-INFINITY, 0.0f);
 #pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            const int r = min(r0 + k, cur.rows - 1);
-                            ml[k] = lane < cn ? __ldcg(reinterpret_cast<const float2 *>(part_of(c + (i0 + lane) * step) + 2 * r))
-                                              : make_float2(-INFINITY, 0.0f);
-#pragma unroll
-                            for (int i = 0; i < kJoin; i++) {
-                                if (i < cn) {
-                                    const float *src = part_of(c + (i0 + i) * step) + 2 * kMaxRows + r * D + lane * N;
-                                    if constexpr (N == 4) {
-                                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(src));
-                                        v[k][i][0] = x.x; v[k][i][1] = x.y; v[k][i][2] = x.z; v[k][i][3] = x.w;
-                                    } else {
-                                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(src));
-                                        v[k][i][0] = x.x; v[k][i][1] = x.y;
-                                    }
+                        for (int i = 0; i < kJoin; i++) {
+                            if (i < cn) {
+                                const float *src = part_of(c + (i0 + i) * step) + 2 * kMaxRows + r * D + lane * N;
+                                if constexpr (N == 4) {
+                                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(src));
+                                    v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
                                 } else {
-#pragma unroll
-                                    for (int j = 0; j < N; j++) v[k][i][j] = 0.0f;
+                                    const float2 x = __ldcg(reinterpret_cast<const float2 *>(src));
+                                    v[i][0] = x.x; v[i][1] = x.y;
                                 }
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < N; j++) v[i][j] = 0.0f;
                             }
                         }
+                        const float top = fmaxf(M, warp_max_f(ml.x)), ms = top == -INFINITY ? 0.0f : top;
+                        const float before = ex2(M - ms), a = ex2(ml.x - ms);
+                        M = top;
+                        den = fmaf(den, before, warp_sum_f(ml.y * a));
 #pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            const float top = fmaxf(M[k], warp_max_f(ml[k].x)), ms = top == -INFINITY ? 0.0f : top;
-                            const float before = ex2(M[k] - ms);
-                            M[k] = top;
-                            a[k] = ex2(ml[k].x - ms);
-                            den[k] = fmaf(den[k], before, warp_sum_f(ml[k].y * a[k]));
+                        for (int j = 0; j < N; j++) acc[j] *= before;
 #pragma unroll
-                            for (int j = 0; j < N; j++) acc[k][j] *= before;
+                        for (int i = 0; i < kJoin; i++) {
+                            const float ai = __shfl_sync(0xffffffffu, a, i);
 #pragma unroll
-                            for (int i = 0; i < kJoin; i++) {
-                                const float ai = __shfl_sync(0xffffffffu, a[k], i);
-#pragma unroll
-                                for (int j = 0; j < N; j++) acc[k][j] = fmaf(v[k][i][j], ai, acc[k][j]);
-                            }
+                            for (int j = 0; j < N; j++) acc[j] = fmaf(v[i][j], ai, acc[j]);
                         }
                     }
+                    if (finish) {
+                        write_out(r, lane * N, acc, den);
+                    } else {
+                        float *dst = part_of(c);
+                        __syncwarp();          // its maximum and sum have been read
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const int r = r0 + k;
-                        if (r >= cur.rows) break;
-                        if (finish) {
-                            write_out(r, lane * N, acc[k], den[k]);
-                        } else {
-                            float *dst = part_of(c);
-                            __syncwarp();          // its maximum and sum have been read
-#pragma unroll
-                            for (int j = 0; j < N; j++) dst[2 * kMaxRows + r * D + lane * N + j] = acc[k][j];
-                            if (lane == 0) *reinterpret_cast<float2 *>(dst + 2 * r) = make_float2(M[k], den[k]);
-                        }
+                        for (int j = 0; j < N; j++) dst[2 * kMaxRows + r * D + lane * N + j] = acc[j];
+                        if (lane == 0) *reinterpret_cast<float2 *>(dst + 2 * r) = make_float2(M, den);
                     }
                 }
             };
@@ -554,7 +518,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                     if (d == 0) *reinterpret_cast<float2 *>(mine + 2 * r) = make_float2(M, den);
                 }
             }
-            __syncthreads();   // the sums are read before the next queries go there
+            fence_async_smem();
+            __syncthreads();   // the sums are read before the next tiles are copied there
             if (!whole_seg) {
                 // Whichever CTA brings a group's last part joins the group, in order;
                 // whichever brings the last group joins the groups.
@@ -568,7 +533,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 }
             }
         }
-        if (!more) break;
+        // ---- a segment's beginning: its first loads
+        if (!next_segment(sg)) break;
+        constexpr int kAhead = 2;             // query rows a warp asks for at once
+        float qv[kAhead][N], sk = 0.0f, sv = 0.0f;
+        int64_t blk = -1;
+        {
+            int tok;
+#pragma unroll
+            for (int i = 0; i < kAhead; i++)
+                if (warp + i * kWarps < sg.rows) load_vals<N>(row_ptr(sg, warp + i * kWarps, tok), qv[i]);
+            blk = lookup(sg, sg.t0 + stream);
+            if (leader)
+                for (int i = 0; i < depth; i++) {
+                    const int t = sg.t0 + stream + i * streams;
+                    if (t >= sg.t1) break;
+                    const int64_t first = i ? lookup(sg, t) : blk;
+#pragma unroll 1
+                    for (int which = 0; which < 2; which++) issue(which, first, done + i);
+                }
+            scales(blk, sk, sv);
+        }
 
         // ---- queries of the chunk to shared memory as f16, scaled per row by a power
         // of two that takes the largest value to [2^14, 2^15): what is 2^-28 of it is still held in full
@@ -612,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
                 for (int i = 0; i < N / 2; i++) {
                     y[i] = hi[i];
-                    if (SPLIT) y[i + kWarps * RR * Sh::kQRow / 4] = lo[i];
+                    if (SPLIT) y[i + q_lower / 4] = lo[i];
                 }
             }
         }
@@ -643,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                     z[u] = a.z;
                     z[2 + u] = a.w;
                     if constexpr (SPLIT) {
-                        const uint4 c = y[kWarps * RR * Sh::kQRow / 16 + h * 8 + i];
+                        const uint4 c = y[q_lower / 16 + h * 8 + i];
                         x[1] = c.x;
                         x[3] = c.y;
                         z[1] = c.z;
@@ -757,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             const uint32_t va = vbase + (slot * 4 + lj) * Sh::kVBlk + ln * 16;
             // a tile's sums start at zero and join the running ones in f32, rounded to
             // nearest: the tensor cores' additions round towards zero
-            constexpr int PV = SPLIT ? 8 : 4;
+            constexpr int PV = 4;
 #pragma unroll
             for (int i0 = 0; i0 < NT; i0 += PV) {
                 uint4 vw[PV];
@@ -812,7 +797,7 @@ cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !set[dev]) {
-        if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem)) != cudaSuccess) return e;
+        if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::smem(kWarps))) != cudaSuccess) return e;
         if (dev < 64) set[dev] = true;
     }
     // warps that share a tile: one for each row tile, up to all eight
@@ -823,15 +808,15 @@ cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
     int group = 1;
     while (group < kWarps && (int64_t)group * Sh::kRows < rows) group *= 2;
     uint8_t *ws = static_cast<uint8_t *>(p.ws);
-    const int ctas = p.num_sms * kCtasPerSm;
+    const int ctas = p.num_sms * (SPLIT && group == 1 ? 3 : 2);
     // a launch's tiles are counted in 32 bits: sequences that could have more go in several
     const int64_t most = (((int64_t)p.c.table_stride * kKvBlock << p.c.page_shift) / kTile + 2) * p.c.heads *
                          ((rows + group * Sh::kRows - 1) / (group * Sh::kRows));
     const int step = (int)std::max<int64_t>(1, std::min<int64_t>(p.b.B, (int64_t)INT_MAX / most));
     for (int s = 0; s < p.b.B; s += step) {
-        e = launch_dependent(kern, dim3(ctas), dim3(kThreads), Sh::kSmem, st, p, s, std::min(p.b.B, s + step), group,
+        e = launch_dependent(kern, dim3(ctas), dim3(kThreads), Sh::smem(group), st, p, s, std::min(p.b.B, s + step), group,
                              g > 1 ? (uint32_t)((1ull << 32) / g + 1) : 0u, reinterpret_cast<int *>(ws + kCounterOff),
-                             reinterpret_cast<float *>(ws + partial_off(ctas)));
+                             reinterpret_cast<float *>(ws + partial_off(p.num_sms * kMaxCtasPerSm)));
         if (e != cudaSuccess) return e;
     }
     if (prompts) return launch_attention_tiles(p, kFewRows, ws + tiles_off(p.num_sms), kTilesBytes, st);
