@@ -268,7 +268,7 @@ int moe_lm_head(moe_ctx *ctx, int32_t T, const float *normed, float *logits, int
  * output projection's input. Device pointers on the context's device
  * throughout; asynchronous on the context's stream; the caller owns all memory
  * named here, the context a fixed workspace. The first of these calls on a
- * context allocates it (about 100 MiB), so make that call before capturing the
+ * context allocates it (about 110 MiB), so make that call before capturing the
  * stream into a graph. Calls on one context, replays of graphs captured from
  * it among them, are serialised by the caller as every other call.
  *
@@ -276,7 +276,8 @@ int moe_lm_head(moe_ctx *ctx, int32_t T, const float *normed, float *logits, int
  * out of range, row_start not ascending or past n_tokens, more than max_new
  * rows, a negative past, a sequence longer than its page table, a slot twice in
  * one append) skips that sequence, or that page, and is reported by
- * moe_device_status as MOE_ERR_TENSOR_BOUNDS. */
+ * moe_device_status as MOE_ERR_TENSOR_BOUNDS; where row_start is out of order,
+ * other sequences of the batch may be skipped as well. */
 
 /* Types of activation rows: ggml_type ids. */
 typedef enum moe_act {
@@ -285,6 +286,7 @@ typedef enum moe_act {
     MOE_ACT_BF16 = 30
 } moe_act;
 
+#define MOE_KV_MAX_TOKENS (1 << 29)   /* of a slot: table_stride * page_tokens */
 #define MOE_KV_BLOCK_TOKENS 16   /* tokens that share a scale, as the blocks of the reference's arena (src/kv.rs:1-4) */
 
 /* One layer's KV cache. A block of 16 tokens and one head is held as signed
@@ -303,7 +305,8 @@ typedef struct moe_kv_cache {
     int32_t n_pages;
     int32_t n_slots;       /* rows of page_table, open_k and open_v */
     int32_t table_stride;  /* page ids of a row */
-    const int32_t *page_table;   /* [n_slots][table_stride]; entries past a sequence's end are not read */
+    const int32_t *page_table;   /* [n_slots][table_stride]; entries past a sequence's end are not
+                                  * read, nor by attention those of pages before every row's window */
     int8_t *k;             /* [n_pages][kv_heads][page_tokens / 16][D / 64][16][64] */
     int8_t *v;             /* [n_pages][kv_heads][page_tokens / 16][D][16] */
     float *k_scale, *v_scale;    /* [n_pages][kv_heads][page_tokens / 16] */
@@ -325,7 +328,7 @@ typedef struct moe_kv_batch {
 /* Norm and rotation of query and key heads: x * rsqrt(mean(x^2) + eps) * norm
  * (per head, where the weight is given), then the first rope_dim values rotated
  * by position * inv_freq[i] and scaled by mscale. Angles are formed in f64; the
- * keys of the cache in f64 throughout, then rounded to f32. */
+ * keys of the cache to 2^-40 of their largest or better, then rounded to f32. */
 typedef struct moe_rope {
     int32_t rope_dim;           /* even, 0 .. head_dim; 0: no rotation */
     int32_t interleaved;        /* 0: value i turns with i + rope_dim / 2; 1: 2i with 2i + 1 */
@@ -376,7 +379,7 @@ int moe_kv_read(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *bat
  * b sees the tokens at positions <= past[b] + i (its own key must be cached),
  * the last opts->window of them; query head h reads key head
  * h / (q_heads / kv_heads). out rows hold q_heads * head_dim values of
- * rows->act, out_stride elements apart. A row whose every page is bad gets
+ * rows->act, out_stride elements apart, and overlap no input. A row whose every page is bad gets
  * zeros. Softmax and sums in f32; with F32 rows the products carry 22 bits of
  * the queries and weights, with 16-bit rows 11. opts may be NULL. */
 int moe_kv_attention(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_attn_opts *opts,

@@ -1456,7 +1456,10 @@ int moe_device_status(moe_ctx *ctx, int32_t *status)
         CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream), "status sync");
         *status = *ctx->status_host;
         if (*status) {
-            CUDA_TRY(ctx, cudaMemsetAsync(ctx->attn_ws, 0, sizeof(int), ctx->stream), "clear status");
+            // after a wait that ran out the arrival counters are as it left them
+            CUDA_TRY(ctx, cudaMemsetAsync(ctx->attn_ws, 0, *status == kErrKvBounds ? sizeof(int) : attn_counter_bytes(ctx->num_sms),
+                                          ctx->stream),
+                     "clear status");
             if (*status != kErrKvBounds)
                 return fail(ctx, MOE_ERR_TIMEOUT, "a bounded device wait ran out in an attention call (status %d)",
                             *status);
@@ -2095,6 +2098,7 @@ int moe_forward_ep(moe_ctx *ctx, int32_t layer, int32_t T, const float *x, float
 // ------------------------------------------------- the attention sublayer
 
 static bool misaligned(const void *p) { return ((uintptr_t)p & 15) != 0; }
+static bool misaligned4(const void *p) { return ((uintptr_t)p & 3) != 0; }   // int32 and f32 arrays
 
 static size_t act_size(int act) { return act == MOE_ACT_F32 ? 4 : 2; }
 
@@ -2110,6 +2114,8 @@ static int check_batch(moe_ctx *ctx, int max_tokens, const moe_kv_batch *b, KvBa
     if (!b->row_start && b->n_tokens != b->n_seqs)
         return fail(ctx, MOE_ERR_INVALID_ARGS, "without row_start a batch has one row per sequence (%d rows, %d sequences)",
                     b->n_tokens, b->n_seqs);
+    if (misaligned4(b->past) || misaligned4(b->row_start) || misaligned4(b->slot))
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "batch arrays must be 4-byte aligned");
     out->B = b->n_seqs;
     out->T = b->n_tokens;
     out->max_new = !b->row_start ? 1 : b->max_new ? std::min(b->max_new, b->n_tokens) : b->n_tokens;
@@ -2125,6 +2131,8 @@ static int check_rope(moe_ctx *ctx, const moe_rope *r, int head_dim, RopeDev *ou
         return fail(ctx, MOE_ERR_INVALID_ARGS, "rope_dim %d must be even, 0..%d", r->rope_dim, head_dim);
     if (!std::isfinite(r->eps) || r->eps < 0.0) return fail(ctx, MOE_ERR_INVALID_ARGS, "eps must be finite and >= 0");
     if (!std::isfinite(r->mscale)) return fail(ctx, MOE_ERR_INVALID_ARGS, "mscale must be finite");
+    if (misaligned4(r->q_norm) || misaligned4(r->k_norm))
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "norm weights must be 4-byte aligned");
     if (r->rope_dim && !r->inv_freq && !(std::isfinite(r->theta) && r->theta > 0.0))
         return fail(ctx, MOE_ERR_INVALID_ARGS, "theta must be positive where inv_freq is not given");
     out->R = r->rope_dim;
@@ -2182,6 +2190,12 @@ static int check_cache(moe_ctx *ctx, const moe_kv_cache *c, const moe_kv_batch *
         return fail(ctx, MOE_ERR_INVALID_ARGS, "null cache array");
     if (misaligned(c->k) || misaligned(c->v) || misaligned(c->open_k) || misaligned(c->open_v))
         return fail(ctx, MOE_ERR_INVALID_ARGS, "cache arrays must be 16-byte aligned");
+    if (misaligned4(c->page_table) || misaligned4(c->k_scale) || misaligned4(c->v_scale))
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "page table and scales must be 4-byte aligned");
+    // the kernels count a launch's tiles of 64 tokens, over the key heads, in 32 bits
+    const int64_t tokens = (int64_t)c->table_stride * c->page_tokens;
+    if (tokens > MOE_KV_MAX_TOKENS || tokens / 64 * c->kv_heads > (1 << 29))
+        return fail(ctx, MOE_ERR_CAPABILITY_MISMATCH, "page tables of %lld tokens with %d key heads", (long long)tokens, c->kv_heads);
     if (!b->slot && b->n_seqs > c->n_slots)
         return fail(ctx, MOE_ERR_TENSOR_BOUNDS, "%d sequences without slots, %d slots", b->n_seqs, c->n_slots);
     *out = KvCacheDev{c->head_dim, c->kv_heads, c->n_pages, c->n_slots, c->table_stride, shift, c->page_table,
@@ -2301,6 +2315,9 @@ static int check_attention(moe_ctx *ctx, int max_tokens, const moe_kv_cache *cac
     if (rows->head_dim != cache->head_dim || rows->kv_heads != cache->kv_heads || rows->q_heads % cache->kv_heads)
         return fail(ctx, MOE_ERR_INVALID_ARGS, "rows of %d query and %d key heads of %d, cache of %d heads of %d",
                     rows->q_heads, rows->kv_heads, rows->head_dim, cache->kv_heads, cache->head_dim);
+    if ((int64_t)batch->n_tokens * (rows->q_heads / cache->kv_heads) > (1 << 30))   // counted in 32 bits
+        return fail(ctx, MOE_ERR_CAPABILITY_MISMATCH, "%d rows of %d query heads a key head", batch->n_tokens,
+                    rows->q_heads / cache->kv_heads);
     p->use_rope = rope != nullptr;
     p->scale = opts && opts->scale != 0.0f ? opts->scale : (float)(1.0 / std::sqrt((double)cache->head_dim));
     if (!std::isfinite(p->scale)) return fail(ctx, MOE_ERR_INVALID_ARGS, "scale must be finite");

@@ -836,6 +836,7 @@ cudaError_t launch_t(const AttnParams &p, cudaStream_t st)
 
 }  // namespace
 
+size_t attn_counter_bytes(int num_sms) { return partial_off(num_sms * kMaxCtasPerSm); }
 size_t attn_workspace_bytes(int num_sms) { return tiles_off(num_sms) + kTilesBytes; }
 
 cudaError_t launch_attention(const AttnParams &p, cudaStream_t st)

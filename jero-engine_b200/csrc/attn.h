@@ -58,6 +58,8 @@ struct AttnParams {
 
 // Bytes of a context's attention workspace.
 size_t attn_workspace_bytes(int num_sms);
+// Of them, from the start: the status word and the arrival counters, zero between calls.
+size_t attn_counter_bytes(int num_sms);
 
 // Attention of the sequences with more than few_rows rows (tokens times query
 // heads of a key head) on tcgen05; the others' rows are left alone.

@@ -165,9 +165,8 @@ __device__ __forceinline__ double root_f64(double x)
 
 constexpr int kAppendWarps = 8, kPer = kKvBlock / kAppendWarps;      // tokens of a warp
 
-// A number as the unevaluated sum of two f32, good to 2^-46 or so: the keys'
-// arithmetic, at f32's rate. (f64 instructions are eight times as dear here:
-// the same kernel in f64 took 52 us where this takes @@.)
+// A number as the unevaluated sum of two f32, good to 2^-45 or so: the keys'
+// arithmetic, at f32's rate (64 tokens of 64 sequences: 8.1 us in f64, 6.9 so).
 struct Two {
     float h, l;
 };
@@ -185,7 +184,7 @@ __device__ __forceinline__ Two dot2(Two a, Two b, Two c, Two d)
     const float s = p + q, t = s - p;
     const float l = ((p - (s - t)) + (q - t)) + (e + f);
     const float h = s + l;
-    return {h, (s - h) + l};
+    return fabsf(s) < INFINITY ? Two{h, (s - h) + l} : Two{s, 0.0f};   // an infinite key stays one
 }
 
 // One CTA per (touched block, group of heads): warp w has the block's tokens
@@ -228,7 +227,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3)
     if (s < 0 || !seq_info(b, s, q) || !seq_in_cache(c, b, s, q, slot) || q.n == 0) return;
     const int total = q.past + q.n, blk0 = q.past / kKvBlock, blk_end = (total + kKvBlock - 1) / kKvBlock;
     const int blk1 = blk0 + (u - (q.row0 / kKvBlock + 2 * s));
-    if (blk1 >= blk_end) return;
+    if (blk1 < blk0 || blk1 >= blk_end) return;     // below: row_start out of order
     // The first block reads the open rows and the last writes them: where both
     // do, one CTA takes the two in turn.
     const bool both = blk_end - 1 > blk0 && q.past % kKvBlock && total % kKvBlock;

@@ -189,7 +189,7 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int e, int g, int
     const bool ok = seq_info(p.b, s, it.q) && seq_in_cache(p.c, p.b, s, it.q, it.slot);
     if (!ok) return false;
     const int first = (e - first_entry(p.b, s, g)) * kRowsItem, rows = it.q.n * g;
-    if (first >= rows || rows <= few_rows) return false;
+    if (first < 0 || first >= rows || rows <= few_rows) return false;   // below 0: row_start out of order
     it.tok = first / g;
     it.rem = first - it.tok * g;
     it.rows = min(kRowsItem, rows - first);

@@ -63,6 +63,8 @@ def test_check_takes_good_arguments():
     _check(_args(rows__act=jm.BF16, cache__page_tokens=16, opts__window=100, rope__rope_dim=0))
     _check(_args(batch=dict(n_seqs=2, n_tokens=7, past=1 << 20, row_start=1 << 20, slot=1 << 20)))
     _check(_args(batch=dict(n_seqs=0, n_tokens=0)))
+    _check(_args(cache__table_stride=1 << 23))
+    _check(_args(max_tokens=1 << 30, batch__n_tokens=1 << 27, batch__row_start=1 << 20, rope__q_norm=(1 << 20) + 4))
 
 
 @pytest.mark.parametrize("over,error", [
@@ -109,6 +111,17 @@ def test_check_takes_good_arguments():
     (dict(out=(1 << 20) + 4), jm.InvalidArguments),
     (dict(out_stride=4095), jm.InvalidArguments),
     (dict(out_stride=2048), jm.TensorBoundsError),
+    (dict(cache__page_table=(1 << 20) + 2), jm.InvalidArguments),
+    (dict(cache__v_scale=(1 << 20) + 1), jm.InvalidArguments),
+    (dict(cache__table_stride=(1 << 23) + 1), jm.CapabilityMismatch),
+    (dict(cache__table_stride=1 << 22, cache__kv_heads=512, rows__kv_heads=512, rows__q_heads=512, rows__q_stride=1 << 16,
+          rows__k_stride=1 << 16, rows__v_stride=1 << 16, out_stride=1 << 16), jm.CapabilityMismatch),
+    (dict(batch__past=(1 << 20) + 2), jm.InvalidArguments),
+    (dict(batch__slot=(1 << 20) + 1), jm.InvalidArguments),
+    (dict(batch__row_start=(1 << 20) + 3), jm.InvalidArguments),
+    (dict(rope__q_norm=(1 << 20) + 2), jm.InvalidArguments),
+    (dict(rope__k_norm=(1 << 20) + 1), jm.InvalidArguments),
+    (dict(max_tokens=1 << 30, batch__n_tokens=(1 << 27) + 1, batch__row_start=1 << 20), jm.CapabilityMismatch),
 ])
 def test_check_refuses(over, error):
     with pytest.raises(error):
@@ -786,3 +799,177 @@ def test_two_contexts_on_two_streams(make):
     for i, (ctx, b, r, out, q) in enumerate(work):
         s.check_attention(out.double().cpu().numpy(), q, [s.lens[i] - 1], [1], [i])
     other.close()
+
+
+# ------------------------------------------------------- batches at the edges
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,hq", [("f32", 8), ("bf16", 16), ("f16", 64)])
+def test_attention_of_more_sequences_than_lanes(make, act, hq):
+    """70 sequences (a plan of several passes) of 8 key heads, more segments than CTAs: runs cross segments."""
+    s = make(act, D=64, q_heads=hq, kv_heads=8, page=16, n_slots=70, pages_per_slot=12)
+    total = [1 + (37 * i) % 190 for i in range(70)]
+    s.append([0] * 30, total[:30], range(30), rows=s.rows(sum(total[:30])))
+    s.append([0] * 40, total[30:], range(30, 70), rows=s.rows(sum(total[30:])))
+    order = s.rng.permutation(70).tolist()
+    past = [total[i] - 1 for i in order]
+    s.attend(past, [1] * 70, order, max_new=1)
+    new = [min(total[i], (i * 5) % 4) for i in order]
+    s.attend([total[i] - n for i, n in zip(order, new)], new, order, behind=2)
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_attention_single_tokens_and_prompts_in_one_call(make, act):
+    s = make(act, D=128, q_heads=8, kv_heads=2, page=32, n_slots=6, pages_per_slot=16)
+    total = [400, 130, 77, 1, 500, 300]
+    s.append([0] * 6, total, range(6), rows=s.rows(sum(total)))
+    new = [1, 100, 0, 1, 5, 300]
+    for scale in (None, -0.05):
+        s.attend([t - n for t, n in zip(total, new)], new, range(6), behind=3, scale=scale)
+    s.attend([t - n for t, n in zip(total, new)], new, range(6), window=50, max_new=300)
+    s.attend([t - 1 for t in total], [1] * 6, range(6), scale=-0.3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16"])
+def test_attention_prompts_past_the_workspace(make, act):
+    """More query rows than the workspace takes at once: several passes over the list."""
+    n = 24 if act == "f32" else 46
+    s = make(act, D=128, q_heads=32, kv_heads=32, page=16, n_slots=n, pages_per_slot=6)
+    new = [65 + i % 7 for i in range(n)]
+    s.append([0] * n, new, range(n), rows=s.rows(sum(new)))
+    s.attend([0] * n, new, range(n))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("D,R,interleaved", [(128, 34, False), (64, 2, False), (128, 6, True), (64, 50, False)])
+def test_step_with_odd_rotations(make, act, D, R, interleaved):
+    """Pairs that do not lie lane by lane, through the append, few rows and many."""
+    s = make(act, D=D, q_heads=6, kv_heads=2, page=16, n_slots=2, pages_per_slot=16)
+    rope, plain = s.rope(rope_dim=R, interleaved=interleaved, mscale=1.25)
+    past = [0, 0]
+    for new in ([70, 3], [1, 1], [90, 30], [2, 1]):
+        r, x, q, k, v = s.rows(sum(new))
+        out = s.out(sum(new), 6)
+        s.ctx.attention(s.cache, s.batch(past, new, [1, 0]), rope, None, r, out.data_ptr(), 6 * D)
+        at, want = 0, np.empty(q.shape)
+        for i, slot in enumerate((1, 0)):
+            pos = past[i] + np.arange(new[i])
+            rows = slice(at, at + new[i])
+            s.ref.append(slot, past[i], plain(k[rows], "k", pos), v[rows])
+            want[rows] = plain(q[rows], "q", pos)
+            at += new[i]
+            past[i] += new[i]
+            s.lens[slot] = past[i]
+            s.check_blocks(slot)
+        # a query value is off by 24 u (|a| + |b|) <= 34 u of its turned pair's length; over a logit's products with
+        # a key's pairs that is at most 48 u |q| |k|, and the largest sum |q_d k_d| of these normal rows is near
+        # 2 / pi |q| |k|: more than an eighth of it
+        s.check_attention(out.double().cpu().numpy(), want, [p - n for p, n in zip(past, new)], new, [1, 0], q_err=8 * 48 * U)
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_append_infinite_keys_turn(make):
+    """A pair with an infinite value turns into infinite values: bytes of +-127, the rest of the block untouched by them."""
+    s = make("f32", D=64, q_heads=2, kv_heads=1, page=16, n_slots=1, pages_per_slot=4)
+    rope, plain = s.rope(norm=False, theta=100.0)
+    r, x, q, k, v = s.rows(20)
+    x[5, 2 * 64 + 3] = float("inf")
+    x[17, 2 * 64 + 60] = float("-inf")
+    k = x.double().cpu().numpy()[:, 128:192].reshape(20, 1, 64)
+    s.append([0], [20], [0], rope, plain, rows=(r, x, q, k, v))
+    assert np.count_nonzero(np.isinf(s.ref.k[0])) == 4
+    s.check_blocks(0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_window_over_freed_pages(make, act):
+    """Pages before every row's window may have left the page table."""
+    s = make(act, D=64, q_heads=8, kv_heads=2, page=32, n_slots=2, pages_per_slot=20)
+    total = [600, 333]
+    s.append([0, 0], total, [0, 1], rows=s.rows(sum(total)))
+    for new, window in (([1, 1], 64), ([4, 2], 100), ([40, 90], 33)):
+        for i, (t, n) in enumerate(zip(total, new)):
+            s.table[i, : max(0, t - n - window + 1) // 32] = -1
+        s.attend([t - n for t, n in zip(total, new)], new, [0, 1], window=window)
+        s.table.copy_(s.t.tensor(s.table_np, dtype=s.t.int32))
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_row_starts_out_of_order(make, act):
+    """Reported, and nothing outside the batch's rows is written; the call after it is right."""
+    s = make(act, D=64, q_heads=2, kv_heads=2, page=32, n_slots=10, pages_per_slot=20)
+    s.append([0], [600], [6], rows=s.rows(600))
+    r, _, _, _, _ = s.rows(600)
+    for starts in ([-9000] * 6 + [300, 600, -9000, 0, 0], [0, 600, 0, 600, 0, 600, 0, 600, 0, 600, 0],
+                   [600, 500, 400, 300, 200, 100, 0, 600, 7, 5, 600], [2 ** 31 - 1, -2 ** 31] * 5 + [600]):
+        b = jm.KvBatch(n_seqs=10, n_tokens=600, past=s.ints([0] * 10), row_start=s.ints(starts))
+        out = s.out(3 * 9100, 2)
+        before = [x.clone() for x in (s.k, s.k_scale)]
+        s.ctx.kv_attention(s.cache, b, None, r, out[9100:].data_ptr(), 128)
+        with pytest.raises(jm.TensorBoundsError):
+            s.ctx.device_status()
+        assert bool((out[:9100] == 123.0).all()) and bool((out[9700:] == 123.0).all())
+        q2, k2 = s.out(9100 * 3, 2), s.out(9100 * 3, 2)
+        rope, _ = s.rope()
+        s.ctx.qk_norm_rope(b, rope, r, s.into(q2[9100:], k2[9100:]))
+        with pytest.raises(jm.TensorBoundsError):
+            s.ctx.device_status()
+        s.ctx.kv_read(s.cache, b, s.into(k=k2[9100:]))
+        with pytest.raises(jm.TensorBoundsError):
+            s.ctx.device_status()
+        for x in (q2, k2):
+            assert bool((x[:9100] == 123.0).all()) and bool((x[9700:] == 123.0).all())
+        assert all(s.t.equal(a.view(s.t.uint8), b.view(s.t.uint8)) for a, b in zip(before, (s.k, s.k_scale)))
+    other = s.table[6].clone()
+    s.table[6] = min(set(range(s.n_pages)) - set(s.table_np.flat))   # the appends below fill a page that nothing else has
+    for starts in ([-9000] * 6 + [300, 600, -9000, 0, 0], [600, 500, 400, 300, 200, 100, 0, 600, 7, 5, 600]):
+        b = jm.KvBatch(n_seqs=10, n_tokens=600, past=s.ints([0] * 10), row_start=s.ints(starts))
+        s.ctx.kv_append(s.cache, b, None, r)
+        with pytest.raises(jm.TensorBoundsError):
+            s.ctx.device_status()
+    s.table[6] = other
+    s.attend([500], [100], [6])
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_two_graphs_share_a_context(make):
+    """Graphs of single tokens and of prompts, captured from one context, replayed in turn many times."""
+    import torch
+    s = make("bf16", D=128, q_heads=16, kv_heads=4, page=64, n_slots=4, pages_per_slot=40)
+    total = [2400, 900, 64, 2000]
+    s.append([0, 0], total[:2], [0, 1], rows=s.rows(3300))
+    s.append([0, 0], total[2:], [2, 3], rows=s.rows(2064))
+    work = []
+    for new in ([1] * 4, [200, 100, 0, 3]):
+        T = sum(new)
+        r, _, q, _, _ = s.rows(T)
+        past = [t - n for t, n in zip(total, new)]
+        work.append((s.batch(past, new, range(4), max_new=max(new)), r, s.out(T, 16), q, past, new))
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    s.ctx.set_stream(stream.cuda_stream)
+    graphs = []
+    for b, r, out, _, _, _ in work:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            s.ctx.kv_attention(s.cache, b, None, r, out.data_ptr(), 16 * 128)
+        graphs.append(g)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for _ in range(20):
+            for g in graphs:
+                g.replay()
+    torch.cuda.synchronize()
+    for _, _, out, q, past, new in work:
+        s.check_attention(out.double().cpu().numpy(), q, past, new, range(4))
+    assert s.ctx.device_status() == 0
