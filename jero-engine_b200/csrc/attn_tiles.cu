@@ -17,7 +17,12 @@
 // The sums O are scaled down only when a row's maximum has grown by more than
 // 2^8 since they were last: the weights then reach 2^8 instead of 1, which f16
 // holds as exactly. With F32 rows queries and weights are split in two f16
-// halves, each half a product of its own: 22 bits for twice the products.
+// halves, each half a product of its own: 22 bits for twice the products. The
+// tensor cores cut a sum off where f32 would round it, some 2^-26 of it lost,
+// one way, with each step of 16; so there TMEM holds the sums of two tiles only
+// and the softmax threads keep their rows' in registers (rounded sums: 7.8e-7
+// off in all over 2500 tokens, 5e-6 with all the tiles in TMEM), which costs
+// room: 201 us instead of 176 (1500 + 1025 tokens of 3 sequences, 32 heads).
 //
 // Bound by the tensor cores and, as much, by the exponentials: 128 x 128
 // weights take 1024 cycles of the 16 a cycle that the SM gives, the two
@@ -33,10 +38,18 @@ namespace jmoe {
 namespace {
 
 constexpr int kRowsTile = 128, kRowsItem = 256, kKv = 128, kHalf = 64;
-constexpr int kSoftWarps = 8, kConvWarps = 4, kMmaWarp = kSoftWarps + kConvWarps;
-constexpr int kThreads = 16 * 32;    // whole warpgroups: three warps beside the product warp only lend registers
-// Registers a thread after the split: 2 x 152 + 2 x 104 = 4 x the launch's 128.
-constexpr int kSoftRegs = 152, kOtherRegs = 104;
+constexpr int kSoftWarps = 8;
+constexpr int kConvWarps = 4, kMmaWarp = kSoftWarps + kConvWarps;
+constexpr int kThreads = 16 * 32;    // whole warpgroups: two warps beside the product warps only lend registers
+// Registers a thread after the split: 2 x (kSoft + kOther) = 4 x the launch's 128.
+// With F32 rows the softmax threads keep their rows' sums.
+template <bool SPLIT>
+struct Regs {
+    static constexpr int kSoft = SPLIT ? 200 : 152, kOther = SPLIT ? 56 : 104;
+};
+// F32 rows: tiles whose products are summed in TMEM before they join the row's
+// sums (one: 210 us where two take 202; four: 198, and over 1e-6 off).
+constexpr int kFold = 2;
 constexpr float kNoScaleLog2 = -80.0f;
 constexpr int kCubic = 4;            // one pair of weights in this many takes the cubic
 constexpr float kLazy = 8.0f;        // growth of a row's maximum (log2) that its sums are left unscaled for
@@ -314,6 +327,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 {
     using Sh = TileShape<D, SPLIT>;
     constexpr int NB = Sh::kBufs, SL = Sh::kSlabs;
+    // a conversion thread's unit of 16 bytes in every kStep-th block; SPLIT: half of them at a time, for the registers
+    constexpr int kStep = kConvWarps * 32 / D, kTurns = SPLIT ? 2 : 1, kIn = 8 / kStep / kTurns;
+    static_assert(kStep >= 1 && kIn >= 1, "threads");
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(8) uint64_t q_full[2], q_free[2], k_full[NB], k_empty[NB], v_full[NB], v_empty[NB], st_full[2], s_full[2][2],
         p_full[2][2], o_sum[2], o_done[2], drained[2];
@@ -373,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp >= kSoftWarps && warp < kMmaWarp) {
         // ============ conversion: cache bytes -> f16 operands. (After a wait that ran out
         // the warps go on through their barriers: every wait then gives up at once.)
-        regs_down<kOtherRegs>();
+        regs_down<Regs<SPLIT>::kOther>();
         const int ct = tid - kSoftWarps * 32, cw = warp - kSoftWarps;
         fence_proxy_async_global();       // the cache as an append before this left it, to the bulk copies
         uint32_t done = 0, staged = 0;
@@ -428,23 +444,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (lane == 0) s_ok[r] = live & 0xFFu;
                 }
-                {
-                    const int tb = ct % D, sub = ct / D, slab = tb / 64, tok = tb % 64 / 4, c = tb % 4 * 2;
+#pragma unroll
+                for (int u = 0; u < kTurns; u++) {
+                    const int tb = ct % D, sub = ct / D + u * kIn * kStep, slab = tb / 64, tok = tb % 64 / 4, c = tb % 4 * 2;
                     uint8_t *dst = sm_k + buf * Sh::kOperand + slab * (kKv * 128) + tok * 128;
-                    const uint32_t src = smem_addr(sm_st) + ct * 16, x = smem_addr(dst) + ((c ^ (tok & 7)) * 16),
+                    const uint32_t src = smem_addr(sm_st) + (sub * D + tb) * 16, x = smem_addr(dst) + ((c ^ (tok & 7)) * 16),
                                    y = smem_addr(dst) + (((c + 1) ^ (tok & 7)) * 16);
-                    uint4 in[8 * D / 128];
+                    uint4 in[kIn];
 #pragma unroll
-                    for (int i = 0; i < 8 * D / 128; i++) in[i] = lds128(src + i * 2048);
+                    for (int i = 0; i < kIn; i++) in[i] = lds128(src + i * (kStep * D * 16));
 #pragma unroll
-                    for (int i = 0; i < 8 * D / 128; i++) {
+                    for (int i = 0; i < kIn; i++) {
                         const uint4 w = in[i];
                         uint4 a, b;
                         bytes_f16(w.x, a.x, a.y);
                         bytes_f16(w.y, a.z, a.w);
                         bytes_f16(w.z, b.x, b.y);
                         bytes_f16(w.w, b.z, b.w);
-                        const uint32_t o = (i * (128 / D) + sub) * (kKvBlock * 128);
+                        const uint32_t o = (i * kStep + sub) * (kKvBlock * 128);
                         sts128(x + o, a);
                         sts128(y + o, b);
                     }
@@ -456,22 +473,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // ---- values: rows are the head's values, 64 tokens a slab
                 ok &= warp_wait(&st_full[1], done & 1, abort_flag, p.err);
                 ok &= warp_wait(&v_empty[buf], ph ^ 1, abort_flag, p.err);
-                {
-                    const int d = ct % D, sub = ct / D;
+#pragma unroll
+                for (int u = 0; u < kTurns; u++) {
+                    const int d = ct % D, sub = ct / D + u * kIn * kStep;
                     uint8_t *dst = sm_v + buf * Sh::kOperand + d * 128;
-                    const uint32_t src = smem_addr(sm_st + Sh::kStage) + ct * 16, base = smem_addr(dst);
-                    uint4 in[8 * D / 128];
+                    const uint32_t src = smem_addr(sm_st + Sh::kStage) + (sub * D + d) * 16, base = smem_addr(dst);
+                    uint4 in[kIn];
 #pragma unroll
-                    for (int i = 0; i < 8 * D / 128; i++) in[i] = lds128(src + i * 2048);
+                    for (int i = 0; i < kIn; i++) in[i] = lds128(src + i * (kStep * D * 16));
 #pragma unroll
-                    for (int i = 0; i < 8 * D / 128; i++) {
+                    for (int i = 0; i < kIn; i++) {
                         const uint4 w = in[i];
                         uint4 a, b;
                         bytes_f16(w.x, a.x, a.y);
                         bytes_f16(w.y, a.z, a.w);
                         bytes_f16(w.z, b.x, b.y);
                         bytes_f16(w.w, b.z, b.w);
-                        const int blk = i * (128 / D) + sub, c = blk % 4 * 2;
+                        const int blk = i * kStep + sub, c = blk % 4 * 2;
                         const uint32_t o = base + blk / 4 * (D * 128);
                         sts128(o + ((c ^ (d & 7)) * 16), a);
                         sts128(o + (((c + 1) ^ (d & 7)) * 16), b);
@@ -490,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int w = 0; w < 2; w++)
                 if (staged) drain_wait(&st_full[w], (staged - 1) & 1);
     } else if (warp >= kMmaWarp) {
-        regs_down<kOtherRegs>();
+        regs_down<Regs<SPLIT>::kOther>();
         if (warp < kMmaWarp + 2) {
             // ============ products: a warp for each row tile
             fence_proxy_async_global();       // the queries as the kernel before left them
@@ -505,13 +523,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) mbar_arrive(&s_full[i][h]);      // with the scales that the keys came with
                 const uint64_t b = dk + ((buf * Sh::kOperand + h * kHalf * 128) >> 4);
 #pragma unroll
-                for (int half = 0; half < (SPLIT ? 2 : 1); half++)
+                for (int half = SPLIT ? 1 : 0; half >= 0; half--)      // the lower halves first: what they lose is small
 #pragma unroll
                     for (int s = 0; s < SL; s++)
 #pragma unroll
                         for (int k = 0; k < 4; k++)
                             mma_ss(ts + h * kHalf, dq + ((half * SL + s) * kRowsTile * 128 >> 4) + 2 * k, b + (s * kKv * 128 >> 4) + 2 * k,
-                                   id_s, half + s + k != 0);
+                                   id_s, (SPLIT && half == 0) || s + k != 0);
                 commit_one(&s_full[i][h]);
             };
             // O: the weights of half h times the values in buffer buf
@@ -521,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int k = 0; k < 4; k++)
 #pragma unroll
                     for (int half = 0; half < (SPLIT ? 2 : 1); half++)
-                        mma_ts(to, ts + h * kHalf + k / 2 * 32 + k % 2 * 8 + half * 16, b + 2 * k, id_o, half + k != 0 ? 1u : acc);
+                        mma_ts(to, ts + h * kHalf + (SPLIT ? k * 16 + half * 8 : k / 2 * 32 + k % 2 * 8), b + 2 * k, id_o, half + k != 0 ? 1u : acc);
                 commit_one(&o_sum[i]);
             };
             uint32_t done = 0, items = 0, turns = 0;     // tiles of the CTA, items and tiles of this row tile
@@ -560,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int h = 0; h < 2; h++) {
                         if (!wait(&p_full[i][h], turns)) break;
                         tc_fence_after();
-                        sums(h, buf, t > 0 || h > 0);
+                        sums(h, buf, (SPLIT ? t % kFold : t) > 0 || h > 0);
                         if (h) commit_one(&v_empty[buf]);
                         if (last) continue;
                         if (h == 0) {
@@ -589,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // ============ softmax: warpgroup w has row tile w, a thread a row
-        regs_up<kSoftRegs>();
+        regs_up<Regs<SPLIT>::kSoft>();
         const int w = warp / 4, r = tid % kRowsTile + w * kRowsTile;
         const uint32_t ts = tmem + w * kKv + ((uint32_t)(warp % 4 * 32) << 16), to = tmem + 2 * kKv + w * D + ((uint32_t)(warp % 4 * 32) << 16);
         uint32_t done = 0, turns = 0, items = 0;       // tiles of the CTA, tiles and items of this row tile
@@ -605,14 +623,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int pos = live ? it.q.past + tok : INT_MAX;
             const float rf = live ? ld_plain(factors + (int64_t)image * kRowsItem + r) : 0.0f;
             float m = -INFINITY, l = 0.0f;
+            [[maybe_unused]] float tot[SPLIT ? D : 1];     // the row's sums of the tiles before, F32 rows
+            if constexpr (SPLIT)
+#pragma unroll
+                for (int i = 0; i < D; i++) tot[i] = 0.0f;
             for (int u = 0; u < 2 * it.tiles; u++) {
                 // ---- half u & 1 of tile u / 2
                 const int h = u & 1, rr = done & 3, tok0 = (it.tile0 + u / 2) * kKv + h * kHalf;
                 if (!(ok = warp_wait(&s_full[w][h], turns & 1, abort_flag, p.err))) break;
                 tc_fence_after();
-                uint32_t s[kHalf];
-                tmem_ld32(ts + h * kHalf, reinterpret_cast<uint32_t (&)[32]>(s[0]));
-                tmem_ld32(ts + h * kHalf + 32, reinterpret_cast<uint32_t (&)[32]>(s[32]));
+                uint32_t s[SPLIT ? 32 : kHalf];
+                if constexpr (!SPLIT) {
+                    tmem_ld32(ts + h * kHalf, reinterpret_cast<uint32_t (&)[32]>(s[0]));
+                    tmem_ld32(ts + h * kHalf + 32, reinterpret_cast<uint32_t (&)[32]>(s[32]));
+                }
                 // factors and offsets of the half's four blocks
                 const float4 sk = *reinterpret_cast<const float4 *>(&s_sk[rr][4 * h]), ls = *reinterpret_cast<const float4 *>(&s_lsv[rr][4 * h]),
                              is = *reinterpret_cast<const float4 *>(&s_isv[rr][4 * h]);
@@ -621,39 +645,51 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int hi = pos - tok0, lo = p.window ? max(-1, pos - p.window - tok0) : -1;   // seen: lo < column <= hi
                 const uint32_t okm = s_ok[rr] >> (4 * h) & 0xFu;
                 const bool whole = __all_sync(0xffffffffu, hi >= kHalf - 1 && (!live || lo < 0)) && okm == 0xFu;
-                tmem_ld_wait();
-                if (!whole) {
-                    // unseen columns to -inf (the other values are finite: cache bytes times f16)
-#pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        const int up = hi - 32 * c, down = lo - 32 * c;
-                        uint32_t mask = up < 0 ? 0u : up >= 31 ? ~0u : (2u << up) - 1;
-                        if (down >= 0) mask &= down >= 31 ? 0u : ~((2u << down) - 1);
-                        mask &= (okm >> (2 * c) & 1 ? 0xFFFFu : 0u) | (okm >> (2 * c) & 2 ? 0xFFFF0000u : 0u);
-#pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (!(mask >> i & 1)) s[32 * c + i] = 0xFF800000u;
-                    }
-                }
-                // ---- the row's maximum
+                if constexpr (!SPLIT) tmem_ld_wait();
+                // columns of 32 that this row sees
+                auto seen = [&](int c) -> uint32_t {
+                    const int up = hi - 32 * c, down = lo - 32 * c;
+                    uint32_t mask = up < 0 ? 0u : up >= 31 ? ~0u : (2u << up) - 1;
+                    if (down >= 0) mask &= down >= 31 ? 0u : ~((2u << down) - 1);
+                    return mask & ((okm >> (2 * c) & 1 ? 0xFFFFu : 0u) | (okm >> (2 * c) & 2 ? 0xFFFF0000u : 0u));
+                };
+                // ---- the row's maximum; unseen columns to -inf (the other values are finite:
+                // cache bytes times f16)
                 float top = -INFINITY;
 #pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    float x[4];
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float v = __uint_as_float(s[b * 16 + i]);
-                        x[i % 4] = i < 4 ? v : fmaxf(x[i % 4], v);
+                for (int c = 0; c < 2; c++) {
+                    uint32_t (&x32)[32] = reinterpret_cast<uint32_t (&)[32]>(s[SPLIT ? 0 : 32 * c]);
+                    if constexpr (SPLIT) {
+                        tmem_ld32(ts + h * kHalf + 32 * c, x32);
+                        tmem_ld_wait();
                     }
-                    const float y = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                    top = fmaxf(top, y == -INFINITY ? -INFINITY : fmaf(y, f[b], off[b]));     // (0 * -inf)
+                    if (!whole) {
+                        const uint32_t mask = seen(c);
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (!(mask >> i & 1)) x32[i] = 0xFF800000u;
+                    }
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        float x[4];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const float v = __uint_as_float(x32[b * 16 + i]);
+                            x[i % 4] = i < 4 ? v : fmaxf(x[i % 4], v);
+                        }
+                        const float y = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                        top = fmaxf(top, y == -INFINITY ? -INFINITY : fmaf(y, f[2 * c + b], off[2 * c + b]));     // (0 * -inf)
+                    }
                 }
                 const bool grow = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
+                [[maybe_unused]] float down = 1.0f;
+                const bool fold = SPLIT && u > 0 && u % (2 * kFold) == 0;      // what TMEM holds joins the row's sums below
                 if (__any_sync(0xffffffffu, grow)) {
                     const float a = grow ? ex2(m - top) : 1.0f;
                     if (grow) m = top;
                     l *= a;
-                    if (u > 0) {
+                    down = a;
+                    if (u > 0 && !fold) {
                         // the sums so far, the other half's product among them (the one before
                         // that is done: these logits came after it)
                         if (!(ok = warp_wait(&o_sum[w], (2 * turns + h - 1) & 1, abort_flag, p.err))) break;
@@ -668,37 +704,77 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tmem_st32(to + c * 32, o);
                         }
                         tmem_st_wait();
+                        if constexpr (SPLIT)
+#pragma unroll
+                            for (int i = 0; i < D; i++) tot[i] *= a;
                     }
                 }
                 // ---- the weights, over the logits they come from
                 const float ms = m == -INFINITY ? 0.0f : m;
+                if constexpr (SPLIT) {
+#pragma unroll 1
+                    for (int b = 0; b < 4; b++) {
+                        uint32_t x16[16], hi8[8], lo8[8];
+                        const float fb = rf * s_sk[rr][4 * h + b], zb = s_lsv[rr][4 * h + b] - ms;
+                        tmem_ld16(ts + h * kHalf + b * 16, x16);
+                        tmem_ld_wait();
+                        if (!whole) {
+                            const uint32_t mask = seen(b / 2) >> (b % 2 * 16);
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    uint32_t hi16[16];
-                    [[maybe_unused]] uint32_t lo16[16];
-#pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        const float ff = whole ? f[2 * c + b] : fmaxf(f[2 * c + b], 1e-30f), z = off[2 * c + b] - ms;    // (0 * -inf)
-                        const f32x2 f2 = pair(ff, ff), z2 = pair(z, z);
+                            for (int i = 0; i < 16; i++)
+                                if (!(mask >> i & 1)) x16[i] = 0xFF800000u;
+                        }
+                        const float ff = whole ? fb : fmaxf(fb, 1e-30f);    // (0 * -inf)
+                        const f32x2 f2 = pair(ff, ff), z2 = pair(zb, zb);
                         f32x2 add = pair(0.0f, 0.0f);
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
-                            const int k = c * 32 + b * 16 + i;
-                            const f32x2 x = fma2(pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), f2, z2);
-                            float2 e;
-                            if (!SPLIT && i / 2 % kCubic == kCubic - 1) e = ex2_cubic(x);
-                            else e = make_float2(ex2(unpair(x).x), ex2(unpair(x).y));
+                            const f32x2 x = fma2(pair(__uint_as_float(x16[i]), __uint_as_float(x16[i + 1])), f2, z2);
+                            const float2 e = make_float2(ex2(unpair(x).x), ex2(unpair(x).y));
                             add = add2(add, pair(e.x, e.y));
-                            hi16[b * 8 + i / 2] = pack_f16(e.x, e.y);
-                            if constexpr (SPLIT) {
-                                const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&hi16[b * 8 + i / 2]));
-                                lo16[b * 8 + i / 2] = pack_f16(e.x - q.x, e.y - q.y);
-                            }
+                            hi8[i / 2] = pack_f16(e.x, e.y);
+                            const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&hi8[i / 2]));
+                            lo8[i / 2] = pack_f16(e.x - q.x, e.y - q.y);
                         }
-                        l = fmaf(unpair(add).x + unpair(add).y, isv[2 * c + b], l);
+                        l = fmaf(unpair(add).x + unpair(add).y, s_isv[rr][4 * h + b], l);
+                        tmem_st8(ts + h * kHalf + b * 16, hi8);
+                        tmem_st8(ts + h * kHalf + b * 16 + 8, lo8);
                     }
-                    tmem_st16(ts + h * kHalf + c * 32, hi16);
-                    if constexpr (SPLIT) tmem_st16(ts + h * kHalf + c * 32 + 16, lo16);
+                    if (fold) {
+                        // (the product before the last is done: these logits came after it)
+                        if (!(ok = warp_wait(&o_sum[w], (2 * turns - 1) & 1, abort_flag, p.err))) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int c = 0; c < D / 32; c++) {
+                            tmem_ld32(to + c * 32, s);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) tot[c * 32 + i] = (tot[c * 32 + i] + __uint_as_float(s[i])) * down;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t hi16[16];
+#pragma unroll
+                        for (int b = 0; b < 2; b++) {
+                            const float ff = whole ? f[2 * c + b] : fmaxf(f[2 * c + b], 1e-30f), z = off[2 * c + b] - ms;    // (0 * -inf)
+                            const f32x2 f2 = pair(ff, ff), z2 = pair(z, z);
+                            f32x2 add = pair(0.0f, 0.0f);
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                const int k = c * 32 + b * 16 + i;
+                                const f32x2 x = fma2(pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), f2, z2);
+                                float2 e;
+                                if (i / 2 % kCubic == kCubic - 1) e = ex2_cubic(x);
+                                else e = make_float2(ex2(unpair(x).x), ex2(unpair(x).y));
+                                add = add2(add, pair(e.x, e.y));
+                                hi16[b * 8 + i / 2] = pack_f16(e.x, e.y);
+                            }
+                            l = fmaf(unpair(add).x + unpair(add).y, isv[2 * c + b], l);
+                        }
+                        tmem_st16(ts + h * kHalf + c * 32, hi16);
+                    }
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -722,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_ld_wait();
                 float v[32];
 #pragma unroll
-                for (int i = 0; i < 32; i++) v[i] = __uint_as_float(o[i]) * inv;
+                for (int i = 0; i < 32; i++) v[i] = (SPLIT ? tot[SPLIT ? c * 32 + i : 0] + __uint_as_float(o[i]) : __uint_as_float(o[i])) * inv;
                 if (live) store_vals<32>(out + c * 32, v);
             }
             tc_fence_before();
@@ -746,6 +822,10 @@ cudaError_t launch_tiles_d(const AttnParams &p, int few_rows, uint8_t *ws, size_
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !set[dev]) {
         if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem)) != cudaSuccess) return e;
+        // the split of the registers must not ask for more than the launch brings: it would wait for good
+        cudaFuncAttributes at;
+        if ((e = cudaFuncGetAttributes(&at, kern)) != cudaSuccess) return e;
+        if (2 * at.numRegs < Regs<kSplit>::kSoft + Regs<kSplit>::kOther) return cudaErrorInvalidConfiguration;
         if (dev < 64) set[dev] = true;
     }
     // the list goes in slices whose queries fit the workspace
