@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kStep = kConvWarps * 32 / D, kTurns = SPLIT ? 2 : 1, kIn = 8 / kStep / kTurns;
     static_assert(kStep >= 1 && kIn >= 1, "threads");
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ __align__(8) uint64_t q_full[2], q_free[2], k_full[NB], k_empty[NB], v_full[NB], v_empty[NB], st_full[2], s_full[2][2],
+    __shared__ __align__(8) uint64_t q_full[2], q_free[2], k_full[NB], k_empty[NB], v_full[NB], v_empty[NB], st_full[2], st_empty[2], s_full[2][2],
         p_full[2][2], o_sum[2], o_done[2], drained[2];
     __shared__ __align__(16) float s_sk[4][8], s_lsv[4][8], s_isv[4][8];
     __shared__ uint32_t s_ok[4];
@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&st_full[i], 1);
+            mbar_init(&st_empty[i], kConvWarps);
             for (int h = 0; h < 2; h++) {
                 mbar_init(&s_full[i][h], 2);      // the products' end, and what the product thread has seen
                 mbar_init(&p_full[i][h], 4);
@@ -390,60 +391,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ============ conversion: cache bytes -> f16 operands. (After a wait that ran out
         // the warps go on through their barriers: every wait then gives up at once.)
         regs_down<Regs<SPLIT>::kOther>();
-        const int ct = tid - kSoftWarps * 32, cw = warp - kSoftWarps;
-        fence_proxy_async_global();       // the cache as an append before this left it, to the bulk copies
-        uint32_t done = 0, staged = 0;
+        const int ct = tid - kSoftWarps * 32;
+        uint32_t done = 0;
         bool ok = true;
         for (int j = 0, have; (have = item(j)) >= 0; j++) {
             if (!have) continue;
-            int64_t at = -1;
-            float sk = 0.0f, sv = 0.0f;
-            // Warp 0: asks for tile t's keys (0) or values (1); lanes 0 .. 7 look after a block each.
-            auto stage = [&](int which, int t) {
-                if (which == 0) {
-                    at = -1;
-                    const int blk = (it.tile0 + t) * (kKv / kKvBlock) + lane, first = blk * kKvBlock;
-                    if (lane < 8 && first <= it.pos_last && (!p.window || first + kKvBlock - 1 > it.pos_first - p.window)) {
-                        at = block_index(p.c, it.slot, blk, head);
-                        if (at < 0) kv_error(p.err);
-                    }
-                }
-                const unsigned n = __popc(__ballot_sync(0xffffffffu, at >= 0));
-                if (lane == 0) mbar_arrive_expect_tx(&st_full[which], n * (kKvBlock * D));
-                __syncwarp();
-                if (at >= 0)
-                    bulk_load(smem_addr(sm_st + which * Sh::kStage + lane * kKvBlock * D),
-                              (which ? p.c.v : p.c.k) + at * (kKvBlock * D), kKvBlock * D, &st_full[which]);
-                if (which == 0) {
-                    sk = sv = 0.0f;
-                    if (at >= 0) {
-                        sk = ld_plain(p.c.k_scale + at);
-                        sv = ld_plain(p.c.v_scale + at);
-                    }
-                }
-            };
-            if (cw == 0) {
-                stage(0, 0);
-                stage(1, 0);
-            }
-            staged = done + 1;
             for (int t = 0; t < it.tiles; t++, done++) {
                 const int buf = done % NB;
                 const uint32_t ph = (done / NB) & 1;
                 // ---- keys: rows are tokens, 64 values a slab
                 ok &= warp_wait(&st_full[0], done & 1, abort_flag, p.err);
                 ok &= warp_wait(&k_empty[buf], ph ^ 1, abort_flag, p.err);
-                if (cw == 0) {
-                    const int r = done & 3;
-                    const unsigned live = __ballot_sync(0xffffffffu, at >= 0);
-                    if (lane < 8) {
-                        const float ls = sv > 0.0f ? lg2(sv) : kNoScaleLog2;
-                        s_sk[r][lane] = sk;
-                        s_lsv[r][lane] = ls;
-                        s_isv[r][lane] = ex2(-ls);
-                    }
-                    if (lane == 0) s_ok[r] = live & 0xFFu;
-                }
 #pragma unroll
                 for (int u = 0; u < kTurns; u++) {
                     const int tb = ct % D, sub = ct / D + u * kIn * kStep, slab = tb / 64, tok = tb % 64 / 4, c = tb % 4 * 2;
@@ -453,6 +411,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint4 in[kIn];
 #pragma unroll
                     for (int i = 0; i < kIn; i++) in[i] = lds128(src + i * (kStep * D * 16));
+                    if (u == kTurns - 1) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&st_empty[0]);
+                    }
 #pragma unroll
                     for (int i = 0; i < kIn; i++) {
                         const uint4 w = in[i];
@@ -467,9 +429,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 fence_async_smem();
-                named_bar(1, kConvWarps * 32);       // every warp has read the staged bytes and written its part
+                __syncwarp();
                 if (lane == 0) mbar_arrive(&k_full[buf]);
-                if (cw == 0 && t + 1 < it.tiles) stage(0, t + 1);
                 // ---- values: rows are the head's values, 64 tokens a slab
                 ok &= warp_wait(&st_full[1], done & 1, abort_flag, p.err);
                 ok &= warp_wait(&v_empty[buf], ph ^ 1, abort_flag, p.err);
@@ -481,6 +442,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint4 in[kIn];
 #pragma unroll
                     for (int i = 0; i < kIn; i++) in[i] = lds128(src + i * (kStep * D * 16));
+                    if (u == kTurns - 1) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&st_empty[1]);
+                    }
 #pragma unroll
                     for (int i = 0; i < kIn; i++) {
                         const uint4 w = in[i];
@@ -496,17 +461,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 fence_async_smem();
-                named_bar(1, kConvWarps * 32);
+                __syncwarp();
                 if (lane == 0) mbar_arrive(&v_full[buf]);
-                if (cw == 0 && t + 1 < it.tiles) {
-                    stage(1, t + 1);
-                    staged = done + 2;
-                }
             }
         }
-        if (!ok && cw == 0)        // copies may still be in flight
-            for (int w = 0; w < 2; w++)
-                if (staged) drain_wait(&st_full[w], (staged - 1) & 1);
     } else if (warp >= kMmaWarp) {
         regs_down<Regs<SPLIT>::kOther>();
         if (warp < kMmaWarp + 2) {
@@ -603,6 +561,62 @@ __global__ void __launch_bounds__(kThreads, 1)
                 commit_one(&drained[i]);
                 drain_wait(&drained[i], 0);
             }
+            __syncwarp();
+        } else if (warp == kMmaWarp + 2) {
+            // ============ loads: lanes 0 .. 7 look after a block of the tile each, a tile ahead
+            fence_proxy_async_global();       // the cache as an append before this left it, to the bulk copies
+            uint32_t done = 0, staged[2] = {0, 0};
+            bool ok = true;
+            for (int j = 0, have; ok && (have = item(j)) >= 0; j++) {
+                if (!have) continue;
+                auto lookup = [&](int t) -> int64_t {
+                    const int blk = (it.tile0 + t) * (kKv / kKvBlock) + lane, first = blk * kKvBlock;
+                    if (t >= it.tiles || lane >= 8 || first > it.pos_last || (p.window && first + kKvBlock - 1 <= it.pos_first - p.window))
+                        return -1;
+                    const int64_t i = block_index(p.c, it.slot, blk, head);
+                    if (i < 0) kv_error(p.err);
+                    return i;
+                };
+                auto scales = [&](int64_t i, float &k, float &v) {
+                    k = i >= 0 ? ld_plain(p.c.k_scale + i) : 0.0f;
+                    v = i >= 0 ? ld_plain(p.c.v_scale + i) : 0.0f;
+                };
+                int64_t at = lookup(0);
+                float sk, sv;
+                scales(at, sk, sv);
+                for (int t = 0; t < it.tiles; t++, done++) {
+                    const unsigned live = __ballot_sync(0xffffffffu, at >= 0);
+                    for (int which = 0; which < 2; which++) {
+                        // read by every conversion warp
+                        if (done && !(ok = warp_wait(&st_empty[which], (done - 1) & 1, abort_flag, p.err))) break;
+                        if (which == 0) {
+                            // (this slot's last tile, four before, has its weights: the keys of the
+                            // one before are converted, so those of three before have been used)
+                            const int r = done & 3;
+                            if (lane < 8) {
+                                const float ls = sv > 0.0f ? lg2(sv) : kNoScaleLog2;
+                                s_sk[r][lane] = sk;
+                                s_lsv[r][lane] = ls;
+                                s_isv[r][lane] = ex2(-ls);
+                            }
+                            if (lane == 0) s_ok[r] = live & 0xFFu;
+                            __syncwarp();
+                        }
+                        if (lane == 0) mbar_arrive_expect_tx(&st_full[which], __popc(live) * (kKvBlock * D));
+                        __syncwarp();
+                        if (at >= 0)
+                            bulk_load(smem_addr(sm_st + which * Sh::kStage + lane * kKvBlock * D),
+                                      (which ? p.c.v : p.c.k) + at * (kKvBlock * D), kKvBlock * D, &st_full[which]);
+                        staged[which] = done + 1;
+                    }
+                    if (!ok) break;
+                    at = lookup(t + 1);
+                    scales(at, sk, sv);
+                }
+            }
+            if (!ok)        // copies may still be in flight
+                for (int which = 0; which < 2; which++)
+                    if (staged[which]) drain_wait(&st_full[which], (staged[which] - 1) & 1);
             __syncwarp();
         }
     } else {
