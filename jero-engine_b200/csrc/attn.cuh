@@ -99,14 +99,36 @@ __device__ __forceinline__ int64_t block_index(const KvCacheDev &c, int slot, in
     return (((int64_t)page * c.heads + head) << c.page_shift) + (blk & ((1 << c.page_shift) - 1));
 }
 
-// cos and sin of an angle in f64, reduced there to [-pi, pi] so that far
-// positions lose nothing, then in f32.
+// An angle less its whole quarter turns, in f64 (far positions lose nothing):
+// the rest, in [-pi/4, pi/4], and the number of turns mod 4, which the low bits
+// of angle * 2/pi + 1.5 * 2^52 hold.
+__device__ __forceinline__ int quarter_turns(double &angle)
+{
+    const double t = fma(angle, 0.6366197723675814, 6755399441055744.0), n = t - 6755399441055744.0;
+    angle = fma(-n, 6.123233995736766e-17, fma(-n, 1.5707963267948966, angle));   // pi / 2 in two parts
+    return __double2loint(t) & 3;
+}
+
+// cos and sin of an angle, in f32 from the rest on: the Taylor series up to x^10
+// and x^9 (the next terms are below 2e-9).
 __device__ __forceinline__ void turn_f32(double angle, float &c, float &s)
 {
-    const double n = rint(angle * 0.15915494309189535);
-    double r = fma(-n, 6.283185307179586, angle);
-    r = fma(-n, 2.4492935982947064e-16, r);   // the rest of 2 pi
-    sincosf((float)r, &s, &c);
+    const int k = quarter_turns(angle);
+    const float x = (float)angle, z = x * x;
+    float a = 1.0f / 362880.0f, b = -1.0f / 3628800.0f;
+    b = fmaf(b, z, 1.0f / 40320.0f);
+    a = fmaf(a, z, -1.0f / 5040.0f);
+    b = fmaf(b, z, -1.0f / 720.0f);
+    a = fmaf(a, z, 1.0f / 120.0f);
+    b = fmaf(b, z, 1.0f / 24.0f);
+    a = fmaf(a, z, -1.0f / 6.0f);
+    b = fmaf(b, z, -0.5f);
+    a = fmaf(a * z, x, x);
+    b = fmaf(b, z, 1.0f);
+    c = k & 1 ? a : b;
+    s = k & 1 ? b : a;
+    if (k == 1 || k == 2) c = -c;
+    if (k >= 2) s = -s;
 }
 
 // Indices of pair i of a head's first R values.

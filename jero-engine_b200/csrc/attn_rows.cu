@@ -17,7 +17,7 @@ constexpr int kRowWarps = 4;
 
 // Norms and rotation: a warp takes a group of a token's heads, kAhead loads of
 // 16 bytes a lane under way before the first is worked on.
-constexpr int kAhead = 4;
+constexpr int kAhead = 2;
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) qk_norm_rope_kernel(KvBatchDev b, const __grid_constant__ RopeDev rope,
@@ -36,17 +36,16 @@ __global__ void __launch_bounds__(kRowWarps * 32) qk_norm_rope_kernel(KvBatchDev
     const int64_t item = (int64_t)blockIdx.x * kRowWarps + warp;
     const int row = (int)(item / groups);
     if (row >= b.T) return;
-    // groups of query heads, then of key heads
-    const int q_heads = in.q ? in.q_heads : 0, q_groups = (q_heads + group - 1) / group, gi = (int)(item - (int64_t)row * groups);
-    const bool is_q = gi < q_groups;
-    const int heads = is_q ? q_heads : in.kv_heads, sub = lane / L::kLanes, d0 = lane % L::kLanes * L::kVals;
-    int h = (is_q ? gi : gi - q_groups) * group + sub;
-    const int head1 = min(heads, h - sub + group);
-    const T *src = static_cast<const T *>(is_q ? in.q : in.k) + row * (is_q ? in.q_stride : in.k_stride) + d0;
-    T *dst = static_cast<T *>(const_cast<void *>(is_q ? out.q : out.k)) + row * (is_q ? out.q_stride : out.k_stride) + d0;
-    const float *norm = is_q ? rope.q_norm : rope.k_norm;
+    // groups of query heads, then of key heads; or, with one group, both in turn
+    const int q_heads = in.q ? in.q_heads : 0, k_heads = in.k ? in.kv_heads : 0, gi = (int)(item - (int64_t)row * groups);
+    const int q_groups = groups == 1 ? 0 : (q_heads + group - 1) / group;
+    const int sub = lane / L::kLanes, d0 = lane % L::kLanes * L::kVals;
+    bool is_q = groups == 1 ? q_heads > 0 : gi < q_groups;
+    int h, head1;
+    const T *src;
+    T *dst;
     float v[kAhead][L::kVals];
-    auto load = [&](int h) {
+    auto load = [&] {
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
             const int x = h + i * L::kHeads;
@@ -56,25 +55,39 @@ __global__ void __launch_bounds__(kRowWarps * 32) qk_norm_rope_kernel(KvBatchDev
                 for (int k = 0; k < L::kVals; k++) v[i][k] = 0.0f;
         }
     };
-    load(h);
+    auto begin = [&] {
+        const int heads = is_q ? q_heads : k_heads;
+        h = groups == 1 ? sub : (is_q ? gi : gi - q_groups) * group + sub;
+        head1 = groups == 1 ? heads : min(heads, h - sub + group);
+        src = static_cast<const T *>(is_q ? in.q : in.k) + row * (is_q ? in.q_stride : in.k_stride) + d0;
+        dst = static_cast<T *>(const_cast<void *>(is_q ? out.q : out.k)) + row * (is_q ? out.q_stride : out.k_stride) + d0;
+        load();
+    };
+    begin();
     const int s = seq_of_row_warp(b, row, lane);
     SeqInfo q;
     if (s < 0 || !seq_info(b, s, q) || row < q.row0 || row >= q.row0 + q.n) return;
     L l;
     l.begin(rope, q.past + row - q.row0, s_y[warp], lane);
-    float w[L::kVals];
-    l.weights(norm, w);
     for (;;) {
+        const float *norm = is_q ? rope.q_norm : rope.k_norm;
+        float w[L::kVals];
+        l.weights(norm, w);
+        for (;;) {
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            const int x = h + i * L::kHeads;
-            if (x - sub >= head1) break;
-            l.turn(v[i], norm != nullptr, w, (float)rope.eps, s_y[warp]);
-            if (x < head1) store_vals<L::kVals>(dst + x * D, v[i]);
+            for (int i = 0; i < kAhead; i++) {
+                const int x = h + i * L::kHeads;
+                if (x - sub >= head1) break;
+                l.turn(v[i], norm != nullptr, w, (float)rope.eps, s_y[warp]);
+                if (x < head1) store_vals<L::kVals>(dst + x * D, v[i]);
+            }
+            h += kAhead * L::kHeads;
+            if (h - sub >= head1) break;
+            load();
         }
-        h += kAhead * L::kHeads;
-        if (h - sub >= head1) break;
-        load(h);
+        if (groups > 1 || !is_q || !k_heads) break;
+        is_q = false;
+        begin();
     }
 }
 
@@ -125,14 +138,13 @@ __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t 
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// cos and sin in f64: the angle less its whole quarter turns, then the Taylor
-// series up to x^14 and x^13 on [-pi/4, pi/4] (the next terms are below 2e-14;
-// the keys are rounded to f32 afterwards). A third of the library function's work.
+// cos and sin in f64, of the angle's rest the Taylor series up to x^14 and x^13
+// (the next terms are below 2e-14; the keys are rounded to f32 afterwards). A
+// third of the library function's work.
 __device__ __forceinline__ void turn_f64(double angle, double &c, double &s)
 {
-    const double n = rint(angle * 0.6366197723675814);       // 2 / pi
-    double x = fma(-n, 1.5707963267948966, angle);
-    x = fma(-n, 6.123233995736766e-17, x);                    // the rest of pi / 2
+    double x = angle;
+    const int k = quarter_turns(x);
     const double z = x * x;
     double a = 1.0 / 6227020800.0, b = -1.0 / 87178291200.0;
     a = fma(a, z, -1.0 / 39916800.0);
@@ -148,7 +160,6 @@ __device__ __forceinline__ void turn_f64(double angle, double &c, double &s)
     a = fma(a * z, x, x);
     b = fma(b, z, -0.5);
     b = fma(b, z, 1.0);
-    const int k = (int)(__double2ll_rn(n) & 3);
     c = k & 1 ? a : b;
     s = k & 1 ? b : a;
     if (k == 1 || k == 2) c = -c;
@@ -516,11 +527,12 @@ cudaError_t by_type(int act, int D, F &&f)
 cudaError_t launch_qk_norm_rope(const KvBatchDev &b, const RopeDev &rope, const AttnRows &in, const AttnRows &out, int D,
                                 int *err, cudaStream_t st)
 {
-    // few tokens: one load a warp, for the shortest time; many: a token's heads up to four loads' worth a turn
+    // few tokens: one load a warp, for the shortest time; many: a warp a token, which forms its angles once
     return by_type(in.act, D, [&](auto d, auto t) {
         using L = HeadLanes<decltype(d)::value, decltype(t)>;
-        const int group = b.T <= 512 ? L::kHeads : kAhead * L::kHeads * 2;
-        const int groups = (in.q ? (in.q_heads + group - 1) / group : 0) + (in.k ? (in.kv_heads + group - 1) / group : 0);
+        const int group = L::kHeads;
+        const int groups =
+            b.T > 512 ? 1 : (in.q ? (in.q_heads + group - 1) / group : 0) + (in.k ? (in.kv_heads + group - 1) / group : 0);
         return launch_dependent(qk_norm_rope_kernel<decltype(d)::value, decltype(t)>,
                                 dim3((unsigned)(((int64_t)b.T * groups + kRowWarps - 1) / kRowWarps)), dim3(kRowWarps * 32), 0, st, b,
                                 rope, in, out, group, groups, err);
