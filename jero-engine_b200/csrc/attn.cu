@@ -29,15 +29,13 @@ namespace jmoe {
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-// CTAs of an SM: one joins its parts while the others stream. Three where eight
-// rows of queries are all that a CTA holds (shared memory), else two.
+// CTAs of an SM: one joins its parts while the others stream. Three where a CTA
+// holds eight rows of queries (registers), else two.
 constexpr int kMaxCtasPerSm = 3;
 constexpr int kTile = 64;                    // tokens of a tile: 4 blocks
-constexpr int kMaxRows = kWarps * 16;        // rows of a chunk
+constexpr int kMaxRows = 16;                 // rows of a chunk, at most
 // A run has at least this many tiles: fewer CTAs share a short sequence.
 constexpr int kMinTiles = 2;
-// Sequences with more rows (new tokens times query heads of a key head) go to attn_tiles.cu.
-constexpr int kFewRows = 64;
 // What beginning and joining one more segment costs a CTA, in tiles.
 constexpr int kSegmentTiles = 8;
 
@@ -177,12 +175,12 @@ struct SeqWork {
     int slot, tile0, tiles, segs;
 };
 
-__device__ __forceinline__ void seq_work(const AttnParams &p, int s, int g, int chunk_rows, SeqWork &w, bool &bad)
+__device__ __forceinline__ void seq_work(const AttnParams &p, int s, int g, int few_rows, int chunk_rows, SeqWork &w, bool &bad)
 {
     const bool listed = seq_info(p.b, s, w.q), cached = seq_in_cache(p.c, p.b, s, w.q, w.slot);
     bad = !listed || !cached;
     w.tile0 = w.tiles = w.segs = 0;
-    if (bad || w.q.n == 0 || w.q.n * g > kFewRows) return;
+    if (bad || w.q.n == 0 || w.q.n * g > few_rows) return;
     w.tile0 = p.window ? max(0, w.q.past - p.window + 1) / kTile : 0;
     w.tiles = (w.q.past + w.q.n - 1) / kTile + 1 - w.tile0;
     w.segs = p.c.heads;
@@ -208,13 +206,13 @@ struct Shape {
     static constexpr int kKBytes = kWarps * 4 * kBlk, kVBytes = kWarps * 4 * kVBlk;
     static constexpr int kRowOff = kKBytes + kVBytes;            // a head row of each warp while it is rotated
     static constexpr int kQOff = kRowOff + kWarps * D * 4;       // queries, upper halves, then the lower ones
-    static constexpr int smem(int group) { return kQOff + group * kRows * kQRow * (SPLIT ? 2 : 1); }
+    static constexpr int kSmem = kQOff + kRows * kQRow * (SPLIT ? 2 : 1);
     static_assert(kWarps * kRows * D * 4 <= kKBytes + kVBytes, "the warps' sums lie where their tiles were");
 };
 
 template <int D, typename T, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
-    attend_stream_kernel(const __grid_constant__ AttnParams p, int seq0, int seq1, int group, uint32_t g_mul, int *counters,
+    attend_stream_kernel(const __grid_constant__ AttnParams p, int seq0, int seq1, int few_rows, uint32_t g_mul, int *counters,
                          float *partials)
 {
     using Sh = Shape<D, SPLIT>;
@@ -227,10 +225,8 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
     float *s_sum = reinterpret_cast<float *>(smem);           // the warps' sums of a finished segment
     const uint32_t kbase = smem_addr(smem), vbase = kbase + Sh::kKBytes;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, ln = lane / 4, lj = lane % 4;
-    const int streams = kWarps / group, stream = warp / group, rt = warp % group, depth = group;
-    const int g = p.rows.q_heads / p.c.heads, chunk_rows = group * RR, me = blockIdx.x;
-    const bool leader = rt == 0;
-    const int q_lower = chunk_rows * Sh::kQRow;
+    const int g = p.rows.q_heads / p.c.heads, me = blockIdx.x;
+    constexpr int q_lower = RR * Sh::kQRow;
     // n / g for numbers below 2^32 / g
     auto over_g = [&](int n) -> int { return g == 1 ? n : (int)__umulhi((uint32_t)n, g_mul); };
 
@@ -238,8 +234,8 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
         for (int i = 0; i < kWarps; i++) {
             mbar_init(&s_full[0][i], 1);
             mbar_init(&s_full[1][i], 1);
-            mbar_init(&s_empty[0][i], group);
-            mbar_init(&s_empty[1][i], group);
+            mbar_init(&s_empty[0][i], 1);
+            mbar_init(&s_empty[1][i], 1);
         }
         s_abort = 0;
         fence_barrier_init();
@@ -253,12 +249,12 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
     SeqWork w;
     bool bad = false;
     w.tiles = w.segs = 0;
-    if (seq0 + lane < seq1) seq_work(p, seq0 + lane, g, chunk_rows, w, bad);
+    if (seq0 + lane < seq1) seq_work(p, seq0 + lane, g, few_rows, RR, w, bad);
     const SeqWork w0 = w;
     int total = w.tiles * w.segs, segs = w.segs;
     for (int s = seq0 + 32 + lane; s < seq1; s += 32) {
         bool worse;
-        seq_work(p, s, g, chunk_rows, w, worse);
+        seq_work(p, s, g, few_rows, RR, w, worse);
         total += w.tiles * w.segs;
         segs += w.segs;
         bad |= worse;
@@ -289,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
         w = w0;
         if (s0 != seq0) {
             w.tiles = w.segs = 0;
-            if (s0 + lane < seq1) seq_work(p, s0 + lane, g, chunk_rows, w, bad);
+            if (s0 + lane < seq1) seq_work(p, s0 + lane, g, few_rows, RR, w, bad);
         }
         const int n = w.segs * (cut ? quot(w.tiles + cut - 1, cut, inv_cut) : w.tiles);
         int last = n;
@@ -320,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                 w.tiles = __shfl_sync(0xffffffffu, w0.tiles, i);
                 w.segs = __shfl_sync(0xffffffffu, w0.segs, i);
             } else {
-                seq_work(p, b, g, chunk_rows, w, bad);
+                seq_work(p, b, g, few_rows, RR, w, bad);
             }
             per = cut ? quot(w.tiles + cut - 1, cut, inv_cut) : w.tiles;
             if (at < base + w.segs * per) break;
@@ -347,9 +343,9 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
         }
         const int chunk = idx < p.c.heads ? 0 : idx / p.c.heads;
         sg.head = idx - chunk * p.c.heads;
-        sg.rows = min(chunk_rows, w.q.n * g - chunk * chunk_rows);
-        sg.tok = chunk ? chunk * chunk_rows / g : 0;
-        sg.rem = chunk * chunk_rows - sg.tok * g;
+        sg.rows = min(RR, w.q.n * g - chunk * RR);
+        sg.tok = chunk ? chunk * RR / g : 0;
+        sg.rem = chunk * RR - sg.tok * g;
         sg.pos_first = w.q.past + sg.tok;
         sg.pos_last = sg.pos_first + over_g(sg.rem + sg.rows - 1);
         return true;
@@ -363,18 +359,17 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
         if (i < 0) kv_error(p.err);
         return i;
     };
-    // The leader warp loads a tile's keys (0) or values (1) into the stream's next slot.
-    // n: tiles that the stream was given before it.
+    // The warp loads a tile's keys (0) or values (1) into its slot. n: tiles that it was
+    // given before it.
     auto issue = [&](int which, int64_t blk, uint32_t n) {
-        const int slot = stream * depth + (int)(n & (depth - 1));
-        uint64_t *full = &s_full[which][slot];
+        uint64_t *full = &s_full[which][warp];
         const unsigned have = __ballot_sync(0xffffffffu, blk >= 0) & 0xFu;
-        // the slot's last tile has been read by every warp of the group
-        if (n >= (uint32_t)depth) tc_spin_wait(&s_empty[which][slot], (n / depth - 1) & 1, &s_abort, p.err);
+        // the slot's last tile has been read
+        if (n) tc_spin_wait(&s_empty[which][warp], (n - 1) & 1, &s_abort, p.err);
         if (lane == 0) mbar_arrive_expect_tx(full, __popc(have) * Sh::kBlk);
         __syncwarp();
         if (lane < 4 && blk >= 0) {
-            const uint32_t dst = which ? vbase + (slot * 4 + lj) * Sh::kVBlk : kbase + (slot * 4 + lj) * Sh::kBlk;
+            const uint32_t dst = which ? vbase + (warp * 4 + lj) * Sh::kVBlk : kbase + (warp * 4 + lj) * Sh::kBlk;
             bulk_load(dst, (which ? p.c.v : p.c.k) + blk * Sh::kBlk, Sh::kBlk, full);
         }
     };
@@ -394,13 +389,13 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
 
     Segment cur, sg;
     bool joining = false;      // cur's tiles are done, its parts not yet joined
-    uint32_t done = 0;         // tiles this stream has taken
+    uint32_t done = 0;         // tiles this warp has taken
     float m[U], l[U], o[NT][SPLIT ? 2 : 4];
     __syncthreads();
     for (;;) {
         // ---- the warps' parts of the segment before, and the CTAs'
         if (joining) {
-            const int taken = cur.t1 - cur.t0, used = min(streams, taken);
+            const int taken = cur.t1 - cur.t0, used = min(kWarps, taken);
             float *part = s_sum + warp * RR * D;
             __syncthreads();          // every warp is done with its tiles
 #pragma unroll
@@ -496,16 +491,15 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
             };
             constexpr int Q4 = D / 4;
             for (int e = tid; e < cur.rows * Q4; e += kThreads) {
-                const int r = e / Q4, d = e % Q4 * 4, wr = r / RR, rr = r % RR;
+                const int r = e / Q4, d = e % Q4 * 4;
                 float M = -INFINITY;
-                for (int i = 0; i < used; i++) M = fmaxf(M, s_m[i * group + wr][rr]);
+                for (int w = 0; w < used; w++) M = fmaxf(M, s_m[w][r]);
                 const float Ms = M == -INFINITY ? 0.0f : M;
                 float acc[4] = {}, den = 0.0f;
-                for (int i = 0; i < used; i++) {
-                    const int w = i * group + wr;
-                    const float a = ex2(s_m[w][rr] - Ms);
-                    const float4 v = *reinterpret_cast<const float4 *>(s_sum + (w * RR + rr) * D + d);
-                    den = fmaf(s_l[w][rr], a, den);
+                for (int w = 0; w < used; w++) {
+                    const float a = ex2(s_m[w][r] - Ms);
+                    const float4 v = *reinterpret_cast<const float4 *>(s_sum + (w * RR + r) * D + d);
+                    den = fmaf(s_l[w][r], a, den);
                     acc[0] = fmaf(v.x, a, acc[0]);
                     acc[1] = fmaf(v.y, a, acc[1]);
                     acc[2] = fmaf(v.z, a, acc[2]);
@@ -543,15 +537,11 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
 #pragma unroll
             for (int i = 0; i < kAhead; i++)
                 if (warp + i * kWarps < sg.rows) load_vals<N>(row_ptr(sg, warp + i * kWarps, tok), qv[i]);
-            blk = lookup(sg, sg.t0 + stream);
-            if (leader)
-                for (int i = 0; i < depth; i++) {
-                    const int t = sg.t0 + stream + i * streams;
-                    if (t >= sg.t1) break;
-                    const int64_t first = i ? lookup(sg, t) : blk;
+            const int t = sg.t0 + warp;
+            blk = lookup(sg, t);
+            if (t < sg.t1)
 #pragma unroll 1
-                    for (int which = 0; which < 2; which++) issue(which, first, done + i);
-                }
+                for (int which = 0; which < 2; which++) issue(which, blk, done);
             scales(blk, sk, sv);
         }
 
@@ -609,10 +599,9 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
         uint32_t qa[KS][4];
         float rf[U];
         int pos[U];
-        const int row_base = rt * RR;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int r = row_base + ln + 8 * u;
+            const int r = ln + 8 * u;
             const bool live = r < sg.rows;
             pos[u] = live ? sg.pos_first + over_g(sg.rem + r) : -1;
             rf[u] = live ? s_rf[r] : 0.0f;
@@ -636,9 +625,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                     }
                 }
         }
-        const int tile_pos0 = sg.pos_first + over_g(sg.rem + min(row_base, sg.rows - 1));   // of the first row
-        const int tile_pos1 = sg.pos_first + over_g(sg.rem + min(row_base + RR, sg.rows) - 1);
-#pragma unroll
+        #pragma unroll
         for (int u = 0; u < U; u++) {
             m[u] = -INFINITY;
             l[u] = 0.0f;
@@ -648,18 +635,16 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
 #pragma unroll
             for (int x = 0; x < (SPLIT ? 2 : 4); x++) o[i][x] = 0.0f;
 
-        // ---- the stream's tiles
-        for (int t = sg.t0 + stream; t < sg.t1; t += streams, done++) {
-            const int slot = stream * depth + (int)(done & (depth - 1));
-            const uint32_t ph = (done / depth) & 1;
-            const int64_t next = lookup(sg, t + streams);
-            const int64_t ahead = depth == 1 ? next : leader ? lookup(sg, t + depth * streams) : -1;
+        // ---- the warp's tiles
+        for (int t = sg.t0 + warp; t < sg.t1; t += kWarps, done++) {
+            const uint32_t ph = done & 1;
+            const int64_t next = lookup(sg, t + kWarps);
             float s[8][4];
-            tc_spin_wait(&s_full[0][slot], ph, &s_abort, p.err);
+            tc_spin_wait(&s_full[0][warp], ph, &s_abort, p.err);
             // column c of the 8-token group i: token 16 (c / 2) + 2 i + (c & 1) of the
             // tile, so that this lane's columns all lie in block lj (four groups at a
             // time: their accumulators do not wait for one another)
-            const uint32_t ka = kbase + (slot * 4 + ln / 2) * Sh::kBlk + (ln & 1) * 64 + lj * 16;
+            const uint32_t ka = kbase + (warp * 4 + ln / 2) * Sh::kBlk + (ln & 1) * 64 + lj * 16;
 #pragma unroll
             for (int i0 = 0; i0 < 8; i0 += 4)
 #pragma unroll
@@ -678,16 +663,16 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                         }
                 }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[0][slot]);
-            const bool reload = leader && t + depth * streams < sg.t1;
-            if (reload) issue(0, ahead, done + depth);
+            if (lane == 0) mbar_arrive(&s_empty[0][warp]);
+            const bool reload = t + kWarps < sg.t1;
+            if (reload) issue(0, next, done + 1);
             float sk_next, sv_next;
             scales(next, sk_next, sv_next);
 
             // ---- weights
             const float lsv = sv > 0.0f ? lg2(sv) : kNoScaleLog2, isv = ex2(-lsv);
             const int tok0 = (sg.tile0 + t) * kTile;
-            const bool clear = tok0 + kTile - 1 <= tile_pos0 && (!p.window || tok0 > tile_pos1 - p.window);
+            const bool clear = tok0 + kTile - 1 <= sg.pos_first && (!p.window || tok0 > sg.pos_last - p.window);
             const bool whole = __all_sync(0xffffffffu, clear && blk >= 0);
             float alpha[U];
 #pragma unroll
@@ -738,8 +723,8 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                     pa[q][3] = pack_f16(s[2 * q + 1][2], s[2 * q + 1][3]);
                 }
             }
-            tc_spin_wait(&s_full[1][slot], ph, &s_abort, p.err);
-            const uint32_t va = vbase + (slot * 4 + lj) * Sh::kVBlk + ln * 16;
+            tc_spin_wait(&s_full[1][warp], ph, &s_abort, p.err);
+            const uint32_t va = vbase + (warp * 4 + lj) * Sh::kVBlk + ln * 16;
             // a tile's sums start at zero and join the running ones in f32, rounded to
             // nearest: the tensor cores' additions round towards zero
             constexpr int PV = 4;
@@ -771,8 +756,8 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                     }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[1][slot]);
-            if (reload) issue(1, ahead, done + depth);
+            if (lane == 0) mbar_arrive(&s_empty[1][warp]);
+            if (reload) issue(1, next, done + 1);
             blk = next;
             sk = sk_next;
             sv = sv_next;
@@ -781,10 +766,22 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
         joining = true;
     }
     // after a wait that ran out, copies may still be in flight
-    if (*(volatile int *)&s_abort && leader)
-        for (int which = 0; which < 2; which++)
-            for (uint32_t n = done > (uint32_t)depth ? done - depth : 0; n < done; n++)
-                drain_wait(&s_full[which][stream * depth + n % depth], (n / depth) & 1);
+    if (*(volatile int *)&s_abort && done)
+        for (int which = 0; which < 2; which++) drain_wait(&s_full[which][warp], (done - 1) & 1);
+}
+
+// Sequences with more rows (new tokens times query heads of a key head) than
+// this go to attn_tiles.cu, which takes 256 rows and a key head a CTA over their
+// whole history: better where such items fill the SMs, while the runs here split
+// a history, but read it anew for each 8 or 16 rows. With 2000 cached tokens, 8
+// key heads, bf16 / f32, us here and there:
+//   1 sequence,  512 rows  39 / 45 and 52 / 76    16 sequences, 32 rows  37 / 45 and 42 / 63
+//   4 sequences, 256 rows  53 / 69 and 51 / 74    16 sequences, 64 rows  56 / 71 and 42 / 64
+//   64 sequences, 16 rows  57 / 75 and 81 / 124   64 sequences, 32 rows  96 / 130 and 83 / 128
+// (1 sequence of 20000, 128 rows: 56 / 78 and 287 / 476.)
+int few_rows(const AttnParams &p)
+{
+    return std::max(16, std::min(512, 40 * p.num_sms / std::max(1, p.b.B * p.c.heads)));
 }
 
 template <int D, typename T, bool SPLIT>
@@ -797,29 +794,26 @@ cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !set[dev]) {
-        if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::smem(kWarps))) != cudaSuccess) return e;
+        if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem)) != cudaSuccess) return e;
         if (dev < 64) set[dev] = true;
     }
-    // warps that share a tile: one for each row tile, up to all eight
     const int g = p.rows.q_heads / p.c.heads;
-    int64_t rows = (int64_t)p.b.max_new * g;
-    const bool prompts = rows > kFewRows;
-    if (prompts) rows = kFewRows;
-    int group = 1;
-    while (group < kWarps && (int64_t)group * Sh::kRows < rows) group *= 2;
+    const int64_t rows = (int64_t)p.b.max_new * g;
+    // tiles are counted in 32 bits: a sequence's, ...
+    const int64_t chunk = (((int64_t)p.c.table_stride * kKvBlock << p.c.page_shift) / kTile + 2) * p.c.heads;
+    const int few = (int)std::min<int64_t>(few_rows(p), INT_MAX / chunk * Sh::kRows);
     uint8_t *ws = static_cast<uint8_t *>(p.ws);
-    const int ctas = p.num_sms * (SPLIT && group == 1 ? 3 : 2);
-    // a launch's tiles are counted in 32 bits: sequences that could have more go in several
-    const int64_t most = (((int64_t)p.c.table_stride * kKvBlock << p.c.page_shift) / kTile + 2) * p.c.heads *
-                         ((rows + group * Sh::kRows - 1) / (group * Sh::kRows));
+    const int ctas = p.num_sms * (SPLIT ? 3 : 2);
+    // ... and a launch's: sequences that could have more go in several
+    const int64_t most = chunk * ((std::min<int64_t>(rows, few) + Sh::kRows - 1) / Sh::kRows);
     const int step = (int)std::max<int64_t>(1, std::min<int64_t>(p.b.B, (int64_t)INT_MAX / most));
     for (int s = 0; s < p.b.B; s += step) {
-        e = launch_dependent(kern, dim3(ctas), dim3(kThreads), Sh::smem(group), st, p, s, std::min(p.b.B, s + step), group,
+        e = launch_dependent(kern, dim3(ctas), dim3(kThreads), Sh::kSmem, st, p, s, std::min(p.b.B, s + step), few,
                              g > 1 ? (uint32_t)((1ull << 32) / g + 1) : 0u, reinterpret_cast<int *>(ws + kCounterOff),
                              reinterpret_cast<float *>(ws + partial_off(p.num_sms * kMaxCtasPerSm)));
         if (e != cudaSuccess) return e;
     }
-    if (prompts) return launch_attention_tiles(p, kFewRows, ws + tiles_off(p.num_sms), kTilesBytes, st);
+    if (rows > few) return launch_attention_tiles(p, few, ws + tiles_off(p.num_sms), kTilesBytes, st);
     return cudaSuccess;
 }
 

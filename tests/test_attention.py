@@ -973,3 +973,21 @@ def test_two_graphs_share_a_context(make):
     for _, _, out, q, past, new in work:
         s.check_attention(out.double().cpu().numpy(), q, past, new, range(4))
     assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,hq,hk,page,window", [(128, 4, 4, 32, 0), (64, 3, 1, 16, 0), (128, 7, 1, 64, 100), (64, 16, 2, 128, 33),
+                                                 (128, 2, 1, 256, 1)])
+def test_attention_of_long_prompts(make, act, D, hq, hk, page, window):
+    """More rows than the runs over the cache take: 256 rows at a time, whole and ragged ones, with and without a history."""
+    g = hq // hk
+    s = make(act, D=D, q_heads=hq, kv_heads=hk, page=page, n_slots=3, pages_per_slot=-(-1400 // page))
+    new = [520 // g + 1, 768 // g + 2, 1025 // g + 1]
+    past = [0, 130, 77]
+    s.append([0] * 3, [p + n for p, n in zip(past, new)], range(3), rows=s.rows(sum(past) + sum(new)))
+    if window:
+        for i, p in enumerate(past):
+            s.table[i, : max(0, p - window + 1) // page] = -1
+    s.attend(past, new, range(3), window=window, behind=1, max_new=max(new))
+    assert s.ctx.device_status() == 0
