@@ -268,7 +268,7 @@ int moe_lm_head(moe_ctx *ctx, int32_t T, const float *normed, float *logits, int
  * output projection's input. Device pointers on the context's device
  * throughout; asynchronous on the context's stream; the caller owns all memory
  * named here, the context a fixed workspace. The first of these calls on a
- * context allocates it (about 110 MiB), so make that call before capturing the
+ * context allocates it (about 90 MiB), so make that call before capturing the
  * stream into a graph. Calls on one context, replays of graphs captured from
  * it among them, are serialised by the caller as every other call.
  *

@@ -4,10 +4,21 @@
 // running maximum m and the sums in f32, in one pass over the cache.
 //
 // attend_stream_kernel: the whole batch's (sequence, row chunk, key head, tile
-// of 64 tokens) list is cut into equal runs, one per CTA, found on the device
-// from the batch arrays. A run's tiles go to the CTA's warps in turn; each warp
-// keeps the softmax of its row tile in registers, and the warps' (and, where a
-// run ends inside a sequence, the CTAs') parts are joined by their maxima.
+// of 64 tokens) list is cut into runs, one per CTA, found on the device from the
+// batch arrays. A run's tiles go to the CTA's warps in turn, each with a slot of
+// shared memory that bulk copies refill; each warp keeps the softmax of the row
+// tile in registers, and the warps' (and, where a segment is cut, the CTAs')
+// parts are joined by their maxima. Warps that shared a tile among several row
+// tiles took longer at every size but one (32 rows over 2000 tokens, 1 sequence:
+// 25 us, a row tile a CTA 14).
+//
+// Bound by the cache's bytes and, as much, by what hides their latency: shared
+// memory holds 192 KB a SM in flight, and a warp's slot waits while its tile is
+// worked on. Without the products the copies alone run at 5.4 TB/s.
+//   64 single tokens over 398752 cached, 4 heads of 128, bf16  92 us, 4.4 TB/s
+//   one token over 131001 cached, F32 rows                     42 us, 3.2 TB/s
+//   one token over 701 cached, F32 rows                        12 us (latency)
+//   66 drafted tokens, 17 sequences, window 1024, f16          16.5 us
 //
 // The products run on mma.m16n8k16 with f16 operands: a decode row tile has 8
 // rows, which the 128-row tcgen05 form would leave 15/16 empty, and the kernel
@@ -30,18 +41,24 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 // CTAs of an SM: one joins its parts while the others stream. Three where a CTA
-// holds eight rows of queries (registers), else two.
+// holds eight rows of queries (a decoder layer's 32 histories 44 us, with two
+// 54), else two (registers).
 constexpr int kMaxCtasPerSm = 3;
 constexpr int kTile = 64;                    // tokens of a tile: 4 blocks
 constexpr int kMaxRows = 16;                 // rows of a chunk, at most
-// A run has at least this many tiles: fewer CTAs share a short sequence.
-constexpr int kMinTiles = 2;
-// What beginning and joining one more segment costs a CTA, in tiles.
+// A run has at least this many tiles, one for each warp: fewer CTAs share a short
+// sequence (one of 200 tokens 8.2 us, with 2 tiles 11.0; of 3000 13.6 and 15.5;
+// 8 of 700 13.6 and 12.8).
+constexpr int kMinTiles = kWarps;
+// What beginning and joining one more segment costs a CTA, in tiles: runs that
+// end with their segment may be longer by this (with 0 and 40 instead of 8: one
+// sequence of 3000 tokens 22.0 and 15.5 us for 15.5, 40 of 3000 44.5 and 47.8
+// for 44.4, 64 of 500 26.2 and 18.8 for 18.7).
 constexpr int kSegmentTiles = 8;
 
-// A segment's parts are joined in groups of this many CTAs, then the groups.
+// A segment's parts are joined in groups of this many CTAs, all of a group's
+// loads under way at once, then the groups.
 constexpr int kJoin = 16;
-
 // Workspace: status word | arrival counters [2][ctas][2] | partials [ctas][2].
 constexpr size_t kCounterOff = 256;
 size_t partial_off(int ctas) { return kCounterOff + ((size_t)ctas * 16 + 255) / 256 * 256; }
@@ -773,15 +790,16 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
 // Sequences with more rows (new tokens times query heads of a key head) than
 // this go to attn_tiles.cu, which takes 256 rows and a key head a CTA over their
 // whole history: better where such items fill the SMs, while the runs here split
-// a history, but read it anew for each 8 or 16 rows. With 2000 cached tokens, 8
-// key heads, bf16 / f32, us here and there:
-//   1 sequence,  512 rows  39 / 45 and 52 / 76    16 sequences, 32 rows  37 / 45 and 42 / 63
-//   4 sequences, 256 rows  53 / 69 and 51 / 74    16 sequences, 64 rows  56 / 71 and 42 / 64
-//   64 sequences, 16 rows  57 / 75 and 81 / 124   64 sequences, 32 rows  96 / 130 and 83 / 128
-// (1 sequence of 20000, 128 rows: 56 / 78 and 287 / 476.)
+// a history, but read it anew for each 8 or 16 rows. With 2000 cached tokens, 4
+// key heads of 128, bf16 / f32, us here and there:
+//   1 sequence,  512 rows  36 / 41 and 52 / 76    16 sequences, 32 rows  35 / 42 and 42 / 63
+//   4 sequences, 256 rows  49 / 65 and 51 / 74    16 sequences, 64 rows  51 / 67 and 42 / 64
+//   64 sequences, 16 rows  53 / 70 and 81 / 124   64 sequences, 32 rows  96 / 130 and 83 / 127
+// (1 sequence of 20000, 128 rows: 51 / 74 and 287 / 476.)
 int few_rows(const AttnParams &p)
 {
-    return std::max(16, std::min(512, 40 * p.num_sms / std::max(1, p.b.B * p.c.heads)));
+    const int fill = (p.rows.act == MOE_ACT_F32 ? 32 : 24) * p.num_sms / std::max(1, p.b.B * p.c.heads);
+    return std::max(16, std::min(512, fill));
 }
 
 template <int D, typename T, bool SPLIT>
@@ -820,7 +838,8 @@ cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
 template <typename T>
 cudaError_t launch_t(const AttnParams &p, cudaStream_t st)
 {
-    // eight rows at a time where no sequence has more (half the registers), or for 22 bits
+    // Eight rows at a time where no sequence has more, or for 22 bits: half the registers, three CTAs
+    // an SM (8 rows of bf16, 64 sequences of 4000 tokens: 72 us, 16 at a time 83; one of 100000: 38 and 40)
     if (sizeof(T) == 4 || (int64_t)p.b.max_new * (p.rows.q_heads / p.c.heads) <= 8)
         return p.c.D == 64 ? launch_stream<64, T, true>(p, st) : launch_stream<128, T, true>(p, st);
     if constexpr (sizeof(T) == 2)

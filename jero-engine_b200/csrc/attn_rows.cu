@@ -2,9 +2,15 @@
 // and key heads with the rotation in the same pass, appending keys and values
 // to the paged 8-bit cache, and reading cached rows back.
 //
-// All three touch each value once and are bound by memory (or, for a decode
-// step's few rows, by the launch): bytes per call = rows in + rows out, and for
-// the append the 8-bit blocks, their scales and the open blocks in f32.
+// All three touch each value once: bytes per call = rows in + rows out, and for
+// the append the 8-bit blocks, their scales and the open blocks in f32. At a
+// decode step's few rows they are bound by the launch and a chain of dependent
+// loads (batch entry, page, rows). At prompts the norms and the append are bound
+// by their instructions and the latencies between them, not yet by memory:
+//   norms and rotation  11093 tokens of 14 + 2 heads of 64, bf16   23 us, 2.0 TB/s
+//                       8 tokens of 32 + 4 heads of 128, f32       4 us
+//   append              8483 tokens of 4 heads of 128, bf16        44 us
+//                       64 tokens of 64 sequences, f32             7 us
 #include <algorithm>
 
 #include "attn.cuh"
@@ -15,8 +21,10 @@ namespace {
 
 constexpr int kRowWarps = 4;
 
-// Norms and rotation: a warp takes a group of a token's heads, kAhead loads of
-// 16 bytes a lane under way before the first is worked on.
+// Norms and rotation: y = x / sqrt(mean x^2 + eps) w, then pairs turned by
+// position * frequency. A warp takes a group of a token's heads, or all of them,
+// kAhead loads of 16 bytes a lane under way before the first is worked on (four:
+// 25.6 us where two take 23.5, the registers).
 constexpr int kAhead = 2;
 
 template <int D, typename T>
@@ -527,12 +535,15 @@ cudaError_t by_type(int act, int D, F &&f)
 cudaError_t launch_qk_norm_rope(const KvBatchDev &b, const RopeDev &rope, const AttnRows &in, const AttnRows &out, int D,
                                 int *err, cudaStream_t st)
 {
-    // few tokens: one load a warp, for the shortest time; many: a warp a token, which forms its angles once
+    // Few warps: one load each, for the shortest time; where that would be many, a
+    // warp a token, which forms its angles once. 32 + 4 heads of 128, bf16, us for
+    // one load a warp and for a warp a token: 64 tokens 4.1 and 9.9, 256 tokens
+    // (4608 warps) 8.9 and 10.1, 512 tokens 13.8 and 10.1, 4096 tokens 87 and 31.
     return by_type(in.act, D, [&](auto d, auto t) {
         using L = HeadLanes<decltype(d)::value, decltype(t)>;
         const int group = L::kHeads;
-        const int groups =
-            b.T > 512 ? 1 : (in.q ? (in.q_heads + group - 1) / group : 0) + (in.k ? (in.kv_heads + group - 1) / group : 0);
+        int groups = (in.q ? (in.q_heads + group - 1) / group : 0) + (in.k ? (in.kv_heads + group - 1) / group : 0);
+        if ((int64_t)b.T * groups > 6144) groups = 1;
         return launch_dependent(qk_norm_rope_kernel<decltype(d)::value, decltype(t)>,
                                 dim3((unsigned)(((int64_t)b.T * groups + kRowWarps - 1) / kRowWarps)), dim3(kRowWarps * 32), 0, st, b,
                                 rope, in, out, group, groups, err);
@@ -543,7 +554,8 @@ cudaError_t launch_kv_append(const KvCacheDev &c, const KvBatchDev &b, const Rop
                              cudaStream_t st)
 {
     // Few blocks: a head a CTA, for the shortest time. Many: two heads share the
-    // angles (8192 tokens of 8 heads: 43.2 us, a head a CTA 44.6, four heads 43.6).
+    // angles. 4 heads of 128, bf16, a head a CTA and two: 1000 tokens 12.0 and
+    // 15.7 us, 4000 tokens 20.4 and 20.4, 8483 tokens 44.6 and 43.2.
     const unsigned blocks = (unsigned)(b.T / kKvBlock + 2 * b.B);
     const int group = blocks >= 512 ? std::min(c.heads, 2) : 1;
     const RopeDev none{};

@@ -24,9 +24,15 @@
 // off in all over 2500 tokens, 5e-6 with all the tiles in TMEM), which costs
 // room: 201 us instead of 176 (1500 + 1025 tokens of 3 sequences, 32 heads).
 //
-// Bound by the tensor cores and, as much, by the exponentials: 128 x 128
-// weights take 1024 cycles of the 16 a cycle that the SM gives, the two
-// products of a row tile 2 x 512.
+// Bound by the chain from one half's logits to the next one's: a softmax warp
+// takes some 2450 cycles for 64 columns (loads 360, maxima 410, a look at their
+// growth 210, weights 920, stores 90), the products and their operands' reads
+// from shared memory about as long for the four halves that are under way, and
+// neither covers the other wholly. 4096 rows of 32 heads over 4096 + 4096
+// tokens, bf16: 500 us, 0.82 PFLOP/s; 2064 rows in 3 prompts, F32 rows: 194 us.
+// (Not better: two threads a row and twice the warps, 578 us: the halves then
+// hand the maxima to one another; a third or half of the weights by the cubic
+// instead of a quarter, 494 and 505.)
 #include <algorithm>
 #include <type_traits>
 
@@ -859,6 +865,8 @@ cudaError_t launch_tiles_d(const AttnParams &p, int few_rows, uint8_t *ws, size_
         const int e1 = (int)std::min(entries, e0 + slice);
         float *factors = reinterpret_cast<float *>(ws + (size_t)(e1 - e0) * p.c.heads * Sh::kImage);
         using L = HeadLanes<D, T>;
+        // few tokens: one load a warp (the whole call with 128 tokens 53 us, grouped 57); many: a group of
+        // heads, which share a token's angles (1024 tokens 76 us, one load a warp 80)
         const int group = p.b.T <= 512 ? L::kHeads : kAhead * L::kHeads * 2, groups = (p.rows.q_heads + group - 1) / group;
         if ((e = launch_dependent(query_tiles_kernel<D, T, kSplit>,
                                   dim3((unsigned)(((int64_t)p.b.T * groups + kQueryWarps - 1) / kQueryWarps)), dim3(kQueryWarps * 32), 0,
