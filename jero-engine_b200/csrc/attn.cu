@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                     }
                 }
         }
-        #pragma unroll
+#pragma unroll
         for (int u = 0; u < U; u++) {
             m[u] = -INFINITY;
             l[u] = 0.0f;
