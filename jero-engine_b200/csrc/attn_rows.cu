@@ -9,7 +9,7 @@
 // by their instructions and the latencies between them, not yet by memory:
 //   norms and rotation  11093 tokens of 14 + 2 heads of 64, bf16   23 us, 2.0 TB/s
 //                       8 tokens of 32 + 4 heads of 128, f32       4 us
-//   append              8483 tokens of 4 heads of 128, bf16        44 us
+//   append              8483 tokens of 4 heads of 128, bf16        41 us
 //                       64 tokens of 64 sequences, f32             7 us
 #include <algorithm>
 
@@ -207,16 +207,18 @@ __device__ __forceinline__ Two dot2(Two a, Two b, Two c, Two d)
 }
 
 // One CTA per (touched block, group of heads): warp w has the block's tokens
-// 2 w and 2 w + 1, a lane D / 32 of their values. The angles are formed once for
+// 2 w and 2 w + 1, a lane D / 32 of their values (four CTAs an SM: 8483 tokens of
+// 4 heads 41 us, three 44, two 50). The angles are formed once for
 // the group, in f64 for every fourth token and from there by turns of the
 // frequency.
 //
-// Flat block index u: sequence s owns the indices from row_start[s] / 16 + 2 s
-// on, at least as many as the blocks its rows can touch (ceil((15 + n) / 16)),
-// so no prefix sum is needed.
+// Flat block index u: `per` indices a sequence, where that many blocks hold
+// max_new rows wherever they begin; with per = 0 sequence s owns the indices from
+// row_start[s] / 16 + 2 s on, at least as many as the blocks its rows can touch
+// (ceil((15 + n) / 16)), so no prefix sum is needed.
 template <int D, typename T>
-__global__ void __launch_bounds__(kAppendWarps * 32, 3)
-    kv_append_kernel(KvCacheDev c, KvBatchDev b, const __grid_constant__ RopeDev rope, int use_rope, AttnRows rows, int group, int *err)
+__global__ void __launch_bounds__(kAppendWarps * 32, 4)
+    kv_append_kernel(KvCacheDev c, KvBatchDev b, const __grid_constant__ RopeDev rope, int use_rope, AttnRows rows, int group, int per, int *err)
 {
     constexpr int N = D / 32;
     __shared__ __align__(16) float4 s_turn[kKvBlock][64];      // [token][place of a pair]: cos and sin, two f32 each
@@ -231,10 +233,14 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3)
     if (tid < 4) s_amax[tid / 2][tid % 2] = 0u;
     pdl_wait();
     pdl_trigger();
-    // the sequence: the last whose indices start at or before u
     int s = 0;
-    for (int i = lane; i < b.B; i += 32) s += row_of(b, i) / kKvBlock + 2 * i <= u;
-    s = __reduce_add_sync(0xffffffffu, s) - 1;
+    if (per) {
+        s = u / per;
+    } else {      // the last whose indices start at or before u
+#pragma unroll 4
+        for (int i = lane; i < b.B; i += 32) s += row_of(b, i) / kKvBlock + 2 * i <= u;
+        s = __reduce_add_sync(0xffffffffu, s) - 1;
+    }
     if (u == 0 && head0 == 0)
         for (int i = tid; i < b.B; i += blockDim.x) {
             SeqInfo qi;
@@ -245,7 +251,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3)
     int slot = -1;
     if (s < 0 || !seq_info(b, s, q) || !seq_in_cache(c, b, s, q, slot) || q.n == 0) return;
     const int total = q.past + q.n, blk0 = q.past / kKvBlock, blk_end = (total + kKvBlock - 1) / kKvBlock;
-    const int blk1 = blk0 + (u - (q.row0 / kKvBlock + 2 * s));
+    const int blk1 = blk0 + (per ? u - s * per : u - (q.row0 / kKvBlock + 2 * s));
     if (blk1 < blk0 || blk1 >= blk_end) return;     // below: row_start out of order
     // The first block reads the open rows and the last writes them: where both
     // do, one CTA takes the two in turn.
@@ -556,12 +562,14 @@ cudaError_t launch_kv_append(const KvCacheDev &c, const KvBatchDev &b, const Rop
     // Few blocks: a head a CTA, for the shortest time. Many: two heads share the
     // angles. 4 heads of 128, bf16, a head a CTA and two: 1000 tokens 12.0 and
     // 15.7 us, 4000 tokens 20.4 and 20.4, 8483 tokens 44.6 and 43.2.
-    const unsigned blocks = (unsigned)(b.T / kKvBlock + 2 * b.B);
+    // a sequence's rows touch at most so many blocks (1024 single tokens 37 us, searched for among 55)
+    const int most = (kKvBlock - 1 + b.max_new + kKvBlock - 1) / kKvBlock, per = most <= 2 ? most : 0;
+    const unsigned blocks = (unsigned)(per ? per * b.B : b.T / kKvBlock + 2 * b.B);
     const int group = blocks >= 512 ? std::min(c.heads, 2) : 1;
     const RopeDev none{};
     return by_type(rows.act, c.D, [&](auto d, auto t) {
         return launch_dependent(kv_append_kernel<decltype(d)::value, decltype(t)>, dim3(blocks, (c.heads + group - 1) / group),
-                                dim3(kAppendWarps * 32), 0, st, c, b, rope ? *rope : none, (int)(rope != nullptr), rows, group,
+                                dim3(kAppendWarps * 32), 0, st, c, b, rope ? *rope : none, (int)(rope != nullptr), rows, group, per,
                                 err);
     });
 }

@@ -991,3 +991,53 @@ def test_attention_of_long_prompts(make, act, D, hq, hk, page, window):
             s.table[i, : max(0, p - window + 1) // page] = -1
     s.attend(past, new, range(3), window=window, behind=1, max_new=max(new))
     assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,max_new", [("f32", 1), ("bf16", 2), ("f16", 17), ("f32", 18)])
+def test_append_with_a_bound_on_rows(make, act, max_new):
+    """The bound chooses how blocks are found: first blocks, last blocks and both at once, and sequences without rows."""
+    s = make(act, D=64, q_heads=2, kv_heads=2, page=16, n_slots=12, pages_per_slot=12)
+    rope, plain = s.rope()
+    past = [(7 * i) % 40 for i in range(12)]
+    s.append([0] * 12, past, range(12), rope, plain)
+    for step in range(4):
+        new = [(max_new + i * 5 + step) % (max_new + 1) for i in range(12)]
+        new[step] = max_new
+        new[5] = 0
+        slots = s.rng.permutation(12).tolist()
+        rows = s.rows(sum(new))
+        r, _, _, k, v = rows
+        at = [past[j] for j in slots]
+        s.ctx.kv_append(s.cache, s.batch(at, new, slots, max_new=max_new), rope, r)
+        row = 0
+        for j, n in zip(slots, new):
+            if n:
+                s.ref.append(j, past[j], plain(k[row:row + n], "k", past[j] + np.arange(n)), v[row:row + n])
+                past[j] += n
+                s.lens[j] = past[j]
+            row += n
+        for j in range(12):
+            if past[j]:
+                s.check_blocks(j)
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,hk", [("f32", 1), ("bf16", 3)])
+def test_attention_of_many_short_sequences(make, act, hk):
+    """300 sequences: several rounds of the plan; histories of a tile, longer ones among them."""
+    n = 300
+    s = make(act, D=64, q_heads=2 * hk, kv_heads=hk, page=32, n_slots=n, pages_per_slot=12)
+    total = [1 + (i * 53) % 60 for i in range(n)]
+    total[17], total[200], total[299] = 380, 300, 1
+    for a in range(0, n, 60):
+        s.append([0] * 60, total[a:a + 60], range(a, a + 60), rows=s.rows(sum(total[a:a + 60])))
+    order = s.rng.permutation(n).tolist()
+    s.attend([total[i] - 1 for i in order], [1] * n, order, max_new=1)
+    b = jm.KvBatch(n_seqs=n, n_tokens=n, past=s.ints([t - 1 for t in total]))       # a row each, slot b
+    r, _, q, _, _ = s.rows(n)
+    out = s.out(n, 2 * hk)
+    s.ctx.kv_attention(s.cache, b, None, r, out.data_ptr(), 2 * hk * 64)
+    s.check_attention(out.double().cpu().numpy(), q, [t - 1 for t in total], [1] * n, range(n))
+    assert s.ctx.device_status() == 0
