@@ -53,6 +53,8 @@ template <bool SPLIT>
 struct Regs {
     static constexpr int kSoft = SPLIT ? 200 : 152, kOther = SPLIT ? 56 : 104;
 };
+// Chunks of a launch that are put in order, at most (a launch of more has several for each SM)
+constexpr int kMaxSorted = 1024;
 // F32 rows: tiles whose products are summed in TMEM before they join the row's
 // sums (one: 210 us where two take 202; four: 198, and over 1e-6 off).
 constexpr int kFold = 2;
@@ -197,14 +199,10 @@ struct Item {
     int slot, tok, rem, rows, pos_first, pos_last, tile0, tiles;
 };
 
-// Entry `e` of the list, by a whole warp; false where it holds no chunk (or one
+// Chunk `e` of the list as one of sequence s; false where it holds none (or one
 // of a sequence with at most few_rows rows, which attn.cu takes).
-__device__ __forceinline__ bool find_item(const AttnParams &p, int e, int g, int few_rows, int lane, Item &it)
+__device__ __forceinline__ bool item_of(const AttnParams &p, int s, int e, int g, int few_rows, Item &it)
 {
-    int n = 0;
-    for (int s = lane; s < p.b.B; s += 32) n += first_entry(p.b, s, g) <= e;
-    const int s = __reduce_add_sync(0xffffffffu, n) - 1;
-    if (s < 0) return false;
     const bool ok = seq_info(p.b, s, it.q) && seq_in_cache(p.c, p.b, s, it.q, it.slot);
     if (!ok) return false;
     const int first = (e - first_entry(p.b, s, g)) * kRowsItem, rows = it.q.n * g;
@@ -217,6 +215,40 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int e, int g, int
     it.tile0 = p.window ? max(0, it.pos_first - p.window + 1) / kKv : 0;
     it.tiles = it.pos_last / kKv + 1 - it.tile0;
     return true;
+}
+
+// The same for a whole warp, which finds the sequence.
+__device__ __forceinline__ bool find_item(const AttnParams &p, int e, int g, int few_rows, int lane, Item &it)
+{
+    int n = 0;
+    for (int s = lane; s < p.b.B; s += 32) n += first_entry(p.b, s, g) <= e;
+    const int s = __reduce_add_sync(0xffffffffu, n) - 1;
+    return s >= 0 && item_of(p, s, e, g, few_rows, it);
+}
+
+// The list's chunks by length, longest first: their places in `order`, by the
+// whole CTA, in time for its last barrier. `length`: room for an int each.
+__device__ __forceinline__ void sort_items(const AttnParams &p, int entry0, int entries, int g, int few_rows, int *length, uint16_t *order)
+{
+    for (int e = threadIdx.x; e < entries; e += kThreads) {
+        int lo = 0, hi = p.b.B;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            (first_entry(p.b, mid, g) <= entry0 + e ? lo : hi) = mid;
+        }
+        Item it;
+        length[e] = item_of(p, lo, entry0 + e, g, few_rows, it) ? it.tiles : 0;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < entries; e += kThreads) {
+        const int mine = length[e];
+        int place = 0;
+#pragma unroll 4
+        for (int i = 0; i < entries; i++) place += length[i] > mine || (length[i] == mine && i < e);
+        order[place] = (uint16_t)e;
+    }
+    fence_async_smem();        // copies are to land where the lengths lay
+    __syncthreads();
 }
 
 template <int D, bool SPLIT>
@@ -341,6 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         p_full[2][2], o_sum[2], o_done[2], drained[2];
     __shared__ __align__(16) float s_sk[4][8], s_lsv[4][8], s_isv[4][8];
     __shared__ uint32_t s_ok[4];
+    __shared__ uint16_t s_order[kMaxSorted];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     uint8_t *sm_q = smem, *sm_k = sm_q + 2 * Sh::kQTile, *sm_v = sm_k + NB * Sh::kOperand, *sm_st = sm_v + NB * Sh::kOperand;
@@ -379,18 +412,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_trigger();
     volatile int *abort_flag = &s_abort;
 
-    // Items go to the CTAs there and back, longest first: neighbours' lengths differ little.
+    // Items go to the CTAs there and back, longest first. (In the list's own order, which
+    // is by length within a sequence only: 3 prompts with F32 rows 194 us instead of 158.)
     const int G = gridDim.x, entries = entry1 - entry0, total = entries * p.c.heads;
+    const bool sorted = entries <= kMaxSorted;
+    if (sorted) sort_items(p, entry0, entries, g, few_rows, reinterpret_cast<int *>(smem), s_order);
     Item it;
     int head = 0, image = 0;
     auto item = [&](int j) -> int {       // 1: an item, 0: none here, -1: the end
         if ((int64_t)j * G >= total) return -1;
         const int64_t u = (j & 1) ? (int64_t)(j + 1) * G - 1 - (int)blockIdx.x : (int64_t)j * G + (int)blockIdx.x;
         if (u >= total) return 0;
-        const int e = (int)(u / p.c.heads);
-        head = (int)(u - (int64_t)e * p.c.heads);
-        image = (entries - 1 - e) * p.c.heads + head;
-        return find_item(p, entry1 - 1 - e, g, few_rows, lane, it) ? 1 : 0;
+        const int i = (int)(u / p.c.heads), e = sorted ? s_order[i] : entries - 1 - i;
+        head = (int)(u - (int64_t)i * p.c.heads);
+        image = e * p.c.heads + head;
+        return find_item(p, entry0 + e, g, few_rows, lane, it) ? 1 : 0;
     };
 
     if (warp >= kSoftWarps && warp < kMmaWarp) {
