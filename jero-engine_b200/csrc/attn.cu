@@ -59,7 +59,7 @@ constexpr int kSegmentTiles = 8;
 // A segment's parts are joined in groups of this many CTAs, all of a group's
 // loads under way at once, then the groups.
 constexpr int kJoin = 16;
-// Workspace: status word | claimed items (kClaimsOff) | arrival counters [2][ctas][2] | partials [ctas][2].
+// Workspace: status word | arrival counters [2][ctas][2] | partials [ctas][2].
 constexpr size_t kCounterOff = 256;
 size_t partial_off(int ctas) { return kCounterOff + ((size_t)ctas * 16 + 255) / 256 * 256; }
 constexpr size_t kPartialBytes = (size_t)kMaxRows * (kMaxHeadDim + 2) * 4;

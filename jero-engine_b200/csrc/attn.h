@@ -56,8 +56,6 @@ struct AttnParams {
     int num_sms;
 };
 
-constexpr size_t kClaimsOff = 128;  // in the workspace: how many items of attn_tiles.cu are claimed
-
 // Bytes of a context's attention workspace.
 size_t attn_workspace_bytes(int num_sms);
 // Of them, from the start: the status word and the arrival counters, zero between calls.

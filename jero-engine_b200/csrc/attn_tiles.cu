@@ -11,7 +11,7 @@
 // halves of 64 tokens (P over S once S has been read) and O (D columns). While
 // a warpgroup weighs one half, the tensor cores add the other half's weights
 // and refill it: with one S of 128 columns a row tile the two waited for one
-// another, and the same work took 561 us where it took 504 then (4096 rows of 32 heads
+// another, and the same work took 561 us instead of 504 (4096 rows of 32 heads
 // over 4096 + 4096 tokens, bf16).
 //
 // The sums O are scaled down only when a row's maximum has grown by more than
@@ -22,17 +22,17 @@
 // one way, with each step of 16; so there TMEM holds the sums of two tiles only
 // and the softmax threads keep their rows' in registers (rounded sums: 7.8e-7
 // off in all over 2500 tokens, 5e-6 with all the tiles in TMEM), which costs
-// room: 201 us where it took 176 then (1500 + 1025 tokens of 3 sequences, 32 heads).
+// room: 201 us instead of 176 (1500 + 1025 tokens of 3 sequences, 32 heads).
 //
 // Bound by the chain from one half's logits to the next one's: a softmax warp
 // takes some 2450 cycles for 64 columns (loads 360, maxima 410, a look at their
 // growth 210, weights 920, stores 90), the products and their operands' reads
 // from shared memory about as long for the four halves that are under way, and
 // neither covers the other wholly. 4096 rows of 32 heads over 4096 + 4096
-// tokens, bf16: 490 us, 0.84 PFLOP/s; 2064 rows in 3 prompts, F32 rows: 158 us.
-// (Not better, at 500 us then: two threads a row and twice the warps, 578: the
-// halves then hand the maxima to one another; a third or half of the weights by
-// the cubic instead of a quarter, 494 and 505.)
+// tokens, bf16: 500 us, 0.82 PFLOP/s; 2064 rows in 3 prompts, F32 rows: 194 us.
+// (Not better: two threads a row and twice the warps, 578 us: the halves then
+// hand the maxima to one another; a third or half of the weights by the cubic
+// instead of a quarter, 494 and 505.)
 #include <algorithm>
 #include <type_traits>
 
@@ -55,7 +55,6 @@ struct Regs {
 };
 // Chunks of a launch that are put in order, at most (a launch of more has several for each SM)
 constexpr int kMaxSorted = 1024;
-constexpr int kClaims = 4;           // items that a CTA has claimed and not all its warps have read
 // F32 rows: tiles whose products are summed in TMEM before they join the row's
 // sums (one: 210 us where two take 202; four: 198, and over 1e-6 off).
 constexpr int kFold = 2;
@@ -229,7 +228,7 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int e, int g, int
 
 // The list's chunks by length, longest first: their places in `order`, by the
 // whole CTA, in time for its last barrier. `length`: room for an int each.
-__device__ __forceinline__ void sort_items(const AttnParams &p, int entry0, int entries, int g, int few_rows, int *length, uint16_t *order, int *live)
+__device__ __forceinline__ void sort_items(const AttnParams &p, int entry0, int entries, int g, int few_rows, int *length, uint16_t *order)
 {
     for (int e = threadIdx.x; e < entries; e += kThreads) {
         int lo = 0, hi = p.b.B;
@@ -247,7 +246,6 @@ __device__ __forceinline__ void sort_items(const AttnParams &p, int entry0, int 
 #pragma unroll 4
         for (int i = 0; i < entries; i++) place += length[i] > mine || (length[i] == mine && i < e);
         order[place] = (uint16_t)e;
-        if (mine) atomicMax(live, place + 1);
     }
     fence_async_smem();        // copies are to land where the lengths lay
     __syncthreads();
@@ -274,7 +272,7 @@ constexpr int kQueryWarps = 4, kAhead = 4;
 template <int D, typename T, bool SPLIT>
 __global__ void __launch_bounds__(kQueryWarps * 32)
     query_tiles_kernel(const __grid_constant__ AttnParams p, int entry0, int entry1, int few_rows, int group, int groups,
-                       uint8_t *images, float *factors, int *claims)
+                       uint8_t *images, float *factors)
 {
     using Sh = TileShape<D, SPLIT>;
     using L = HeadLanes<D, T>;
@@ -282,7 +280,6 @@ __global__ void __launch_bounds__(kQueryWarps * 32)
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     pdl_wait();
     pdl_trigger();
-    if (blockIdx.x == 0 && threadIdx.x == 0) *claims = 0;
     const int64_t item = (int64_t)blockIdx.x * kQueryWarps + warp;
     const int row = (int)(item / groups);
     if (row >= p.b.T) return;
@@ -364,7 +361,7 @@ __global__ void __launch_bounds__(kQueryWarps * 32)
 template <int D, typename T, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     attend_tiles_kernel(const __grid_constant__ AttnParams p, int entry0, int entry1, int few_rows, const uint8_t *images,
-                        const float *factors, int *claims)
+                        const float *factors)
 {
     using Sh = TileShape<D, SPLIT>;
     constexpr int NB = Sh::kBufs, SL = Sh::kSlabs;
@@ -377,8 +374,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ __align__(16) float s_sk[4][8], s_lsv[4][8], s_isv[4][8];
     __shared__ uint32_t s_ok[4];
     __shared__ uint16_t s_order[kMaxSorted];
-    __shared__ __align__(8) uint64_t c_full[kClaims], c_empty[kClaims];
-    __shared__ int s_claim[kClaims], s_live;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     uint8_t *sm_q = smem, *sm_k = sm_q + 2 * Sh::kQTile, *sm_v = sm_k + NB * Sh::kOperand, *sm_st = sm_v + NB * Sh::kOperand;
@@ -405,11 +400,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&q_free[i], 1);
             mbar_init(&drained[i], 1);
         }
-        for (int i = 0; i < kClaims; i++) {
-            mbar_init(&c_full[i], 1);
-            mbar_init(&c_empty[i], kSoftWarps + kConvWarps + 2);
-        }
-        s_live = 0;
         s_abort = 0;
         fence_barrier_init();
     }
@@ -422,45 +412,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_trigger();
     volatile int *abort_flag = &s_abort;
 
-    // Items go to the CTAs longest first, the first one by its number, then as they ask
-    // for more. (Dealt out there and back: 496 us where this takes 490; in the list's own
-    // order, which is by length within a sequence only, 3 prompts with F32 rows 194 us
-    // instead of 158.) The loading warp claims, the others read what it has claimed.
-    const int G = gridDim.x, entries = entry1 - entry0;
+    // Items go to the CTAs there and back, longest first. (In the list's own order, which
+    // is by length within a sequence only: 3 prompts with F32 rows 194 us instead of 158.)
+    const int G = gridDim.x, entries = entry1 - entry0, total = entries * p.c.heads;
     const bool sorted = entries <= kMaxSorted;
-    if (sorted) sort_items(p, entry0, entries, g, few_rows, reinterpret_cast<int *>(smem), s_order, &s_live);
-    const int total = (sorted ? s_live : entries) * p.c.heads;
+    if (sorted) sort_items(p, entry0, entries, g, few_rows, reinterpret_cast<int *>(smem), s_order);
     Item it;
     int head = 0, image = 0;
-    auto take = [&](int u) -> int {       // 1: an item, 0: none here, -1: the end
-        if (u >= total) return -1;
-        const int i = u / p.c.heads, e = sorted ? s_order[i] : entries - 1 - i;
-        head = u - i * p.c.heads;
+    auto item = [&](int j) -> int {       // 1: an item, 0: none here, -1: the end
+        if ((int64_t)j * G >= total) return -1;
+        const int64_t u = (j & 1) ? (int64_t)(j + 1) * G - 1 - (int)blockIdx.x : (int64_t)j * G + (int)blockIdx.x;
+        if (u >= total) return 0;
+        const int i = (int)(u / p.c.heads), e = sorted ? s_order[i] : entries - 1 - i;
+        head = (int)(u - (int64_t)i * p.c.heads);
         image = e * p.c.heads + head;
         return find_item(p, entry0 + e, g, few_rows, lane, it) ? 1 : 0;
-    };
-    auto item = [&](int j) -> int {
-        const int at = j % kClaims;
-        if (!warp_wait(&c_full[at], (j / kClaims) & 1, abort_flag, p.err)) return -1;
-        const int u = s_claim[at];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&c_empty[at]);
-        return take(u);
-    };
-    auto claim = [&](int j) -> int {
-        const int at = j % kClaims;
-        if (j >= kClaims && !warp_wait(&c_empty[at], (j / kClaims - 1) & 1, abort_flag, p.err)) return -1;
-        int u = blockIdx.x;
-        if (j) {
-            if (lane == 0) u = G + atomicAdd(claims, 1);
-            u = __shfl_sync(0xffffffffu, u, 0);
-        }
-        if (lane == 0) {
-            s_claim[at] = u;
-            mbar_arrive(&c_full[at]);
-        }
-        __syncwarp();
-        return take(u);
     };
 
     if (warp >= kSoftWarps && warp < kMmaWarp) {
@@ -643,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             fence_proxy_async_global();       // the cache as an append before this left it, to the bulk copies
             uint32_t done = 0, staged[2] = {0, 0};
             bool ok = true;
-            for (int j = 0, have; ok && (have = claim(j)) >= 0; j++) {
+            for (int j = 0, have; ok && (have = item(j)) >= 0; j++) {
                 if (!have) continue;
                 auto lookup = [&](int t) -> int64_t {
                     const int blk = (it.tile0 + t) * (kKv / kKvBlock) + lane, first = blk * kKvBlock;
@@ -930,7 +896,6 @@ cudaError_t launch_tiles_d(const AttnParams &p, int few_rows, uint8_t *ws, size_
     const int64_t entries = (int64_t)p.b.T * g / kRowsItem + p.b.B;
     const size_t per = (size_t)p.c.heads * (Sh::kImage + kRowsItem * 4);
     const int64_t slice = (int64_t)(ws_bytes / per);
-    int *claims = reinterpret_cast<int *>(static_cast<uint8_t *>(p.ws) + kClaimsOff);
     if (slice < 1) return cudaErrorInvalidValue;
     for (int64_t e0 = 0; e0 < entries; e0 += slice) {
         const int e1 = (int)std::min(entries, e0 + slice);
@@ -941,11 +906,11 @@ cudaError_t launch_tiles_d(const AttnParams &p, int few_rows, uint8_t *ws, size_
         const int group = p.b.T <= 512 ? L::kHeads : kAhead * L::kHeads * 2, groups = (p.rows.q_heads + group - 1) / group;
         if ((e = launch_dependent(query_tiles_kernel<D, T, kSplit>,
                                   dim3((unsigned)(((int64_t)p.b.T * groups + kQueryWarps - 1) / kQueryWarps)), dim3(kQueryWarps * 32), 0,
-                                  st, p, (int)e0, e1, few_rows, group, groups, ws, factors, claims)) != cudaSuccess)
+                                  st, p, (int)e0, e1, few_rows, group, groups, ws, factors)) != cudaSuccess)
             return e;
         const int grid = (int)std::min<int64_t>(p.num_sms, (e1 - e0) * p.c.heads);
         if ((e = launch_dependent(kern, dim3(grid), dim3(kThreads), Sh::kSmem, st, p, (int)e0, e1, few_rows, (const uint8_t *)ws,
-                                  (const float *)factors, claims)) != cudaSuccess)
+                                  (const float *)factors)) != cudaSuccess)
             return e;
     }
     return cudaSuccess;
