@@ -11,7 +11,7 @@
 // halves of 64 tokens (P over S once S has been read) and O (D columns). While
 // a warpgroup weighs one half, the tensor cores add the other half's weights
 // and refill it: with one S of 128 columns a row tile the two waited for one
-// another, and the same work took 561 us instead of 504 (4096 rows of 32 heads
+// another, and the same work took 561 us where it took 504 then (4096 rows of 32 heads
 // over 4096 + 4096 tokens, bf16).
 //
 // The sums O are scaled down only when a row's maximum has grown by more than
@@ -22,14 +22,14 @@
 // one way, with each step of 16; so there TMEM holds the sums of two tiles only
 // and the softmax threads keep their rows' in registers (rounded sums: 7.8e-7
 // off in all over 2500 tokens, 5e-6 with all the tiles in TMEM), which costs
-// room: 201 us instead of 176 (1500 + 1025 tokens of 3 sequences, 32 heads).
+// room: 201 us where it took 176 then (1500 + 1025 tokens of 3 sequences, 32 heads).
 //
 // Bound by the chain from one half's logits to the next one's: a softmax warp
 // takes some 2450 cycles for 64 columns (loads 360, maxima 410, a look at their
 // growth 210, weights 920, stores 90), the products and their operands' reads
 // from shared memory about as long for the four halves that are under way, and
 // neither covers the other wholly. 4096 rows of 32 heads over 4096 + 4096
-// tokens, bf16: 500 us, 0.82 PFLOP/s; 2064 rows in 3 prompts, F32 rows: 194 us.
+// tokens, bf16: 500 us, 0.82 PFLOP/s; 2064 tokens in 3 prompts, F32 rows: 158 us.
 // (Not better: two threads a row and twice the warps, 578 us: the halves then
 // hand the maxima to one another; a third or half of the weights by the cubic
 // instead of a quarter, 494 and 505.)
@@ -177,6 +177,23 @@ __device__ __forceinline__ void commit_one(uint64_t *bar)
         "elect.sync _|e, 0xffffffff;\n\t"
         "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
         : "memory");
+}
+
+// TMEM to registers, load and wait in one: between the two the registers do not
+// hold the values yet, and the compiler, which does not know, may move or spill them.
+__device__ __forceinline__ void tmem_get32(uint32_t taddr, uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_get16(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr)
+                 : "memory");
 }
 
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -689,10 +706,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = warp_wait(&s_full[w][h], turns & 1, abort_flag, p.err))) break;
                 tc_fence_after();
                 uint32_t s[SPLIT ? 32 : kHalf];
-                if constexpr (!SPLIT) {
-                    tmem_ld32(ts + h * kHalf, reinterpret_cast<uint32_t (&)[32]>(s[0]));
-                    tmem_ld32(ts + h * kHalf + 32, reinterpret_cast<uint32_t (&)[32]>(s[32]));
-                }
                 // factors and offsets of the half's four blocks
                 const float4 sk = *reinterpret_cast<const float4 *>(&s_sk[rr][4 * h]), ls = *reinterpret_cast<const float4 *>(&s_lsv[rr][4 * h]),
                              is = *reinterpret_cast<const float4 *>(&s_isv[rr][4 * h]);
@@ -704,7 +717,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // (a copy of its own for halves that every row sees whole: F32 rows 201 -> 194 us)
                 auto weigh = [&](auto whole_half) {
                     constexpr bool WHOLE = decltype(whole_half)::value;
-                if constexpr (!SPLIT) tmem_ld_wait();
+                if constexpr (!SPLIT) {
+                    tmem_get32(ts + h * kHalf, reinterpret_cast<uint32_t (&)[32]>(s[0]));
+                    tmem_get32(ts + h * kHalf + 32, reinterpret_cast<uint32_t (&)[32]>(s[32]));
+                }
                 // columns of 32 that this row sees
                 auto seen = [&](int c) -> uint32_t {
                     const int up = hi - 32 * c, down = lo - 32 * c;
@@ -719,8 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int c = 0; c < 2; c++) {
                     uint32_t (&x32)[32] = reinterpret_cast<uint32_t (&)[32]>(s[SPLIT ? 0 : 32 * c]);
                     if constexpr (SPLIT) {
-                        tmem_ld32(ts + h * kHalf + 32 * c, x32);
-                        tmem_ld_wait();
+                        tmem_get32(ts + h * kHalf + 32 * c, x32);
                     }
                     if constexpr (!WHOLE) {
                         const uint32_t mask = seen(c);
@@ -756,8 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
                         for (int c = 0; c < D / 32; c++) {
                             uint32_t o[32];
-                            tmem_ld32(to + c * 32, o);
-                            tmem_ld_wait();
+                            tmem_get32(to + c * 32, o);
 #pragma unroll
                             for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
                             tmem_st32(to + c * 32, o);
@@ -775,8 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int b = 0; b < 4; b++) {
                         uint32_t x16[16], hi8[8], lo8[8];
                         const float fb = rf * s_sk[rr][4 * h + b], zb = s_lsv[rr][4 * h + b] - ms;
-                        tmem_ld16(ts + h * kHalf + b * 16, x16);
-                        tmem_ld_wait();
+                        tmem_get16(ts + h * kHalf + b * 16, x16);
                         if constexpr (!WHOLE) {
                             const uint32_t mask = seen(b / 2) >> (b % 2 * 16);
 #pragma unroll
@@ -805,8 +818,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc_fence_after();
 #pragma unroll
                         for (int c = 0; c < D / 32; c++) {
-                            tmem_ld32(to + c * 32, s);
-                            tmem_ld_wait();
+                            tmem_get32(to + c * 32, s);
 #pragma unroll
                             for (int i = 0; i < 32; i++) tot[c * 32 + i] = (tot[c * 32 + i] + __uint_as_float(s[i])) * down;
                         }
@@ -857,8 +869,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {
                 uint32_t o[32];
-                tmem_ld32(to + c * 32, o);
-                tmem_ld_wait();
+                tmem_get32(to + c * 32, o);
                 float v[32];
 #pragma unroll
                 for (int i = 0; i < 32; i++) v[i] = (SPLIT ? tot[SPLIT ? c * 32 + i : 0] + __uint_as_float(o[i]) : __uint_as_float(o[i])) * inv;
