@@ -470,10 +470,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint4 in[kIn];
 #pragma unroll
                     for (int i = 0; i < kIn; i++) in[i] = lds128(src + i * (kStep * D * 16));
-                    if (u == kTurns - 1) {
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&st_empty[0]);
-                    }
 #pragma unroll
                     for (int i = 0; i < kIn; i++) {
                         const uint4 w = in[i];
@@ -489,7 +485,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 fence_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&k_full[buf]);
+                if (lane == 0) {
+                    mbar_arrive(&st_empty[0]);      // only now: what was loaded has been used
+                    mbar_arrive(&k_full[buf]);
+                }
                 // ---- values: rows are the head's values, 64 tokens a slab
                 ok &= warp_wait(&st_full[1], done & 1, abort_flag, p.err);
                 ok &= warp_wait(&v_empty[buf], ph ^ 1, abort_flag, p.err);
@@ -501,10 +500,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint4 in[kIn];
 #pragma unroll
                     for (int i = 0; i < kIn; i++) in[i] = lds128(src + i * (kStep * D * 16));
-                    if (u == kTurns - 1) {
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&st_empty[1]);
-                    }
 #pragma unroll
                     for (int i = 0; i < kIn; i++) {
                         const uint4 w = in[i];
@@ -521,7 +516,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 fence_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&v_full[buf]);
+                if (lane == 0) {
+                    mbar_arrive(&st_empty[1]);      // only now: what was loaded has been used
+                    mbar_arrive(&v_full[buf]);
+                }
             }
         }
     } else if (warp >= kMmaWarp) {

@@ -1041,3 +1041,23 @@ def test_attention_of_many_short_sequences(make, act, hk):
     s.ctx.kv_attention(s.cache, b, None, r, out.data_ptr(), 2 * hk * 64)
     s.check_attention(out.double().cpu().numpy(), q, [t - 1 for t in total], [1] * n, range(n))
     assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_long_prompts_give_the_same_bits_every_time(make, act):
+    """Several chunks a CTA, staged one behind another: right, and the same run after run."""
+    s = make(act, D=64, q_heads=32, kv_heads=4, page=32, n_slots=3, pages_per_slot=34)
+    past, new = [300, 200, 250], [700, 390, 512]
+    for i in range(3):
+        s.append([0], [past[i] + new[i]], [i], rows=s.rows(past[i] + new[i]))
+    r, _, q, _, _ = s.rows(sum(new))
+    b = s.batch(past, new, range(3), max_new=700)
+    first = None
+    for _ in range(40):
+        out = s.out(sum(new), 32)
+        s.ctx.kv_attention(s.cache, b, None, r, out.data_ptr(), 32 * 64)
+        first = out if first is None else first
+        assert s.t.equal(first, out)
+    s.check_attention(first.double().cpu().numpy(), q, past, new, range(3))
+    assert s.ctx.device_status() == 0
