@@ -2,7 +2,8 @@
 // the mathematics of attn.cu for row chunks of 256 (tokens of a sequence times
 // the query heads of one key head), two tiles of 128 rows a CTA.
 //
-// Per 128 cached tokens: four conversion warps turn the cache's bytes into f16
+// Per 128 cached tokens: a warp looks up the pages and stages the cache's bytes
+// a tile ahead, four conversion warps turn the cache's bytes into f16
 // operands in shared memory (exact; K-major, 128-byte swizzle: a value block
 // lies as [D][16 tokens] in the cache, so neither keys nor values are
 // transposed), one thread issues S = Q K^T (tcgen05.mma, M 128, N 64) and
@@ -46,7 +47,7 @@ namespace {
 constexpr int kRowsTile = 128, kRowsItem = 256, kKv = 128, kHalf = 64;
 constexpr int kSoftWarps = 8;
 constexpr int kConvWarps = 4, kMmaWarp = kSoftWarps + kConvWarps;
-constexpr int kThreads = 16 * 32;    // whole warpgroups: two warps beside the product warps only lend registers
+constexpr int kThreads = 16 * 32;    // whole warpgroups: one warp beside the product warps and the loading one only lends registers
 // Registers a thread after the split: 2 x (kSoft + kOther) = 4 x the launch's 128.
 // With F32 rows the softmax threads keep their rows' sums.
 template <bool SPLIT>
