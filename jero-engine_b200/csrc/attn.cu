@@ -119,10 +119,10 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
                  : "memory");
 }
 
-// c += a b, and c = a b.
+// c += a b, and c = a b. (volatile: they stay before the refill of the slot that b came from)
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                  "{%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -130,10 +130,10 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 
 __device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%10, %10, %10, %10};"
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
     using Sh = Shape<D, SPLIT>;
     constexpr int RR = Sh::kRows, U = SPLIT ? 1 : 2, NT = D / 8, KS = D / 16, N = D / 32;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(8) uint64_t s_full[2][kWarps], s_empty[2][kWarps];   // keys, values
+    __shared__ __align__(8) uint64_t s_full[2][kWarps];       // keys, values
     __shared__ float s_m[kWarps][RR], s_l[kWarps][RR], s_rf[kMaxRows];
     __shared__ int s_last, s_abort;
     uint8_t *s_q = smem + Sh::kQOff;                          // queries: f16 rows, with SPLIT the lower halves behind them
@@ -251,8 +251,6 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
         for (int i = 0; i < kWarps; i++) {
             mbar_init(&s_full[0][i], 1);
             mbar_init(&s_full[1][i], 1);
-            mbar_init(&s_empty[0][i], 1);
-            mbar_init(&s_empty[1][i], 1);
         }
         s_abort = 0;
         fence_barrier_init();
@@ -397,19 +395,24 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
         if (i < 0) kv_error(p.err);
         return i;
     };
-    // The warp loads a tile's keys (0) or values (1) into its slot. n: tiles that it was
-    // given before it.
-    auto issue = [&](int which, int64_t blk, uint32_t n) {
+    // The warp loads a tile's keys (0) or values (1) into its slot.
+    auto issue = [&](int which, int64_t blk) {
         uint64_t *full = &s_full[which][warp];
         const unsigned have = __ballot_sync(0xffffffffu, blk >= 0) & 0xFu;
-        // the slot's last tile has been read
-        if (n) tc_spin_wait(&s_empty[which][warp], (n - 1) & 1, &s_abort, p.err);
         if (lane == 0) mbar_arrive_expect_tx(full, __popc(have) * Sh::kBlk);
         __syncwarp();
         if (lane < 4 && blk >= 0) {
             const uint32_t dst = which ? vbase + (warp * 4 + lj) * Sh::kVBlk : kbase + (warp * 4 + lj) * Sh::kBlk;
             bulk_load(dst, (which ? p.c.v : p.c.k) + blk * Sh::kBlk, Sh::kBlk, full);
         }
+    };
+    // A slot is its warp's own and is refilled once its bytes have been used: every lane
+    // puts its reads of the tile before the bulk copies that are issued after this. (The
+    // copies go through another proxy, which neither the products' order nor a barrier
+    // of the warp holds back alone.)
+    auto given_back = [&] {
+        fence_async_smem();
+        __syncwarp();
     };
     auto scales = [&](int64_t i, float &k, float &v) {
         k = v = 0.0f;
@@ -579,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
             blk = lookup(sg, t);
             if (t < sg.t1)
 #pragma unroll 1
-                for (int which = 0; which < 2; which++) issue(which, blk, done);
+                for (int which = 0; which < 2; which++) issue(which, blk);
             scales(blk, sk, sv);
         }
 
@@ -700,10 +703,11 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                             else mma16816(s[i0 + i], qa[h * 4 + q], b0, b1);
                         }
                 }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[0][warp]);
             const bool reload = t + kWarps < sg.t1;
-            if (reload) issue(0, next, done + 1);
+            if (reload) {
+                given_back();
+                issue(0, next);
+            }
             float sk_next, sv_next;
             scales(next, sk_next, sv_next);
 
@@ -793,9 +797,10 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                         }
                     }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[1][warp]);
-            if (reload) issue(1, next, done + 1);
+            if (reload) {
+                given_back();
+                issue(1, next);
+            }
             blk = next;
             sk = sk_next;
             sv = sv_next;

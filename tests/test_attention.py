@@ -1061,3 +1061,30 @@ def test_long_prompts_give_the_same_bits_every_time(make, act):
         assert s.t.equal(first, out)
     s.check_attention(first.double().cpu().numpy(), q, past, new, range(3))
     assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+def test_few_rows_give_the_same_bits_every_time(make, act):
+    """A warp's slots refilled several times a segment, and segments one behind another in a CTA: right,
+    and the same run after run."""
+    s = make(act, D=128, q_heads=16, kv_heads=4, page=64, n_slots=34, pages_per_slot=40)
+    total = [2500, 1999] + [300 + 7 * (i % 9) for i in range(32)]
+    s.append([0], total[:1], [0], rows=s.rows(total[0]))
+    s.append([0], total[1:2], [1], rows=s.rows(total[1]))
+    for a in (2, 12, 23):
+        b = min(34, a + 11)
+        s.append([0] * (b - a), total[a:b], range(a, b), rows=s.rows(sum(total[a:b])))
+    for new in ([1] * 34, [2, 3] + [1 + i % 3 for i in range(32)], [1]):
+        n = len(new)
+        r, _, q, _, _ = s.rows(sum(new))
+        past = [t - m for t, m in zip(total, new)]
+        b = s.batch(past, new, range(n), max_new=max(new))
+        first = None
+        for _ in range(40):
+            out = s.out(sum(new), 16)
+            s.ctx.kv_attention(s.cache, b, None, r, out.data_ptr(), 16 * 128)
+            first = out if first is None else first
+            assert s.t.equal(first, out)
+        s.check_attention(first.double().cpu().numpy(), q, past, new, range(n))
+    assert s.ctx.device_status() == 0
