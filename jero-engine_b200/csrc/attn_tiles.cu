@@ -289,8 +289,8 @@ constexpr int kQueryWarps = 4, kAhead = 4;
 
 template <int D, typename T, bool SPLIT>
 __global__ void __launch_bounds__(kQueryWarps * 32)
-    query_tiles_kernel(const __grid_constant__ AttnParams p, int entry0, int entry1, int few_rows, int group, int groups,
-                       uint8_t *images, float *factors)
+    query_tiles_kernel(const __grid_constant__ AttnParams p, int entry0, int entry1, int head0, int heads, int few_rows, int group,
+                       int groups, uint8_t *images, float *factors)
 {
     using Sh = TileShape<D, SPLIT>;
     using L = HeadLanes<D, T>;
@@ -342,10 +342,10 @@ __global__ void __launch_bounds__(kQueryWarps * 32)
             for (int k = 0; k < L::kVals; k++) amax = fmaxf(amax, fabsf(a[k]));
             amax = l.head_max(amax);
             const int kvh = x / g, flat = tok * g + x - kvh * g, e = entry + flat / kRowsItem, r = flat % kRowsItem;
-            if (x >= head1 || e < entry0 || e >= entry1) continue;
+            if (x >= head1 || e < entry0 || e >= entry1 || kvh < head0 || kvh >= head0 + heads) continue;
             const int ex = max(-112, (int)(__float_as_uint(amax) >> 23) - 127);
             float up = __int_as_float((14 - ex + 127) << 23);
-            const int64_t image = (int64_t)(e - entry0) * p.c.heads + kvh;
+            const int64_t image = (int64_t)(e - entry0) * heads + kvh - head0;
             if (d0 == 0) factors[image * kRowsItem + r] = __int_as_float((ex - 14 + 127) << 23) * fabsf(p.scale) * 1.4426950408889634f;
             if (p.scale < 0.0f) up = -up;      // the factors are not negative: maxima stay maxima
             uint32_t hi[L::kVals / 2], lo[L::kVals / 2];
@@ -378,8 +378,8 @@ __global__ void __launch_bounds__(kQueryWarps * 32)
 
 template <int D, typename T, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
-    attend_tiles_kernel(const __grid_constant__ AttnParams p, int entry0, int entry1, int few_rows, const uint8_t *images,
-                        const float *factors)
+    attend_tiles_kernel(const __grid_constant__ AttnParams p, int entry0, int entry1, int head0, int heads, int few_rows,
+                        const uint8_t *images, const float *factors)
 {
     using Sh = TileShape<D, SPLIT>;
     constexpr int NB = Sh::kBufs, SL = Sh::kSlabs;
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // Items go to the CTAs there and back, longest first. (In the list's own order, which
     // is by length within a sequence only: 3 prompts with F32 rows 194 us instead of 158.)
-    const int G = gridDim.x, entries = entry1 - entry0, total = entries * p.c.heads;
+    const int G = gridDim.x, entries = entry1 - entry0, total = entries * heads;
     const bool sorted = entries <= kMaxSorted;
     if (sorted) sort_items(p, entry0, entries, g, few_rows, reinterpret_cast<int *>(smem), s_order);
     Item it;
@@ -441,9 +441,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if ((int64_t)j * G >= total) return -1;
         const int64_t u = (j & 1) ? (int64_t)(j + 1) * G - 1 - (int)blockIdx.x : (int64_t)j * G + (int)blockIdx.x;
         if (u >= total) return 0;
-        const int i = (int)(u / p.c.heads), e = sorted ? s_order[i] : entries - 1 - i;
-        head = (int)(u - (int64_t)i * p.c.heads);
-        image = e * p.c.heads + head;
+        const int i = (int)(u / heads), e = sorted ? s_order[i] : entries - 1 - i, h = (int)(u - (int64_t)i * heads);
+        head = head0 + h;
+        image = e * heads + h;
         return find_item(p, entry0 + e, g, few_rows, lane, it) ? 1 : 0;
     };
 
@@ -901,27 +901,32 @@ cudaError_t launch_tiles_d(const AttnParams &p, int few_rows, uint8_t *ws, size_
         if (2 * at.numRegs < Regs<kSplit>::kSoft + Regs<kSplit>::kOther) return cudaErrorInvalidConfiguration;
         if (dev < 64) set[dev] = true;
     }
-    // the list goes in slices whose queries fit the workspace
+    // the list goes in slices whose queries fit the workspace: of its chunks, and where not even one chunk's
+    // fit (more than 635 key heads of F32 rows of 128) of the key heads too
     const int g = p.rows.q_heads / p.c.heads;
     const int64_t entries = (int64_t)p.b.T * g / kRowsItem + p.b.B;
-    const size_t per = (size_t)p.c.heads * (Sh::kImage + kRowsItem * 4);
-    const int64_t slice = (int64_t)(ws_bytes / per);
-    if (slice < 1) return cudaErrorInvalidValue;
-    for (int64_t e0 = 0; e0 < entries; e0 += slice) {
-        const int e1 = (int)std::min(entries, e0 + slice);
-        float *factors = reinterpret_cast<float *>(ws + (size_t)(e1 - e0) * p.c.heads * Sh::kImage);
-        using L = HeadLanes<D, T>;
-        // few tokens: one load a warp (the whole call with 128 tokens 53 us, grouped 57); many: a group of
-        // heads, which share a token's angles (1024 tokens 76 us, one load a warp 80)
-        const int group = p.b.T <= 512 ? L::kHeads : kAhead * L::kHeads * 2, groups = (p.rows.q_heads + group - 1) / group;
-        if ((e = launch_dependent(query_tiles_kernel<D, T, kSplit>,
-                                  dim3((unsigned)(((int64_t)p.b.T * groups + kQueryWarps - 1) / kQueryWarps)), dim3(kQueryWarps * 32), 0,
-                                  st, p, (int)e0, e1, few_rows, group, groups, ws, factors)) != cudaSuccess)
-            return e;
-        const int grid = (int)std::min<int64_t>(p.num_sms, (e1 - e0) * p.c.heads);
-        if ((e = launch_dependent(kern, dim3(grid), dim3(kThreads), Sh::kSmem, st, p, (int)e0, e1, few_rows, (const uint8_t *)ws,
-                                  (const float *)factors)) != cudaSuccess)
-            return e;
+    constexpr size_t kPerHead = Sh::kImage + kRowsItem * 4;
+    const int fit = (int)std::min<size_t>(p.c.heads, ws_bytes / kPerHead);
+    if (fit < 1) return cudaErrorInvalidValue;
+    const int64_t slice = (int64_t)(ws_bytes / (fit * kPerHead));
+    using L = HeadLanes<D, T>;
+    // few tokens: one load a warp (the whole call with 128 tokens 53 us, grouped 57); many: a group of
+    // heads, which share a token's angles (1024 tokens 76 us, one load a warp 80)
+    const int group = p.b.T <= 512 ? L::kHeads : kAhead * L::kHeads * 2, groups = (p.rows.q_heads + group - 1) / group;
+    for (int h0 = 0; h0 < p.c.heads; h0 += fit) {
+        const int heads = std::min(fit, p.c.heads - h0);
+        for (int64_t e0 = 0; e0 < entries; e0 += slice) {
+            const int e1 = (int)std::min(entries, e0 + slice);
+            float *factors = reinterpret_cast<float *>(ws + (size_t)(e1 - e0) * heads * Sh::kImage);
+            if ((e = launch_dependent(query_tiles_kernel<D, T, kSplit>,
+                                      dim3((unsigned)(((int64_t)p.b.T * groups + kQueryWarps - 1) / kQueryWarps)), dim3(kQueryWarps * 32),
+                                      0, st, p, (int)e0, e1, h0, heads, few_rows, group, groups, ws, factors)) != cudaSuccess)
+                return e;
+            const int grid = (int)std::min<int64_t>(p.num_sms, (e1 - e0) * heads);
+            if ((e = launch_dependent(kern, dim3(grid), dim3(kThreads), Sh::kSmem, st, p, (int)e0, e1, h0, heads, few_rows,
+                                      (const uint8_t *)ws, (const float *)factors)) != cudaSuccess)
+                return e;
+        }
     }
     return cudaSuccess;
 }

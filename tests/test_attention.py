@@ -1088,3 +1088,13 @@ def test_few_rows_give_the_same_bits_every_time(make, act):
             assert s.t.equal(first, out)
         s.check_attention(first.double().cpu().numpy(), q, past, new, range(n))
     assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_prompts_of_more_key_heads_than_the_workspace_takes(make):
+    """640 key heads with F32 rows of 128: not one chunk of rows of all heads fits the prompts' workspace."""
+    s = make("f32", D=128, q_heads=640, kv_heads=640, page=16, n_slots=2, pages_per_slot=3)
+    past, new = [3, 20], [20, 17]
+    s.append([0, 0], [p + n for p, n in zip(past, new)], [1, 0], rows=s.rows(sum(past) + sum(new)))
+    s.attend(past, new, [1, 0], behind=1, max_new=20)
+    assert s.ctx.device_status() == 0
