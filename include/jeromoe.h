@@ -405,6 +405,13 @@ int moe_residency_summary(const moe_ctx *ctx, moe_residency *out);
  * check met a bad batch entry or page (above). */
 int moe_device_status(moe_ctx *ctx, int32_t *status);
 
+/* Fault injection for tests (no counterpart in the reference): leaves ctx as a
+ * bounded wait that ran out in a forward, in an attention call, or in both
+ * leaves it, the status word set and the attention's arrival counters not back
+ * at zero, without a device fault. Needs a layer upload, or an attention call,
+ * before. */
+int moe_debug_timeout(moe_ctx *ctx, int32_t forward, int32_t attention);
+
 /* ---- per-kernel timing (the device counterpart of PassTiming, src/engine.rs:136) ---- */
 
 typedef struct moe_kernel_time {

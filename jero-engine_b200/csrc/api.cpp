@@ -2097,6 +2097,24 @@ int moe_forward_ep(moe_ctx *ctx, int32_t layer, int32_t T, const float *x, float
 
 // ------------------------------------------------- the attention sublayer
 
+int moe_debug_timeout(moe_ctx *ctx, int32_t forward, int32_t attention)
+{
+    if (!ctx) return fail(nullptr, MOE_ERR_INVALID_ARGS, "null context");
+    if ((forward && !ctx->scratch.err) || (attention && !ctx->attn_ws))
+        return fail(ctx, MOE_ERR_INVALID_ARGS, "no such call was made on this context");
+    DeviceGuard guard;
+    CUDA_TRY(ctx, cudaSetDevice(ctx->spec.device), "cudaSetDevice");
+    // status words of kErrTimeout (1), arrival counters that are not back at zero
+    const std::vector<int> ones(attn_counter_bytes(ctx->num_sms) / sizeof(int), 1);
+    if (forward)
+        CUDA_TRY(ctx, cudaMemcpyAsync(ctx->scratch.err, ones.data(), sizeof(int), cudaMemcpyHostToDevice, ctx->stream), "set status");
+    if (attention)
+        CUDA_TRY(ctx, cudaMemcpyAsync(ctx->attn_ws, ones.data(), ones.size() * sizeof(int), cudaMemcpyHostToDevice, ctx->stream),
+                 "set status");
+    CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream), "status sync");
+    return MOE_OK;
+}
+
 static bool misaligned(const void *p) { return ((uintptr_t)p & 15) != 0; }
 static bool misaligned4(const void *p) { return ((uintptr_t)p & 3) != 0; }   // int32 and f32 arrays
 

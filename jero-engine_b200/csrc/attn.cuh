@@ -63,7 +63,8 @@ __device__ __forceinline__ void store_vals(T *p, const float (&v)[N])
     }
 }
 
-__device__ __forceinline__ void kv_error(int *err) { atomicExch(err, kErrKvBounds); }
+// A wait that ran out is left in the word: after one no output of the call is good.
+__device__ __forceinline__ void kv_error(int *err) { atomicCAS(err, 0, kErrKvBounds); }
 
 __device__ __forceinline__ int row_of(const KvBatchDev &b, int s) { return b.row_start ? ld_plain(b.row_start + s) : s; }
 

@@ -176,6 +176,7 @@ EXPORTS = {
     "moe_ep_unique_id": (C.c_int, [C.c_void_p]),
     "moe_ep_init": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p]),
     "moe_ep_reset": (C.c_int, [C.c_void_p]),
+    "moe_debug_timeout": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32]),
     "moe_debug_ep_fault": (C.c_int, [C.c_void_p, C.c_uint32, C.c_int64]),
     "moe_forward_ep": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                  C.c_int32]),
@@ -483,6 +484,10 @@ class Context:
         r = moe_residency()
         _check(lib.moe_residency_summary(self.h, C.byref(r)), self.h)
         return r
+
+    def debug_timeout(self, forward=False, attention=False):
+        """Test hook: leaves the context as a bounded wait that ran out leaves it (moe_debug_timeout)."""
+        _check(lib.moe_debug_timeout(self.h, int(forward), int(attention)), self.h)
 
     def debug_capture_block_sums(self, device_ptr: int, n_ints: int):
         """Raw int32 block sums of the int8 tensor-core gate/up launch go to this

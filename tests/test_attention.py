@@ -1098,3 +1098,20 @@ def test_prompts_of_more_key_heads_than_the_workspace_takes(make):
     s.append([0, 0], [p + n for p, n in zip(past, new)], [1, 0], rows=s.rows(sum(past) + sum(new)))
     s.attend(past, new, [1, 0], behind=1, max_new=20)
     assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_a_timeout_outlasts_a_bad_entry(make):
+    """A wait that ran out is reported as such whatever is found after it, and the call after the report is right."""
+    s = make("f32", D=128, q_heads=8, kv_heads=2, page=64, n_slots=2, pages_per_slot=48)
+    s.append([0], [3000], [0], rows=s.rows(3000))
+    s.attend([2999], [1], [0])
+    s.ctx.debug_timeout(attention=True)
+    r, _, _, _, _ = s.rows(1)
+    out = s.out(1, 8)
+    s.ctx.kv_attention(s.cache, s.batch([10], [1], [5]), None, r, out.data_ptr(), 1024)
+    with pytest.raises(jm.DeviceTimeout):
+        s.ctx.device_status()
+    assert s.ctx.device_status() == 0
+    s.attend([2999], [1], [0])
+    assert s.ctx.device_status() == 0
