@@ -402,7 +402,8 @@ int moe_residency_summary(const moe_ctx *ctx, moe_residency *out);
  * stream). *status != 0 (and MOE_ERR_TIMEOUT) when a bounded wait inside a
  * kernel gave up since the last check; host-pointer forwards check it themselves.
  * *status != 0 and MOE_ERR_TENSOR_BOUNDS when an attention call since the last
- * check met a bad batch entry or page (above). */
+ * check met a bad batch entry or page (above). A wait that ran out comes first;
+ * the message then names the other as well. */
 int moe_device_status(moe_ctx *ctx, int32_t *status);
 
 /* Fault injection for tests (no counterpart in the reference): leaves ctx as a

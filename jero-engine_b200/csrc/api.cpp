@@ -172,7 +172,7 @@ struct moe_ctx {
     int32_t *dbg_isum = nullptr;   // moe_debug_capture_block_sums
     uint64_t dbg_isum_cap = 0;
     int num_sms = 148;
-    int *status_host = nullptr;   // pinned word for the device status flag
+    int *status_host = nullptr;   // two pinned words for the device status flags
     float *stack_buf = nullptr;   // moe_prefill_ffn_layers: the hidden rows on the device
     size_t stack_buf_n = 0;
     // the LM head (moe_lm_head_upload / moe_lm_head)
@@ -842,7 +842,7 @@ int moe_ctx_create(const moe_device_spec *spec, moe_ctx **out)
     ctx->stream = ctx->own_stream;
     if ((e = cudaDeviceGetAttribute(&ctx->num_sms, cudaDevAttrMultiProcessorCount, spec->device)) != cudaSuccess)
         return cuda_fail(nullptr, e, "cudaDeviceGetAttribute");
-    if ((e = cudaMallocHost(&ctx->status_host, sizeof(int))) != cudaSuccess)
+    if ((e = cudaMallocHost(&ctx->status_host, 2 * sizeof(int))) != cudaSuccess)
         return cuda_fail(nullptr, e, "cudaMallocHost");
     *ctx->status_host = 0;
     *out = ctx.release();
@@ -1448,45 +1448,37 @@ int moe_device_status(moe_ctx *ctx, int32_t *status)
 {
     if (!ctx || !status) return fail(nullptr, MOE_ERR_INVALID_ARGS, "null argument");
     *status = 0;
-    if (ctx->attn_ws) {   // the attention calls' own word
-        DeviceGuard guard;
-        CUDA_TRY(ctx, cudaSetDevice(ctx->spec.device), "cudaSetDevice");
-        CUDA_TRY(ctx, cudaMemcpyAsync(ctx->status_host, ctx->attn_ws, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream),
-                 "copy status");
-        CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream), "status sync");
-        *status = *ctx->status_host;
-        if (*status) {
-            // after a wait that ran out the arrival counters are as it left them
-            CUDA_TRY(ctx, cudaMemsetAsync(ctx->attn_ws, 0, *status == kErrKvBounds ? sizeof(int) : attn_counter_bytes(ctx->num_sms),
-                                          ctx->stream),
-                     "clear status");
-            if (*status != kErrKvBounds)
-                return fail(ctx, MOE_ERR_TIMEOUT, "a bounded device wait ran out in an attention call (status %d)",
-                            *status);
-            return fail(ctx, MOE_ERR_TENSOR_BOUNDS,
-                        "an attention call met a batch entry, slot or page id out of range (or a slot twice)");
-        }
-    }
-    // the context's word, or (LM head calls before any layer upload) the head's own
+    // two words: of the forwards (the context's, or, for LM head calls before any layer upload, the
+    // head's own), and of the attention calls
     int *word = ctx->scratch.err ? ctx->scratch.err : ctx->head.errw;
+    DeviceGuard guard;
     CUDA_TRY(ctx, cudaSetDevice(ctx->spec.device), "cudaSetDevice");
-    if (!word) {
-        CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream), "status sync");
-        return MOE_OK;
-    }
-    CUDA_TRY(ctx, cudaMemcpyAsync(ctx->status_host, word, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream),
-             "copy status");
+    int *host = ctx->status_host;
+    host[0] = host[1] = 0;
+    if (word) CUDA_TRY(ctx, cudaMemcpyAsync(&host[0], word, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream), "copy status");
+    if (ctx->attn_ws)
+        CUDA_TRY(ctx, cudaMemcpyAsync(&host[1], ctx->attn_ws, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream), "copy status");
     CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream), "status sync");
-    *status = *ctx->status_host;
-    if (*status) {
-        CUDA_TRY(ctx, cudaMemsetAsync(word, 0, sizeof(int), ctx->stream), "clear status");
-        if (ctx->ep.world && (*status == kErrEpTimeout || *status == kErrEpDesync)) {
-            ctx->ep.p2p_broken = true;
-            return fail(ctx, MOE_ERR_TIMEOUT,
-                        "a bounded peer-rank wait failed (status %d); call moe_ep_reset on every rank", *status);
-        }
-        return fail(ctx, MOE_ERR_TIMEOUT, "a bounded device wait ran out (status %d)", *status);
+    const int forward = host[0], attention = host[1];
+    if (forward) CUDA_TRY(ctx, cudaMemsetAsync(word, 0, sizeof(int), ctx->stream), "clear status");
+    if (attention)   // after a wait that ran out the arrival counters are as it left them
+        CUDA_TRY(ctx, cudaMemsetAsync(ctx->attn_ws, 0, attention == kErrKvBounds ? sizeof(int) : attn_counter_bytes(ctx->num_sms),
+                                      ctx->stream),
+                 "clear status");
+    *status = forward ? forward : attention;
+    const char *also = !attention ? ""
+                       : attention == kErrKvBounds ? "; an attention call met a batch entry, slot or page id out of range"
+                                                   : "; one of an attention call too";
+    if (forward && ctx->ep.world && (forward == kErrEpTimeout || forward == kErrEpDesync)) {
+        ctx->ep.p2p_broken = true;
+        return fail(ctx, MOE_ERR_TIMEOUT,
+                    "a bounded peer-rank wait failed (status %d); call moe_ep_reset on every rank%s", forward, also);
     }
+    if (forward) return fail(ctx, MOE_ERR_TIMEOUT, "a bounded device wait of a forward ran out (status %d)%s", forward, also);
+    if (attention == kErrKvBounds)
+        return fail(ctx, MOE_ERR_TENSOR_BOUNDS,
+                    "an attention call met a batch entry, slot or page id out of range (or a slot twice)");
+    if (attention) return fail(ctx, MOE_ERR_TIMEOUT, "a bounded device wait ran out in an attention call (status %d)", attention);
     return MOE_OK;
 }
 

@@ -1115,3 +1115,32 @@ def test_a_timeout_outlasts_a_bad_entry(make):
     assert s.ctx.device_status() == 0
     s.attend([2999], [1], [0])
     assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_status_of_forwards_and_attention_at_once():
+    """moe_device_status reports a forward's wait that ran out although an attention call met a bad entry too."""
+    import synth
+    cfg = synth.CONFIGS[2].scaled(E=16, I=256, H=512)
+    s = Setup("f32", D=64, q_heads=4, kv_heads=2)
+    d, keep = synth.desc_for(cfg, synth.build_weights(cfg))
+    s.ctx.upload(0, d)
+
+    def bad_entry():
+        s.ctx.kv_attention(s.cache, s.batch([0], [1], [99]), None, s.rows(1)[0], s.out(1, 4).data_ptr(), 256)
+
+    bad_entry()
+    with pytest.raises(jm.TensorBoundsError):
+        s.ctx.device_status()
+    for forward, attention in ((True, False), (True, True), (False, True)):
+        bad_entry()
+        s.ctx.debug_timeout(forward=forward, attention=attention)
+        with pytest.raises(jm.DeviceTimeout) as e:
+            s.ctx.device_status()
+        assert ("attention" in str(e.value)) and ("forward" in str(e.value)) == forward
+        assert s.ctx.device_status() == 0
+    s.ctx.debug_timeout(forward=True)
+    with pytest.raises(jm.DeviceTimeout):
+        s.ctx.device_status()
+    assert s.ctx.device_status() == 0
+    s.close()
