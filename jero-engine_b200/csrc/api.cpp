@@ -1169,6 +1169,8 @@ int moe_forward_block(moe_ctx *ctx, int32_t layer, int32_t T, const float *hidde
 // (run_prefill_with_hidden, src/qwen_deepseek.rs:2217-2316: every layer per
 // token), because each sublayer treats its tokens independently; with host
 // pointers the rows cross PCIe once each way for the whole stack.
+static int read_status(moe_ctx *ctx, int32_t *status, bool of_attention);
+
 int moe_prefill_ffn_layers(moe_ctx *ctx, int32_t first_layer, int32_t n_layers, int32_t T, float *hidden,
                            int32_t ptr_kind)
 {
@@ -1211,7 +1213,7 @@ int moe_prefill_ffn_layers(moe_ctx *ctx, int32_t first_layer, int32_t n_layers, 
     if (ptr_kind == MOE_PTR_HOST) {
         CUDA_TRY(ctx, cudaMemcpyAsync(hidden, rows, n * 4, cudaMemcpyDeviceToHost, st), "copy hidden");
         int32_t status = 0;
-        const int rc = moe_device_status(ctx, &status);   // synchronises the stream
+        const int rc = read_status(ctx, &status, false);   // synchronises the stream
         if (rc != MOE_OK) return rc;
         if (status) return fail(ctx, MOE_ERR_TIMEOUT, "a bounded device wait ran out (status %d)", status);
     }
@@ -1447,6 +1449,12 @@ int moe_layer_set_ffn_norm(moe_ctx *ctx, int32_t layer, const float *weight, flo
 int moe_device_status(moe_ctx *ctx, int32_t *status)
 {
     if (!ctx || !status) return fail(nullptr, MOE_ERR_INVALID_ARGS, "null argument");
+    return read_status(ctx, status, true);
+}
+
+// Without of_attention: the forwards' word alone; the attention calls' stays for the next check.
+static int read_status(moe_ctx *ctx, int32_t *status, bool of_attention)
+{
     *status = 0;
     // two words: of the forwards (the context's, or, for LM head calls before any layer upload, the
     // head's own), and of the attention calls
@@ -1456,7 +1464,7 @@ int moe_device_status(moe_ctx *ctx, int32_t *status)
     int *host = ctx->status_host;
     host[0] = host[1] = 0;
     if (word) CUDA_TRY(ctx, cudaMemcpyAsync(&host[0], word, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream), "copy status");
-    if (ctx->attn_ws)
+    if (of_attention && ctx->attn_ws)
         CUDA_TRY(ctx, cudaMemcpyAsync(&host[1], ctx->attn_ws, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream), "copy status");
     CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream), "status sync");
     const int forward = host[0], attention = host[1];

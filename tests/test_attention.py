@@ -1144,3 +1144,22 @@ def test_status_of_forwards_and_attention_at_once():
         s.ctx.device_status()
     assert s.ctx.device_status() == 0
     s.close()
+
+
+@pytest.mark.gpu
+def test_prefill_leaves_the_attentions_status(make):
+    """A host-pointer prefill reports its own waits only: a bad entry of an attention call before it stays for the
+    next check."""
+    import synth
+    cfg = synth.CONFIGS[2].scaled(E=16, I=256, H=512)
+    s = make("f32", D=64, q_heads=4, kv_heads=2)
+    d, keep = synth.desc_for(cfg, synth.build_weights(cfg))
+    s.ctx.upload(0, d)
+    s.ctx.set_ffn_norm(0, None, 1e-6)
+    hidden = synth.gen_x(cfg, 9)
+    want = s.ctx.prefill_ffn_layers(0, 1, hidden.copy())
+    s.ctx.kv_attention(s.cache, s.batch([0], [1], [99]), None, s.rows(1)[0], s.out(1, 4).data_ptr(), 256)
+    np.testing.assert_array_equal(s.ctx.prefill_ffn_layers(0, 1, hidden.copy()), want)
+    with pytest.raises(jm.TensorBoundsError):
+        s.ctx.device_status()
+    assert s.ctx.device_status() == 0
