@@ -287,6 +287,7 @@ typedef enum moe_act {
 } moe_act;
 
 #define MOE_KV_MAX_TOKENS (1 << 29)   /* of a slot: table_stride * page_tokens */
+#define MOE_ROPE_MAX_FREQ 65536.0     /* the largest |inv_freq| (radians a token) */
 #define MOE_KV_BLOCK_TOKENS 16   /* tokens that share a scale, as the blocks of the reference's arena (src/kv.rs:1-4) */
 
 /* One layer's KV cache. A block of 16 tokens and one head is held as signed
@@ -327,13 +328,15 @@ typedef struct moe_kv_batch {
 
 /* Norm and rotation of query and key heads: x * rsqrt(mean(x^2) + eps) * norm
  * (per head, where the weight is given), then the first rope_dim values rotated
- * by position * inv_freq[i] and scaled by mscale. Angles are formed in f64; the
- * keys of the cache to 2^-40 of their largest or better, then rounded to f32. */
+ * by position * inv_freq[i] and scaled by mscale. Angles are formed in f64, to
+ * 2^-53 of their size (at most 2^47: no frequency is above MOE_ROPE_MAX_FREQ);
+ * beyond that the keys of the cache are good to 2^-40 of their largest or
+ * better, then rounded to f32. */
 typedef struct moe_rope {
     int32_t rope_dim;           /* even, 0 .. head_dim; 0: no rotation */
     int32_t interleaved;        /* 0: value i turns with i + rope_dim / 2; 1: 2i with 2i + 1 */
     double theta;               /* inv_freq[i] = theta^(-2i / rope_dim) where inv_freq is NULL */
-    const double *inv_freq;     /* host memory, [rope_dim / 2], or NULL */
+    const double *inv_freq;     /* host memory, [rope_dim / 2], or NULL; at most MOE_ROPE_MAX_FREQ in magnitude */
     double mscale;              /* 0 counts as 1 */
     double eps;
     const float *q_norm, *k_norm;   /* device, [head_dim] each, or NULL: no norm */

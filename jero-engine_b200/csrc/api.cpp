@@ -2161,7 +2161,10 @@ static int check_rope(moe_ctx *ctx, const moe_rope *r, int head_dim, RopeDev *ou
     out->k_norm = r->k_norm;
     for (int i = 0; i < r->rope_dim / 2; i++) {
         out->inv[i] = r->inv_freq ? r->inv_freq[i] : std::pow(r->theta, -2.0 * i / r->rope_dim);
-        if (!std::isfinite(out->inv[i])) return fail(ctx, MOE_ERR_INVALID_ARGS, "inv_freq[%d] is not finite", i);
+        // the kernels take whole quarter turns off angles up to 2^47; positions are below 2^31
+        if (!(std::fabs(out->inv[i]) <= MOE_ROPE_MAX_FREQ))
+            return fail(ctx, MOE_ERR_INVALID_ARGS, "inv_freq[%d] is %g (finite, at most %g in magnitude)", i, out->inv[i],
+                        MOE_ROPE_MAX_FREQ);
     }
     return MOE_OK;
 }

@@ -102,7 +102,8 @@ __device__ __forceinline__ int64_t block_index(const KvCacheDev &c, int slot, in
 
 // An angle less its whole quarter turns, in f64 (far positions lose nothing):
 // the rest, in [-pi/4, pi/4], and the number of turns mod 4, which the low bits
-// of angle * 2/pi + 1.5 * 2^52 hold.
+// of angle * 2/pi + 1.5 * 2^52 hold: for angles up to 2^47 (MOE_ROPE_MAX_FREQ
+// times a position), where the rounding of 2/pi (2^-53) moves the rest by 2 % at most.
 __device__ __forceinline__ int quarter_turns(double &angle)
 {
     const double t = fma(angle, 0.6366197723675814, 6755399441055744.0), n = t - 6755399441055744.0;

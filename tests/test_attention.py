@@ -1163,3 +1163,52 @@ def test_prefill_leaves_the_attentions_status(make):
     with pytest.raises(jm.TensorBoundsError):
         s.ctx.device_status()
     assert s.ctx.device_status() == 0
+
+
+# -------------------------------------------------------- rotation frequencies
+
+
+def test_check_takes_frequencies_up_to_the_limit():
+    _check(_args(rope__inv_freq=[jm.ROPE_MAX_FREQ] * 64))
+    _check(_args(rope__inv_freq=[-jm.ROPE_MAX_FREQ] + [0.0] * 63))
+    _check(_args(rope__theta=1e-4))
+
+
+@pytest.mark.parametrize("rope", [dict(inv_freq=[1e20] * 64), dict(inv_freq=[1.0] * 63 + [-65537.0]), dict(theta=1e-20),
+                                  dict(theta=5e-324), dict(inv_freq=[float("nan")] * 64)])
+def test_check_refuses_frequencies_past_the_limit(rope):
+    with pytest.raises(jm.InvalidArguments):
+        _check(_args(rope={"rope_dim": 128, **rope}))
+
+
+def test_quarter_turns_hold_up_to_the_limit_and_not_far_past_it():
+    """The device's reduction in exact arithmetic: up to the largest angle that the checks let through the rest stays in
+    [-pi/4, pi/4], and 2 % for the rounding of 2/pi (2^47 2/pi 2^-53 quarter turns)."""
+    from fractions import Fraction as F
+
+    def rest(angle):
+        t = float(F(angle) * F(0.6366197723675814) + F(6755399441055744.0))     # an fma rounds once, as float() does
+        n = F(t - 6755399441055744.0)
+        return abs(float(F(float(F(angle) - n * F(1.5707963267948966))) - n * F(6.123233995736766e-17)))
+
+    rng = np.random.default_rng(3)
+    for scale in (1.0, 2.0 ** 20, 2.0 ** 40, jm.ROPE_MAX_FREQ * (2.0 ** 31 - 1)):
+        assert max(rest(float(a)) for a in scale * rng.uniform(-1, 1, 200)) <= 1.02 * np.pi / 4
+    assert rest(1e20) > 100.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_norm_rope_of_the_largest_angles(make, act):
+    s = make(act, D=64)
+    f = jm.ROPE_MAX_FREQ / (1.0 + np.arange(32)) * np.where(np.arange(32) % 3 == 0, -1.0, 1.0)
+    rope, plain = s.rope(64, False, False, inv_freq=f)
+    pos = [(1 << 31) - 5000, (1 << 30) + 1, 7, 0]
+    r, x, q, k, _ = s.rows(4)
+    oq, ok = s.out(4, s.hq), s.out(4, s.hk)
+    s.ctx.qk_norm_rope(jm.KvBatch(n_seqs=4, n_tokens=4, past=s.ints(pos)), rope, r, s.into(oq, ok))
+    for got, y, which in ((oq, q, "q"), (ok, k, "k")):
+        ref = plain(y, which, pos)      # the angle is the same product in f64, numpy reduces it exactly
+        size = np.max(np.abs(y), axis=-1, keepdims=True) * 2
+        # at 1.02 pi / 4 the series' next terms, x^11 / 11! and x^12 / 12!, are below 3e-9 < u / 16
+        assert np.all(np.abs(got.double().cpu().numpy() - ref) <= 25 * U * size + HALF_STEP[act] * np.abs(ref) * (1 + 2 ** -7))
