@@ -6,6 +6,8 @@
 #include <cuda_fp16.h>
 #include <limits.h>
 
+#include <type_traits>
+
 #include "../../include/jeromoe.h"
 #include "attn.h"
 #include "ptx.cuh"
@@ -148,6 +150,41 @@ __device__ __forceinline__ int seq_of_row_warp(const KvBatchDev &b, int row, int
     return __reduce_add_sync(0xffffffffu, n) - 1;
 }
 
+// A norm's factor 1 / sqrt(mean square + eps), in f32, is good where the mean lies
+// well inside f32's range: squares that underflow are then far below it, and
+// none has overflowed.
+__device__ __forceinline__ bool plain_root(float inv) { return inv > 0.0f && inv < 1e10f; }
+
+// Where it does not (values above some 1e18 or below 1e-10, which only F32 and
+// BF16 rows have): a head in LANES lanes, N values in each, is scaled by the power
+// of two d that takes its largest value to [1, 2), and its factor formed anew, with
+// eps d^2. Where that would be above 2^100 the squares are nothing beside it, and a
+// d of 2^60 keeps it in range. The whole warp comes here; heads with !mine are left alone.
+template <int N, int LANES>
+__device__ __forceinline__ void scale_head(float (&v)[N], float &inv, double eps, bool mine)
+{
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) amax = fmaxf(amax, fabsf(v[i]));
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const int e = min(126, max(-126, (int)(__float_as_uint(amax) >> 23) - 127));
+    float d = mine ? __int_as_float((127 - e) << 23) : 1.0f, add = (float)(eps * (double)d * (double)d);
+    if (mine && add > 0x1p100f) {
+        d = 0x1p60f;
+        add = (float)(eps * 0x1p120);
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        v[i] *= d;
+        ss = fmaf(v[i], v[i], ss);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (mine) inv = rsqrtf(ss * (1.0f / (N * LANES)) + add);
+}
+
 // A token's heads by one warp, 16 bytes of a head to a lane: the lane's values
 // lie at the same place of every head, so its angles and norm weights are
 // fetched once for the token and stay in registers.
@@ -202,19 +239,34 @@ struct HeadLanes {
         for (int o = kLanes / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
         return v;
     }
-    // v normed (norm) and turned, in f32; the whole warp, each kLanes a head.
-    __device__ __forceinline__ void turn(float (&v)[kVals], bool norm, const float (&w)[kVals], float eps, float *y) const
+    // M heads at a time normed, in f32; the whole warp, each kLanes a head.
+    template <int M>
+    __device__ __forceinline__ void norms(float (&v)[M][kVals], const float (&w)[kVals], double eps) const
     {
-        if (norm) {
+        float inv[M];
+        bool plain = true;
+#pragma unroll
+        for (int h = 0; h < M; h++) {
             float ss = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kVals; i++) ss = fmaf(v[i], v[i], ss);
+            for (int i = 0; i < kVals; i++) ss = fmaf(v[h][i], v[h][i], ss);
 #pragma unroll
             for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = rsqrtf(ss * (1.0f / D) + eps);
-#pragma unroll
-            for (int i = 0; i < kVals; i++) v[i] = v[i] * inv * w[i];
+            inv[h] = rsqrtf(ss * (1.0f / D) + (float)eps);
+            if (!std::is_same<T, __half>::value) plain &= plain_root(inv[h]);
         }
+        // (one vote for all of them: with one for each they wait for one another)
+        if (!__all_sync(0xffffffffu, plain))
+#pragma unroll
+            for (int h = 0; h < M; h++) scale_head<kVals, kLanes>(v[h], inv[h], eps, !plain_root(inv[h]));
+#pragma unroll
+        for (int h = 0; h < M; h++)
+#pragma unroll
+            for (int i = 0; i < kVals; i++) v[h][i] = v[h][i] * inv[h] * w[i];
+    }
+    // v turned, in f32; the whole warp.
+    __device__ __forceinline__ void turn(float (&v)[kVals], float *y) const
+    {
         if (!turns) return;
         float other[kVals];
         if (inter) {
@@ -261,7 +313,8 @@ __device__ __forceinline__ void norm_rope_vals(float (&v)[D / 32], const float *
         for (int i = 0; i < N; i++) ss = fmaf(v[i], v[i], ss);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = 1.0f / sqrtf(ss * (1.0f / D) + (float)r.eps);
+        float inv = 1.0f / sqrtf(ss * (1.0f / D) + (float)r.eps);
+        if (!plain_root(inv)) scale_head<N, 32>(v, inv, r.eps, true);
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = v[i] * inv * ld_plain(w + lane * N + i);
     }

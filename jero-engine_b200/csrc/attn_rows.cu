@@ -24,11 +24,11 @@ constexpr int kRowWarps = 4;
 // Norms and rotation: y = x / sqrt(mean x^2 + eps) w, then pairs turned by
 // position * frequency. A warp takes a group of a token's heads, or all of them,
 // kAhead loads of 16 bytes a lane under way before the first is worked on (four:
-// 25.6 us where two take 23.5, the registers).
+// 25.6 us where two take 23.5, the registers; five CTAs an SM 22.9, four 27.5).
 constexpr int kAhead = 2;
 
 template <int D, typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) qk_norm_rope_kernel(KvBatchDev b, const __grid_constant__ RopeDev rope,
+__global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 8 : 5) qk_norm_rope_kernel(KvBatchDev b, const __grid_constant__ RopeDev rope,
                                                                       AttnRows in, AttnRows out, int group, int groups, int *err)
 {
     using L = HeadLanes<D, T>;
@@ -82,11 +82,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) qk_norm_rope_kernel(KvBatchDev
         float w[L::kVals];
         l.weights(norm, w);
         for (;;) {
+            if (norm) l.norms(v, w, rope.eps);
 #pragma unroll
             for (int i = 0; i < kAhead; i++) {
                 const int x = h + i * L::kHeads;
                 if (x - sub >= head1) break;
-                l.turn(v[i], norm != nullptr, w, (float)rope.eps, s_y[warp]);
+                l.turn(v[i], s_y[warp]);
                 if (x < head1) store_vals<L::kVals>(dst + x * D, v[i]);
             }
             h += kAhead * L::kHeads;

@@ -1212,3 +1212,56 @@ def test_norm_rope_of_the_largest_angles(make, act):
         size = np.max(np.abs(y), axis=-1, keepdims=True) * 2
         # at 1.02 pi / 4 the series' next terms, x^11 / 11! and x^12 / 12!, are below 3e-9 < u / 16
         assert np.all(np.abs(got.double().cpu().numpy() - ref) <= 25 * U * size + HALF_STEP[act] * np.abs(ref) * (1 + 2 ** -7))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("D,eps", [(128, 0.0), (64, 1e-6)])
+def test_norm_of_rows_whose_squares_leave_f32(make, act, D, eps):
+    """Rows whose sum of squares overflows or underflows 32 bits have a norm like any other."""
+    s = make(act, D=D, q_heads=6, kv_heads=3)
+    rope, plain = s.rope(eps=eps)
+    r, x, _, _, _ = s.rows(8)
+    gain = [1e19, 1.0, 1e30, 1e36, 1e-19, 1e-25, 1e-30, 3e18]
+    x *= s.t.tensor(gain, dtype=s.dtype, device="cuda")[:, None]
+    f = x.double().cpu().numpy()
+    a, b = s.hq * D, (s.hq + s.hk) * D
+    oq, ok = s.out(8, s.hq), s.out(8, s.hk)
+    pos = [0, 5, 1 << 20, 130, 7, 9, 1000, 3]
+    s.ctx.qk_norm_rope(jm.KvBatch(n_seqs=8, n_tokens=8, past=s.ints(pos)), rope, r, s.into(oq, ok))
+    for got, y, which in ((oq, f[:, :a].reshape(8, -1, D), "q"), (ok, f[:, a:b].reshape(8, -1, D), "k")):
+        ref = plain(y, which, pos)
+        size = 2 * np.max(np.abs(ref), axis=-1, keepdims=True) * np.sqrt(2.0)
+        # (bf16 holds values below its normal range, 2^-126, to 2^-134 only; f32 to 2^-150)
+        tiny = 2.0 ** -134 if act == "bf16" else 2.0 ** -150
+        err = np.abs(got.double().cpu().numpy() - ref)
+        assert np.all(err <= 24 * U * size + HALF_STEP[act] * np.abs(ref) * (1 + 2 ** -7) + tiny), (which, err.max(axis=(1, 2)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("scale,eps", [(1e30, 1e-6), (1e-25, 0.0)])
+def test_step_of_rows_whose_squares_leave_f32(make, act, scale, eps):
+    """The same for the queries of the whole step, of few rows and of many."""
+    s = make(act, D=64, q_heads=8, kv_heads=2, page=16, n_slots=2, pages_per_slot=16)
+    rope, plain = s.rope(eps=eps)
+    past = [0, 0]
+    for new in ([150, 3], [1, 1]):
+        r, x, _, _, v = s.rows(sum(new))
+        x[:, : 10 * 64] *= scale
+        f = x.double().cpu().numpy()
+        q, k = f[:, :512].reshape(-1, 8, 64), f[:, 512:640].reshape(-1, 2, 64)
+        out = s.out(sum(new), 8)
+        s.ctx.attention(s.cache, s.batch(past, new, range(2)), rope, None, r, out.data_ptr(), 8 * 64)
+        at, want = 0, np.empty(q.shape)
+        for i in range(2):
+            pos = past[i] + np.arange(new[i])
+            rows = slice(at, at + new[i])
+            s.ref.append(i, past[i], plain(k[rows], "k", pos), v[rows])
+            want[rows] = plain(q[rows], "q", pos)
+            at += new[i]
+            past[i] += new[i]
+            s.lens[i] = past[i]
+            s.check_blocks(i)
+        s.check_attention(out.double().cpu().numpy(), want, [p - n for p, n in zip(past, new)], new, range(2), q_err=48 * U)
+    assert s.ctx.device_status() == 0
