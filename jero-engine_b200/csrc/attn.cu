@@ -71,24 +71,6 @@ size_t tiles_off(int num_sms)
     return partial_off(num_sms * kMaxCtasPerSm) + (size_t)num_sms * kMaxCtasPerSm * 2 * kPartialBytes;
 }
 
-// Values of a sequence without a scale (an all-zero block): far below any real
-// scale (>= 2^-74), so its weights stay small and its sums in range.
-constexpr float kNoScaleLog2 = -80.0f;
-
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ float lg2(float x)
-{
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Adds with acquire and release at GPU scope: what the CTA wrote before its
 // last barrier is seen by whoever counts after it.
 __device__ __forceinline__ int atom_add_acq_rel(int *p, int v)
@@ -508,8 +490,8 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                         }
                         const float top = fmaxf(M, warp_max_f(ml.x)), ms = top == -INFINITY ? 0.0f : top;
                         const float before = ex2(M - ms), a = ex2(ml.x - ms);
+                        den = scale_den(den, before, M - ms) + warp_sum_f(scale_den(ml.y, a, ml.x - ms));
                         M = top;
-                        den = fmaf(den, before, warp_sum_f(ml.y * a));
 #pragma unroll
                         for (int j = 0; j < N; j++) acc[j] *= before;
 #pragma unroll
@@ -540,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                 for (int w = 0; w < used; w++) {
                     const float a = ex2(s_m[w][r] - Ms);
                     const float4 v = *reinterpret_cast<const float4 *>(s_sum + (w * RR + r) * D + d);
-                    den = fmaf(s_l[w][r], a, den);
+                    den += scale_den(s_l[w][r], a, s_m[w][r] - Ms);
                     acc[0] = fmaf(v.x, a, acc[0]);
                     acc[1] = fmaf(v.y, a, acc[1]);
                     acc[2] = fmaf(v.z, a, acc[2]);
@@ -734,22 +716,23 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                         s[i][2 * u + x] = v;
                         mx[i % 4] = i < 4 && x == 0 ? v : fmaxf(mx[i % 4], v);
                     }
-                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));      // of this lane's block
+                float top = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const float mn = fmaxf(m[u], top), ms = mn == -INFINITY ? 0.0f : mn;
-                alpha[u] = ex2(m[u] - ms);
+                const float step = m[u] - ms, ref = block_ref(ms, mine);
+                alpha[u] = ex2(step);
                 m[u] = mn;
                 float sum[4];
 #pragma unroll
                 for (int i = 0; i < 8; i++)
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const float e = ex2(s[i][2 * u + x] - ms);
+                        const float e = ex2(s[i][2 * u + x] - ref);
                         s[i][2 * u + x] = e;
                         sum[i % 4] = i < 4 && x == 0 ? e : sum[i % 4] + e;
                     }
-                l[u] = fmaf(l[u], alpha[u], ((sum[0] + sum[1]) + (sum[2] + sum[3])) * isv);
+                l[u] = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), ref == ms ? isv : ex2(ref - ms - lsv), scale_den(l[u], alpha[u], step));
             }
             // A fragments of the weights: k step q takes tokens 4 q .. 4 q + 3 of each lane's block
             uint32_t pa[4][4];

@@ -27,6 +27,42 @@ __device__ __forceinline__ void from_f32(float &d, float v) { d = v; }
 __device__ __forceinline__ void from_f32(__half &d, float v) { d = __float2half_rn(v); }
 __device__ __forceinline__ void from_f32(__nv_bfloat16 &d, float v) { d = __float2bfloat16_rn(v); }
 
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x)
+{
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Attention's weights carry the scale of their block's values, 2^(logit + log2 sv - m)
+// with m the row's largest such exponent, and the denominator takes it out again.
+// Scales range over 2^-74 .. 2^121, further than the exponents of f32 reach, and a
+// block far below the largest one adds nothing to the sums but counts in the
+// denominator like any other: there its weights are formed from an exponent of
+// their own, kFar above the block's largest (so that they are zero as f16), and
+// rescaled with what that exponent is below m.
+constexpr float kFar = 60.0f;
+// Values of a block without a scale (all zeros): far below any real scale (>= 2^-74),
+// so their weights stay small and the sums in range.
+constexpr float kNoScaleLog2 = -80.0f;
+
+// The exponent that a block's weights are formed from. top: the block's largest, -inf for none seen.
+__device__ __forceinline__ float block_ref(float ms, float top) { return top > -INFINITY ? fminf(ms, top + kFar) : ms; }
+
+// l 2^x for a denominator l, where 2^x alone may underflow (x down to -250).
+__device__ __forceinline__ float scale_den(float l, float a, float x)       // a = ex2(x)
+{
+    if (x > -100.0f) return l * a;
+    const float h = ex2(0.5f * x);
+    return l * h * h;
+}
+
 // Loads of memory that a kernel before this one may have written: this kernel
 // may have been launched while that one ran, so none goes through the read-only path.
 template <typename T>

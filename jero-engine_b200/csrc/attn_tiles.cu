@@ -59,22 +59,11 @@ constexpr int kMaxSorted = 1024;
 // F32 rows: tiles whose products are summed in TMEM before they join the row's
 // sums (one: 210 us where two take 202; four: 198, and over 1e-6 off).
 constexpr int kFold = 2;
-constexpr float kNoScaleLog2 = -80.0f;
 constexpr int kCubic = 4;            // one pair of weights in this many takes the cubic
+// A tile with a block whose scale is below 2^-kWide of the largest so far takes the halves' general form
+// (blocks of zeros where values reach 8 or so). Closer ones lose weights of 2^-50 of the largest at most.
+constexpr float kWide = 76.0f;
 constexpr float kLazy = 8.0f;        // growth of a row's maximum (log2) that its sums are left unscaled for
-
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float lg2(float x)
-{
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar)
 {
@@ -629,6 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int j = 0, have; ok && (have = item(j)) >= 0; j++) {
                 if (!have) continue;
+                float largest = -INFINITY;        // log2 of the item's scales so far
                 auto lookup = [&](int t) -> int64_t {
                     const int blk = (it.tile0 + t) * (kKv / kKvBlock) + lane, first = blk * kKvBlock;
                     if (t >= it.tiles || lane >= 8 || first > it.pos_last || (p.window && first + kKvBlock - 1 <= it.pos_first - p.window))
@@ -653,13 +643,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                             // (this slot's last tile, four before, has its weights: the keys of the
                             // one before are converted, so those of three before have been used)
                             const int r = done & 3;
+                            const float ls = sv > 0.0f ? lg2(sv) : kNoScaleLog2;
+                            float big = at >= 0 ? ls : -INFINITY;
+#pragma unroll
+                            for (int o = 4; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                            largest = fmaxf(largest, big);      // (lanes 0 .. 7)
+                            const bool wide = __any_sync(0xffffffffu, at >= 0 && ls < largest - kWide);
                             if (lane < 8) {
-                                const float ls = sv > 0.0f ? lg2(sv) : kNoScaleLog2;
                                 s_sk[r][lane] = sk;
                                 s_lsv[r][lane] = ls;
                                 s_isv[r][lane] = ex2(-ls);
                             }
-                            if (lane == 0) s_ok[r] = live & 0xFFu;
+                            if (lane == 0) s_ok[r] = (live & 0xFFu) | (wide ? 0x100u : 0u);
                             __syncwarp();
                         }
                         if (lane == 0) mbar_arrive_expect_tx(&st_full[which], __popc(live) * (kKvBlock * D));
@@ -713,8 +708,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float f[4] = {rf * sk.x, rf * sk.y, rf * sk.z, rf * sk.w}, off[4] = {ls.x, ls.y, ls.z, ls.w},
                             isv[4] = {is.x, is.y, is.z, is.w};
                 const int hi = pos - tok0, lo = p.window ? max(-1, pos - p.window - tok0) : -1;   // seen: lo < column <= hi
-                const uint32_t okm = s_ok[rr] >> (4 * h) & 0xFu;
-                const bool whole = __all_sync(0xffffffffu, hi >= kHalf - 1 && (!live || lo < 0)) && okm == 0xFu;
+                const uint32_t flags = s_ok[rr], okm = flags >> (4 * h) & 0xFu;
+                const bool whole = __all_sync(0xffffffffu, hi >= kHalf - 1 && (!live || lo < 0)) && okm == 0xFu && !(flags & 0x100u);
                 // (a copy of its own for halves that every row sees whole: F32 rows 201 -> 194 us)
                 auto weigh = [&](auto whole_half) {
                     constexpr bool WHOLE = decltype(whole_half)::value;
@@ -732,6 +727,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // ---- the row's maximum; unseen columns to -inf (the other values are finite:
                 // cache bytes times f16)
                 float top = -INFINITY;
+                [[maybe_unused]] float ref[4];      // the blocks' largest
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     uint32_t (&x32)[32] = reinterpret_cast<uint32_t (&)[32]>(s[SPLIT ? 0 : 32 * c]);
@@ -753,7 +749,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                             x[i % 4] = i < 4 ? v : fmaxf(x[i % 4], v);
                         }
                         const float y = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                        top = fmaxf(top, y == -INFINITY ? -INFINITY : fmaf(y, f[2 * c + b], off[2 * c + b]));     // (0 * -inf)
+                        const float z = y == -INFINITY ? -INFINITY : fmaf(y, f[2 * c + b], off[2 * c + b]);       // (0 * -inf)
+                        if constexpr (!WHOLE) ref[2 * c + b] = z;
+                        top = fmaxf(top, z);
                     }
                 }
                 const bool grow = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
@@ -761,8 +759,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const bool fold = SPLIT && u > 0 && u % (2 * kFold) == 0;      // what TMEM holds joins the row's sums below
                 if (__any_sync(0xffffffffu, grow)) {
                     const float a = grow ? ex2(m - top) : 1.0f;
-                    if (grow) m = top;
-                    l *= a;
+                    if (grow) {
+                        l = scale_den(l, a, m - top);
+                        m = top;
+                    }
                     down = a;
                     if (u > 0 && !fold) {
                         // the sums so far, the other half's product among them (the one before
@@ -785,18 +785,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 // ---- the weights, over the logits they come from
                 const float ms = m == -INFINITY ? 0.0f : m;
+                // a block's exponent, and what takes its scale out of the denominator (nothing counts where the
+                // row sees none of it: the cubic is 2^-126 at least)
+                auto take_out = [&](float top_b, float off_b, float isv_b, float &r) -> float {
+                    r = block_ref(ms, top_b);
+                    return top_b == -INFINITY ? 0.0f : r == ms ? isv_b : ex2(r - ms - off_b);
+                };
                 if constexpr (SPLIT) {
 #pragma unroll 1
                     for (int b = 0; b < 4; b++) {
                         uint32_t x16[16], hi8[8], lo8[8];
-                        const float fb = rf * s_sk[rr][4 * h + b], zb = s_lsv[rr][4 * h + b] - ms;
+                        const float fb = rf * s_sk[rr][4 * h + b], ob = s_lsv[rr][4 * h + b];
+                        float ib = s_isv[rr][4 * h + b], rb = ms;
                         tmem_get16(ts + h * kHalf + b * 16, x16);
                         if constexpr (!WHOLE) {
                             const uint32_t mask = seen(b / 2) >> (b % 2 * 16);
 #pragma unroll
                             for (int i = 0; i < 16; i++)
                                 if (!(mask >> i & 1)) x16[i] = 0xFF800000u;
+                            float y = __uint_as_float(x16[0]);
+#pragma unroll
+                            for (int i = 1; i < 16; i++) y = fmaxf(y, __uint_as_float(x16[i]));
+                            ib = take_out(y == -INFINITY ? y : fmaf(y, fb, ob), ob, ib, rb);
                         }
+                        const float zb = ob - rb;
                         const float ff = WHOLE ? fb : fmaxf(fb, 1e-30f);    // (0 * -inf)
                         const f32x2 f2 = pair(ff, ff), z2 = pair(zb, zb);
                         f32x2 add = pair(0.0f, 0.0f);
@@ -809,7 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&hi8[i / 2]));
                             lo8[i / 2] = pack_f16(e.x - q.x, e.y - q.y);
                         }
-                        l = fmaf(unpair(add).x + unpair(add).y, s_isv[rr][4 * h + b], l);
+                        l = fmaf(unpair(add).x + unpair(add).y, ib, l);
                         tmem_st8(ts + h * kHalf + b * 16, hi8);
                         tmem_st8(ts + h * kHalf + b * 16 + 8, lo8);
                     }
@@ -830,7 +842,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         uint32_t hi16[16];
 #pragma unroll
                         for (int b = 0; b < 2; b++) {
-                            const float ff = WHOLE ? f[2 * c + b] : fmaxf(f[2 * c + b], 1e-30f), z = off[2 * c + b] - ms;    // (0 * -inf)
+                            float ib = isv[2 * c + b], rb = ms;
+                            if constexpr (!WHOLE) ib = take_out(ref[2 * c + b], off[2 * c + b], ib, rb);
+                            const float ff = WHOLE ? f[2 * c + b] : fmaxf(f[2 * c + b], 1e-30f), z = off[2 * c + b] - rb;    // (0 * -inf)
                             const f32x2 f2 = pair(ff, ff), z2 = pair(z, z);
                             f32x2 add = pair(0.0f, 0.0f);
 #pragma unroll
@@ -843,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 add = add2(add, pair(e.x, e.y));
                                 hi16[b * 8 + i / 2] = pack_f16(e.x, e.y);
                             }
-                            l = fmaf(unpair(add).x + unpair(add).y, isv[2 * c + b], l);
+                            l = fmaf(unpair(add).x + unpair(add).y, ib, l);
                         }
                         tmem_st16(ts + h * kHalf + c * 32, hi16);
                     }

@@ -86,3 +86,33 @@ def attend(q, kq, ks, vq, vs, past, scale, window, bad=()):
             p = np.exp(e - e.max())
             out[i, h] = p @ v[kv][seen] / p.sum()
     return out, big, float(np.max(np.abs(v))) if v.size else 0.0
+
+
+def attend_bound(q, kq, ks, vq, vs, past, scale, window, part, floor):
+    """attend's outputs, with a bound on each of them for a kernel whose weights are off by at most `part`
+    relative, and by `floor` of the largest p_j * (scale of v_j) of the row where they are small:
+    2 part sum p_j |v_j| + floor max(p_j s_j) sum |byte of v_j|. part(A, S): A the row's largest sum |q_d k_d| * scale,
+    S its scales' largest |log2 s_j|. Blocks of zeros have no scale: they count with 2^-80, far below any other, which
+    their weights are formed with (a floor of 2^-80 p_j floor, absolute)."""
+    n, hq, D = q.shape
+    hk = kq.shape[0]
+    k = (kq.astype(np.float64) * ks.astype(np.float64)[..., None, None]).reshape(hk, -1, D)
+    byte = np.abs(vq.astype(np.float64)).reshape(hk, -1, D)
+    sv = np.repeat(vs.astype(np.float64), BLOCK, axis=1)
+    v = vq.astype(np.float64).reshape(hk, -1, D) * sv[..., None]
+    weight = np.where(sv > 0, sv, 2.0 ** -80)
+    size = np.abs(np.log2(weight))
+    out, tol = np.zeros((n, hq, D)), np.zeros((n, hq, D))
+    for i in range(n):
+        pos = past + i
+        seen = slice(max(0, pos - window + 1) if window else 0, pos + 1)
+        for h in range(hq):
+            kv = h // (hq // hk)
+            qq = np.asarray(q[i, h], dtype=np.float64)
+            e = k[kv, seen] @ qq * scale
+            A = float(np.max(np.abs(k[kv, seen]) @ np.abs(qq)) * abs(scale))
+            p = np.exp(e - e.max())
+            p /= p.sum()
+            out[i, h] = p @ v[kv, seen]
+            tol[i, h] = 2 * part(A, float(size[kv, seen].max())) * (p @ np.abs(v[kv, seen])) + floor * np.max(p * weight[kv, seen]) * byte[kv, seen].sum(0)
+    return out, tol

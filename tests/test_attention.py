@@ -1265,3 +1265,63 @@ def test_step_of_rows_whose_squares_leave_f32(make, act, scale, eps):
             s.check_blocks(i)
         s.check_attention(out.double().cpu().numpy(), want, [p - n for p, n in zip(past, new)], new, range(2), q_err=48 * U)
     assert s.ctx.device_status() == 0
+
+
+# ------------------------------------------------- value scales far apart
+
+
+def check_rows(s, got, q, past, new, slots, scale=None, window=0, q_err=0.0):
+    """Every output against a bound of its own. With the notation of the head of this file: a weight is off by
+    part = 2 A (2^-22 + (D + 8) u + q_err) + 2^-21 + its rounding (2^-22, or with 16-bit rows 2^-11, the cubic's
+    7.5e-5 in it) + (L + 64) u, relative, and where it is below f16's normal range by half a step of 2^-24 of the
+    row's largest: 2^-25. Its exponent is logit log2 e + log2 s - m, formed in two sums of at most
+    E = 1.45 A + 2 S, S the largest |log2 s|, so off by 2 u E, and log2 s by 2^-22 S. An output below the normal
+    range of its type is rounded to a fixed step, at most half of it off: 2^-25 (f16), 2^-134 (bf16), 2^-150 (f32).
+    Returns, for each head, how often the largest output holds the bound."""
+    scale = scale or 1.0 / np.sqrt(s.D)
+    at, big = 0, np.zeros(s.hq)
+    for p, n, slot in zip(past, new, slots):
+        if not n:
+            continue
+        o, tol = ao.attend_bound(
+            q[at:at + n], *s.device_blocks(slot), p, scale, window,
+            lambda A, S: 2 * A * (2.0 ** -22 + (s.D + 8) * U + q_err) + 2.0 ** -21 + 2 * U * (1.45 * A + 2 * S)
+            + 2.0 ** -22 * S + (2.0 ** -22 if s.act == "f32" else 2.0 ** -11) + (p + n + 64) * U, 2.0 ** -25)
+        tol += HALF_STEP[s.act] * np.abs(o) + {"f16": 2.0 ** -25, "bf16": 2.0 ** -134, "f32": 2.0 ** -150}[s.act]
+        err = np.abs(got[at:at + n] - o)
+        assert np.all(err <= tol), (slot, float((err / tol).max()), np.argwhere(err > tol)[:5].tolist())
+        big = np.maximum(big, (np.abs(o) / tol).max(axis=(0, 2)))
+        at += n
+    return big
+
+
+def _gains(act, rng, n):
+    """Per token: blocks of 16 whose values differ by many orders of magnitude, zeros among them."""
+    pick = [0.0, 1e-7, 1e-3, 1.0, 3e4] if act == "f16" else [0.0, 1e-18, 1e-3, 1.0, 1e10, 1e20, 1e30]
+    block = rng.choice(len(pick), -(-n // 16))
+    return np.repeat(np.array(pick)[block], 16)[:n]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,n", [(64, 230), (128, 520)])
+def test_value_scales_far_apart(make, act, D, n):
+    """Weights count in the denominator whatever the scale of their block's values is: many rows and few, blocks of
+    zeros, and a head whose first blocks are far below its last ones."""
+    s = make(act, D=D, q_heads=8, kv_heads=2, page=16, n_slots=2, pages_per_slot=-(-n // 16))
+    r, x, q, k, v = s.rows(n)
+    b = 10 * D
+    gain = np.stack([_gains(act, s.rng, n), np.where(np.arange(n) < n // 2, 0.0, 3e4 if act == "f16" else 1e30)], axis=1)
+    gain[n // 4: n // 3, 1] = 1e-6 if act == "f16" else 1e-15
+    x[:, b:] *= s.t.tensor(np.repeat(gain, D, axis=1), device="cuda").to(s.dtype)
+    v = x.double().cpu().numpy()[:, b:].reshape(n, 2, D)
+    s.append([0], [n], [1], rows=(r, x, q, k, v))
+    s.check_blocks(1, exact_keys=True)
+    for new, scale, window in ((n, None, 0), (n - 31, 2.0, 0), (n - 40, None, 70), (1, None, 0), (3, 2.0, 0), (5, None, 40)):
+        r, _, q, _, _ = s.rows(new)
+        out = s.out(new, 8)
+        s.ctx.kv_attention(s.cache, s.batch([n - new], [new], [1], max_new=new), jm.AttnOpts(scale=scale or 0.0, window=window), r,
+                           out.data_ptr(), 8 * D)
+        big = check_rows(s, out.double().cpu().numpy(), q, [n - new], [new], [1], scale, window)
+        assert np.all(big > 20), big      # zeros would not pass
+    assert s.ctx.device_status() == 0
