@@ -1325,3 +1325,126 @@ def test_value_scales_far_apart(make, act, D, n):
         big = check_rows(s, out.double().cpu().numpy(), q, [n - new], [new], [1], scale, window)
         assert np.all(big > 20), big      # zeros would not pass
     assert s.ctx.device_status() == 0
+
+
+# --------------------------------------------------- the bits of F32 rows
+
+
+def _rms(x):
+    return float(np.sqrt(np.mean(np.square(x))))
+
+
+def error_share(got, o):
+    """The root mean square of each head's error, as a share of its outputs': the largest head's."""
+    return max(_rms(got[:, h] - o[:, h]) / _rms(o[:, h]) for h in range(o.shape[1]))
+
+
+# What F32 rows may be off by in the root mean square, as a share of the outputs', with normal queries, keys and
+# values of D values and logits within +-8. The errors of a token's weight that differ from token to token:
+#   queries and weights rounded to 22 bits      2^-23 each, a logit sum |q k| / |q| |k| of them: below 2^-22
+#   logits summed in f32                        8 steps of 2^-25 of |logit| <= 8: below 2^-20 worst, a third of it rms
+#   their exponent, in two sums of at most 32   2 * 32 u ln 2 / sqrt 3 = 2^-19.6
+#   log2 of the block's scale, 2^-22 of 6       2^-19.9 with ln 2
+#   the exponential 2^-22; sums over tiles in f32, L / 64 chained roundings that are random: below 2^-21
+# in all 2^-18.5 = 2.7e-6 of sqrt(sum p^2 v^2), which for values of mean zero is the outputs' own root mean square.
+F32_SHARE = 3e-6
+
+
+def _emulated(q, kq, ks, vq, vs, past, scale, drop):
+    """attend with queries and weights in two f16 halves, `drop` of them ("q", "p" or neither) with the upper only."""
+    def halves(x, low):
+        up = 2.0 ** (14 - np.floor(np.log2(np.max(np.abs(x), axis=-1, keepdims=True))))
+        hi = (x * up).astype(np.float16).astype(np.float64)
+        lo = (x * up - hi).astype(np.float16).astype(np.float64)
+        return (hi + (lo if low else 0.0)) / up
+    n, hq, D = q.shape
+    hk = kq.shape[0]
+    k = (kq.astype(np.float64) * ks.astype(np.float64)[..., None, None]).reshape(hk, -1, D)
+    sv = np.repeat(vs.astype(np.float64), 16, axis=1)
+    out = np.zeros((n, hq, D))
+    for i in range(n):
+        for h in range(hq):
+            kv, L = h // (hq // hk), past + i + 1
+            e = k[kv, :L] @ halves(q[i, h], drop != "q") * scale + np.log(sv[kv, :L])
+            w = np.exp(e - e.max())
+            out[i, h] = halves(w, drop != "p") @ vq[kv].reshape(-1, D)[:L].astype(np.float64) / (w / sv[kv, :L]).sum()
+    return out
+
+
+@pytest.mark.parametrize("D,L", [(128, 300), (64, 300), (128, 17), (128, 2500)])
+def test_a_dropped_half_is_seen(D, L):
+    """The measure above rejects products of 11 bits, of the queries or of the weights, and takes those of 22."""
+    rng = np.random.default_rng(D + L)
+    cache = ao.Cache()
+    cache.append(0, 0, rng.standard_normal((L, 2, D)), rng.standard_normal((L, 2, D)))
+    blocks = *cache.blocks(0, "k"), *cache.blocks(0, "v")
+    q = rng.standard_normal((3, 4, D)).astype(np.float32).astype(np.float64)
+    o, _, _ = ao.attend(q, *blocks, L - 3, 1 / np.sqrt(D), 0)
+    for drop, seen in (("", False), ("q", True), ("p", True)):
+        share = error_share(_emulated(q, *blocks, L - 3, 1 / np.sqrt(D), drop), o)
+        assert (share > 10 * F32_SHARE) == seen and (share < F32_SHARE / 10) == (not seen), (drop, share)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,hq,hk", [(128, 8, 2), (64, 6, 2)])
+def test_f32_rows_keep_22_bits(make, D, hq, hk):
+    """Single tokens, drafts, and prompts of several tiles, with and without a history."""
+    s = make("f32", D=D, q_heads=hq, kv_heads=hk, page=64, n_slots=3, pages_per_slot=42)
+    for slot, n in enumerate((2600, 333, 1100)):
+        s.append([0], [n], [slot], rows=s.rows(n))
+    for past, new in (([2599, 332, 1099], [1] * 3), ([2597, 330, 1094], [3, 3, 6]), ([2300, 0, 900], [300, 333, 200])):
+        r, _, q, _, _ = s.rows(sum(new))
+        out = s.out(sum(new), hq)
+        s.ctx.kv_attention(s.cache, s.batch(past, new, range(3), max_new=max(new)), None, r, out.data_ptr(), hq * D)
+        got, at = out.double().cpu().numpy(), 0
+        for slot, (p, n) in enumerate(zip(past, new)):
+            o, _, _ = ao.attend(q[at:at + n], *s.device_blocks(slot), p, 1 / np.sqrt(D), 0)
+            share = error_share(got[at:at + n], o)
+            assert share < F32_SHARE, (slot, p, n, share)
+            at += n
+    assert s.ctx.device_status() == 0
+
+
+# And 16-bit rows: the output's rounding, at most half a step and evenly spread over it (1 / sqrt 3), the same of the
+# weights' to f16 (2^-12), and the cubic's 7.5e-5 for a quarter of them: sqrt((2^-11)^2 + (2^-12)^2) / sqrt 3 and
+# 4e-5 for f16 rows = 3.2e-4, 2^-8 / sqrt 3 = 2.26e-3 for bf16 rows, where the other two add 1e-5.
+ROWS_SHARE = {"f16": 3.3e-4, "bf16": 2.3e-3}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f16", "bf16"])
+@pytest.mark.parametrize("D,hq,hk", [(128, 8, 2), (64, 6, 2)])
+def test_16_bit_rows_lose_their_rounding_only(make, act, D, hq, hk):
+    s = make(act, D=D, q_heads=hq, kv_heads=hk, page=64, n_slots=3, pages_per_slot=42)
+    for slot, n in enumerate((2600, 333, 1100)):
+        s.append([0], [n], [slot], rows=s.rows(n))
+    for past, new in (([2599, 332, 1099], [1] * 3), ([2595, 330, 1091], [5, 3, 9]), ([2300, 0, 900], [300, 333, 200])):
+        r, _, q, _, _ = s.rows(sum(new))
+        out = s.out(sum(new), hq)
+        s.ctx.kv_attention(s.cache, s.batch(past, new, range(3), max_new=max(new)), None, r, out.data_ptr(), hq * D)
+        got, at = out.double().cpu().numpy(), 0
+        for slot, (p, n) in enumerate(zip(past, new)):
+            o, _, _ = ao.attend(q[at:at + n], *s.device_blocks(slot), p, 1 / np.sqrt(D), 0)
+            share = error_share(got[at:at + n], o)
+            assert share < ROWS_SHARE[act], (slot, p, n, share)
+            at += n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,hq,hk,page,window", [(128, 16, 2, 64, 0), (64, 14, 2, 16, 0), (128, 5, 1, 32, 50)])
+def test_every_output_within_a_bound_of_its_own(make, act, D, hq, hk, page, window):
+    """Lengths around block, page and tile ends, single tokens to prompts, each output against what its row can be off by."""
+    s = make(act, D=D, q_heads=hq, kv_heads=hk, page=page, n_slots=8, pages_per_slot=-(-448 // page))
+    total = [1, 2, 15, 16, 17, 64, 129, 440]
+    s.append([0] * 8, total, range(8), rows=s.rows(sum(total)))
+    for new in ([1] * 8, [1, 2, 3, 5, 8, 9, 17, 33], [1, 0, 15, 16, 1, 64, 129, 440]):
+        slots = s.rng.permutation(8)
+        n = [new[i] for i in slots]
+        past = [total[i] - new[i] for i in slots]
+        r, _, q, _, _ = s.rows(sum(n))
+        out = s.out(sum(n), hq)
+        s.ctx.kv_attention(s.cache, s.batch(past, n, slots, max_new=max(n)), jm.AttnOpts(window=window), r, out.data_ptr(), hq * D)
+        big = check_rows(s, out.double().cpu().numpy(), q, past, n, slots, window=window)
+        assert np.all(big > 50), big
+    assert s.ctx.device_status() == 0
