@@ -170,7 +170,7 @@ typedef struct moe_residency {
     int32_t upload_count;
     uint64_t resident_bytes;        /* device bytes held by layer weights */
     uint64_t gguf_bytes;            /* GGUF bytes those uploads consumed */
-    uint64_t scratch_bytes;
+    uint64_t scratch_bytes;         /* the forwards' working set, and the attention calls' once there was one */
 } moe_residency;
 
 typedef struct moe_ctx moe_ctx;
@@ -268,8 +268,11 @@ int moe_lm_head(moe_ctx *ctx, int32_t T, const float *normed, float *logits, int
  * output projection's input. Device pointers on the context's device
  * throughout; asynchronous on the context's stream; the caller owns all memory
  * named here, the context a fixed workspace. The first of these calls on a
- * context allocates it (about 90 MiB), so make that call before capturing the
- * stream into a graph. Calls on one context, replays of graphs captured from
+ * context allocates it, so make that call before capturing the stream into a
+ * graph. Contexts without such calls have none: moe_admission_check does not
+ * count it, and a caller that will make them adds MOE_ATTENTION_WORKSPACE_BYTES
+ * to spec->reserve_bytes, which uploads then leave free. Once allocated it is
+ * part of moe_residency's scratch_bytes. Calls on one context, replays of graphs captured from
  * it among them, are serialised by the caller as every other call.
  *
  * What the device finds wrong in batch arrays or page tables (a slot or page id
@@ -286,6 +289,7 @@ typedef enum moe_act {
     MOE_ACT_BF16 = 30
 } moe_act;
 
+#define MOE_ATTENTION_WORKSPACE_BYTES ((uint64_t)96 << 20)   /* at most; about 88 MiB on 148 SMs */
 #define MOE_KV_MAX_TOKENS (1 << 29)   /* of a slot: table_stride * page_tokens */
 #define MOE_ROPE_MAX_FREQ 65536.0     /* the largest |inv_freq| (radians a token) */
 #define MOE_KV_BLOCK_TOKENS 16   /* tokens that share a scale, as the blocks of the reference's arena (src/kv.rs:1-4) */

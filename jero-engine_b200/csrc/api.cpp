@@ -1536,7 +1536,7 @@ int moe_residency_summary(const moe_ctx *ctx, moe_residency *out)
         out->gguf_bytes += L.gguf_bytes;
     }
     out->upload_count = ctx->upload_count;
-    out->scratch_bytes = ctx->scratch.bytes;
+    out->scratch_bytes = ctx->scratch.bytes + (ctx->attn_ws ? attn_workspace_bytes(ctx->num_sms) : 0);
     return MOE_OK;
 }
 

@@ -61,15 +61,16 @@ constexpr int kSegmentTiles = 8;
 constexpr int kJoin = 16;
 // Workspace: status word | arrival counters [2][ctas][2] | partials [ctas][2].
 constexpr size_t kCounterOff = 256;
-size_t partial_off(int ctas) { return kCounterOff + ((size_t)ctas * 16 + 255) / 256 * 256; }
+constexpr size_t partial_off(int ctas) { return kCounterOff + ((size_t)ctas * 16 + 255) / 256 * 256; }
 constexpr size_t kPartialBytes = (size_t)kMaxRows * (kMaxHeadDim + 2) * 4;
 
 // Behind them the queries of attn_tiles.cu, a slice of the rows at a time.
 constexpr size_t kTilesBytes = (size_t)80 << 20;
-size_t tiles_off(int num_sms)
+constexpr size_t tiles_off(int num_sms)
 {
     return partial_off(num_sms * kMaxCtasPerSm) + (size_t)num_sms * kMaxCtasPerSm * 2 * kPartialBytes;
 }
+static_assert(tiles_off(148) + kTilesBytes <= MOE_ATTENTION_WORKSPACE_BYTES, "what callers set aside");
 
 // Adds with acquire and release at GPU scope: what the CTA wrote before its
 // last barrier is seen by whoever counts after it.

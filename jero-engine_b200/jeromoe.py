@@ -42,6 +42,7 @@ FLAG_FUSED_I8_NEVER, FLAG_FUSED_I8_ALWAYS = 64, 128   # the fused launch's f16 /
 TENSOR_CORE_MIN_TOKENS = 256
 STREAM_LEGACY = 1       # Context.set_stream: the legacy default stream (0 is the context's own)
 KV_BLOCK_TOKENS = 16
+ATTENTION_WORKSPACE_BYTES = 96 << 20   # what a context's first attention call allocates, at most: part of reserve_bytes
 ROPE_MAX_FREQ = 65536.0   # the largest |inv_freq| of a Rope
 
 # ------------------------------------------------------------------- structs

@@ -1448,3 +1448,28 @@ def test_every_output_within_a_bound_of_its_own(make, act, D, hq, hk, page, wind
         big = check_rows(s, out.double().cpu().numpy(), q, past, n, slots, window=window)
         assert np.all(big > 50), big
     assert s.ctx.device_status() == 0
+
+
+# -------------------------------------------------------------- its workspace
+
+
+def test_admission_leaves_room_for_the_workspace():
+    """A caller sets the workspace aside as part of the reserve; without it the admission is what it was."""
+    import synth
+    from test_host import _fake_desc
+    d = [_fake_desc(synth.CONFIGS[2], np.zeros(16, dtype=np.uint8))]
+    need = jm.admission_check(0, 64, d, free_bytes=1 << 40).total_required_bytes
+    room = jm.ATTENTION_WORKSPACE_BYTES
+    jm.admission_check(0, 64, d, free_bytes=need)
+    fp = jm.admission_check(0, 64, d, free_bytes=need + room, reserve_bytes=room)
+    assert fp.total_required_bytes == need and fp.budget_bytes == need
+    with pytest.raises(jm.InsufficientLockableMemory):
+        jm.admission_check(0, 64, d, free_bytes=need + room - 1, reserve_bytes=room)
+
+
+@pytest.mark.gpu
+def test_residency_counts_the_workspace(make):
+    s = make("f32", D=64, q_heads=2, kv_heads=2)
+    assert s.ctx.residency().scratch_bytes == 0
+    s.append([0], [20], [0], rows=s.rows(20))
+    assert 80 << 20 <= s.ctx.residency().scratch_bytes <= jm.ATTENTION_WORKSPACE_BYTES
