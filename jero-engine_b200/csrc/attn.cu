@@ -95,13 +95,6 @@ __device__ __forceinline__ float warp_sum_f(float v)
     return v;
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar)
-{
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                 "l"(src), "r"(bytes), "r"(smem_addr(bar))
-                 : "memory");
-}
-
 // c += a b, and c = a b. (volatile: they stay before the refill of the slot that b came from)
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
@@ -120,23 +113,6 @@ __device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a
 }
 
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-
-// Four signed bytes to f16 pairs: byte + 128 under the exponent of 1024, minus 1152.
-__device__ __forceinline__ void bytes_f16(uint32_t w, uint32_t &lo, uint32_t &hi)
-{
-    const uint32_t u = w ^ 0x80808080u;
-    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
-    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), bias), y = __hsub2(*reinterpret_cast<__half2 *>(&b), bias);
-    lo = *reinterpret_cast<const uint32_t *>(&x);
-    hi = *reinterpret_cast<const uint32_t *>(&y);
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float a, float b)
-{
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
 
 // a and b as f16 pairs hi + lo (22 bits).
 __device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32_t &lo)

@@ -14,11 +14,6 @@
 
 namespace jmoe {
 
-template <int ACT> struct ActType;
-template <> struct ActType<MOE_ACT_F32> { using T = float; };
-template <> struct ActType<MOE_ACT_F16> { using T = __half; };
-template <> struct ActType<MOE_ACT_BF16> { using T = __nv_bfloat16; };
-
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -38,6 +33,31 @@ __device__ __forceinline__ float lg2(float x)
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// An untiled copy to shared memory, counted by a barrier.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(smem_addr(bar))
+                 : "memory");
+}
+
+// Four signed bytes to f16 pairs: byte + 128 under the exponent of 1024, minus 1152.
+__device__ __forceinline__ void bytes_f16(uint32_t w, uint32_t &lo, uint32_t &hi)
+{
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), bias), y = __hsub2(*reinterpret_cast<__half2 *>(&b), bias);
+    lo = *reinterpret_cast<const uint32_t *>(&x);
+    hi = *reinterpret_cast<const uint32_t *>(&y);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
 }
 
 // Attention's weights carry the scale of their block's values, 2^(logit + log2 sv - m)
@@ -369,14 +389,6 @@ __device__ __forceinline__ void norm_rope_vals(float (&v)[D / 32], const float *
         y[ab.y] = b * c + a * s;
     }
     __syncwarp();
-}
-
-template <int D, typename T>
-__device__ __forceinline__ void norm_rope_head(const T *x, const float *w, const RopeDev &r, int pos, float *y, int lane)
-{
-    float v[D / 32];
-    load_vals<D / 32>(x + lane * (D / 32), v);
-    norm_rope_vals<D>(v, w, r, pos, y, lane);
 }
 
 }  // namespace jmoe

@@ -65,30 +65,6 @@ constexpr int kCubic = 4;            // one pair of weights in this many takes t
 constexpr float kWide = 76.0f;
 constexpr float kLazy = 8.0f;        // growth of a row's maximum (log2) that its sums are left unscaled for
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar)
-{
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                 "l"(src), "r"(bytes), "r"(smem_addr(bar))
-                 : "memory");
-}
-
-// Four signed bytes to f16 pairs: byte + 128 under the exponent of 1024, minus 1152.
-__device__ __forceinline__ void bytes_f16(uint32_t w, uint32_t &lo, uint32_t &hi)
-{
-    const uint32_t u = w ^ 0x80808080u;
-    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
-    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), bias), y = __hsub2(*reinterpret_cast<__half2 *>(&b), bias);
-    lo = *reinterpret_cast<const uint32_t *>(&x);
-    hi = *reinterpret_cast<const uint32_t *>(&y);
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float a, float b)
-{
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 // Two f32 at a time.
 using f32x2 = uint64_t;
 __device__ __forceinline__ f32x2 pair(float a, float b)
@@ -713,155 +689,155 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // (a copy of its own for halves that every row sees whole: F32 rows 201 -> 194 us)
                 auto weigh = [&](auto whole_half) {
                     constexpr bool WHOLE = decltype(whole_half)::value;
-                if constexpr (!SPLIT) {
-                    tmem_get32(ts + h * kHalf, reinterpret_cast<uint32_t (&)[32]>(s[0]));
-                    tmem_get32(ts + h * kHalf + 32, reinterpret_cast<uint32_t (&)[32]>(s[32]));
-                }
-                // columns of 32 that this row sees
-                auto seen = [&](int c) -> uint32_t {
-                    const int up = hi - 32 * c, down = lo - 32 * c;
-                    uint32_t mask = up < 0 ? 0u : up >= 31 ? ~0u : (2u << up) - 1;
-                    if (down >= 0) mask &= down >= 31 ? 0u : ~((2u << down) - 1);
-                    return mask & ((okm >> (2 * c) & 1 ? 0xFFFFu : 0u) | (okm >> (2 * c) & 2 ? 0xFFFF0000u : 0u));
-                };
-                // ---- the row's maximum; unseen columns to -inf (the other values are finite:
-                // cache bytes times f16)
-                float top = -INFINITY;
-                [[maybe_unused]] float ref[4];      // the blocks' largest
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    uint32_t (&x32)[32] = reinterpret_cast<uint32_t (&)[32]>(s[SPLIT ? 0 : 32 * c]);
-                    if constexpr (SPLIT) {
-                        tmem_get32(ts + h * kHalf + 32 * c, x32);
+                    if constexpr (!SPLIT) {
+                        tmem_get32(ts + h * kHalf, reinterpret_cast<uint32_t (&)[32]>(s[0]));
+                        tmem_get32(ts + h * kHalf + 32, reinterpret_cast<uint32_t (&)[32]>(s[32]));
                     }
-                    if constexpr (!WHOLE) {
-                        const uint32_t mask = seen(c);
-#pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (!(mask >> i & 1)) x32[i] = 0xFF800000u;
-                    }
-#pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        float x[4];
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const float v = __uint_as_float(x32[b * 16 + i]);
-                            x[i % 4] = i < 4 ? v : fmaxf(x[i % 4], v);
-                        }
-                        const float y = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                        const float z = y == -INFINITY ? -INFINITY : fmaf(y, f[2 * c + b], off[2 * c + b]);       // (0 * -inf)
-                        if constexpr (!WHOLE) ref[2 * c + b] = z;
-                        top = fmaxf(top, z);
-                    }
-                }
-                const bool grow = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
-                [[maybe_unused]] float down = 1.0f;
-                const bool fold = SPLIT && u > 0 && u % (2 * kFold) == 0;      // what TMEM holds joins the row's sums below
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float a = grow ? ex2(m - top) : 1.0f;
-                    if (grow) {
-                        l = scale_den(l, a, m - top);
-                        m = top;
-                    }
-                    down = a;
-                    if (u > 0 && !fold) {
-                        // the sums so far, the other half's product among them (the one before
-                        // that is done: these logits came after it)
-                        if (!(ok = warp_wait(&o_sum[w], (2 * turns + h - 1) & 1, abort_flag, p.err))) return;
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int c = 0; c < D / 32; c++) {
-                            uint32_t o[32];
-                            tmem_get32(to + c * 32, o);
-#pragma unroll
-                            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-                            tmem_st32(to + c * 32, o);
-                        }
-                        tmem_st_wait();
-                        if constexpr (SPLIT)
-#pragma unroll
-                            for (int i = 0; i < D; i++) tot[i] *= a;
-                    }
-                }
-                // ---- the weights, over the logits they come from
-                const float ms = m == -INFINITY ? 0.0f : m;
-                // a block's exponent, and what takes its scale out of the denominator (nothing counts where the
-                // row sees none of it: the cubic is 2^-126 at least)
-                auto take_out = [&](float top_b, float off_b, float isv_b, float &r) -> float {
-                    r = block_ref(ms, top_b);
-                    return top_b == -INFINITY ? 0.0f : r == ms ? isv_b : ex2(r - ms - off_b);
-                };
-                if constexpr (SPLIT) {
-#pragma unroll 1
-                    for (int b = 0; b < 4; b++) {
-                        uint32_t x16[16], hi8[8], lo8[8];
-                        const float fb = rf * s_sk[rr][4 * h + b], ob = s_lsv[rr][4 * h + b];
-                        float ib = s_isv[rr][4 * h + b], rb = ms;
-                        tmem_get16(ts + h * kHalf + b * 16, x16);
-                        if constexpr (!WHOLE) {
-                            const uint32_t mask = seen(b / 2) >> (b % 2 * 16);
-#pragma unroll
-                            for (int i = 0; i < 16; i++)
-                                if (!(mask >> i & 1)) x16[i] = 0xFF800000u;
-                            float y = __uint_as_float(x16[0]);
-#pragma unroll
-                            for (int i = 1; i < 16; i++) y = fmaxf(y, __uint_as_float(x16[i]));
-                            ib = take_out(y == -INFINITY ? y : fmaf(y, fb, ob), ob, ib, rb);
-                        }
-                        const float zb = ob - rb;
-                        const float ff = WHOLE ? fb : fmaxf(fb, 1e-30f);    // (0 * -inf)
-                        const f32x2 f2 = pair(ff, ff), z2 = pair(zb, zb);
-                        f32x2 add = pair(0.0f, 0.0f);
-#pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            const f32x2 x = fma2(pair(__uint_as_float(x16[i]), __uint_as_float(x16[i + 1])), f2, z2);
-                            const float2 e = make_float2(ex2(unpair(x).x), ex2(unpair(x).y));
-                            add = add2(add, pair(e.x, e.y));
-                            hi8[i / 2] = pack_f16(e.x, e.y);
-                            const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&hi8[i / 2]));
-                            lo8[i / 2] = pack_f16(e.x - q.x, e.y - q.y);
-                        }
-                        l = fmaf(unpair(add).x + unpair(add).y, ib, l);
-                        tmem_st8(ts + h * kHalf + b * 16, hi8);
-                        tmem_st8(ts + h * kHalf + b * 16 + 8, lo8);
-                    }
-                    if (fold) {
-                        // (the product before the last is done: these logits came after it)
-                        if (!(ok = warp_wait(&o_sum[w], (2 * turns - 1) & 1, abort_flag, p.err))) return;
-                        tc_fence_after();
-#pragma unroll
-                        for (int c = 0; c < D / 32; c++) {
-                            tmem_get32(to + c * 32, s);
-#pragma unroll
-                            for (int i = 0; i < 32; i++) tot[c * 32 + i] = (tot[c * 32 + i] + __uint_as_float(s[i])) * down;
-                        }
-                    }
-                } else {
+                    // columns of 32 that this row sees
+                    auto seen = [&](int c) -> uint32_t {
+                        const int up = hi - 32 * c, down = lo - 32 * c;
+                        uint32_t mask = up < 0 ? 0u : up >= 31 ? ~0u : (2u << up) - 1;
+                        if (down >= 0) mask &= down >= 31 ? 0u : ~((2u << down) - 1);
+                        return mask & ((okm >> (2 * c) & 1 ? 0xFFFFu : 0u) | (okm >> (2 * c) & 2 ? 0xFFFF0000u : 0u));
+                    };
+                    // ---- the row's maximum; unseen columns to -inf (the other values are finite:
+                    // cache bytes times f16)
+                    float top = -INFINITY;
+                    [[maybe_unused]] float ref[4];      // the blocks' largest
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
-                        uint32_t hi16[16];
+                        uint32_t (&x32)[32] = reinterpret_cast<uint32_t (&)[32]>(s[SPLIT ? 0 : 32 * c]);
+                        if constexpr (SPLIT) {
+                            tmem_get32(ts + h * kHalf + 32 * c, x32);
+                        }
+                        if constexpr (!WHOLE) {
+                            const uint32_t mask = seen(c);
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                if (!(mask >> i & 1)) x32[i] = 0xFF800000u;
+                        }
 #pragma unroll
                         for (int b = 0; b < 2; b++) {
-                            float ib = isv[2 * c + b], rb = ms;
-                            if constexpr (!WHOLE) ib = take_out(ref[2 * c + b], off[2 * c + b], ib, rb);
-                            const float ff = WHOLE ? f[2 * c + b] : fmaxf(f[2 * c + b], 1e-30f), z = off[2 * c + b] - rb;    // (0 * -inf)
-                            const f32x2 f2 = pair(ff, ff), z2 = pair(z, z);
+                            float x[4];
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                const float v = __uint_as_float(x32[b * 16 + i]);
+                                x[i % 4] = i < 4 ? v : fmaxf(x[i % 4], v);
+                            }
+                            const float y = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                            const float z = y == -INFINITY ? -INFINITY : fmaf(y, f[2 * c + b], off[2 * c + b]);       // (0 * -inf)
+                            if constexpr (!WHOLE) ref[2 * c + b] = z;
+                            top = fmaxf(top, z);
+                        }
+                    }
+                    const bool grow = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
+                    [[maybe_unused]] float down = 1.0f;
+                    const bool fold = SPLIT && u > 0 && u % (2 * kFold) == 0;      // what TMEM holds joins the row's sums below
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float a = grow ? ex2(m - top) : 1.0f;
+                        if (grow) {
+                            l = scale_den(l, a, m - top);
+                            m = top;
+                        }
+                        down = a;
+                        if (u > 0 && !fold) {
+                            // the sums so far, the other half's product among them (the one before
+                            // that is done: these logits came after it)
+                            if (!(ok = warp_wait(&o_sum[w], (2 * turns + h - 1) & 1, abort_flag, p.err))) return;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D / 32; c++) {
+                                uint32_t o[32];
+                                tmem_get32(to + c * 32, o);
+#pragma unroll
+                                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+                                tmem_st32(to + c * 32, o);
+                            }
+                            tmem_st_wait();
+                            if constexpr (SPLIT)
+#pragma unroll
+                                for (int i = 0; i < D; i++) tot[i] *= a;
+                        }
+                    }
+                    // ---- the weights, over the logits they come from
+                    const float ms = m == -INFINITY ? 0.0f : m;
+                    // a block's exponent, and what takes its scale out of the denominator (nothing counts where the
+                    // row sees none of it: the cubic is 2^-126 at least)
+                    auto take_out = [&](float top_b, float off_b, float isv_b, float &r) -> float {
+                        r = block_ref(ms, top_b);
+                        return top_b == -INFINITY ? 0.0f : r == ms ? isv_b : ex2(r - ms - off_b);
+                    };
+                    if constexpr (SPLIT) {
+#pragma unroll 1
+                        for (int b = 0; b < 4; b++) {
+                            uint32_t x16[16], hi8[8], lo8[8];
+                            const float fb = rf * s_sk[rr][4 * h + b], ob = s_lsv[rr][4 * h + b];
+                            float ib = s_isv[rr][4 * h + b], rb = ms;
+                            tmem_get16(ts + h * kHalf + b * 16, x16);
+                            if constexpr (!WHOLE) {
+                                const uint32_t mask = seen(b / 2) >> (b % 2 * 16);
+#pragma unroll
+                                for (int i = 0; i < 16; i++)
+                                    if (!(mask >> i & 1)) x16[i] = 0xFF800000u;
+                                float y = __uint_as_float(x16[0]);
+#pragma unroll
+                                for (int i = 1; i < 16; i++) y = fmaxf(y, __uint_as_float(x16[i]));
+                                ib = take_out(y == -INFINITY ? y : fmaf(y, fb, ob), ob, ib, rb);
+                            }
+                            const float zb = ob - rb;
+                            const float ff = WHOLE ? fb : fmaxf(fb, 1e-30f);    // (0 * -inf)
+                            const f32x2 f2 = pair(ff, ff), z2 = pair(zb, zb);
                             f32x2 add = pair(0.0f, 0.0f);
 #pragma unroll
                             for (int i = 0; i < 16; i += 2) {
-                                const int k = c * 32 + b * 16 + i;
-                                const f32x2 x = fma2(pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), f2, z2);
-                                float2 e;
-                                if (i / 2 % kCubic == kCubic - 1) e = ex2_cubic(x);
-                                else e = make_float2(ex2(unpair(x).x), ex2(unpair(x).y));
+                                const f32x2 x = fma2(pair(__uint_as_float(x16[i]), __uint_as_float(x16[i + 1])), f2, z2);
+                                const float2 e = make_float2(ex2(unpair(x).x), ex2(unpair(x).y));
                                 add = add2(add, pair(e.x, e.y));
-                                hi16[b * 8 + i / 2] = pack_f16(e.x, e.y);
+                                hi8[i / 2] = pack_f16(e.x, e.y);
+                                const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&hi8[i / 2]));
+                                lo8[i / 2] = pack_f16(e.x - q.x, e.y - q.y);
                             }
                             l = fmaf(unpair(add).x + unpair(add).y, ib, l);
+                            tmem_st8(ts + h * kHalf + b * 16, hi8);
+                            tmem_st8(ts + h * kHalf + b * 16 + 8, lo8);
                         }
-                        tmem_st16(ts + h * kHalf + c * 32, hi16);
+                        if (fold) {
+                            // (the product before the last is done: these logits came after it)
+                            if (!(ok = warp_wait(&o_sum[w], (2 * turns - 1) & 1, abort_flag, p.err))) return;
+                            tc_fence_after();
+#pragma unroll
+                            for (int c = 0; c < D / 32; c++) {
+                                tmem_get32(to + c * 32, s);
+#pragma unroll
+                                for (int i = 0; i < 32; i++) tot[c * 32 + i] = (tot[c * 32 + i] + __uint_as_float(s[i])) * down;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            uint32_t hi16[16];
+#pragma unroll
+                            for (int b = 0; b < 2; b++) {
+                                float ib = isv[2 * c + b], rb = ms;
+                                if constexpr (!WHOLE) ib = take_out(ref[2 * c + b], off[2 * c + b], ib, rb);
+                                const float ff = WHOLE ? f[2 * c + b] : fmaxf(f[2 * c + b], 1e-30f), z = off[2 * c + b] - rb;    // (0 * -inf)
+                                const f32x2 f2 = pair(ff, ff), z2 = pair(z, z);
+                                f32x2 add = pair(0.0f, 0.0f);
+#pragma unroll
+                                for (int i = 0; i < 16; i += 2) {
+                                    const int k = c * 32 + b * 16 + i;
+                                    const f32x2 x = fma2(pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), f2, z2);
+                                    float2 e;
+                                    if (i / 2 % kCubic == kCubic - 1) e = ex2_cubic(x);
+                                    else e = make_float2(ex2(unpair(x).x), ex2(unpair(x).y));
+                                    add = add2(add, pair(e.x, e.y));
+                                    hi16[b * 8 + i / 2] = pack_f16(e.x, e.y);
+                                }
+                                l = fmaf(unpair(add).x + unpair(add).y, ib, l);
+                            }
+                            tmem_st16(ts + h * kHalf + c * 32, hi16);
+                        }
                     }
-                }
                 };
                 if (whole) weigh(std::true_type{});
                 else weigh(std::false_type{});
