@@ -388,12 +388,15 @@ int moe_kv_read(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *bat
  * h / (q_heads / kv_heads). out rows hold q_heads * head_dim values of
  * rows->act, out_stride elements apart, and overlap no input. A row whose every page is bad gets
  * zeros. Softmax and sums in f32; with F32 rows the products carry 22 bits of
- * the queries and weights, with 16-bit rows 11. opts may be NULL. */
+ * the queries and weights, with 16-bit rows 11: with F16 rows the weights' add
+ * as much to an output's error as its own rounding, 1.4 times that in all.
+ * opts may be NULL. */
 int moe_kv_attention(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_attn_opts *opts,
                      const moe_qkv_rows *rows, void *out, int64_t out_stride);
 
 /* The whole step: moe_kv_append of rows->k and rows->v, then moe_kv_attention
- * of rows->q, normed and rotated (in f32) as it is read. */
+ * of rows->q, normed and rotated (in f32) as it is read; the products then carry
+ * 22 bits of F16 rows' queries too, 11 of BF16 rows'. */
 int moe_attention(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rope *rope,
                   const moe_attn_opts *opts, const moe_qkv_rows *rows, void *out, int64_t out_stride);
 

@@ -824,9 +824,9 @@ cudaError_t launch_stream(const AttnParams &p, cudaStream_t st)
 template <typename T>
 cudaError_t launch_t(const AttnParams &p, cudaStream_t st)
 {
-    // Eight rows at a time where no sequence has more, or for 22 bits: half the registers, three CTAs
+    // Eight rows at a time where no sequence has more, or for queries of 22 bits: half the registers, three CTAs
     // an SM (8 rows of bf16, 64 sequences of 4000 tokens: 72 us, 16 at a time 83; one of 100000: 38 and 40)
-    if (sizeof(T) == 4 || (int64_t)p.b.max_new * (p.rows.q_heads / p.c.heads) <= 8)
+    if (keep_queries<T>(p) || (int64_t)p.b.max_new * (p.rows.q_heads / p.c.heads) <= 8)
         return p.c.D == 64 ? launch_stream<64, T, true>(p, st) : launch_stream<128, T, true>(p, st);
     if constexpr (sizeof(T) == 2)
         return p.c.D == 64 ? launch_stream<64, T, false>(p, st) : launch_stream<128, T, false>(p, st);

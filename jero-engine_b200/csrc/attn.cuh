@@ -83,6 +83,16 @@ __device__ __forceinline__ float scale_den(float l, float a, float x)       // a
     return l * h * h;
 }
 
+// Queries take two halves of 11 bits with F32 rows, and with F16 rows that are normed
+// and turned as they are read: cut to one, they add as much to an output's error as
+// its rounding to f16 (1.7 times that in all; so 1.0 to 1.3 times). BF16 rows' own
+// rounding hides it, and rows that come as they are fit one half.
+template <typename T>
+inline bool keep_queries(const AttnParams &p)
+{
+    return sizeof(T) == 4 || (std::is_same<T, __half>::value && p.use_rope);
+}
+
 // Loads of memory that a kernel before this one may have written: this kernel
 // may have been launched while that one ran, so none goes through the read-only path.
 template <typename T>

@@ -24,6 +24,9 @@
 // and the softmax threads keep their rows' in registers (rounded sums: 7.8e-7
 // off in all over 2500 tokens, 5e-6 with all the tiles in TMEM), which costs
 // room: 201 us where it took 176 then (1500 + 1025 tokens of 3 sequences, 32 heads).
+// F16 rows that are normed and turned on the way here have their queries split
+// too, for errors of 2.7e-4 where one half gives 3.5e-4 and rounding alone 2.1e-4:
+// 658 us, 543 with one half (4096 rows over 4096 + 4096 tokens, the append with them).
 //
 // Bound by the chain from one half's logits to the next one's: a softmax warp
 // takes some 2450 cycles for 64 columns (loads 360, maxima 410, a look at their
@@ -95,8 +98,8 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
 // 2^x of a pair on the multiply-add pipes, which have room where the
 // exponential's own is full: x = n + f with n its nearest integer (the low bits
 // of x + 1.5 * 2^23), and a cubic for 2^f on [-1/2, 1/2] with the smallest
-// largest relative error, 7.5e-5 (2^-13.7), below the 2^-12 that the weights'
-// rounding to f16 brings.
+// largest relative error, 7.5e-5 (2^-13.7), below the 2^-12 to 2^-11 that the
+// weights' rounding to f16 brings.
 __device__ __forceinline__ float2 ex2_cubic(f32x2 x)
 {
     float2 v = unpair(x);
@@ -234,11 +237,12 @@ __device__ __forceinline__ void sort_items(const AttnParams &p, int entry0, int 
     __syncthreads();
 }
 
-template <int D, bool SPLIT>
+// QS: queries in two halves of 11 bits.
+template <int D, bool QS>
 struct TileShape {
     static constexpr int kSlabs = D / 64;
-    static constexpr int kQTile = (SPLIT ? 2 : 1) * kSlabs * kRowsTile * 128;   // bytes of a row tile's queries
-    static constexpr int kBufs = SPLIT ? 1 : 2;
+    static constexpr int kQTile = (QS ? 2 : 1) * kSlabs * kRowsTile * 128;      // bytes of a row tile's queries
+    static constexpr int kBufs = QS ? 1 : 2;
     static constexpr int kOperand = kKv * D * 2;                                // bytes of a key or value operand
     static constexpr int kStage = kKv * D;                                      // ... and of the cache's bytes behind it
     static constexpr int kSmem = 2 * kQTile + 2 * kBufs * kOperand + 2 * kStage;
@@ -253,12 +257,12 @@ struct TileShape {
 // CTAs an SM (a layer's 4 prompts 143.5 us, four 148.4).
 constexpr int kQueryWarps = 4, kAhead = 4;
 
-template <int D, typename T, bool SPLIT>
+template <int D, typename T, bool QS>
 __global__ void __launch_bounds__(kQueryWarps * 32, sizeof(T) == 4 ? 0 : 5)
     query_tiles_kernel(const __grid_constant__ AttnParams p, int entry0, int entry1, int head0, int heads, int few_rows, int group,
                        int groups, uint8_t *images, float *factors)
 {
-    using Sh = TileShape<D, SPLIT>;
+    using Sh = TileShape<D, QS>;
     using L = HeadLanes<D, T>;
     __shared__ __align__(16) float s_y[kQueryWarps][L::kScratch];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -320,7 +324,7 @@ __global__ void __launch_bounds__(kQueryWarps * 32, sizeof(T) == 4 ? 0 : 5)
             for (int k = 0; k < L::kVals / 2; k++) {
                 const float y = a[2 * k] * up, z = a[2 * k + 1] * up;
                 hi[k] = pack_f16(y, z);
-                if constexpr (SPLIT) {
+                if constexpr (QS) {
                     const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[k]));
                     lo[k] = pack_f16(y - f.x, z - f.y);
                 }
@@ -330,9 +334,10 @@ __global__ void __launch_bounds__(kQueryWarps * 32, sizeof(T) == 4 ? 0 : 5)
                            (((d0 % 64) / 8) ^ (rt & 7)) * 16 + d0 % 8 * 2;
             if constexpr (L::kVals == 8) {
                 *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if constexpr (QS) *reinterpret_cast<uint4 *>(dst + Sh::kQTile / 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             } else {
                 *reinterpret_cast<uint2 *>(dst) = make_uint2(hi[0], hi[1]);
-                if constexpr (SPLIT) *reinterpret_cast<uint2 *>(dst + Sh::kQTile / 2) = make_uint2(lo[0], lo[1]);
+                if constexpr (QS) *reinterpret_cast<uint2 *>(dst + Sh::kQTile / 2) = make_uint2(lo[0], lo[1]);
             }
         }
         h += kAhead * L::kHeads;
@@ -343,12 +348,12 @@ __global__ void __launch_bounds__(kQueryWarps * 32, sizeof(T) == 4 ? 0 : 5)
 
 // ------------------------------------------------------------ attention
 
-template <int D, typename T, bool SPLIT>
+template <int D, typename T, bool SPLIT, bool QS>
 __global__ void __launch_bounds__(kThreads, 1)
     attend_tiles_kernel(const __grid_constant__ AttnParams p, int entry0, int entry1, int head0, int heads, int few_rows,
                         const uint8_t *images, const float *factors)
 {
-    using Sh = TileShape<D, SPLIT>;
+    using Sh = TileShape<D, QS>;
     constexpr int NB = Sh::kBufs, SL = Sh::kSlabs;
     // a conversion thread's unit of 16 bytes in every kStep-th block; SPLIT: half of them at a time, for the registers
     constexpr int kStep = kConvWarps * 32 / D, kTurns = SPLIT ? 2 : 1, kIn = 8 / kStep / kTurns;
@@ -506,13 +511,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) mbar_arrive(&s_full[i][h]);      // with the scales that the keys came with
                 const uint64_t b = dk + ((buf * Sh::kOperand + h * kHalf * 128) >> 4);
 #pragma unroll
-                for (int half = SPLIT ? 1 : 0; half >= 0; half--)      // the lower halves first: what they lose is small
+                for (int half = QS ? 1 : 0; half >= 0; half--)      // the lower halves first: what they lose is small
 #pragma unroll
                     for (int s = 0; s < SL; s++)
 #pragma unroll
                         for (int k = 0; k < 4; k++)
                             mma_ss(ts + h * kHalf, dq + ((half * SL + s) * kRowsTile * 128 >> 4) + 2 * k, b + (s * kKv * 128 >> 4) + 2 * k,
-                                   id_s, (SPLIT && half == 0) || s + k != 0);
+                                   id_s, (QS && half == 0) || s + k != 0);
                 commit_one(&s_full[i][h]);
             };
             // O: the weights of half h times the values in buffer buf
@@ -875,12 +880,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
-template <int D, typename T>
+template <int D, typename T, bool QS>
 cudaError_t launch_tiles_d(const AttnParams &p, int few_rows, uint8_t *ws, size_t ws_bytes, cudaStream_t st)
 {
     constexpr bool kSplit = sizeof(T) == 4;
-    using Sh = TileShape<D, kSplit>;
-    auto kern = attend_tiles_kernel<D, T, kSplit>;
+    using Sh = TileShape<D, QS>;
+    auto kern = attend_tiles_kernel<D, T, kSplit, QS>;
     static bool set[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -910,7 +915,7 @@ cudaError_t launch_tiles_d(const AttnParams &p, int few_rows, uint8_t *ws, size_
         for (int64_t e0 = 0; e0 < entries; e0 += slice) {
             const int e1 = (int)std::min(entries, e0 + slice);
             float *factors = reinterpret_cast<float *>(ws + (size_t)(e1 - e0) * heads * Sh::kImage);
-            if ((e = launch_dependent(query_tiles_kernel<D, T, kSplit>,
+            if ((e = launch_dependent(query_tiles_kernel<D, T, QS>,
                                       dim3((unsigned)(((int64_t)p.b.T * groups + kQueryWarps - 1) / kQueryWarps)), dim3(kQueryWarps * 32),
                                       0, st, p, (int)e0, e1, h0, heads, few_rows, group, groups, ws, factors)) != cudaSuccess)
                 return e;
@@ -928,7 +933,14 @@ cudaError_t launch_tiles_d(const AttnParams &p, int few_rows, uint8_t *ws, size_
 template <typename T>
 static cudaError_t launch_tiles_t(const AttnParams &p, int few_rows, uint8_t *ws, size_t ws_bytes, cudaStream_t st)
 {
-    return p.c.D == 64 ? launch_tiles_d<64, T>(p, few_rows, ws, ws_bytes, st) : launch_tiles_d<128, T>(p, few_rows, ws, ws_bytes, st);
+    if constexpr (!std::is_same<T, __nv_bfloat16>::value)
+        if (keep_queries<T>(p))
+            return p.c.D == 64 ? launch_tiles_d<64, T, true>(p, few_rows, ws, ws_bytes, st)
+                               : launch_tiles_d<128, T, true>(p, few_rows, ws, ws_bytes, st);
+    if constexpr (sizeof(T) == 2)
+        return p.c.D == 64 ? launch_tiles_d<64, T, false>(p, few_rows, ws, ws_bytes, st)
+                           : launch_tiles_d<128, T, false>(p, few_rows, ws, ws_bytes, st);
+    return cudaErrorInvalidValue;
 }
 
 cudaError_t launch_attention_tiles(const AttnParams &p, int few_rows, void *ws, size_t ws_bytes, cudaStream_t st)
