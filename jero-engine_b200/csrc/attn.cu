@@ -15,9 +15,9 @@
 // Bound by the cache's bytes and, as much, by what hides their latency: shared
 // memory holds 192 KB a SM in flight, and a warp's slot waits while its tile is
 // worked on. Without the products the copies alone run at 5.4 TB/s.
-//   64 single tokens over 398752 cached, 4 heads of 128, bf16  92 us, 4.4 TB/s
-//   one token over 131001 cached, F32 rows                     42 us, 3.2 TB/s
-//   one token over 701 cached, F32 rows                        12 us (latency)
+//   64 single tokens over 398752 cached, 4 heads of 128, bf16  91 to 95 us, 4.4 TB/s
+//   one token over 131001 cached, F32 rows                     40 us, 3.3 TB/s
+//   one token over 701 cached, F32 rows                        11.5 us (latency)
 //   66 drafted tokens, 17 sequences, window 1024, f16          16.5 us
 //
 // The products run on mma.m16n8k16 with f16 operands: a decode row tile has 8
@@ -25,11 +25,14 @@
 // is bound by the cache's bytes. Cache bytes are exact in f16. Queries are
 // scaled per row by a power of two; with F32 rows they and the weights are
 // split in two f16 halves that take the upper and lower 8 rows of the same
-// instruction, so 22 bits cost no more than 11.
+// instruction, so 22 bits cost no more than 11 there. With 16-bit rows one f16
+// each: the weights' rounding adds 2.1e-4 in the root mean square, as much as an
+// F16 output's own. (F16 rows that are normed and turned here take the split
+// form: see keep_queries.)
 //
 // The value scale sv of a block enters as a term of the exponent: the weights
 // w = exp2(s + log2 sv - m) stay in (0, 1] whatever the scales, and p = w / sv
-// is summed for the denominator.
+// is summed for the denominator (attn.cuh: where scales are far apart).
 #include <algorithm>
 
 #include "attn.cuh"

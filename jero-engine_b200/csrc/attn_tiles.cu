@@ -33,7 +33,7 @@
 // growth 210, weights 920, stores 90), the products and their operands' reads
 // from shared memory about as long for the four halves that are under way, and
 // neither covers the other wholly. 4096 rows of 32 heads over 4096 + 4096
-// tokens, bf16: 500 us, 0.82 PFLOP/s; 2064 tokens in 3 prompts, F32 rows: 158 us.
+// tokens, bf16: 507 us, 0.81 PFLOP/s; 2064 tokens in 3 prompts, F32 rows: 160 us.
 // (Not better: two threads a row and twice the warps, 578 us: the halves then
 // hand the maxima to one another; a third or half of the weights by the cubic
 // instead of a quarter, 494 and 505.)
