@@ -15,9 +15,9 @@
 // Bound by the cache's bytes and, as much, by what hides their latency: shared
 // memory holds 192 KB a SM in flight, and a warp's slot waits while its tile is
 // worked on. Without the products the copies alone run at 5.4 TB/s.
-//   64 single tokens over 398752 cached, 4 heads of 128, bf16  91 to 95 us, 4.4 TB/s
-//   one token over 131001 cached, F32 rows                     40 us, 3.3 TB/s
-//   one token over 701 cached, F32 rows                        11.5 us (latency)
+//   64 single tokens over 398752 cached, 4 heads of 128, bf16  95 us, 4.3 TB/s
+//   one token over 131001 cached, F32 rows                     41 us, 3.3 TB/s
+//   one token over 701 cached, F32 rows                        12 us (latency)
 //   66 drafted tokens, 17 sequences, window 1024, f16          16.5 us
 //
 // The products run on mma.m16n8k16 with f16 operands: a decode row tile has 8
@@ -357,8 +357,11 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
         if (i < 0) kv_error(p.err);
         return i;
     };
-    // The warp loads a tile's keys (0) or values (1) into its slot.
+    // The warp loads a tile's keys (0) or values (1) into its slot. Not after a wait that
+    // ran out: the slot's barrier then still counts the copies before.
+    uint32_t stuck = 0;               // 0: none did; else 1 + 2 * (tiles taken before) + whether the keys after it were under way
     auto issue = [&](int which, int64_t blk) {
+        if (stuck) return;
         uint64_t *full = &s_full[which][warp];
         const unsigned have = __ballot_sync(0xffffffffu, blk >= 0) & 0xFu;
         if (lane == 0) mbar_arrive_expect_tx(full, __popc(have) * Sh::kBlk);
@@ -643,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
             const uint32_t ph = done & 1;
             const int64_t next = lookup(sg, t + kWarps);
             float s[8][4];
-            tc_spin_wait(&s_full[0][warp], ph, &s_abort, p.err);
+            if (!__all_sync(0xffffffffu, tc_spin_wait(&s_full[0][warp], ph, &s_abort, p.err)) && !stuck) stuck = 1 + 2 * done;
             // column c of the 8-token group i: token 16 (c / 2) + 2 i + (c & 1) of the
             // tile, so that this lane's columns all lie in block lj (four groups at a
             // time: their accumulators do not wait for one another)
@@ -728,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                     pa[q][3] = pack_f16(s[2 * q + 1][2], s[2 * q + 1][3]);
                 }
             }
-            tc_spin_wait(&s_full[1][warp], ph, &s_abort, p.err);
+            if (!__all_sync(0xffffffffu, tc_spin_wait(&s_full[1][warp], ph, &s_abort, p.err)) && !stuck) stuck = 1 + 2 * done + reload;
             const uint32_t va = vbase + (warp * 4 + lj) * Sh::kVBlk + ln * 16;
             // a tile's sums start at zero and join the running ones in f32, rounded to
             // nearest: the tensor cores' additions round towards zero
@@ -772,8 +775,11 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
         joining = true;
     }
     // after a wait that ran out, copies may still be in flight
-    if (*(volatile int *)&s_abort && done)
-        for (int which = 0; which < 2; which++) drain_wait(&s_full[which][warp], (done - 1) & 1);
+    if (stuck) {
+        const uint32_t tile = (stuck - 1) / 2;
+        drain_wait(&s_full[0][warp], (tile + ((stuck - 1) & 1)) & 1);
+        drain_wait(&s_full[1][warp], tile & 1);
+    }
 }
 
 // Sequences with more rows (new tokens times query heads of a key head) than
