@@ -326,7 +326,8 @@ typedef struct moe_kv_batch {
     const int32_t *past;        /* [n_seqs] */
     const int32_t *row_start;   /* [n_seqs + 1], or NULL: sequence b has the one row b */
     const int32_t *slot;        /* [n_seqs] rows of the page table, or NULL: sequence b has slot b */
-    int32_t max_new;            /* upper bound on a sequence's rows (chooses kernels); 0: n_tokens */
+    int32_t max_new;            /* upper bound on a sequence's rows; 0: n_tokens. It chooses kernels: single tokens
+                                 * that come with row_start are faster with 1 */
     int32_t _pad;
 } moe_kv_batch;
 
@@ -396,7 +397,8 @@ int moe_kv_attention(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch
 
 /* The whole step: moe_kv_append of rows->k and rows->v, then moe_kv_attention
  * of rows->q, normed and rotated (in f32) as it is read; the products then carry
- * 22 bits of F16 rows' queries too, 11 of BF16 rows'. */
+ * 22 bits of F16 rows' queries too, 11 of BF16 rows'. A sequence whose append
+ * is refused on the device (a slot twice) attends over the cache as it stands. */
 int moe_attention(moe_ctx *ctx, const moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rope *rope,
                   const moe_attn_opts *opts, const moe_qkv_rows *rows, void *out, int64_t out_stride);
 

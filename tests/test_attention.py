@@ -1504,3 +1504,128 @@ def test_step_of_16_bit_rows_loses_their_rounding_only(make, act, D, hq, hk):
             at += new[i]
             past[i] += new[i]
     assert s.ctx.device_status() == 0
+
+
+# ------------------------------------------------------- sizes past the usual
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_cache_past_32_bits(make, act):
+    """Bytes beyond 2^32: 4.9 GiB each of keys and values, the sequences' pages spread over them."""
+    s = make(act, D=128, q_heads=16, kv_heads=8, page=256, n_slots=2, pages_per_slot=10000)
+    assert s.k.numel() > 1 << 32
+    s.table_np[0, :3] = s.n_pages - 1, 0, s.n_pages - 2     # and the very ends of them
+    s.table_np[1, :2] = s.n_pages - 3, s.n_pages // 2
+    used = set(s.table_np[0, :3]) | set(s.table_np[1, :2])
+    for i in range(2):
+        free = [p for p in s.table_np[i, 5:] if p not in used][:7]
+        s.table_np[i, 3 - i: 8] = free[: 5 + i]
+        used |= set(free)
+    s.table.copy_(s.t.tensor(s.table_np, dtype=s.t.int32))
+    total = [1500, 700]
+    s.append([0, 0], total, [0, 1], rows=s.rows(2200))
+    for i in range(2):
+        s.check_blocks(i, exact_keys=True)
+    for new in ([1, 1], [5, 300]):
+        s.attend([t - n for t, n in zip(total, new)], new, [0, 1], max_new=max(new))
+    ok, ov = s.out(700, 8), s.out(700, 8)
+    s.ctx.kv_read(s.cache, s.batch([0], [700], [1]), s.into(k=ok, v=ov))
+    kq, ks, vq, vs = s.device_blocks(1)
+    for got, q, sc in ((ok, kq, ks), (ov, vq, vs)):
+        val = (q.astype(np.float32) * sc[..., None, None]).reshape(8, -1, 128)[:, :700].transpose(1, 0, 2)
+        assert s.t.equal(got.cpu(), s.t.tensor(val).to(s.dtype))
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16"])
+def test_attention_of_a_list_too_long_to_sort(make, act):
+    """1200 sequences, prompts among single tokens: more chunks of rows than a launch puts in order."""
+    n = 1200
+    s = make(act, D=64, q_heads=3, kv_heads=1, page=16, n_slots=n, pages_per_slot=5)
+    new = [(7 * i) % 50 + 20 if i % 40 == 0 else i % 2 for i in range(n)]
+    total = [m + (11 * i) % 9 if m else 0 for i, m in enumerate(new)]
+    for a in range(0, n, 300):
+        s.append([0] * 300, total[a:a + 300], range(a, a + 300), rows=s.rows(max(1, sum(total[a:a + 300]))))
+    order = s.rng.permutation(n).tolist()
+    s.attend([total[i] - new[i] for i in order], [new[i] for i in order], order, behind=1, max_new=max(new))
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("hq,new", [(1024, [1, 3]), (512, [1, 1]), (509, [2, 0])])
+def test_many_query_heads_a_key_head(make, act, hq, new):
+    s = make(act, D=64, q_heads=hq, kv_heads=1, page=32, n_slots=2, pages_per_slot=8)
+    total = [200, 77]
+    s.append([0, 0], total, [0, 1], rows=s.rows(277))
+    s.attend([t - n for t, n in zip(total, new)], new, [0, 1], max_new=max(new))
+    rope, plain = s.rope()
+    past = [t for t in total]
+    r, x, q, k, v = s.rows(sum(new))
+    out = s.out(sum(new), hq)
+    s.ctx.attention(s.cache, s.batch(past, new, [0, 1], max_new=max(new)), rope, None, r, out.data_ptr(), hq * 64)
+    want, at = np.empty(q.shape), 0
+    for i in range(2):
+        pos = past[i] + np.arange(new[i])
+        if new[i]:
+            s.ref.append(i, past[i], plain(k[at:at + new[i]], "k", pos), v[at:at + new[i]])
+            want[at:at + new[i]] = plain(q[at:at + new[i]], "q", pos)
+        s.lens[i] = past[i] + new[i]
+        at += new[i]
+    s.check_attention(out.double().cpu().numpy(), want, past, new, [0, 1], q_err=48 * U)
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,hq,hk,R,interleaved", [(64, 7, 3, 64, False), (128, 5, 2, 64, True), (64, 1, 1, 34, False)])
+def test_norm_rope_of_many_tokens(make, act, D, hq, hk, R, interleaved):
+    """A warp a token for all its heads: head counts that do not fill its last load, queries or keys alone, no norm on one."""
+    s = make(act, D=D, q_heads=hq, kv_heads=hk)
+    rope, plain = s.rope(R, interleaved)
+    T = 4000
+    past, new = [0, 1 << 20, 9, 77], [1500, 0, 2499, 1]
+    r, x, q, k, _ = s.rows(T + 3)
+    b = s.batch(past, new, range(4), behind=3)
+    pos = np.concatenate([p + np.arange(n) for p, n in zip(past, new)])
+    for which in ("qk", "q", "k"):
+        oq, ok = s.out(T + 3, hq), s.out(T + 3, hk)
+        part = jm.QkvRows(**{f: getattr(r, f) for f, _ in r._fields_})
+        part.q, part.k = (r.q if "q" in which else None), (r.k if "k" in which else None)
+        s.ctx.qk_norm_rope(b, rope, part, s.into(oq, ok))
+        for got, y, name in ((oq, q, "q"), (ok, k, "k")):
+            got = got.double().cpu().numpy()
+            if name not in which:
+                assert np.all(got == 123.0)
+                continue
+            ref = plain(y[:T], name, pos)
+            size = 2 * np.max(np.abs(ref), axis=-1, keepdims=True) * np.sqrt(2.0)
+            assert np.all(np.abs(got[:T] - ref) <= 24 * U * size + HALF_STEP[act] * np.abs(ref) * (1 + 2 ** -7))
+            assert np.all(got[T:] == 123.0)
+    assert s.ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_step_with_a_slot_twice(make):
+    """The whole step refuses a slot's second appearance: the first and the other sequences are right, and so is the
+    call after it."""
+    s = make("f32", D=64, q_heads=4, kv_heads=2, page=16, n_slots=3, pages_per_slot=8)
+    s.append([0] * 3, [40, 30, 20], range(3), rows=s.rows(90))
+    for new in ([1, 1, 1], [20, 1, 30]):
+        r, x, q, k, v = s.rows(sum(new))
+        out = s.out(sum(new), 4)
+        past = [s.lens[0], s.lens[2], s.lens[0]]
+        s.ctx.attention(s.cache, s.batch(past, new, [0, 2, 0]), None, None, r, out.data_ptr(), 256)
+        with pytest.raises(jm.TensorBoundsError):
+            s.ctx.device_status()
+        at = 0
+        for slot, n in ((0, new[0]), (2, new[1])):
+            s.ref.append(slot, s.lens[slot], k[at:at + n], v[at:at + n])
+            s.lens[slot] += n
+            s.check_blocks(slot, exact_keys=True)
+            at += n
+        s.check_attention(out.double().cpu().numpy()[:at], q[:at], past[:2], new[:2], [0, 2])
+    s.attend([s.lens[0] - 1], [1], [0])
+    assert s.ctx.device_status() == 0
