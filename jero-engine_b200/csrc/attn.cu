@@ -15,7 +15,7 @@
 // Bound by the cache's bytes and, as much, by what hides their latency: shared
 // memory holds 192 KB a SM in flight, and a warp's slot waits while its tile is
 // worked on. Without the products the copies alone run at 5.4 TB/s.
-//   64 single tokens over 398752 cached, 4 heads of 128, bf16  95 us, 4.3 TB/s
+//   64 single tokens over 398752 cached, 4 heads of 128, bf16  96 us, 4.3 TB/s
 //   one token over 131001 cached, F32 rows                     41 us, 3.3 TB/s
 //   one token over 701 cached, F32 rows                        12 us (latency)
 //   66 drafted tokens, 17 sequences, window 1024, f16          16.5 us
@@ -34,6 +34,7 @@
 // w = exp2(s + log2 sv - m) stay in (0, 1] whatever the scales, and p = w / sv
 // is summed for the denominator (attn.cuh: where scales are far apart).
 #include <algorithm>
+#include <type_traits>
 
 #include "attn.cuh"
 #include "kernels.h"
@@ -357,13 +358,20 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
         if (i < 0) kv_error(p.err);
         return i;
     };
-    // The warp loads a tile's keys (0) or values (1) into its slot. Not after a wait that
-    // ran out: the slot's barrier then still counts the copies before.
-    uint32_t stuck = 0;               // 0: none did; else 1 + 2 * (tiles taken before) + whether the keys after it were under way
-    auto issue = [&](int which, int64_t blk) {
-        if (stuck) return;
+    // The warp loads a tile's keys (0) or values (1) into its slot. `refill`: a tile of the
+    // segment was there, the n-th that the warp was given is to follow. Nothing is loaded
+    // once a wait of the CTA has run out: the slot's barrier may then still count the copies
+    // before. (Lane 31 brings the flag to the ballot; segments end with the first such one:
+    // in all 96 us instead of 95 for the 64 single tokens.)
+    uint32_t held = 0;                // 0: none did; else 1 + 2 n + which of the first load held back
+    auto issue = [&](auto refill, int which, int64_t blk, uint32_t n) {
+        constexpr bool REFILL = decltype(refill)::value;
         uint64_t *full = &s_full[which][warp];
-        const unsigned have = __ballot_sync(0xffffffffu, blk >= 0) & 0xFu;
+        const unsigned all = __ballot_sync(0xffffffffu, REFILL && lane == 31 ? *(volatile int *)&s_abort != 0 : blk >= 0), have = all & 0xFu;
+        if (REFILL && all >> 31) {
+            if (!held) held = 1 + 2 * n + which;
+            return;
+        }
         if (lane == 0) mbar_arrive_expect_tx(full, __popc(have) * Sh::kBlk);
         __syncwarp();
         if (lane < 4 && blk >= 0) {
@@ -534,7 +542,8 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
             }
         }
         // ---- a segment's beginning: its first loads
-        if (!next_segment(sg)) break;
+        // (all waits lie between two barriers: every thread reads the same flag here)
+        if (*(volatile int *)&s_abort || !next_segment(sg)) break;
         constexpr int kAhead = 2;             // query rows a warp asks for at once
         float qv[kAhead][N], sk = 0.0f, sv = 0.0f;
         int64_t blk = -1;
@@ -547,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
             blk = lookup(sg, t);
             if (t < sg.t1)
 #pragma unroll 1
-                for (int which = 0; which < 2; which++) issue(which, blk);
+                for (int which = 0; which < 2; which++) issue(std::false_type{}, which, blk, done);
             scales(blk, sk, sv);
         }
 
@@ -646,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
             const uint32_t ph = done & 1;
             const int64_t next = lookup(sg, t + kWarps);
             float s[8][4];
-            if (!__all_sync(0xffffffffu, tc_spin_wait(&s_full[0][warp], ph, &s_abort, p.err)) && !stuck) stuck = 1 + 2 * done;
+            tc_spin_wait(&s_full[0][warp], ph, &s_abort, p.err);
             // column c of the 8-token group i: token 16 (c / 2) + 2 i + (c & 1) of the
             // tile, so that this lane's columns all lie in block lj (four groups at a
             // time: their accumulators do not wait for one another)
@@ -671,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
             const bool reload = t + kWarps < sg.t1;
             if (reload) {
                 given_back();
-                issue(0, next);
+                issue(std::true_type{}, 0, next, done + 1);
             }
             float sk_next, sv_next;
             scales(next, sk_next, sv_next);
@@ -731,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
                     pa[q][3] = pack_f16(s[2 * q + 1][2], s[2 * q + 1][3]);
                 }
             }
-            if (!__all_sync(0xffffffffu, tc_spin_wait(&s_full[1][warp], ph, &s_abort, p.err)) && !stuck) stuck = 1 + 2 * done + reload;
+            tc_spin_wait(&s_full[1][warp], ph, &s_abort, p.err);
             const uint32_t va = vbase + (warp * 4 + lj) * Sh::kVBlk + ln * 16;
             // a tile's sums start at zero and join the running ones in f32, rounded to
             // nearest: the tensor cores' additions round towards zero
@@ -765,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
             }
             if (reload) {
                 given_back();
-                issue(1, next);
+                issue(std::true_type{}, 1, next, done + 1);
             }
             blk = next;
             sk = sk_next;
@@ -775,10 +784,11 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 2)
         joining = true;
     }
     // after a wait that ran out, copies may still be in flight
-    if (stuck) {
-        const uint32_t tile = (stuck - 1) / 2;
-        drain_wait(&s_full[0][warp], (tile + ((stuck - 1) & 1)) & 1);
-        drain_wait(&s_full[1][warp], tile & 1);
+    if (*(volatile int *)&s_abort) {
+        // loads of each kind: all that were asked for, or those before the first one held back
+        const uint32_t values = held ? (held - 1) / 2 : done, keys = values + (held ? (held - 1) & 1 : 0);
+        if (keys) drain_wait(&s_full[0][warp], (keys - 1) & 1);
+        if (values) drain_wait(&s_full[1][warp], (values - 1) & 1);
     }
 }
 
